@@ -1,0 +1,101 @@
+// The residual step between two blocks, one launch (the stack's moe_stack_norm with a norm behind the block, a gate
+// and other types):
+//   a = h rsqrt(mean(h^2) + post_eps) post_w   (or h itself)
+//   v = x + scale gate a;   out = v;   normed = v rsqrt(mean(v^2) + pre_eps) pre_w
+// gate: none, one value per token, per channel or per value, as it is or through a sigmoid. v stays in fp32 from the
+// sum to `normed`; out and normed are rounded once. A group of 256 threads takes a token's row, 8 neighbouring
+// values per thread and step, all of them in registers between the two sums of squares, whose partial sums meet
+// in fixed order. out may be x, and normed h, in place.
+// Constants: 0 h (0: none, v = x) 2 h stride 4 x 6 x stride 8 out (0: none) 10 out stride 12 normed (0: none)
+// 14 normed stride 16 post weight (0: none) 18 pre weight (0: none) 20 gate (0: none) 22 gate's token stride
+// 24 gate's channel step (0 or 1) 25 types (h | x << 4 | out << 8 | normed << 12 | gate << 16) 26 flags (1 post norm,
+// 2 sigmoid) 27 E 28 post eps 29 pre eps 30 scale (fp32 bits) 31 tokens. Weights are fp32.
+#pragma once
+#include "rows.h"
+
+// Sum over the group's four waves, in their order.
+__device__ __forceinline__ float bn_group_sum(float v, float *part) {
+    v = gd_wave_sum_dpp(v);
+    if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+template <int STEPS>
+__device__ __forceinline__ void block_norm_body(const GdArgs &a) {
+    __shared__ float part[2][4];
+    const uint32_t E = a.c[27], types = a.c[25], flags = a.c[26];
+    const uint32_t ht = types & 15u, xt = types >> 4 & 15u, ot = types >> 8 & 15u, nt = types >> 12 & 15u, gt = types >> 16 & 15u;
+    const uint64_t H = gd_addr(a, 0), X = gd_addr(a, 4), O = gd_addr(a, 8), N = gd_addr(a, 12), PW = gd_addr(a, 16),
+                   NW = gd_addr(a, 18), G = gd_addr(a, 20);
+    const uint64_t hs = gd_addr(a, 2), xs = gd_addr(a, 6), os = gd_addr(a, 10), ns = gd_addr(a, 14), gs = gd_addr(a, 22);
+    const bool channel = a.c[24] != 0u, post = flags & 1u, sigmoid = flags & 2u;
+    const float scale = gd_bits_f32(a.c[30]);
+    const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= a.c[31]) return;
+    const bool hw = row_aligned(H, hs, ht), xw = row_aligned(X, xs, xt), ow = row_aligned(O, os, ot), nw = row_aligned(N, ns, nt),
+               gw = row_aligned(G, gs, gt), pw = row_aligned(PW, 0, ROW_F32), ww = row_aligned(NW, 0, ROW_F32);
+    float v[STEPS][8], x[STEPS][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        const uint32_t i = (k * 256u + threadIdx.x) * 8u;
+        row_load8(X + ((row * xs) << row_shift(xt)), i, E, xt, xw, x[k]);
+        if (H) row_load8(H + ((row * hs) << row_shift(ht)), i, E, ht, hw, v[k]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
+    }
+    if (H) {
+        float r = scale;
+        if (post) {
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ss += v[k][j] * v[k][j];
+            r = scale / sqrtf(bn_group_sum(ss, part[0]) / (float)E + gd_bits_f32(a.c[28]));
+        }
+        if (G && !channel) {
+            const float g = row_load(G, row * gs, gt);
+            r *= sigmoid ? gd_sigmoid_accurate(g) : g;
+        }
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const uint32_t i = (k * 256u + threadIdx.x) * 8u;
+            float w[8], g[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = g[j] = 1.f;
+            if (PW) row_load8(PW, i, E, ROW_F32, pw, w);
+            if (G && channel) {
+                row_load8(G + ((row * gs) << row_shift(gt)), i, E, gt, gw, g);
+                if (sigmoid)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[j] = gd_sigmoid_accurate(g[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[k][j] += v[k][j] * r * w[j] * g[j];
+        }
+    }
+    if (O)
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+            row_store8(O + ((row * os) << row_shift(ot)), (k * 256u + threadIdx.x) * 8u, E, ot, ow, x[k]);
+    if (!N) return;
+    ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += x[k][j] * x[k][j];  // values past the row's end are zeros
+    const float r = 1.0f / sqrtf(bn_group_sum(ss, part[1]) / (float)E + gd_bits_f32(a.c[29]));
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        const uint32_t i = (k * 256u + threadIdx.x) * 8u;
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = 1.f;
+        if (NW) row_load8(NW, i, E, ROW_F32, ww, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] *= x[k][j] * r;
+        row_store8(N + ((row * ns) << row_shift(nt)), i, E, nt, nw, w);
+    }
+}

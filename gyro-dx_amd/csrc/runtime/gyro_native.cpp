@@ -809,7 +809,8 @@ extern "C" gd_result gd_dispatch_on(gd_context *c, gd_pipeline *p, const uint32_
         x > 65535 || y > 65535 || z > 65535)
         return kInvalidArg;
     GD_HIP(hipSetDevice(c->device));
-    return launch(c, p, c->table, constants, count, x, y, z, stream ? (hipStream_t)stream : c->compute);
+    return launch(c, p, c->table, constants, count, x, y, z,
+                  stream == GD_STREAM_DEFAULT ? nullptr : stream ? (hipStream_t)stream : c->compute);
 }
 
 extern "C" gd_result gd_wrap_memory(gd_context *c, void *device_address, uint64_t bytes, gd_buffer **out,

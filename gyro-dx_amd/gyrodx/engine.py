@@ -1,4 +1,4 @@
-"""ctypes binding of the C++ MoE layer engine (include/gyro_moe.h)."""
+"""ctypes binding of the C++ MoE layer engine (include/gyro_moe.h) and its operators (include/gyro_ops.h)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -19,6 +19,48 @@ class LayerDesc(C.Structure):
                 ("types", C.c_void_p), ("SF", C.c_uint32), ("sh_gate", C.c_void_p), ("sh_up", C.c_void_p),
                 ("sh_down", C.c_void_p), ("sh_gate_inp", C.c_void_p), ("norm_weight", C.c_void_p),
                 ("norm_eps", C.c_float), ("sh_type", C.c_uint32)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_uint64), ("type", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class MatrixDesc(C.Structure):
+    _fields_ = [("format", C.c_uint32), ("rows", C.c_uint32), ("cols", C.c_uint32), ("group", C.c_uint32)] + \
+        [(p + f, C.c_void_p) for p in ("", "up_") for f in ("quants", "scales", "mins")]
+
+
+class BlockNormDesc(C.Structure):
+    _fields_ = [("E", C.c_uint32), ("post", C.c_uint32), ("gate_kind", C.c_uint32), ("gate_act", C.c_uint32),
+                ("h", Rows), ("x", Rows), ("out", Rows), ("normed", Rows), ("gate", Rows),
+                ("post_weight", C.c_void_p), ("pre_weight", C.c_void_p), ("post_eps", C.c_float),
+                ("pre_eps", C.c_float), ("scale", C.c_float), ("reserved", C.c_uint32)]
+
+
+class LogprobsDesc(C.Structure):
+    _fields_ = [("logits", Rows), ("V", C.c_uint32), ("given", C.c_uint32), ("top", C.c_uint32),
+                ("tokens_64", C.c_uint32), ("scale", C.c_float), ("reserved", C.c_uint32), ("tokens", C.c_void_p),
+                ("tokens_stride", C.c_uint64), ("logprobs", C.c_void_p), ("logprobs_stride", C.c_uint64),
+                ("entropy", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
+                ("top_stride", C.c_uint64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+# 4-bit matrix formats (gm_matrix_desc) and the operators' activations and element types.
+MATRIX_FORMATS = {"q4_0": 0, "q4_1": 1, "q4": 2}
+ACTS = {"none": 0, "silu": 1, "sigmoid": 2}
+GATE_TOKEN, GATE_CHANNEL, GATE_VALUE = 1, 2, 3
+_TYPE_NAMES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2, "torch.int32": 3, "torch.int64": 4,
+               "torch.uint8": 5}
+_type_codes = {}  # dtype object -> its code in _TYPE_NAMES
+
+
+def _type(t, allowed, what):
+    code = _type_codes.get(t.dtype)
+    if code is None:
+        code = _type_codes[t.dtype] = _TYPE_NAMES.get(str(t.dtype), -1)
+    if code not in allowed:
+        raise ValueError(f"{what}: dtype {t.dtype} is not taken")
+    return code
 
 
 # GGML type of a shared expert's matrices (src/kernels.zig:7-10) -> the engine's gm_layer_desc code.
@@ -57,6 +99,14 @@ def lib() -> C.CDLL:
         L.gm_run_stack.argtypes = [vp, u32, u32, u32, u32, C.POINTER(u32), u32, C.POINTER(C.c_double),
                                    C.POINTER(C.c_double)]
         L.gm_forward_decode_noalloc.argtypes = [vp, u32, vp, u32, vp, vp]
+        L.gm_load_operators.argtypes = [vp]
+        L.gm_add_matrix.argtypes = [vp, C.POINTER(MatrixDesc), C.POINTER(u32)]
+        L.gm_release_matrix.argtypes = [vp, u32]
+        L.gm_linear.argtypes = [vp, u32, C.POINTER(Rows), u32, C.POINTER(Rows), u32, u32, C.c_float, vp]
+        L.gm_block_norm.argtypes = [vp, C.POINTER(BlockNormDesc), u32, vp]
+        L.gm_logprobs_workspace.argtypes = [u32, u32, u32]
+        L.gm_logprobs_workspace.restype = C.c_uint64
+        L.gm_logprobs.argtypes = [vp, C.POINTER(LogprobsDesc), u32, vp]
         _lib = L
     return _lib
 
@@ -74,7 +124,9 @@ class Engine:
         if rc != 0:
             raise RuntimeError(f"gm_create failed ({rc})")
         self.max_tok = max_tok
+        self.adapter = adapter
         self.E = None
+        self._matrices = {}
 
     def _check(self, rc, what):
         if rc != 0:
@@ -201,3 +253,147 @@ class Engine:
         out = np.empty((n, self.E), np.float32)
         self._check(lib().gm_read_outputs(self._h, _f32p(out), n), "gm_read_outputs")
         return out
+
+    # ---- operators around the layers, on device tensors ------------------------------------------
+    # Tensors are torch tensors (or objects with their shape, dtype, stride(), data_ptr() and get_device()) on the
+    # engine's GPU; `stream` is a hipStream_t as torch gives it (torch.cuda.current_stream().cuda_stream; 0 is the
+    # default stream). Each call queues its work and returns. include/gyro_ops.h states the formulas.
+
+    def load_operators(self):
+        """Loads the operators' kernels, so that first calls may be captured into a graph."""
+        self._check(lib().gm_load_operators(self._h), "gm_load_operators")
+
+    def add_matrix(self, fmt: str, rows: int, cols: int, data, up=None, group: int = 32) -> int:
+        """Uploads a 4-bit matrix (or, with `up`, a gated pair) and returns its index. fmt "q4_0" or "q4_1": `data`
+        is the uint8 array of its GGUF blocks; "q4": (quants uint8 [rows, cols / 2], scales float16 [rows,
+        cols / group], mins float16 or None)."""
+        if fmt not in MATRIX_FORMATS:
+            raise ValueError(f"matrix format {fmt!r} is none of {sorted(MATRIX_FORMATS)}")
+        keep = []
+
+        def parts(m):
+            m = m if fmt == "q4" else (m, None, None)
+            if len(m) != 3:
+                raise ValueError("a q4 matrix is (quants, scales, mins or None)")
+            if rows <= 0 or cols <= 0 or group <= 0 or cols % group:
+                raise ValueError("a matrix has rows, and columns in whole groups")
+            block = {"q4_0": 18, "q4_1": 20}.get(fmt)
+            want = [(np.uint8, rows * cols // 32 * block if block else rows * cols // 2),
+                    (np.float16, rows * (cols // group)), (np.float16, rows * (cols // group))]
+            out = []
+            for a, (dtype, size), name in zip(m, want, ("quants", "scales", "mins")):
+                if a is not None:
+                    a = np.ascontiguousarray(a)
+                    if a.dtype != dtype or a.size != size:
+                        raise ValueError(f"{name}: {a.dtype} x {a.size}, not {np.dtype(dtype)} x {size}")
+                    keep.append(a)
+                out.append(None if a is None else a.ctypes.data)
+            return out
+
+        d = MatrixDesc(MATRIX_FORMATS[fmt], rows, cols, group, *parts(data), *(parts(up) if up is not None else ()))
+        idx = C.c_uint32()
+        self._check(lib().gm_add_matrix(self._h, C.byref(d), C.byref(idx)), "gm_add_matrix")
+        self._matrices[idx.value] = (rows, cols)
+        return idx.value
+
+    def release_matrix(self, matrix: int):
+        if self._h:
+            self._check(lib().gm_release_matrix(self._h, matrix), "gm_release_matrix")
+            self._matrices.pop(matrix, None)
+
+    def _rows(self, t, n, cols, what):
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != n or shape[1] != cols:
+            raise ValueError(f"{what}: shape {tuple(shape)}, not {(n, cols)}")
+        if t.get_device() != self.adapter:
+            raise ValueError(f"{what}: not on the engine's GPU")
+        stride, step = t.stride()
+        if step != 1 and cols > 1:
+            raise ValueError(f"{what}: the values of a row are not neighbours")
+        return Rows(t.data_ptr(), stride, _type(t, (0, 1, 2), what))
+
+    def _flat(self, t, size, types, what):
+        """Address of a contiguous tensor of `size` values (None: no tensor)."""
+        if t is None:
+            return None
+        if t.numel() != size or not t.is_contiguous():
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, not {size} neighbouring values")
+        if t.get_device() != self.adapter:
+            raise ValueError(f"{what}: not on the engine's GPU")
+        _type(t, types, what)
+        return t.data_ptr()
+
+    def linear(self, matrix: int, x, y, act: str = "none", accumulate: bool = False, scale: float = 1.0,
+               stream: int = 0):
+        """y = act(scale W x) per row (+ y with accumulate), or scale silu(G x) * (U x) of a gated pair."""
+        if matrix not in self._matrices:
+            raise ValueError(f"no matrix {matrix}")
+        rows, cols = self._matrices[matrix]
+        n = x.shape[0]
+        xr, yr = self._rows(x, n, cols, "x"), self._rows(y, n, rows, "y")
+        rc = lib().gm_linear(self._h, matrix, xr, n, yr, ACTS[act], accumulate, scale, stream)
+        if rc:
+            self._check(rc, "gm_linear")
+
+    def block_norm(self, h, x, out=None, normed=None, post: bool = False, post_weight=None, post_eps: float = 1e-6,
+                   gate=None, gate_act: str = "none", scale: float = 1.0, pre_weight=None, pre_eps: float = 1e-6,
+                   stream: int = 0):
+        """out = v = x + scale * gate * a with a = RMSNorm(h) (post) or h, normed = RMSNorm(v). `gate` is [n, 1] (per
+        token), [1, E] (per channel) or [n, E]; weights are fp32 [E]. h None: v = x."""
+        n, E = x.shape
+        d = BlockNormDesc(E, post)
+        d.x = self._rows(x, n, E, "x")
+        if h is not None:
+            d.h = self._rows(h, n, E, "h")
+        if out is not None:
+            d.out = self._rows(out, n, E, "out")
+        if normed is not None:
+            d.normed = self._rows(normed, n, E, "normed")
+        if gate is not None:
+            shape = tuple(gate.shape)
+            d.gate_kind = GATE_VALUE if shape == (n, E) else GATE_CHANNEL if shape == (1, E) else GATE_TOKEN
+            d.gate = self._rows(gate, *{GATE_VALUE: (n, E), GATE_CHANNEL: (1, E), GATE_TOKEN: (n, 1)}[d.gate_kind], "gate")
+            d.gate_act = ACTS[gate_act]
+        d.post_weight = self._flat(post_weight, E, (0,), "post_weight")
+        d.pre_weight = self._flat(pre_weight, E, (0,), "pre_weight")
+        d.post_eps, d.pre_eps, d.scale = post_eps, pre_eps, scale
+        rc = lib().gm_block_norm(self._h, d, n, stream)
+        if rc:
+            self._check(rc, "gm_block_norm")
+
+    @staticmethod
+    def logprobs_workspace(n: int, V: int, top: int = 0) -> int:
+        """Bytes of the workspace that logprobs() of n rows of V logits takes."""
+        return lib().gm_logprobs_workspace(n, V, top)
+
+    def logprobs(self, logits, workspace=None, tokens=None, logprob=None, entropy=None, top_ids=None,
+                 top_logprobs=None, scale: float = 1.0, stream: int = 0):
+        """Log probabilities of `tokens` (int32 or int64 [n, given]) under softmax(scale * logits) into logprob (fp32
+        [n, given]), the entropy (fp32 [n]), and the largest logits' ids (int32 [n, top]) and log probabilities.
+        workspace: a uint8 tensor of at least logprobs_workspace() bytes, not shared with calls that may overlap."""
+        n, V = logits.shape
+        d = LogprobsDesc(self._rows(logits, n, V, "logits"), V)
+        d.scale = scale
+        if tokens is not None:
+            d.given = tokens.shape[-1]
+            d.tokens = self._flat(tokens, n * d.given, (3, 4), "tokens")
+            d.tokens_64 = _type(tokens, (3, 4), "tokens") == 4
+            if logprob is None:
+                raise ValueError("tokens without logprob")
+            d.logprobs = self._flat(logprob, n * d.given, (0,), "logprob")
+            d.tokens_stride = d.logprobs_stride = d.given
+        elif logprob is not None:
+            raise ValueError("logprob without tokens")
+        d.entropy = self._flat(entropy, n, (0,), "entropy")
+        if (top_ids is None) != (top_logprobs is None):
+            raise ValueError("top_ids and top_logprobs go together")
+        if top_ids is not None:
+            d.top = d.top_stride = top_ids.shape[-1]
+            d.top_ids = self._flat(top_ids, n * d.top, (3,), "top_ids")
+            d.top_logprobs = self._flat(top_logprobs, n * d.top, (0,), "top_logprobs")
+        if workspace is not None:
+            d.workspace_bytes = workspace.numel()
+            d.workspace = self._flat(workspace, d.workspace_bytes, (5,), "workspace")
+        rc = lib().gm_logprobs(self._h, d, n, stream)
+        if rc:
+            self._check(rc, "gm_logprobs")

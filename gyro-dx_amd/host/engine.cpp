@@ -26,6 +26,7 @@
 #include "decode_split.h"
 #include "device.h"
 #include "gyro_moe.h"
+#include "row_ops.h"
 
 // Intermediate buffers of gm_forward_decode_noalloc: router logits, routes, the rotated input,
 // the gate/up partials and the shared expert's rows. One copy per GPU, alive until the process
@@ -433,6 +434,78 @@ class Engine {
         }
     }
 
+    // The operators of row_ops.h; their kernels load with the first matrix or call that takes them.
+    RowOps ops;
+    // Uploads a matrix and lays it out (q4_repack); a gated pair's halves go through one source buffer in turn.
+    uint32_t add_matrix(const gm_matrix_desc &d) {
+        Matrix m = RowOps::describe(d);
+        ops.load("q4_repack");
+        ops.load("mv_q4");
+        const uint64_t bytes = RowOps::layout(m), qb = (RowOps::quant_bytes(d) + 255) & ~uint64_t(255),
+                       sb = d.scales ? (RowOps::scale_bytes(d) + 255) & ~uint64_t(255) : 0, mb = d.mins ? sb : 0;
+        struct Held {
+            Device &dev;
+            Buffer b;
+            ~Held() { dev.release(b); }
+        } src{dev, {}}, out{dev, {}};
+        out.b = dev.buffer(bytes, Kind::device);
+        src.b = dev.buffer(qb + sb + mb, Kind::device);
+        const void *parts[2][3] = {{d.quants, d.scales, d.mins}, {d.up_quants, d.up_scales, d.up_mins}};
+        for (uint32_t half = 0; half < (m.gated ? 2u : 1u); ++half) {
+            upload_bytes(src.b, 0, parts[half][0], RowOps::quant_bytes(d));
+            if (sb) upload_bytes(src.b, qb, parts[half][1], RowOps::scale_bytes(d));
+            if (mb) upload_bytes(src.b, qb + sb, parts[half][2], RowOps::scale_bytes(d));
+            Constants c;
+            c.set(0, d.format);
+            c.set(1, m.rows);
+            c.set(2, m.cols);
+            c.set(3, m.chunks);
+            c.set(4, m.lg);
+            c.set(5, m.tiles / (m.gated ? 2u : 1u));
+            c.set(6, m.gated ? 2u : 1u);
+            c.set(7, half);
+            c.set64(8, src.b.gpu);
+            c.set64(10, src.b.gpu + qb);
+            if (mb) c.set64(12, src.b.gpu + qb + sb);
+            c.set64(14, out.b.gpu);
+            c.set64(16, out.b.gpu + m.scales);
+            if (m.mins) c.set64(18, out.b.gpu + m.minima);
+            const uint64_t groups = ((uint64_t)c.w[5] * m.chunks * 64 + 255) / 256;
+            dev.begin();
+            dev.dispatch(ops.pipes.at("q4_repack"), c.w, 60, (uint32_t)std::min<uint64_t>(groups, 65535),
+                         (uint32_t)((groups + 65534) / 65535), 1);
+            dev.wait(dev.submit());
+        }
+        m.data = out.b;
+        out.b = Buffer{};
+        return ops.keep(std::move(m));
+    }
+    void launch(const Launch &l, void *stream) {
+        if (!l.x) return;
+        auto it = ops.pipes.find(l.kernel);
+        if (it == ops.pipes.end()) {
+            // Loading may allocate, which a capture does not take.
+            hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+            if (stream && hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess) status = hipStreamCaptureStatusActive;
+            require(status == hipStreamCaptureStatusNone,
+                    "the operator's kernel is not loaded: call gm_load_operators or the operator once before a capture");
+            require(ops.files.count(l.kernel) != 0, "operator kernel missing from the kernel directory");
+            ops.load(l.kernel);
+            it = ops.pipes.find(l.kernel);
+        }
+        check(gd_dispatch_on(dev.ctx, it->second, l.c.w, 60, l.x, l.y, 1, stream ? stream : GD_STREAM_DEFAULT), "gd_dispatch_on");
+    }
+    // upload() of any number of bytes: the last word is filled up with zeros (the buffer has room).
+    void upload_bytes(const Buffer &dst, uint64_t off, const void *src, uint64_t bytes) {
+        const uint64_t whole = bytes & ~uint64_t(3);
+        if (whole) upload(dst, off, src, whole);
+        if (bytes > whole) {
+            uint32_t word = 0;
+            std::memcpy(&word, static_cast<const uint8_t *>(src) + whole, bytes - whole);
+            upload(dst, off + whole, &word, 4);
+        }
+    }
+
     void load_kernels(const std::string &dir) {
         DIR *d = opendir(dir.c_str());
         if (!d) throw NativeError(-1, "kernel directory not found: " + dir);
@@ -440,7 +513,9 @@ class Engine {
             std::string name = ent->d_name;
             if (name.size() > 3 && name.compare(name.size() - 3, 3, ".co") == 0) {
                 const std::string kernel = name.substr(0, name.size() - 3), file = dir + "/" + name;
-                if (kernel.rfind("moe_decode_gu", 0) == 0 || kernel.rfind("moe_decode_down", 0) == 0)
+                if (RowOps::owns(kernel))
+                    ops.files[kernel] = file;
+                else if (kernel.rfind("moe_decode_gu", 0) == 0 || kernel.rfind("moe_decode_down", 0) == 0)
                     decode_files[kernel] = file;
                 else
                     pipes[kernel] = dev.pipeline(read_file(file));
@@ -607,9 +682,12 @@ class Engine {
         dev.wait(dev.submit());
     }
 
-    void create(const std::string &kernel_dir, uint32_t adapter, uint32_t tokens_per_call) {
+    uint32_t adapter = 0;
+    void create(const std::string &kernel_dir, uint32_t device, uint32_t tokens_per_call) {
+        adapter = device;
         max_tok = tokens_per_call;
         dev.init(adapter);
+        ops.loader = [this](const std::string &file) { return dev.pipeline(read_file(file)); };
         load_kernels(kernel_dir);
         staging = dev.buffer(kStagingBytes, Kind::host);
         status = dev.buffer(256, Kind::host);
@@ -1710,5 +1788,74 @@ extern "C" int gm_read_outputs(gm_engine *g, float *y, uint32_t n_total) {
         Engine &e = g->e;
         if (n_total > e.n_tokens) throw gyro::NativeError(-1, "more outputs than tokens");
         e.download(e.outputs, y, (uint64_t)n_total * e.E * 4);
+    });
+}
+
+// ---- operators around the layers (row_ops.h) ----
+
+namespace {
+// The caller's current device, put back when a call is done (the runtime's calls select the engine's).
+struct KeepDevice {
+    int device = 0;
+    bool known;
+    KeepDevice() : known(hipGetDevice(&device) == hipSuccess) {}
+    ~KeepDevice() {
+        if (known) (void)hipSetDevice(device);
+    }
+};
+}  // namespace
+
+extern "C" int gm_load_operators(gm_engine *g) {
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.ops.load("");
+    });
+}
+
+extern "C" int gm_add_matrix(gm_engine *g, const gm_matrix_desc *d, uint32_t *out_index) {
+    if (!d || !out_index) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        *out_index = g->e.add_matrix(*d);
+    });
+}
+
+extern "C" int gm_release_matrix(gm_engine *g, uint32_t matrix) {
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.ops.matrix(matrix);
+        // The matrix's readers are on the callers' streams.
+        if (hipSetDevice((int)g->e.adapter) != hipSuccess || hipDeviceSynchronize() != hipSuccess)
+            throw gyro::NativeError(-1, "gm_release_matrix: the device's work did not finish");
+        g->e.dev.release(g->e.ops.matrices[matrix].data);
+    });
+}
+
+extern "C" int gm_linear(gm_engine *g, uint32_t matrix, const gm_rows *x, uint32_t n, const gm_rows *y, uint32_t act,
+                         uint32_t accumulate, float scale, void *stream) {
+    if (!x || !y) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(gyro::RowOps::linear(g->e.ops.matrix(matrix), g->e.cus, *x, n, *y, act, accumulate, scale), stream);
+    });
+}
+
+extern "C" int gm_block_norm(gm_engine *g, const gm_block_norm_desc *d, uint32_t n, void *stream) {
+    if (!d) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(gyro::RowOps::block_norm(*d, n), stream);
+    });
+}
+
+extern "C" uint64_t gm_logprobs_workspace(uint32_t n, uint32_t V, uint32_t top) {
+    return gyro::RowOps::logprobs_workspace(n, V, top);
+}
+
+extern "C" int gm_logprobs(gm_engine *g, const gm_logprobs_desc *d, uint32_t n, void *stream) {
+    if (!d) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(gyro::RowOps::logprobs(*d, n), stream);
     });
 }

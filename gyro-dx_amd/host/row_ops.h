@@ -1,0 +1,263 @@
+// The operators around the MoE layers (gm_linear, gm_block_norm, gm_logprobs): argument checks, the choice of a
+// build, its constants and grid. The engine launches what they return. Their kernels (csrc/kernels/mv_q4.h, block_norm.h, logprobs.hip) take every address
+// in the launch's constants, so a call needs no table entry and may be captured.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <functional>
+#include <map>
+#include <string>
+#include <vector>
+
+#include "device.h"
+#include "gyro_ops.h"
+
+namespace gyro {
+
+inline void require(bool ok, const char *what) {
+    if (!ok) throw NativeError((gd_result)0x80070057u, what);  // E_INVALIDARG
+}
+
+// The constants of a launch, set by position.
+struct Constants {
+    uint32_t w[60] = {};
+    void set(int i, uint32_t v) { w[i] = v; }
+    void set64(int i, uint64_t v) {
+        w[i] = (uint32_t)v;
+        w[i + 1] = (uint32_t)(v >> 32);
+    }
+    void set(int i, const void *p) { set64(i, (uint64_t)(uintptr_t)p); }
+    void set(int i, float v) { std::memcpy(&w[i], &v, 4); }
+};
+
+// A launch: the kernel, its constants and grid (x 0: nothing to do).
+struct Launch {
+    const char *kernel = nullptr;
+    Constants c;
+    uint32_t x = 0, y = 0;
+};
+
+struct Matrix {
+    Buffer data;  // quants, scales, minima (q4_repack)
+    uint32_t rows = 0, cols = 0, lg = 0, tiles = 0, chunks = 0;
+    bool gated = false, mins = false;
+    uint64_t scales = 0, minima = 0;  // byte offsets
+};
+
+class RowOps {
+  public:
+    std::map<std::string, std::string, std::less<>> files;  // kernels not loaded yet
+    std::map<std::string, gd_pipeline *, std::less<>> pipes;
+    std::vector<Matrix> matrices;
+
+    static bool owns(const std::string &kernel) {
+        return kernel.rfind("mv_q4", 0) == 0 || kernel == "q4_repack" || kernel.rfind("block_norm", 0) == 0 ||
+               kernel.rfind("logprobs", 0) == 0;
+    }
+    using Loader = std::function<gd_pipeline *(const std::string &file)>;
+    Loader loader;
+    void load(const std::string &prefix) {
+        for (auto it = files.begin(); it != files.end();) {
+            if (it->first.rfind(prefix, 0) != 0) {
+                ++it;
+                continue;
+            }
+            pipes[it->first] = loader(it->second);
+            it = files.erase(it);
+        }
+    }
+
+    // ---- linear ----
+
+    static uint64_t layout(Matrix &m) {
+        const uint64_t units = (uint64_t)m.tiles * m.chunks, per = 128u >> m.lg;
+        m.scales = units * 1024;
+        m.minima = m.scales + units * 16 * per * 2;
+        return m.mins ? m.minima + units * 16 * per * 2 : m.minima;
+    }
+    // Source bytes of a matrix's quants, and of its scales or minima (format GM_MATRIX_Q4).
+    static uint64_t quant_bytes(const gm_matrix_desc &d) {
+        const uint64_t n = (uint64_t)d.rows * d.cols;
+        return d.format == GM_MATRIX_Q4_0 ? n / 32 * 18 : d.format == GM_MATRIX_Q4_1 ? n / 32 * 20 : n / 2;
+    }
+    static uint64_t scale_bytes(const gm_matrix_desc &d) { return (uint64_t)d.rows * (d.cols / d.group) * 2; }
+
+    static Matrix describe(const gm_matrix_desc &d) {
+        require(d.format <= GM_MATRIX_Q4, "unknown matrix format");
+        require(d.group == 32 || (d.format == GM_MATRIX_Q4 && (d.group == 64 || d.group == 128)),
+                "a matrix's group is 32, or 64 or 128 in the format of separate scales");
+        require(d.rows && d.cols && d.cols % d.group == 0, "a matrix has rows, and columns in whole groups");
+        require(d.rows <= 1u << 26 && d.cols <= 1u << 20, "a matrix has at most 2^26 rows and 2^20 columns");
+        const bool arrays = d.format == GM_MATRIX_Q4;
+        require(d.quants && (!arrays || d.scales), "a matrix needs its quants and scales");
+        require(arrays || (!d.scales && !d.mins && !d.up_scales && !d.up_mins), "GGUF blocks hold their own scales");
+        require(d.up_quants ? (!arrays || d.up_scales) && !d.mins == !d.up_mins : !d.up_scales && !d.up_mins,
+                "a gated pair's matrices have one format");
+        Matrix m;
+        m.rows = d.rows;
+        m.cols = d.cols;
+        m.lg = d.group == 32 ? 5 : d.group == 64 ? 6 : 7;
+        m.gated = d.up_quants != nullptr;
+        m.mins = d.format == GM_MATRIX_Q4_1 || (arrays && d.mins);
+        m.tiles = (d.rows + 15) / 16 * (m.gated ? 2u : 1u);
+        m.chunks = (d.cols + 127) / 128;
+        const uint64_t limit = uint64_t(4) << 30;
+        require(layout(m) <= limit && quant_bytes(d) <= limit, "a matrix takes at most 4 GiB");
+        return m;
+    }
+
+    const Matrix &matrix(uint32_t i) const {
+        require(i < matrices.size() && matrices[i].data.handle, "no such matrix");
+        return matrices[i];
+    }
+    uint32_t keep(Matrix &&m) {
+        for (uint32_t i = 0; i < matrices.size(); ++i)
+            if (!matrices[i].data.handle) {
+                matrices[i] = std::move(m);
+                return i;
+            }
+        matrices.push_back(std::move(m));
+        return (uint32_t)matrices.size() - 1;
+    }
+
+    static void check_rows(const gm_rows &r, uint32_t n, uint32_t cols, bool output, const char *what) {
+        require(r.data != nullptr && r.type <= GM_F16, what);
+        const uint64_t size = r.type == GM_F32 ? 4 : 2;
+        require((uintptr_t)r.data % size == 0, what);
+        require(r.stride <= uint64_t(1) << 40, what);
+        require(!output || n <= 1 || r.stride >= cols, what);
+    }
+
+    static Launch linear(const Matrix &m, uint32_t cus, const gm_rows &x, uint32_t n, const gm_rows &y, uint32_t act,
+                         uint32_t accumulate, float scale) {
+        Launch l;
+        if (!n) return l;  // of no rows there may be no memory
+        check_rows(x, n, m.cols, false, "gm_linear: x");
+        check_rows(y, n, m.rows, true, "gm_linear: y");
+        require(act <= GM_ACT_SIGMOID && (!m.gated || act == GM_ACT_NONE), "gm_linear: act");
+        require(n <= 1u << 18, "gm_linear takes at most 2^18 tokens");
+        Constants &c = l.c;
+        c.set64(0, m.data.gpu);
+        c.set64(2, m.data.gpu + m.scales);
+        c.set64(4, m.mins ? m.data.gpu + m.minima : 0);
+        c.set(6, m.tiles);
+        c.set(7, m.chunks);
+        c.set(8, m.lg);
+        c.set(9, m.cols);
+        c.set(10, m.rows);
+        c.set(11, m.gated ? 1u : 0u);
+        c.set(12, x.data);
+        c.set64(14, x.stride);
+        c.set(16, x.type);
+        c.set(17, n);
+        c.set(18, y.data);
+        c.set64(20, y.stride);
+        c.set(22, y.type);
+        c.set(23, act);
+        c.set(24, accumulate ? 1u : 0u);
+        c.set(25, scale);
+        uint32_t wk = 1;
+        while (wk < 8 && wk * 2 <= m.chunks) wk *= 2;
+        c.set(26, wk);
+        const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u;
+        const bool few = m.tiles / (4 * (8 / wk)) < cus;
+        const uint32_t run = (few ? 2u : 4u) * (8 / wk), runs = (m.tiles + run - 1) / run;
+        l.kernel = few ? "mv_q4_s" : "mv_q4";
+        l.x = std::min(runs, 2 * cus);
+        l.y = (n + per - 1) / per;
+        return l;
+    }
+
+    // ---- block norm ----
+
+    static Launch block_norm(const gm_block_norm_desc &d, uint32_t n) {
+        Launch l;
+        if (!n) return l;  // of no rows there may be no memory
+        require(d.E && d.E <= 16384, "gm_block_norm takes rows of 1 to 16384 values");
+        require(d.out.data || d.normed.data, "gm_block_norm: no output");
+        check_rows(d.x, n, d.E, false, "gm_block_norm: x");
+        if (d.h.data) check_rows(d.h, n, d.E, false, "gm_block_norm: h");
+        if (d.out.data) check_rows(d.out, n, d.E, true, "gm_block_norm: out");
+        if (d.normed.data) check_rows(d.normed, n, d.E, true, "gm_block_norm: normed");
+        require(d.gate_kind <= GM_GATE_VALUE && (d.gate_act == GM_ACT_NONE || d.gate_act == GM_ACT_SIGMOID), "gm_block_norm: gate");
+        const bool gate = d.gate_kind != GM_GATE_NONE;
+        require(d.h.data || (!gate && !d.post), "gm_block_norm: a gate or a post norm without h");
+        if (gate) check_rows(d.gate, n, d.E, false, "gm_block_norm: gate");
+        require(d.post || !d.post_weight, "gm_block_norm: a post weight without the post norm");
+        require((uintptr_t)d.post_weight % 4 == 0 && (uintptr_t)d.pre_weight % 4 == 0, "gm_block_norm: weights");
+        require(d.post_eps >= 0 && d.pre_eps >= 0, "gm_block_norm: eps");
+        Constants &c = l.c;
+        c.set(0, d.h.data);
+        c.set64(2, d.h.stride);
+        c.set(4, d.x.data);
+        c.set64(6, d.x.stride);
+        c.set(8, d.out.data);
+        c.set64(10, d.out.stride);
+        c.set(12, d.normed.data);
+        c.set64(14, d.normed.stride);
+        c.set(16, d.post_weight);
+        c.set(18, d.pre_weight);
+        if (gate) c.set(20, d.gate.data);
+        c.set64(22, d.gate_kind == GM_GATE_CHANNEL ? 0 : d.gate.stride);
+        c.set(24, d.gate_kind >= GM_GATE_CHANNEL ? 1u : 0u);
+        c.set(25, d.h.type | d.x.type << 4 | d.out.type << 8 | d.normed.type << 12 | d.gate.type << 16);
+        c.set(26, (d.post ? 1u : 0u) | (d.gate_act == GM_ACT_SIGMOID ? 2u : 0u));
+        c.set(27, d.E);
+        c.set(28, d.post_eps);
+        c.set(29, d.pre_eps);
+        c.set(30, d.scale);
+        c.set(31, n);
+        l.kernel = d.E <= 4096 ? "block_norm" : "block_norm_l";
+        l.x = std::min(n, 65535u);
+        l.y = (uint32_t)(((uint64_t)n + 65534) / 65535);
+        return l;
+    }
+
+    // ---- log probabilities ----
+
+    static uint64_t logprobs_workspace(uint32_t, uint32_t, uint32_t) { return 0; }
+
+    static Launch logprobs(const gm_logprobs_desc &d, uint32_t n) {
+        Launch l;
+        if (!n) return l;  // of no rows there may be no memory
+        require(d.V && d.V < 1u << 31, "gm_logprobs: V");
+        check_rows(d.logits, n, d.V, false, "gm_logprobs: logits");
+        require(d.scale > 0 && std::isfinite(d.scale), "gm_logprobs: scale");
+        require(d.given <= 64 && d.top <= 64 && d.top <= d.V, "gm_logprobs: given, top");
+        require(!d.given || (d.tokens && d.logprobs && (uintptr_t)d.tokens % (d.tokens_64 ? 8 : 4) == 0 &&
+                             (uintptr_t)d.logprobs % 4 == 0 && (n <= 1 || d.logprobs_stride >= d.given)),
+                "gm_logprobs: tokens and logprobs");
+        require(!d.top || (d.top_ids && d.top_logprobs && (uintptr_t)d.top_ids % 4 == 0 &&
+                           (uintptr_t)d.top_logprobs % 4 == 0 && (n <= 1 || d.top_stride >= d.top)),
+                "gm_logprobs: top_ids and top_logprobs");
+        require((uintptr_t)d.entropy % 4 == 0 && (d.given || d.entropy || d.top), "gm_logprobs: no output");
+        const uint64_t need = logprobs_workspace(n, d.V, d.top);
+        require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0),
+                "gm_logprobs: workspace");
+        Constants &c = l.c;
+        c.set(0, d.logits.data);
+        c.set64(2, d.logits.stride);
+        c.set(4, d.logits.type);
+        c.set(5, d.V);
+        c.set(6, d.scale);
+        c.set(7, d.top);
+        c.set(8, d.tokens);
+        c.set64(10, d.tokens_stride);
+        c.set(12, d.given);
+        c.set(13, d.tokens_64 ? 1u : 0u);
+        c.set(14, d.logprobs);
+        c.set64(16, d.logprobs_stride);
+        c.set(18, d.entropy);
+        c.set(20, d.top_ids);
+        c.set(22, d.top_logprobs);
+        c.set64(24, d.top_stride);
+        c.set(26, n);
+        l.kernel = "logprobs";
+        l.x = std::min(n, 65535u);
+        l.y = (uint32_t)(((uint64_t)n + 65534) / 65535);
+        return l;
+    }
+};
+
+}  // namespace gyro

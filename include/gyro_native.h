@@ -168,8 +168,9 @@ GD_API gd_result gd_dispatch_timed(gd_context *context, gd_pipeline *pipeline, c
 
 /* Extension with no counterpart in the reference ABI, for callers that run outside a recording
  * (the MoE engine's no-allocation entry point): launches at once on `stream`, a hipStream_t of
- * the context's device (NULL: the context's compute stream), with the checks of gd_dispatch but
- * no gd_begin / gd_submit bracket and no ticket. */
+ * the context's device (NULL: the context's compute stream; GD_STREAM_DEFAULT: the device's null
+ * stream), with the checks of gd_dispatch but no gd_begin / gd_submit bracket and no ticket. */
+#define GD_STREAM_DEFAULT ((void *)1)
 GD_API gd_result gd_dispatch_on(gd_context *context, gd_pipeline *pipeline, const uint32_t *constants,
     uint32_t constant_count, uint32_t groups_x, uint32_t groups_y, uint32_t groups_z, void *stream);
 /* Extension with no counterpart in the reference ABI: gives memory the caller owns (device

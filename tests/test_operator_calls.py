@@ -1,0 +1,256 @@
+"""The operators' argument checks, builds and grids (host/row_ops.h) and their binding, on the CPU: every call that the
+headers refuse, none of which reaches a launch, and the layout sizes of matrices."""
+import ctypes as C
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from gyrodx import engine
+from gyrodx.engine import BlockNormDesc, Engine, LogprobsDesc, MatrixDesc, Rows
+from test_abi import declared, exported
+
+ROOT = Path(__file__).resolve().parents[1]
+BUILD = ROOT / "gyro-dx_amd" / "build"
+
+SHIM = r"""
+#include "row_ops.h"
+using namespace gyro;
+template <class F> static int run(char *why, F f) {
+    try { f(); return 0; } catch (const NativeError &e) { std::strncpy(why, e.what(), 199); return e.code; }
+}
+static void tell(const Launch &l, uint32_t *out, char *why) {
+    out[0] = l.x; out[1] = l.y;
+    std::memcpy(out + 2, l.c.w, sizeof(l.c.w));
+    std::strncpy(why, l.kernel ? l.kernel : "", 199);
+}
+extern "C" int plan_matrix(const gm_matrix_desc *d, uint64_t *out, char *why) {
+    return run(why, [&] { Matrix m = RowOps::describe(*d); out[0] = RowOps::layout(m); out[1] = m.tiles; out[2] = m.chunks;
+                          out[3] = m.scales; out[4] = m.minima; });
+}
+extern "C" int plan_linear(const gm_matrix_desc *d, const gm_rows *x, uint32_t n, const gm_rows *y, uint32_t act,
+                           uint32_t accumulate, float scale, uint32_t *out, char *why) {
+    return run(why, [&] { Matrix m = RowOps::describe(*d); RowOps::layout(m);
+                          tell(RowOps::linear(m, 256, *x, n, *y, act, accumulate, scale), out, why); });
+}
+extern "C" int plan_norm(const gm_block_norm_desc *d, uint32_t n, uint32_t *out, char *why) {
+    return run(why, [&] { tell(RowOps::block_norm(*d, n), out, why); });
+}
+extern "C" int plan_logprobs(const gm_logprobs_desc *d, uint32_t n, uint32_t *out, char *why) {
+    return run(why, [&] { tell(RowOps::logprobs(*d, n), out, why); });
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def shim(tmp_path_factory):
+    d = tmp_path_factory.mktemp("ops")
+    (d / "shim.cpp").write_text(SHIM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", str(ROOT / "include"), "-I",
+                    str(ROOT / "gyro-dx_amd" / "host"), "-o", str(d / "shim.so"), str(d / "shim.cpp")], check=True)
+    L = C.CDLL(str(d / "shim.so"))
+    L.plan_linear.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p,
+                              C.c_char_p]
+    return L
+
+
+A = 0x10000  # an address that no check may follow
+
+
+def rows(type=0, stride=1 << 20, data=A):
+    return Rows(data, stride, type)
+
+
+def matrix(fmt=0, rows=64, cols=256, group=32, **more):
+    d = MatrixDesc(fmt, rows, cols, group, quants=A)
+    if fmt == 2:
+        d.scales = A
+    for k, v in more.items():
+        setattr(d, k, v)
+    return d
+
+
+def call(f, *args):
+    why, out = C.create_string_buffer(200), (C.c_uint32 * 62)()
+    rc = f(*[C.byref(a) if isinstance(a, C.Structure) else a for a in args], out, why)
+    return rc, why.value.decode(), out[0], out[1]
+
+
+def test_header_is_exported():
+    names = declared("gyro_ops.h", "gm_")
+    assert len(names) == 7, names
+    assert not set(names) - exported(BUILD / "libgyro_moe.so")
+
+
+def test_struct_layouts():
+    """Offsets of the header's structs (64-bit pointers)."""
+    assert C.sizeof(Rows) == 24 and Rows.stride.offset == 8 and Rows.type.offset == 16
+    assert C.sizeof(MatrixDesc) == 64 and MatrixDesc.quants.offset == 16 and MatrixDesc.up_quants.offset == 40
+    assert C.sizeof(BlockNormDesc) == 168 and BlockNormDesc.h.offset == 16 and BlockNormDesc.post_weight.offset == 136
+    assert C.sizeof(LogprobsDesc) == 128 and LogprobsDesc.tokens.offset == 48 and LogprobsDesc.workspace.offset == 112
+
+
+@pytest.mark.parametrize("d,tiles,chunks,per,mins", [
+    (matrix(), 4, 2, 4, 0), (matrix(rows=17, cols=32), 2, 1, 4, 0), (matrix(1, rows=16, cols=160), 1, 2, 4, 1),
+    (matrix(2, group=64, cols=192), 4, 2, 2, 0), (matrix(2, group=128, mins=A), 4, 2, 1, 1),
+    (matrix(rows=17, up_quants=A), 4, 2, 4, 0)])
+def test_matrix_layout(shim, d, tiles, chunks, per, mins):
+    out, why = (C.c_uint64 * 5)(), C.create_string_buffer(200)
+    assert shim.plan_matrix(C.byref(d), out, why) == 0, why.value
+    units = tiles * chunks
+    assert list(out) == [units * (1024 + 32 * per * (1 + mins)), tiles, chunks, units * 1024, units * (1024 + 32 * per)]
+
+
+@pytest.mark.parametrize("d", [
+    matrix(3), matrix(group=64), matrix(1, group=128), matrix(2, group=16), matrix(2, group=256, cols=512),
+    matrix(rows=0), matrix(cols=0), matrix(cols=48), matrix(2, group=128, cols=192), matrix(quants=None),
+    matrix(2, scales=None), matrix(scales=A), matrix(mins=A), matrix(up_scales=A), matrix(2, up_scales=A),
+    matrix(2, up_quants=A), matrix(2, up_quants=A, up_scales=A, mins=A), matrix(2, up_quants=A, up_scales=A, up_mins=A),
+    matrix(rows=1 << 26, cols=256), matrix(rows=1 << 27, cols=32), matrix(rows=1, cols=1 << 21)])
+def test_matrix_refusals(shim, d):
+    out, why = (C.c_uint64 * 5)(), C.create_string_buffer(200)
+    assert shim.plan_matrix(C.byref(d), out, why) < 0 and why.value
+
+
+def test_linear_refusals(shim):
+    m, g = matrix(), matrix(up_quants=A)
+    ok = lambda d=m, x=rows(), n=4, y=rows(), act=0, acc=0, scale=1.0: call(shim.plan_linear, d, x, n, y, act, acc, scale)  # noqa: E731
+    assert ok()[0] == 0 and ok()[2] >= 1
+    assert ok(n=0)[0] == 0 and ok(n=0)[2] == 0
+    assert ok(x=rows(stride=0))[0] == 0 and ok(y=rows(stride=0), n=1)[0] == 0
+    for bad in (dict(x=rows(data=None)), dict(y=rows(data=None)), dict(x=rows(type=3)), dict(y=rows(type=7)),
+                dict(x=rows(data=A + 2)), dict(y=rows(type=1, data=A + 1)), dict(y=rows(stride=63)), dict(act=3),
+                dict(d=g, act=1), dict(n=(1 << 18) + 1), dict(x=rows(stride=1 << 41))):
+        rc, why, *_ = ok(**bad)
+        assert rc < 0 and why, bad
+
+
+def test_linear_grids(shim):
+    """Any token count and matrix fits the grid's 65535 groups a dimension."""
+    for fmt, r, c in ((0, 1, 32), (0, 131072, 2048), (2, 100003, 2560), (0, 1 << 22, 1024)):
+        for type in (0, 1, 2):
+            for n in (1, 5, 6, 64, 1023, 1 << 18):
+                rc, why, x, y = call(shim.plan_linear, matrix(fmt, r, c), rows(type), n, rows(stride=r), 0, 0, 1.0)
+                assert rc == 0 and 1 <= x <= 65535 and 1 <= y <= 65535, (r, c, type, n, why, x, y)
+
+
+def norm(**kw):
+    d = BlockNormDesc(E=100, post=0, h=rows(), x=rows(), out=rows(), normed=rows(), post_eps=1e-6, pre_eps=1e-6, scale=1.0)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_block_norm_refusals(shim):
+    none = Rows()
+    for good in (norm(), norm(h=none), norm(out=none), norm(normed=none), norm(post=1, post_weight=A), norm(E=16384),
+                 norm(gate_kind=3, gate=rows(1))):
+        assert call(shim.plan_norm, good, 3)[0] == 0
+    assert call(shim.plan_norm, norm(), 0)[2] == 0
+    assert call(shim.plan_norm, norm(), 70000)[2:] == (65535, 2)
+    for bad in (norm(E=0), norm(E=16385), norm(out=none, normed=none), norm(x=none), norm(x=rows(9)), norm(h=rows(data=A + 1)),
+                norm(out=rows(stride=99)), norm(normed=rows(stride=0)), norm(gate_kind=4, gate=rows()),
+                norm(gate_kind=1), norm(gate_kind=1, gate=rows(), gate_act=1), norm(h=none, gate_kind=1, gate=rows()),
+                norm(h=none, post=1), norm(post_weight=A), norm(post=1, post_weight=A + 2), norm(pre_weight=A + 1),
+                norm(post_eps=-1.0), norm(pre_eps=float("nan"))):
+        rc, why, *_ = call(shim.plan_norm, bad, 3)
+        assert rc < 0 and why
+
+
+def lp(n=3, **kw):
+    d = LogprobsDesc(logits=rows(), V=1000, given=1, top=5, tokens_64=1, scale=1.0, tokens=A, tokens_stride=1, logprobs=A,
+                     logprobs_stride=1, entropy=A, top_ids=A, top_logprobs=A, top_stride=5, workspace=A, workspace_bytes=1 << 40)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_logprobs_refusals(shim):
+    for good in (lp(), lp(given=0, tokens=None, logprobs=None), lp(top=0, top_ids=None, top_logprobs=None), lp(entropy=None),
+                 lp(V=5), lp(V=70000, top=64, given=64, top_stride=64, logprobs_stride=64, tokens_stride=64)):
+        rc, why, *_ = call(shim.plan_logprobs, good, 3)
+        assert rc == 0, why
+    assert call(shim.plan_logprobs, lp(), 0)[2] == 0
+    assert call(shim.plan_logprobs, lp(), 200000)[2:] == (65535, 4)
+    for bad in (lp(V=0), lp(V=1 << 31), lp(logits=Rows()), lp(logits=rows(5)), lp(logits=rows(data=A + 1)), lp(scale=0.0),
+                lp(scale=-1.0), lp(scale=float("nan")), lp(scale=float("inf")), lp(given=65), lp(top=65), lp(V=4),
+                lp(tokens=None), lp(logprobs=None), lp(tokens=A + 4), lp(tokens_64=0, tokens=A + 2), lp(logprobs=A + 2),
+                lp(logprobs_stride=0), lp(top_ids=None), lp(top_logprobs=None), lp(top_ids=A + 1), lp(top_stride=4),
+                lp(entropy=A + 2), lp(given=0, top=0, entropy=None)):
+        rc, why, *_ = call(shim.plan_logprobs, bad, 3)
+        assert rc < 0 and why
+
+
+# ---- the binding's own checks ----
+
+@pytest.fixture
+def eng():
+    """An engine without a device: tensors on the CPU pass its device check, and a call that passes every check ends
+    at the missing handle."""
+    e = Engine.__new__(Engine)
+    e._h, e.adapter, e._matrices = C.c_void_p(), -1, {0: (64, 96)}
+    return e
+
+
+def reached(f, *args, **kw):
+    with pytest.raises(RuntimeError, match="no engine"):
+        f(*args, **kw)
+
+
+def refused(f, *args, **kw):
+    with pytest.raises((ValueError, KeyError)):
+        f(*args, **kw)
+
+
+def test_binding_linear(eng):
+    x, y = torch.zeros(3, 96), torch.zeros(3, 64)
+    reached(eng.linear, 0, x, y)
+    reached(eng.linear, 0, torch.zeros(3, 100)[:, 4:], y.half())
+    for bad in ((1, x, y), (0, x[:, :95], y), (0, x, y[:2]), (0, x.double(), y), (0, x, y.int()), (0, x, torch.zeros(64, 3).T),
+                (0, x[0], y)):
+        refused(eng.linear, *bad)
+    refused(eng.linear, 0, x, y, act="gelu")
+    eng.adapter = 0
+    refused(eng.linear, 0, x, y)
+
+
+def test_binding_matrix(eng):
+    q, s = np.zeros((4, 32), np.uint8), np.zeros((4, 2), np.float16)
+    reached(eng.add_matrix, "q4", 4, 64, (q, s, None))
+    reached(eng.add_matrix, "q4", 4, 64, (q, s, s), up=(q, s, s))
+    reached(eng.add_matrix, "q4_0", 4, 64, np.zeros((4, 36), np.uint8))
+    for bad in (("q5", 4, 64, q), ("q4", 4, 64, (q, s)), ("q4", 4, 64, (q.astype(np.int8), s, None)), ("q4", 4, 64, (q[:3], s, None)),
+                ("q4", 4, 64, (q, s.astype(np.float32), None)), ("q4", 4, 64, (q, s, s[:1])), ("q4_0", 4, 64, q),
+                ("q4_1", 4, 64, np.zeros((4, 36), np.uint8)), ("q4", 0, 64, (q, s, None)), ("q4", 4, 48, (q, s, None))):
+        refused(eng.add_matrix, *bad)
+
+
+def test_binding_block_norm(eng):
+    x, w = torch.zeros(3, 8), torch.zeros(8)
+    reached(eng.block_norm, x, x, x, x, post=True, post_weight=w, gate=torch.zeros(3, 1), pre_weight=w)
+    reached(eng.block_norm, None, x, None, x.half(), gate=None)
+    for kw in (dict(gate=torch.zeros(2, 8)), dict(gate=torch.zeros(8)), dict(gate=torch.zeros(3, 1), gate_act="tanh"),
+               dict(pre_weight=w[:7]), dict(pre_weight=w.half()), dict(post_weight=torch.zeros(16)[::2]), dict(normed=x[:2])):
+        refused(eng.block_norm, x, x, x, **kw)
+    refused(eng.block_norm, x[:2], x, x)
+
+
+def test_binding_logprobs(eng):
+    x, t, o = torch.zeros(3, 50), torch.zeros(3, 1, dtype=torch.int64), torch.zeros(3, 1)
+    ids, top = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 4)
+    reached(eng.logprobs, x, tokens=t, logprob=o, entropy=torch.zeros(3), top_ids=ids, top_logprobs=top)
+    for kw in (dict(tokens=t), dict(logprob=o), dict(tokens=t.double(), logprob=o), dict(tokens=t, logprob=o.half()),
+               dict(tokens=t[:2], logprob=o), dict(entropy=torch.zeros(2)), dict(top_ids=ids), dict(top_logprobs=top),
+               dict(top_ids=ids.long(), top_logprobs=top), dict(top_ids=ids, top_logprobs=top[:, :3]),
+               dict(entropy=torch.zeros(3), workspace=torch.zeros(4))):
+        refused(eng.logprobs, x, **kw)
+
+
+def test_workspace_sizes():
+    f = engine.lib().gm_logprobs_workspace
+    assert f(0, 1000, 5) == 0
+    for n in (1, 5, 64, 1023, 70000):
+        for V in (1, 50, 4096, 131072):
+            assert f(n, V, 0) <= f(n, V, min(V, 64)) < 1 << 40
