@@ -1,88 +1,89 @@
-// Rows of logits to the log probabilities of given tokens, the entropy and the top alternatives: with m = max x,
-// d = scale (x - m) (the difference first: the scale may not take the type's lowest value out of range),
-// S = sum exp(d), T = sum d exp(d):
-//   logprob[j] = d[token j] - log S,   entropy = log S - T / S,   the `top` largest x, equal ones by id.
-// One group per row. S and T are running sums: a larger maximum rescales them.
-// Constants: 0 x 2 x stride 4 type 5 V 6 scale (fp32 bits) 7 top 8 tokens 10 tokens' stride 12 given 13 token type
-// (0 int32, 1 int64) 14 logprob 16 logprob stride 18 entropy (0: none) 20 ids 22 top logprobs 24 top stride 26 n.
-#include "rows.h"
-
-struct LpState {
-    float m, s, t;
-};
-__device__ __forceinline__ LpState lp_join(const LpState &p, const LpState &q, float scale) {
-    LpState o;
-    o.m = fmaxf(p.m, q.m);
-    // At least -1e30, so that a term of exp 0 stays 0 and no NaN.
-    auto diff = [&](const LpState &r) {
-        const float d = scale * (r.m - o.m);
-        return r.s == 0.f ? 0.f : d < -1e30f ? -1e30f : d;
-    };
-    const float dp = diff(p), dq = diff(q);
-    const float ep = __expf(dp), eq = __expf(dq);
-    o.s = p.s * ep + q.s * eq;
-    o.t = ep * (p.t + p.s * dp) + eq * (q.t + q.s * dq);
-    return o;
-}
-// Value i's place in the order: falling values, NaNs first, equal ones by index. Never 0, and below the start ~0.
-__device__ __forceinline__ uint64_t lp_key(float x, uint32_t i) {
-    uint32_t u = gd_f32_bits(x + 0.0f);
-    u = x != x ? 0xfffffffeu : u & 0x80000000u ? ~u : u | 0x80000000u;
-    return (uint64_t)u << 32 | (uint32_t)~i;
-}
+// Log probabilities, entropy and top alternatives of rows of logits (logprobs.h): a group of four waves per row, or per
+// part of one, wave w taking batches w, w + 4, ... of it. Grid: (row blocks of 65535, parts) as y = row block * parts + part.
+#include "logprobs.h"
 
 GD_PIPELINE_NAMED(logprobs, 256) {
-    __shared__ LpState st[4];
-    __shared__ uint64_t best[4];
-    const uint32_t V = a.c[5], type = a.c[4], top = a.c[7], lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    __shared__ uint64_t lists[LP_WAVES * LP_LIST];
+    __shared__ uint64_t merged[LP_WAVES * LP_TOP];
+    __shared__ LpSums sums[LP_WAVES];
+    const uint32_t V = a.c[5], type = a.c[4], top = a.c[7], parts = a.c[27];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t part = blockIdx.y % parts;
+    const uint64_t row = (uint64_t)(blockIdx.y / parts) * gridDim.x + blockIdx.x;
     if (row >= a.c[26]) return;
     const float scale = gd_bits_f32(a.c[6]);
     const uint64_t X = gd_addr(a, 0) + ((row * gd_addr(a, 2)) << row_shift(type));
-    LpState p = {-INFINITY, 0.f, 0.f};
-    for (uint32_t i = threadIdx.x; i < V; i += 256u) {
-        const float x = row_load(X, i, type);
-        if (x == -INFINITY) continue;
-        p = lp_join(p, LpState{x, 1.f, 0.f}, scale);
+    LpGiven given = {0.f, 1};
+    if (parts == 1u) given = lp_given(a, row, X);
+
+    // Values are counted from the 16-byte boundary at or before the row: the row is [from, to).
+    const uint32_t from = (uint32_t)(X & 15u) >> row_shift(type), to = from + V;
+    const uint64_t base = X & ~15ull;
+    const uint32_t batches = (to + LP_BATCH - 1u) / LP_BATCH;
+    const uint32_t b0 = (uint32_t)((uint64_t)batches * part / parts), b1 = (uint32_t)((uint64_t)batches * (part + 1u) / parts);
+    LpTop l = {lists + wave * LP_LIST, 0u, top, -INFINITY};
+    LpSums p = {-INFINITY, 0.f, 0.f};
+    for (uint32_t b = b0 + wave; b < b1; b += LP_WAVES) {
+        const uint32_t first = b * LP_BATCH;
+        float x[32];
+        const bool whole = first >= from && first + LP_BATCH <= to;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t i = first + 512u * j + 8u * lane;
+            float v[8];
+            if (whole) {
+                row_load8(base, i, i + 8u, type, true, v);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    v[e] = i + e >= from && i + e < to ? row_load(base, i + e, type) : -INFINITY;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) x[8 * j + e] = v[e];
+        }
+        float most = x[0];
+#pragma unroll
+        for (uint32_t i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
+        // The lane's sums so far move to the new maximum; a maximum of -infinity counts as 0 (no term yet).
+        const float m = fmaxf(p.m, most), ref = m == -INFINITY ? 0.f : m;
+        const float back = lp_diff(p.m, ref, scale), shrink = __expf(back);
+        p.t = shrink * (p.t + p.s * back);
+        p.s *= shrink;
+        p.m = m;
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            const float d = scale * (x[i] - ref), e = __expf(d);
+            s += e;
+            t += e * fmaxf(d, -1e30f);
+        }
+        p.s += s;
+        p.t += t;
+        if (top) lp_add(l, x, first - from, most, p.s != p.s);
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const LpState q = {__shfl_xor(p.m, o, 64), __shfl_xor(p.s, o, 64), __shfl_xor(p.t, o, 64)};
-        p = lp_join(p, q, scale);
+    p = lp_wave_join(p, scale);
+    if (lane == 0) sums[wave] = p;
+    if (top) {
+        uint32_t bound;
+        l.c = lp_cut(l.list, l.c, top, bound);
+        lp_wave_sync();
+        if (lane < top) merged[wave * top + lane] = lane < l.c ? l.list[lane] : lp_nothing(wave * LP_TOP + lane);
     }
-    if (lane == 0) st[wave] = p;
     __syncthreads();
-    p = lp_join(lp_join(st[0], st[1], scale), lp_join(st[2], st[3], scale), scale);
-    const bool none = p.s == 0.f;
-    const float logs = none ? 0.f : logf(p.s);
-    auto logprob = [&](float x) { return none ? -INFINITY : scale * (x - p.m) - logs; };
-    if (threadIdx.x == 0 && gd_addr(a, 18)) gd_at<float>(gd_addr(a, 18))[row] = none ? 0.f : logs - p.t / p.s;
-    if (threadIdx.x < a.c[12]) {
-        const uint64_t at = row * gd_addr(a, 10) + threadIdx.x;
-        const int64_t token = a.c[13] ? gd_at<const int64_t>(gd_addr(a, 8))[at] : gd_at<const int32_t>(gd_addr(a, 8))[at];
-        float v = token < 0 ? 0.f : __builtin_nanf("");
-        if (token >= 0 && token < (int64_t)V) v = logprob(row_load(X, (uint64_t)token, type));
-        gd_at<float>(gd_addr(a, 14))[row * gd_addr(a, 16) + threadIdx.x] = v;
+    if (wave) return;
+    p = lp_join(lp_join(sums[0], sums[1], scale), lp_join(sums[2], sums[3], scale), scale);
+    if (parts == 1u) {
+        lp_finish(a, row, X, p, given, merged, LP_WAVES * top);
+        return;
     }
-    uint64_t last = ~0ull;
-    for (uint32_t k = 0; k < top; ++k) {
-        uint64_t b = 0;
-        for (uint32_t i = threadIdx.x; i < V; i += 256u) {
-            const uint64_t key = lp_key(row_load(X, i, type), i);
-            if (key < last && key > b) b = key;
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t q = (uint64_t)__shfl_xor((long long)b, o, 64);
-            b = q > b ? q : b;
-        }
-        __syncthreads();
-        if (lane == 0) best[wave] = b;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) b = best[w] > b ? best[w] : b;
-        last = b;
-        if (threadIdx.x == 0) {
-            const uint32_t id = min(~(uint32_t)b, V - 1u);
-            gd_at<uint32_t>(gd_addr(a, 20))[row * gd_addr(a, 24) + k] = id;
-            gd_at<float>(gd_addr(a, 22))[row * gd_addr(a, 24) + k] = logprob(row_load(X, id, type));
+    const uint64_t out = lp_part(a, row, part);
+    if (lane == 0) gd_at<gd_f32x4>(out)[0] = gd_f32x4{p.m, p.s, p.t, 0.f};
+    if (top) {
+        uint32_t bound;
+        lp_cut(merged, LP_WAVES * top, top, bound);
+        if (lane < top) {
+            const uint64_t p = merged[lane];
+            gd_at<uint64_t>(out + 16u)[lane] = p >> 32 ? p : lp_nothing(part * LP_TOP + lane);
         }
     }
 }

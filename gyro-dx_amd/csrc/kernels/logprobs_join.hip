@@ -1,0 +1,32 @@
+// Joins the parts of rows that several groups of logprobs shared (logprobs.h): a group per row, a wave per quarter of
+// the parts' places (at most 32 parts of at most 64).
+#include "logprobs.h"
+
+GD_PIPELINE_NAMED(logprobs_join, 256) {
+    __shared__ uint64_t lists[LP_WAVES * LP_LIST];
+    __shared__ uint64_t merged[LP_WAVES * LP_TOP];
+    const uint32_t top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= a.c[26]) return;
+    const float scale = gd_bits_f32(a.c[6]);
+    const uint64_t X = gd_addr(a, 0) + ((row * gd_addr(a, 2)) << row_shift(a.c[4]));
+    const LpGiven given = lp_given(a, row, X);
+    LpSums p = {-INFINITY, 0.f, 0.f};
+    if (wave == 0 && lane < parts) {
+        const gd_f32x4 v = gd_at<const gd_f32x4>(lp_part(a, row, lane))[0];
+        p = LpSums{v[0], v[1], v[2]};
+    }
+    if (top) {
+        // Wave w: parts w, w + 4, ..., up to 8 of them.
+        uint64_t *list = lists + wave * LP_LIST;
+        uint32_t c = 0, bound;
+        for (uint32_t part = wave; part < parts; part += LP_WAVES, c += top)
+            if (lane < top) list[c + lane] = gd_at<const uint64_t>(lp_part(a, row, part) + 16u)[lane];
+        lp_wave_sync();
+        c = lp_cut(list, c, top, bound);
+        if (lane < top) merged[wave * top + lane] = lane < c ? list[lane] : lp_nothing((parts + wave) * LP_TOP + lane);
+        __syncthreads();
+    }
+    if (wave) return;
+    lp_finish(a, row, X, lp_wave_join(p, scale), given, merged, LP_WAVES * top);
+}

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -52,6 +53,13 @@ GATE_TOKEN, GATE_CHANNEL, GATE_VALUE = 1, 2, 3
 _TYPE_NAMES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2, "torch.int32": 3, "torch.int64": 4,
                "torch.uint8": 5}
 _type_codes = {}  # dtype object -> its code in _TYPE_NAMES
+_ROW_TYPES, _FLOAT, _INT32, _INTS, _UINT8 = (0, 1, 2), (0,), (3,), (3, 4), (5,)
+
+# The structs above as bytes, which ctypes passes several times faster than it fills a Structure.
+_PACK_ROWS = struct.Struct("@PQII").pack
+_PACK_NORM = struct.Struct("@4I" + 5 * "PQII" + "PP4f").pack
+_PACK_LOGPROBS = struct.Struct("@PQII4IfIPQPQPPPQPQ").pack
+_NO_ROWS = (0, 0, 0)
 
 
 def _type(t, allowed, what):
@@ -102,11 +110,11 @@ def lib() -> C.CDLL:
         L.gm_load_operators.argtypes = [vp]
         L.gm_add_matrix.argtypes = [vp, C.POINTER(MatrixDesc), C.POINTER(u32)]
         L.gm_release_matrix.argtypes = [vp, u32]
-        L.gm_linear.argtypes = [vp, u32, C.POINTER(Rows), u32, C.POINTER(Rows), u32, u32, C.c_float, vp]
-        L.gm_block_norm.argtypes = [vp, C.POINTER(BlockNormDesc), u32, vp]
+        L.gm_linear.argtypes = [vp, u32, vp, u32, vp, u32, u32, C.c_float, vp]
+        L.gm_block_norm.argtypes = [vp, vp, u32, vp]
         L.gm_logprobs_workspace.argtypes = [u32, u32, u32]
         L.gm_logprobs_workspace.restype = C.c_uint64
-        L.gm_logprobs.argtypes = [vp, C.POINTER(LogprobsDesc), u32, vp]
+        L.gm_logprobs.argtypes = [vp, vp, u32, vp]
         _lib = L
     return _lib
 
@@ -301,21 +309,19 @@ class Engine:
             self._check(lib().gm_release_matrix(self._h, matrix), "gm_release_matrix")
             self._matrices.pop(matrix, None)
 
-    def _rows(self, t, n, cols, what):
-        shape = t.shape
-        if len(shape) != 2 or shape[0] != n or shape[1] != cols:
-            raise ValueError(f"{what}: shape {tuple(shape)}, not {(n, cols)}")
+    def _rows(self, t, shape, what):
+        """(address, stride, type) of a tensor of rows."""
+        if t.shape != shape:
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, not {shape}")
         if t.get_device() != self.adapter:
             raise ValueError(f"{what}: not on the engine's GPU")
         stride, step = t.stride()
-        if step != 1 and cols > 1:
+        if step != 1 and shape[1] > 1:
             raise ValueError(f"{what}: the values of a row are not neighbours")
-        return Rows(t.data_ptr(), stride, _type(t, (0, 1, 2), what))
+        return t.data_ptr(), stride, _type(t, _ROW_TYPES, what)
 
     def _flat(self, t, size, types, what):
-        """Address of a contiguous tensor of `size` values (None: no tensor)."""
-        if t is None:
-            return None
+        """Address of a contiguous tensor of `size` values."""
         if t.numel() != size or not t.is_contiguous():
             raise ValueError(f"{what}: shape {tuple(t.shape)}, not {size} neighbouring values")
         if t.get_device() != self.adapter:
@@ -330,8 +336,8 @@ class Engine:
             raise ValueError(f"no matrix {matrix}")
         rows, cols = self._matrices[matrix]
         n = x.shape[0]
-        xr, yr = self._rows(x, n, cols, "x"), self._rows(y, n, rows, "y")
-        rc = lib().gm_linear(self._h, matrix, xr, n, yr, ACTS[act], accumulate, scale, stream)
+        rc = lib().gm_linear(self._h, matrix, _PACK_ROWS(*self._rows(x, (n, cols), "x"), 0), n,
+                             _PACK_ROWS(*self._rows(y, (n, rows), "y"), 0), ACTS[act], accumulate, scale, stream)
         if rc:
             self._check(rc, "gm_linear")
 
@@ -340,23 +346,21 @@ class Engine:
                    stream: int = 0):
         """out = v = x + scale * gate * a with a = RMSNorm(h) (post) or h, normed = RMSNorm(v). `gate` is [n, 1] (per
         token), [1, E] (per channel) or [n, E]; weights are fp32 [E]. h None: v = x."""
-        n, E = x.shape
-        d = BlockNormDesc(E, post)
-        d.x = self._rows(x, n, E, "x")
-        if h is not None:
-            d.h = self._rows(h, n, E, "h")
-        if out is not None:
-            d.out = self._rows(out, n, E, "out")
-        if normed is not None:
-            d.normed = self._rows(normed, n, E, "normed")
+        shape = tuple(x.shape)
+        n, E = shape
+        kind, g = 0, _NO_ROWS
         if gate is not None:
-            shape = tuple(gate.shape)
-            d.gate_kind = GATE_VALUE if shape == (n, E) else GATE_CHANNEL if shape == (1, E) else GATE_TOKEN
-            d.gate = self._rows(gate, *{GATE_VALUE: (n, E), GATE_CHANNEL: (1, E), GATE_TOKEN: (n, 1)}[d.gate_kind], "gate")
-            d.gate_act = ACTS[gate_act]
-        d.post_weight = self._flat(post_weight, E, (0,), "post_weight")
-        d.pre_weight = self._flat(pre_weight, E, (0,), "pre_weight")
-        d.post_eps, d.pre_eps, d.scale = post_eps, pre_eps, scale
+            gs = tuple(gate.shape)
+            kind, gs = (GATE_VALUE, shape) if gs == shape else (GATE_CHANNEL, (1, E)) if gs == (1, E) else (GATE_TOKEN, (n, 1))
+            g = self._rows(gate, gs, "gate")
+        xr = self._rows(x, shape, "x")
+        hr = self._rows(h, shape, "h") if h is not None else _NO_ROWS
+        out_r = self._rows(out, shape, "out") if out is not None else _NO_ROWS
+        nr = self._rows(normed, shape, "normed") if normed is not None else _NO_ROWS
+        d = _PACK_NORM(E, post, kind, ACTS[gate_act], *hr, 0, *xr, 0, *out_r, 0, *nr, 0, *g, 0,
+                       self._flat(post_weight, E, _FLOAT, "post_weight") if post_weight is not None else 0,
+                       self._flat(pre_weight, E, _FLOAT, "pre_weight") if pre_weight is not None else 0,
+                       post_eps, pre_eps, scale, 0)
         rc = lib().gm_block_norm(self._h, d, n, stream)
         if rc:
             self._check(rc, "gm_block_norm")
@@ -372,28 +376,28 @@ class Engine:
         [n, given]), the entropy (fp32 [n]), and the largest logits' ids (int32 [n, top]) and log probabilities.
         workspace: a uint8 tensor of at least logprobs_workspace() bytes, not shared with calls that may overlap."""
         n, V = logits.shape
-        d = LogprobsDesc(self._rows(logits, n, V, "logits"), V)
-        d.scale = scale
+        x = self._rows(logits, (n, V), "logits")
+        given = top = wide = ws_bytes = tp = lp = ip = kp = ws = 0
         if tokens is not None:
-            d.given = tokens.shape[-1]
-            d.tokens = self._flat(tokens, n * d.given, (3, 4), "tokens")
-            d.tokens_64 = _type(tokens, (3, 4), "tokens") == 4
             if logprob is None:
                 raise ValueError("tokens without logprob")
-            d.logprobs = self._flat(logprob, n * d.given, (0,), "logprob")
-            d.tokens_stride = d.logprobs_stride = d.given
+            given = tokens.shape[-1]
+            tp = self._flat(tokens, n * given, _INTS, "tokens")
+            wide = _type_codes[tokens.dtype] == 4
+            lp = self._flat(logprob, n * given, _FLOAT, "logprob")
         elif logprob is not None:
             raise ValueError("logprob without tokens")
-        d.entropy = self._flat(entropy, n, (0,), "entropy")
         if (top_ids is None) != (top_logprobs is None):
             raise ValueError("top_ids and top_logprobs go together")
         if top_ids is not None:
-            d.top = d.top_stride = top_ids.shape[-1]
-            d.top_ids = self._flat(top_ids, n * d.top, (3,), "top_ids")
-            d.top_logprobs = self._flat(top_logprobs, n * d.top, (0,), "top_logprobs")
+            top = top_ids.shape[-1]
+            ip = self._flat(top_ids, n * top, _INT32, "top_ids")
+            kp = self._flat(top_logprobs, n * top, _FLOAT, "top_logprobs")
         if workspace is not None:
-            d.workspace_bytes = workspace.numel()
-            d.workspace = self._flat(workspace, d.workspace_bytes, (5,), "workspace")
+            ws_bytes = workspace.numel()
+            ws = self._flat(workspace, ws_bytes, _UINT8, "workspace")
+        d = _PACK_LOGPROBS(*x, 0, V, given, top, wide, scale, 0, tp, given, lp, given,
+                           self._flat(entropy, n, _FLOAT, "entropy") if entropy is not None else 0, ip, kp, top, ws, ws_bytes)
         rc = lib().gm_logprobs(self._h, d, n, stream)
         if rc:
             self._check(rc, "gm_logprobs")

@@ -480,20 +480,24 @@ class Engine {
         out.b = Buffer{};
         return ops.keep(std::move(m));
     }
+    // The operator's kernel, loaded if this is its first call: which may allocate, and a capture does not take.
+    gd_pipeline *op_kernel(const char *name, void *stream) {
+        auto it = ops.pipes.find(name);
+        if (it != ops.pipes.end()) return it->second;
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (stream && hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess) status = hipStreamCaptureStatusActive;
+        require(status == hipStreamCaptureStatusNone,
+                "the operator's kernel is not loaded: call gm_load_operators or the operator once before a capture");
+        require(ops.files.count(name) != 0, "operator kernel missing from the kernel directory");
+        ops.load(name);
+        return ops.pipes.at(name);
+    }
     void launch(const Launch &l, void *stream) {
         if (!l.x) return;
-        auto it = ops.pipes.find(l.kernel);
-        if (it == ops.pipes.end()) {
-            // Loading may allocate, which a capture does not take.
-            hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-            if (stream && hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess) status = hipStreamCaptureStatusActive;
-            require(status == hipStreamCaptureStatusNone,
-                    "the operator's kernel is not loaded: call gm_load_operators or the operator once before a capture");
-            require(ops.files.count(l.kernel) != 0, "operator kernel missing from the kernel directory");
-            ops.load(l.kernel);
-            it = ops.pipes.find(l.kernel);
-        }
-        check(gd_dispatch_on(dev.ctx, it->second, l.c.w, 60, l.x, l.y, 1, stream ? stream : GD_STREAM_DEFAULT), "gd_dispatch_on");
+        void *const on = stream ? stream : GD_STREAM_DEFAULT;
+        gd_pipeline *const first = op_kernel(l.kernel, stream), *const next = l.next ? op_kernel(l.next, stream) : nullptr;
+        check(gd_dispatch_on(dev.ctx, first, l.c.w, 60, l.x, l.y, 1, on), "gd_dispatch_on");
+        if (next) check(gd_dispatch_on(dev.ctx, next, l.c.w, 60, l.next_x, l.next_y, 1, on), "gd_dispatch_on");
     }
     // upload() of any number of bytes: the last word is filled up with zeros (the buffer has room).
     void upload_bytes(const Buffer &dst, uint64_t off, const void *src, uint64_t bytes) {

@@ -31,11 +31,11 @@ struct Constants {
     void set(int i, float v) { std::memcpy(&w[i], &v, 4); }
 };
 
-// A launch: the kernel, its constants and grid (x 0: nothing to do).
+// A launch: the kernel, its constants and grid (x 0: nothing to do), and one of the same constants after it.
 struct Launch {
-    const char *kernel = nullptr;
+    const char *kernel = nullptr, *next = nullptr;
     Constants c;
-    uint32_t x = 0, y = 0;
+    uint32_t x = 0, y = 0, next_x = 0, next_y = 0;
 };
 
 struct Matrix {
@@ -216,7 +216,16 @@ class RowOps {
 
     // ---- log probabilities ----
 
-    static uint64_t logprobs_workspace(uint32_t, uint32_t, uint32_t) { return 0; }
+    // Groups that share a row: enough that the rows' groups fill the device, each of their four waves with a batch
+    // of 2048 logits at least.
+    static uint32_t logprobs_parts(uint32_t n, uint32_t V) {
+        const uint32_t batches = (V + 7 + 2047) / 2048;
+        return std::max(1u, std::min({32u, (batches + 3) / 4, 768 / std::max(1u, n)}));
+    }
+    static uint64_t logprobs_workspace(uint32_t n, uint32_t V, uint32_t top) {
+        const uint32_t parts = logprobs_parts(n, V);
+        return parts == 1 ? 0 : (uint64_t)n * parts * (16 + 8ull * ((top + 1) & ~1u));
+    }
 
     static Launch logprobs(const gm_logprobs_desc &d, uint32_t n) {
         Launch l;
@@ -253,9 +262,17 @@ class RowOps {
         c.set(22, d.top_logprobs);
         c.set64(24, d.top_stride);
         c.set(26, n);
+        const uint32_t parts = logprobs_parts(n, d.V);
+        c.set(27, parts);
+        c.set(28, d.workspace);
         l.kernel = "logprobs";
         l.x = std::min(n, 65535u);
-        l.y = (uint32_t)(((uint64_t)n + 65534) / 65535);
+        l.y = (uint32_t)(((uint64_t)n + 65534) / 65535) * parts;
+        if (parts > 1) {
+            l.next = "logprobs_join";
+            l.next_x = l.x;
+            l.next_y = l.y / parts;
+        }
         return l;
     }
 };
