@@ -33,15 +33,13 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
     const float scale = gd_bits_f32(a.c[30]);
     const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.c[31]) return;
-    const bool hw = row_aligned(H, hs, ht), xw = row_aligned(X, xs, xt), ow = row_aligned(O, os, ot), nw = row_aligned(N, ns, nt),
-               gw = row_aligned(G, gs, gt), pw = row_aligned(PW, 0, ROW_F32), ww = row_aligned(NW, 0, ROW_F32);
     float v[STEPS][8], x[STEPS][8];
     float ss = 0.f;
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
         const uint32_t i = (k * 256u + threadIdx.x) * 8u;
-        row_load8(X + ((row * xs) << row_shift(xt)), i, E, xt, xw, x[k]);
-        if (H) row_load8(H + ((row * hs) << row_shift(ht)), i, E, ht, hw, v[k]);
+        row_load8(X + ((row * xs) << row_shift(xt)), i, E, xt, x[k]);
+        if (H) row_load8(H + ((row * hs) << row_shift(ht)), i, E, ht, v[k]);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
@@ -65,9 +63,9 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
             float w[8], g[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = g[j] = 1.f;
-            if (PW) row_load8(PW, i, E, ROW_F32, pw, w);
+            if (PW) row_load8(PW, i, E, ROW_F32, w);
             if (G && channel) {
-                row_load8(G + ((row * gs) << row_shift(gt)), i, E, gt, gw, g);
+                row_load8(G + ((row * gs) << row_shift(gt)), i, E, gt, g);
                 if (sigmoid)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) g[j] = gd_sigmoid_accurate(g[j]);
@@ -79,7 +77,7 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
     if (O)
 #pragma unroll
         for (int k = 0; k < STEPS; ++k)
-            row_store8(O + ((row * os) << row_shift(ot)), (k * 256u + threadIdx.x) * 8u, E, ot, ow, x[k]);
+            row_store8(O + ((row * os) << row_shift(ot)), (k * 256u + threadIdx.x) * 8u, E, ot, x[k]);
     if (!N) return;
     ss = 0.f;
 #pragma unroll
@@ -93,9 +91,9 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
         float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = 1.f;
-        if (NW) row_load8(NW, i, E, ROW_F32, ww, w);
+        if (NW) row_load8(NW, i, E, ROW_F32, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] *= x[k][j] * r;
-        row_store8(N + ((row * ns) << row_shift(nt)), i, E, nt, nw, w);
+        row_store8(N + ((row * ns) << row_shift(nt)), i, E, nt, w);
     }
 }

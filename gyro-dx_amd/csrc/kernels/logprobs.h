@@ -32,20 +32,28 @@ struct LpSums {
 // scale (a - b), at least -1e30 so that an exp of 0 times it is 0.
 __device__ __forceinline__ float lp_diff(float a, float b, float scale) { return fmaxf(scale * (a - b), -1e30f); }
 
-__device__ __forceinline__ LpSums lp_join(const LpSums &p, const LpSums &q, float scale) {
-    LpSums o;
-    o.m = fmaxf(p.m, q.m);
-    const float m = o.m == -INFINITY ? 0.f : o.m;
-    const float dp = lp_diff(p.m, m, scale), dq = lp_diff(q.m, m, scale), ep = __expf(dp), eq = __expf(dq);
-    o.s = p.s * ep + q.s * eq;
-    o.t = ep * (p.t + p.s * dp) + eq * (q.t + q.s * dq);
-    return o;
+// Moves p's sums to the maximum m >= p.m (-infinity: there is no term yet, and any reference will do).
+__device__ __forceinline__ void lp_move(LpSums &p, float m, float scale) {
+    const float d = lp_diff(p.m, m == -INFINITY ? 0.f : m, scale), e = __expf(d);
+    p.t = e * (p.t + p.s * d);
+    p.s *= e;
+    p.m = m;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float lp_dpp_max_step(float v) {
+    return fmaxf(v, gd_bits_f32((uint32_t)__builtin_amdgcn_update_dpp((int)0xff800000, (int)gd_f32_bits(v), CTRL, ROWS, 0xf, false)));
+}
+// Sums of the wave's lanes, in every lane: one maximum by DPP, then two sums (gd_wave_sum_dpp's steps).
 __device__ __forceinline__ LpSums lp_wave_join(LpSums p, float scale) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        p = lp_join(p, LpSums{__shfl_xor(p.m, o, 64), __shfl_xor(p.s, o, 64), __shfl_xor(p.t, o, 64)}, scale);
-    return p;
+    float m = p.m;
+    m = lp_dpp_max_step<0x111, 0xf>(m);
+    m = lp_dpp_max_step<0x112, 0xf>(m);
+    m = lp_dpp_max_step<0x114, 0xf>(m);
+    m = lp_dpp_max_step<0x118, 0xf>(m);
+    m = lp_dpp_max_step<0x142, 0xa>(m);
+    m = lp_dpp_max_step<0x143, 0xc>(m);
+    lp_move(p, gd_bits_f32((uint32_t)__builtin_amdgcn_readlane((int)gd_f32_bits(m), 63)), scale);
+    return {p.m, gd_wave_sum_dpp(p.s), gd_wave_sum_dpp(p.t)};
 }
 
 // Order of a value: falling with it, NaNs above all, both zeros alike; never 0 nor ~0.
@@ -53,13 +61,16 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
     const uint32_t u = gd_f32_bits(x + 0.0f);
     return x != x ? 0xfffffffeu : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// A value of the order u, -infinity's or above it; of a NaN's +infinity, so that only NaNs are not at or below it.
-__device__ __forceinline__ float lp_value(uint32_t u) {
-    if (u > 0xff800000u) return INFINITY;
-    if (u == 0x7fffffffu) u = 0x7ffffffeu;  // between the smallest negative value and the zeros
-    return gd_bits_f32(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+// A value of the order u, -infinity's or above it.
+__device__ __forceinline__ float lp_value(uint32_t u) { return gd_bits_f32(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+// A bound that exactly the values of orders above u pass (of orders up to infinity's): no value lies between the
+// smallest negative one and the zeros, and only NaNs are not at or below +infinity.
+__device__ __forceinline__ float lp_bound(uint32_t u) {
+    return u > 0xff800000u ? INFINITY : lp_value(u == 0x7fffffffu ? 0x7ffffffeu : u);
 }
 __device__ __forceinline__ uint64_t lp_place(float x, uint32_t i) { return (uint64_t)lp_order(x) << 32 | (uint32_t)~i; }
+// A place below every value's, for a list that is not full; no two alike (n < 2^31).
+__device__ __forceinline__ uint64_t lp_nothing(uint32_t n) { return n + 1u; }
 
 __device__ __forceinline__ void lp_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -69,61 +80,66 @@ __device__ __forceinline__ uint32_t lp_before(uint64_t mask) {  // set bits of t
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// A place below every value's, for a list that is not full; no two alike (n < 2^31).
-__device__ __forceinline__ uint64_t lp_nothing(uint32_t n) { return n + 1u; }
-
-// Cuts list[0 .. c) (c <= LP_LIST, unique places) to its `top` largest, in no order; returns their count and, where
-// something was cut, the order of the last in `bound`. One wave.
-__device__ __forceinline__ uint32_t lp_cut(uint64_t *list, uint32_t c, uint32_t top, uint32_t &bound) {
-    if (c <= top) return c;
-    const uint32_t lane = threadIdx.x & 63u, steps = (c + 63u) >> 6;
+// Moves the `top` largest of list[0 .. c) (top <= c <= LP_LIST, unique places) to out[0 .. top), in no order; out may
+// be list. Returns the order of the last of them. One wave. Code is kept small: at one batch per wave, what an
+// instruction costs is fetching it.
+__device__ __forceinline__ uint32_t lp_cut(const uint64_t *list, uint32_t c, uint32_t top, uint64_t *out) {
+    const uint32_t lane = threadIdx.x & 63u;
     uint32_t hi[LP_LIST / 64], lo[LP_LIST / 64];
     lp_wave_sync();
 #pragma unroll
     for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
-        const uint64_t p = lane + 64u * r < c ? list[lane + 64u * r] : 0ull;
-        hi[r] = (uint32_t)(p >> 32);
-        lo[r] = (uint32_t)p;
+        hi[r] = lo[r] = 0u;
+        if (64u * r < c) {
+            const uint64_t p = list[min(lane + 64u * r, c - 1u)];
+            if (lane + 64u * r < c) {
+                hi[r] = (uint32_t)(p >> 32);
+                lo[r] = (uint32_t)p;
+            }
+        }
     }
     lp_wave_sync();
-    // The largest value reached by `top` orders, then, of those that equal it, the largest reached by the rest.
-    uint32_t at = 0, count = c;
+    // The largest order that `top` reach, then, of those that equal it, the largest low word that the rest reach.
+    uint32_t at = 0, low = 0, count = c, above = 0;
     for (uint32_t bit = 0x80000000u; bit && count != top; bit >>= 1) {
+        const uint32_t probe = at | bit;
         uint32_t n = 0;
 #pragma unroll
-        for (uint32_t r = 0; r < LP_LIST / 64; ++r)
-            if (r < steps) n += __popcll(__ballot(hi[r] >= (at | bit)));
+        for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
+            if (64u * r >= c) break;
+            n += __popcll(__ballot(hi[r] >= probe));
+        }
         if (n >= top) {
-            at |= bit;
+            at = probe;
+            count = n;
+        } else {
+            above = n;  // at the end, what is above `at`
+        }
+    }
+    for (uint32_t bit = 0x80000000u; bit && count != top; bit >>= 1) {
+        const uint32_t probe = low | bit;
+        uint32_t n = above;
+#pragma unroll
+        for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
+            if (64u * r >= c) break;
+            n += __popcll(__ballot(hi[r] == at && lo[r] >= probe));
+        }
+        if (n >= top) {
+            low = probe;
             count = n;
         }
     }
-    uint32_t low = 0;
-    if (count != top) {
-        uint32_t above = 0;
-#pragma unroll
-        for (uint32_t r = 0; r < LP_LIST / 64; ++r)
-            if (r < steps) above += __popcll(__ballot(hi[r] > at));
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            uint32_t n = above;
-#pragma unroll
-            for (uint32_t r = 0; r < LP_LIST / 64; ++r)
-                if (r < steps) n += __popcll(__ballot(hi[r] == at && lo[r] >= (low | bit)));
-            if (n >= top) low |= bit;
-        }
-    }
-    uint32_t out = 0;
+    uint32_t o = 0;
 #pragma unroll
     for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
-        if (r >= steps) break;
-        const bool keep = count == top ? hi[r] >= at : hi[r] > at || (hi[r] == at && lo[r] >= low);
+        if (64u * r >= c) break;
+        const bool keep = hi[r] > at || (hi[r] == at && lo[r] >= low);
         const uint64_t mask = __ballot(keep);
-        if (keep) list[out + lp_before(mask)] = (uint64_t)hi[r] << 32 | lo[r];
-        out += __popcll(mask);
+        if (keep) out[o + lp_before(mask)] = (uint64_t)hi[r] << 32 | lo[r];
+        o += __popcll(mask);
     }
     lp_wave_sync();
-    bound = at;
-    return out;
+    return at;
 }
 
 // One wave's share of a row's top: its list, the count and the bound (values at or below it are out). -infinity is
@@ -135,105 +151,115 @@ struct LpTop {
     float bound;
 };
 
-// The 32 values of a lane, x[8 j + e] being value first + 512 j + 8 lane + e of the row (-infinity outside it).
-// gd_rounded: the compiler makes ballots and orders again where they are used again, instead of keeping 32 of them.
-__device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], uint32_t first, float most, bool nan) {
-    if (!__any(nan || !(most <= l.bound))) return;
-    const uint32_t at0 = first + 8u * (threadIdx.x & 63u);
-    auto count = [&](float bound) {
-        const float b = gd_rounded(bound);
+// Adds to the list what may be among the top of the 32 values of a lane, x[8 j + e] being value at(j) + e of the row
+// (-infinity outside it). gd_rounded: the compiler makes ballots and orders again where they are used again, instead
+// of keeping 32 of them.
+template <typename F>
+__device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, bool nan) {
+    float group[4];  // maxima of 8
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        group[j] = x[8 * j];
+#pragma unroll
+        for (uint32_t e = 1; e < 8; ++e) group[j] = fmaxf(group[j], x[8 * j + e]);
+    }
+    auto groups = [&](float bound) {
         uint32_t n = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) n += __popcll(__ballot(!(x[i] <= b)));
+        for (uint32_t j = 0; j < 4; ++j) n += __popcll(__ballot(!(group[j] <= bound)));
         return n;
     };
     float bound = l.bound;
-    uint32_t n = count(bound);
-    if (l.c + n > LP_LIST && l.c > l.top) {
-        uint32_t last = 0;
-        l.c = lp_cut(l.list, l.c, l.top, last);
-        bound = l.bound = lp_value(last);
-        n = count(bound);
-    }
-    if (l.c + n > LP_LIST) {
-        // A lower bound of the batch's top-th value from the maxima of 8, by their leading 16 bits.
-        uint32_t group[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            float m = x[8 * j];
-#pragma unroll
-            for (uint32_t e = 1; e < 8; ++e) m = fmaxf(m, x[8 * j + e]);
-            group[j] = lp_order(m);
+    uint32_t n = nan ? 256u : groups(bound);  // a maximum leaves out NaNs
+    if (!n) return;
+    if (l.c + 8u * n > LP_LIST) {
+        if (l.c > l.top) {
+            bound = l.bound = lp_bound(lp_cut(l.list, l.c, l.top, l.list));
+            l.c = l.top;
         }
-        uint32_t at = 0;
+        // A lower bound of the batch's top-th value from the maxima of 8, by their leading bits: up to 16, fewer where
+        // no more than 8 maxima too many reach it.
+        uint32_t order[4], leading = 0, count = 256;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) order[j] = lp_order(group[j]);
 #pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+        for (uint32_t bit = 0x80000000u; bit >= 0x10000u && count > l.top + 8u; bit >>= 1) {
             uint32_t reached = 0;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) reached += __popcll(__ballot(group[j] >= (at | bit)));
-            if (reached >= l.top) at |= bit;
+            for (uint32_t j = 0; j < 4; ++j) reached += __popcll(__ballot(order[j] >= (leading | bit)));
+            if (reached >= l.top) {
+                leading |= bit;
+                count = reached;
+            }
         }
-        if (at > lp_order(-INFINITY)) {
-            const float low = lp_value(at - 1u);
+        if (leading > lp_order(-INFINITY)) {
+            const float low = lp_bound(leading - 1u);
             if (!(low <= bound)) bound = low;
         }
-        n = count(bound);
-    }
-    if (l.c + n <= LP_LIST) {
+        n = 0;
         const float b = gd_rounded(bound);
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-            const bool take = !(x[i] <= b);
-            const uint64_t mask = __ballot(take);
-            if (!mask) continue;
-            if (take) l.list[l.c + lp_before(mask)] = lp_place(x[i], at0 + 512u * (i >> 3) + (i & 7u));
-            l.c += __popcll(mask);
-        }
-    } else {
-        // The batch's own top, exactly (more than LP_LIST of its values are above the bound): the largest order that
-        // `top` of its values reach, what is above it, and of those that equal it the first.
-        auto order = [&](float v) {
-            const float w = gd_rounded(v);
-            return w <= bound ? 0u : lp_order(w);
-        };
-        uint32_t at = 0;
+        for (uint32_t i = 0; i < 32; ++i) n += __popcll(__ballot(!(x[i] <= b)));
+        if (l.c + n > LP_LIST) {
+            // The batch's own top, exactly: the largest order that `top` of its values reach, what is above it, and of
+            // those that equal it the first.
+            auto exact = [&](float v) {
+                const float w = gd_rounded(v);
+                return w <= bound ? 0u : lp_order(w);
+            };
+            uint32_t last = 0, left = l.top;
 #pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            uint32_t reached = 0;
+            for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                uint32_t reached = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) reached += __popcll(__ballot(order(x[i]) >= (at | bit)));
-            if (reached >= l.top) at |= bit;
+                for (uint32_t i = 0; i < 32; ++i) reached += __popcll(__ballot(exact(x[i]) >= (last | bit)));
+                if (reached >= l.top) last |= bit;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) {
+                const bool take = exact(x[i]) > last;
+                const uint64_t mask = __ballot(take);
+                if (!mask) continue;
+                if (take) l.list[l.c + lp_before(mask)] = lp_place(x[i], at(i >> 3) + (i & 7u));
+                l.c += __popcll(mask);
+                left -= __popcll(mask);  // fewer than `top` are above
+            }
+            // 512 values of a step in order: by lane, then within its 8.
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                if (!left) break;
+                uint32_t mine = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) mine += exact(x[8 * j + e]) == last ? 1u : 0u;
+                const uint32_t upto = gd_wave_scan_u32(mine), all = __shfl(upto, 63, 64);
+                uint32_t pos = upto - mine;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    if (exact(x[8 * j + e]) == last) {
+                        if (pos < left) l.list[l.c + pos] = lp_place(x[8 * j + e], at(j) + e);
+                        ++pos;
+                    }
+                const uint32_t took = min(all, left);
+                l.c += took;
+                left -= took;
+            }
+            lp_wave_sync();
+            l.bound = lp_bound(last);
+            return;
         }
-        uint32_t left = l.top;
+    }
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-            const bool take = order(x[i]) > at;
+    for (uint32_t j = 0; j < 4; ++j) {
+        if (!nan && !__any(!(group[j] <= bound))) continue;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const float v = x[8 * j + e];
+            const bool take = !(v <= bound);
             const uint64_t mask = __ballot(take);
             if (!mask) continue;
-            if (take) l.list[l.c + lp_before(mask)] = lp_place(x[i], at0 + 512u * (i >> 3) + (i & 7u));
+            if (take) l.list[l.c + lp_before(mask)] = lp_place(v, at(j) + e);
             l.c += __popcll(mask);
-            left -= __popcll(mask);  // fewer than `top` are above
         }
-        // 512 values of a step in order: by lane, then within its 8.
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            if (!left) break;
-            uint32_t mine = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) mine += order(x[8 * j + e]) == at ? 1u : 0u;
-            const uint32_t upto = gd_wave_scan_u32(mine), all = __shfl(upto, 63, 64);
-            uint32_t pos = upto - mine;
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                if (order(x[8 * j + e]) == at) {
-                    if (pos < left) l.list[l.c + pos] = lp_place(x[8 * j + e], at0 + 512u * j + e);
-                    ++pos;
-                }
-            const uint32_t took = min(all, left);
-            l.c += took;
-            left -= took;
-        }
-        bound = lp_value(at);
     }
     lp_wave_sync();
     if (l.c >= l.top && !(bound <= l.bound)) l.bound = bound;
@@ -254,9 +280,9 @@ __device__ __forceinline__ LpGiven lp_given(const GdArgs &a, uint64_t row, uint6
     return g;
 }
 
-// The row's outputs from its sums and the list of `c` <= 4 LP_TOP places in LDS; the first wave.
+// The row's outputs from its sums and its `top` places (list, in LDS, in any order); the first wave.
 __device__ __forceinline__ void lp_finish(const GdArgs &a, uint64_t row, uint64_t X, const LpSums &p, const LpGiven &g,
-                                          uint64_t *list, uint32_t c) {
+                                          const uint64_t *list) {
     const float scale = gd_bits_f32(a.c[6]);
     const bool none = p.s == 0.f;
     const float logs = none ? 0.f : logf(p.s);
@@ -267,27 +293,29 @@ __device__ __forceinline__ void lp_finish(const GdArgs &a, uint64_t row, uint64_
         gd_at<float>(gd_addr(a, 14))[row * gd_addr(a, 16) + lane] =
             g.kind == 0 ? logprob(g.x) : g.kind == 1 ? 0.f : __builtin_nanf("");
     if (!top) return;
-    uint32_t bound;
-    lp_cut(list, c, top, bound);
     const uint64_t mine = lane < top ? list[lane] : 0ull;
-    const bool real = (mine >> 32) != 0;
+    const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine;
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (uint32_t k = 0; k < top; ++k) {
+        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, (int)k) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)lo, (int)k);
+        rank += other > mine ? 1u : 0u;
+    }
     const auto ids = gd_at<uint32_t>(gd_addr(a, 20)) + row * gd_addr(a, 24);
     const auto tops = gd_at<float>(gd_addr(a, 22)) + row * gd_addr(a, 24);
-    uint32_t rank = 0;
-    for (uint32_t k = 0; k < top; ++k) rank += list[k] > mine ? 1u : 0u;
-    if (real) {
-        const uint32_t id = ~(uint32_t)mine;
-        ids[rank] = id;
-        tops[rank] = logprob(row_load(X, id, a.c[4]));
+    if (hi) {
+        ids[rank] = ~lo;
+        tops[rank] = logprob(lp_value(hi));
     }
     // What is missing are the first logits of -infinity.
-    for (uint32_t found = __popcll(__ballot(real)), i = 0; found < top && i < a.c[5]; i += 64u) {
+    for (uint32_t found = __popcll(__ballot(hi != 0u)), i = 0; found < top && i < a.c[5]; i += 64u) {
         const bool hit = i + lane < a.c[5] && row_load(X, i + lane, a.c[4]) == -INFINITY;
         const uint64_t mask = __ballot(hit);
-        const uint32_t at = found + lp_before(mask);
-        if (hit && at < top) {
-            ids[at] = i + lane;
-            tops[at] = logprob(-INFINITY);
+        const uint32_t to = found + lp_before(mask);
+        if (hit && to < top) {
+            ids[to] = i + lane;
+            tops[to] = logprob(-INFINITY);
         }
         found += __popcll(mask);
     }
@@ -296,4 +324,105 @@ __device__ __forceinline__ void lp_finish(const GdArgs &a, uint64_t row, uint64_
 // Workspace of a row's part: the sums (4 words), then `top` places, in 16-byte units.
 __device__ __forceinline__ uint64_t lp_part(const GdArgs &a, uint64_t row, uint32_t part) {
     return gd_addr(a, 28) + (row * a.c[27] + part) * (16u + 8ull * ((a.c[7] + 1u) & ~1u));
+}
+
+// A group of four waves takes a row, or a part of one, wave w batches w, w + 4, ... of it. Grid: x rows (up to 65535),
+// y = (rows / 65535) * parts + part.
+template <uint32_t TYPE>
+__device__ __forceinline__ void logprobs_body(const GdArgs &a) {
+    __shared__ uint64_t lists[LP_WAVES * LP_LIST];
+    __shared__ uint64_t merged[LP_LIST];
+    __shared__ LpSums sums[LP_WAVES];
+    __shared__ uint32_t counts[LP_WAVES];
+    const uint32_t V = a.c[5], top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t part = blockIdx.y % parts;
+    const uint64_t row = (uint64_t)(blockIdx.y / parts) * gridDim.x + blockIdx.x;
+    if (row >= a.c[26]) return;
+    const float scale = gd_bits_f32(a.c[6]);
+    const uint64_t X = gd_addr(a, 0) + ((row * gd_addr(a, 2)) << row_shift(TYPE));
+    LpGiven given = {0.f, 1};
+    if (parts == 1u) given = lp_given(a, row, X);
+    const uint32_t batches = (V + LP_BATCH - 1u) / LP_BATCH;
+    const uint32_t b0 = (uint32_t)((uint64_t)batches * part / parts), b1 = (uint32_t)((uint64_t)batches * (part + 1u) / parts);
+    LpTop l = {lists + wave * LP_LIST, 0u, top, -INFINITY};
+    LpSums p = {-INFINITY, 0.f, 0.f};
+    for (uint32_t b = b0 + wave; b < b1; b += LP_WAVES) {
+        const uint32_t first = b * LP_BATCH + 8u * lane;
+        float x[32];
+        // Eight values at a time; a lane that reaches past the row reads the row's last eight and leaves out (as
+        // -infinity) those before its own. A row of fewer than eight is one lane's.
+        auto at = [&](uint32_t j) { return V < 8u ? first + 512u * j : min(first + 512u * j, V - 8u); };
+        if (V >= 8u) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                float v[8];
+                row_load8<TYPE>(X, at(j), v);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) x[8 * j + e] = v[e];
+            }
+            if (b + 1u == batches) {
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i)
+                    if (at(i >> 3) + (i & 7u) < first + 512u * (i >> 3)) x[i] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) x[i] = i < 8u && first + i < V ? row_load(X, first + i, TYPE) : -INFINITY;
+        }
+        float most = x[0];
+#pragma unroll
+        for (uint32_t i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
+        lp_move(p, fmaxf(p.m, most), scale);
+        const float ref = p.m == -INFINITY ? 0.f : p.m;
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            const float d = scale * (x[i] - ref), e = __expf(d);
+            s += e;
+            t += e * fmaxf(d, -1e30f);
+        }
+        p.s += s;
+        p.t += t;
+        if (top) lp_add(l, x, at, __any(p.s != p.s));
+    }
+    p = lp_wave_join(p, scale);
+    if (lane == 0) {
+        sums[wave] = p;
+        counts[wave] = l.c;
+    }
+    __syncthreads();
+    if (top) {
+        // The waves' lists side by side, each cut to its top first where they are too long together; the first `top`
+        // places of a short one are filled up.
+        uint32_t c[LP_WAVES], total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < LP_WAVES; ++w) total += c[w] = counts[w];
+        const bool cut = total > LP_LIST - top;
+        uint32_t start = 0, mine = l.c;
+#pragma unroll
+        for (uint32_t w = 0; w < LP_WAVES; ++w)
+            if (w < wave) start += cut ? min(c[w], top) : c[w];
+        if (cut && l.c > top) {
+            lp_cut(l.list, l.c, top, l.list);
+            mine = top;
+        }
+        for (uint32_t i = lane; i < mine; i += 64u) merged[start + i] = l.list[i];
+        if (wave == LP_WAVES - 1u && start + mine < top)
+            for (uint32_t i = start + mine + lane; i < top; i += 64u) merged[i] = lp_nothing(part * LP_TOP + i);
+        __syncthreads();
+        if (wave) return;
+        total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < LP_WAVES; ++w) total += cut ? min(c[w], top) : c[w];
+        if (total > top) lp_cut(merged, total, top, merged);
+    }
+    if (wave) return;
+    p = lp_wave_join(lane < LP_WAVES ? sums[lane] : LpSums{-INFINITY, 0.f, 0.f}, scale);
+    if (parts == 1u) {
+        lp_finish(a, row, X, p, given, merged);
+        return;
+    }
+    const uint64_t out = lp_part(a, row, part);
+    if (lane == 0) gd_at<gd_f32x4>(out)[0] = gd_f32x4{p.m, p.s, p.t, 0.f};
+    if (lane < top) gd_at<uint64_t>(out + 16u)[lane] = merged[lane];
 }

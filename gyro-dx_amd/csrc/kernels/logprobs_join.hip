@@ -1,5 +1,5 @@
 // Joins the parts of rows that several groups of logprobs shared (logprobs.h): a group per row, a wave per quarter of
-// the parts' places (at most 32 parts of at most 64).
+// the parts' places (at most 32 parts of at most 64), or the first wave alone where all of them fit its list.
 #include "logprobs.h"
 
 GD_PIPELINE_NAMED(logprobs_join, 256) {
@@ -16,17 +16,27 @@ GD_PIPELINE_NAMED(logprobs_join, 256) {
         const gd_f32x4 v = gd_at<const gd_f32x4>(lp_part(a, row, lane))[0];
         p = LpSums{v[0], v[1], v[2]};
     }
+    const bool alone = parts * top <= LP_LIST;
     if (top) {
-        // Wave w: parts w, w + 4, ..., up to 8 of them.
         uint64_t *list = lists + wave * LP_LIST;
-        uint32_t c = 0, bound;
-        for (uint32_t part = wave; part < parts; part += LP_WAVES, c += top)
-            if (lane < top) list[c + lane] = gd_at<const uint64_t>(lp_part(a, row, part) + 16u)[lane];
-        lp_wave_sync();
-        c = lp_cut(list, c, top, bound);
-        if (lane < top) merged[wave * top + lane] = lane < c ? list[lane] : lp_nothing((parts + wave) * LP_TOP + lane);
-        __syncthreads();
+        const uint32_t step = alone ? 1u : LP_WAVES, total = parts * top;
+        if (alone && wave == 0) {
+            for (uint32_t i = lane; i < total; i += 64u) {
+                const uint32_t part = i / top;
+                list[i] = gd_at<const uint64_t>(lp_part(a, row, part) + 16u)[i - part * top];
+            }
+            lp_cut(list, total, top, merged);
+        } else if (!alone) {
+            // Wave w: parts w, w + 4, ..., up to 8 of them.
+            uint32_t c = 0;
+            for (uint32_t part = wave; part < parts; part += step, c += top)
+                if (lane < top) list[c + lane] = gd_at<const uint64_t>(lp_part(a, row, part) + 16u)[lane];
+            lp_cut(list, c, top, list);  // more than 512 places: every wave has a part
+            if (lane < top) merged[wave * top + lane] = list[lane];
+            __syncthreads();
+            if (wave == 0) lp_cut(merged, LP_WAVES * top, top, merged);
+        }
     }
     if (wave) return;
-    lp_finish(a, row, X, lp_wave_join(p, scale), given, merged, LP_WAVES * top);
+    lp_finish(a, row, X, lp_wave_join(p, scale), given, merged);
 }

@@ -72,7 +72,6 @@ __device__ __forceinline__ void mv_q4_body(const GdArgs &a) {
     gd_u32x4 *xl = reinterpret_cast<gd_u32x4 *>(pool + red_bytes);
     const uint32_t seg = min(chunks, (MQ_POOL - red_bytes) / (rows * 256u));  // chunks per segment
     const uint32_t units = seg * 16u;                                          // 16-byte units per operand row
-    const bool wide = row_aligned(X, xs, xt);
     const uint32_t arow = min(col, rows - 1u);
 
     const float bias = minima ? -16.f : -24.f;
@@ -92,7 +91,7 @@ __device__ __forceinline__ void mv_q4_body(const GdArgs &a) {
                 for (uint32_t i = tid; i < nt * units; i += 64u * MQ_WAVES) {
                     const uint32_t t = i / units, u = i - t * units;
                     float v[8];
-                    row_load8(X + (((uint64_t)(t0 + t) * xs) << row_shift(xt)), c0 * 128u + u * 8u, cols, xt, wide, v);
+                    row_load8(X + (((uint64_t)(t0 + t) * xs) << row_shift(xt)), c0 * 128u + u * 8u, cols, xt, v);
                     mq_planes(v, P, [&](uint32_t p, gd_u32x4 w) {
                         const uint32_t r = t * P + p;
                         xl[r * units + (u ^ (r & 15u))] = w;

@@ -36,37 +36,42 @@ __device__ __forceinline__ void row_store(uint64_t base, uint64_t i, uint32_t ty
     else gd_at<uint16_t>(base)[i] = (uint16_t)row_bits16(v, type);
 }
 
-// Whether every 8-value group of rows at `base`, `stride` values apart, starts on a 16-byte boundary
-// (fp32 groups are two 16-byte loads).
-__device__ __forceinline__ bool row_aligned(uint64_t base, uint64_t stride, uint32_t type) {
-    return ((base | (stride << row_shift(type))) & 15u) == 0;
-}
+// 16-byte accesses at any address of the type's alignment (a row starts where the caller's stride puts it).
+typedef gd_u32x4 gd_u32x4_any __attribute__((aligned(2)));
+typedef gd_f32x4 gd_f32x4_any __attribute__((aligned(4)));
 
-// Values i .. i + 7 of a row, those from `n` on as zeros; `wide`: the row is row_aligned and i a multiple of 8.
-__device__ __forceinline__ void row_load8(uint64_t row, uint32_t i, uint32_t n, uint32_t type, bool wide, float (&v)[8]) {
-    if (wide && i + 8u <= n) {
-        if (type == ROW_F32) {
-            const gd_f32x4 a = gd_at<const gd_f32x4>(row + 4ull * i)[0], b = gd_at<const gd_f32x4>(row + 4ull * i)[1];
+// Values i .. i + 7 of a row.
+template <uint32_t TYPE>
+__device__ __forceinline__ void row_load8(uint64_t row, uint32_t i, float (&v)[8]) {
+    if constexpr (TYPE == ROW_F32) {
+        const gd_f32x4 a = gd_at<const gd_f32x4_any>(row + 4ull * i)[0], b = gd_at<const gd_f32x4_any>(row + 4ull * i)[1];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = a[j];
-                v[4 + j] = b[j];
-            }
-        } else {
-            const gd_u32x4 w = gd_at<const gd_u32x4>(row + 2ull * i)[0];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[2 * j] = row_value16(w[j] & 0xffffu, type);
-                v[2 * j + 1] = row_value16(w[j] >> 16, type);
-            }
+        for (int j = 0; j < 4; ++j) {
+            v[j] = a[j];
+            v[4 + j] = b[j];
         }
+    } else {
+        const gd_u32x4 w = gd_at<const gd_u32x4_any>(row + 2ull * i)[0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = row_value16(w[j] & 0xffffu, TYPE);
+            v[2 * j + 1] = row_value16(w[j] >> 16, TYPE);
+        }
+    }
+}
+// As before, of a type known at run time, those from `n` on as zeros.
+__device__ __forceinline__ void row_load8(uint64_t row, uint32_t i, uint32_t n, uint32_t type, float (&v)[8]) {
+    if (i + 8u <= n) {
+        if (type == ROW_F32) row_load8<ROW_F32>(row, i, v);
+        else if (type == ROW_BF16) row_load8<ROW_BF16>(row, i, v);
+        else row_load8<ROW_F16>(row, i, v);
         return;
     }
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) v[j] = i + j < n ? row_load(row, i + j, type) : 0.f;
 }
-__device__ __forceinline__ void row_store8(uint64_t row, uint32_t i, uint32_t n, uint32_t type, bool wide, const float (&v)[8]) {
-    if (wide && i + 8u <= n) {
+__device__ __forceinline__ void row_store8(uint64_t row, uint32_t i, uint32_t n, uint32_t type, const float (&v)[8]) {
+    if (i + 8u <= n) {
         if (type == ROW_F32) {
             gd_f32x4 a, b;
 #pragma unroll
@@ -74,13 +79,13 @@ __device__ __forceinline__ void row_store8(uint64_t row, uint32_t i, uint32_t n,
                 a[j] = v[j];
                 b[j] = v[4 + j];
             }
-            gd_at<gd_f32x4>(row + 4ull * i)[0] = a;
-            gd_at<gd_f32x4>(row + 4ull * i)[1] = b;
+            gd_at<gd_f32x4_any>(row + 4ull * i)[0] = a;
+            gd_at<gd_f32x4_any>(row + 4ull * i)[1] = b;
         } else {
             gd_u32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = row_bits16(v[2 * j], type) | row_bits16(v[2 * j + 1], type) << 16;
-            gd_at<gd_u32x4>(row + 2ull * i)[0] = w;
+            gd_at<gd_u32x4_any>(row + 2ull * i)[0] = w;
         }
         return;
     }

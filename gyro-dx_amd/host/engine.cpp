@@ -489,7 +489,7 @@ class Engine {
         require(status == hipStreamCaptureStatusNone,
                 "the operator's kernel is not loaded: call gm_load_operators or the operator once before a capture");
         require(ops.files.count(name) != 0, "operator kernel missing from the kernel directory");
-        ops.load(name);
+        ops.load(name);  // and its other types' builds
         return ops.pipes.at(name);
     }
     void launch(const Launch &l, void *stream) {

@@ -219,7 +219,7 @@ class RowOps {
     // Groups that share a row: enough that the rows' groups fill the device, each of their four waves with a batch
     // of 2048 logits at least.
     static uint32_t logprobs_parts(uint32_t n, uint32_t V) {
-        const uint32_t batches = (V + 7 + 2047) / 2048;
+        const uint32_t batches = (V + 2047) / 2048;
         return std::max(1u, std::min({32u, (batches + 3) / 4, 768 / std::max(1u, n)}));
     }
     static uint64_t logprobs_workspace(uint32_t n, uint32_t V, uint32_t top) {
@@ -265,7 +265,7 @@ class RowOps {
         const uint32_t parts = logprobs_parts(n, d.V);
         c.set(27, parts);
         c.set(28, d.workspace);
-        l.kernel = "logprobs";
+        l.kernel = d.logits.type == GM_F32 ? "logprobs" : d.logits.type == GM_BF16 ? "logprobs_b" : "logprobs_h";
         l.x = std::min(n, 65535u);
         l.y = (uint32_t)(((uint64_t)n + 65534) / 65535) * parts;
         if (parts > 1) {
