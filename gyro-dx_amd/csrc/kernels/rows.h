@@ -7,6 +7,7 @@ enum { ROW_F32 = 0, ROW_BF16 = 1, ROW_F16 = 2 };
 
 typedef __bf16 gd_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float gd_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t gd_u32x2 __attribute__((ext_vector_type(2)));
 
 // The address in constants W and W + 1, in global address space (global loads, not flat ones).
 template <typename T>

@@ -441,6 +441,7 @@ class Engine {
         Matrix m = RowOps::describe(d);
         ops.load("q4_repack");
         ops.load("mv_q4");
+        ops.load("mm_q4");
         const uint64_t bytes = RowOps::layout(m), qb = (RowOps::quant_bytes(d) + 255) & ~uint64_t(255),
                        sb = d.scales ? (RowOps::scale_bytes(d) + 255) & ~uint64_t(255) : 0, mb = d.mins ? sb : 0;
         struct Held {
@@ -448,7 +449,7 @@ class Engine {
             Buffer b;
             ~Held() { dev.release(b); }
         } src{dev, {}}, out{dev, {}};
-        out.b = dev.buffer(bytes, Kind::device);
+        out.b = dev.buffer(bytes + 8, Kind::device);  // scales are read 8 bytes at a time
         src.b = dev.buffer(qb + sb + mb, Kind::device);
         const void *parts[2][3] = {{d.quants, d.scales, d.mins}, {d.up_quants, d.up_scales, d.up_mins}};
         for (uint32_t half = 0; half < (m.gated ? 2u : 1u); ++half) {

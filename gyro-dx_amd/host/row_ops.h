@@ -52,7 +52,7 @@ class RowOps {
     std::vector<Matrix> matrices;
 
     static bool owns(const std::string &kernel) {
-        return kernel.rfind("mv_q4", 0) == 0 || kernel == "q4_repack" || kernel.rfind("block_norm", 0) == 0 ||
+        return kernel.rfind("mv_q4", 0) == 0 || kernel.rfind("mm_q4", 0) == 0 || kernel == "q4_repack" || kernel.rfind("block_norm", 0) == 0 ||
                kernel.rfind("logprobs", 0) == 0;
     }
     using Loader = std::function<gd_pipeline *(const std::string &file)>;
@@ -157,13 +157,31 @@ class RowOps {
         c.set(23, act);
         c.set(24, accumulate ? 1u : 0u);
         c.set(25, scale);
-        uint32_t wk = 1;
-        while (wk < 8 && wk * 2 <= m.chunks) wk *= 2;
-        c.set(26, wk);
         const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u;
-        const bool few = m.tiles / (4 * (8 / wk)) < cus;
-        const uint32_t run = (few ? 2u : 4u) * (8 / wk), runs = (m.tiles + run - 1) / run;
-        l.kernel = few ? "mv_q4_s" : "mv_q4";
+        const char *em = getenv("MM"); 
+        if (em ? em[0] == '1' : n > per) {
+            static const char *const names[2][3] = {{"mm_q4_f", "mm_q4_b", "mm_q4_h"}, {"mm_q4_fm", "mm_q4_bm", "mm_q4_hm"}};
+            uint32_t best = 1, cost = ~0u;
+            for (uint32_t t = 1; t <= (x.type == GM_F32 ? 3u : 4u); ++t) {
+                const uint32_t k = (n + 16 * t - 1) / (16 * t) * (28 + 16 * t);
+                if (k <= cost) {
+                    cost = k;
+                    best = t;
+                }
+            }
+            const char *et = getenv("MMT"); if (et) best = atoi(et);
+            c.set(26, best);
+            l.kernel = names[m.mins ? 1 : 0][x.type];
+            l.x = (m.tiles + 15) / 16;
+            l.y = (n + 16 * best - 1) / (16 * best);
+            return l;
+        }
+        uint32_t wk = 1;
+        while (wk < 8 && wk * 2 <= m.chunks && m.tiles / 2 * wk < 16 * cus) wk *= 2;
+        c.set(26, wk);
+        const char *ew = getenv("MQW"); if (ew) { wk = atoi(ew); c.set(26, wk); }
+        const uint32_t run = 2 * (8 / wk), runs = (m.tiles + run - 1) / run;
+        l.kernel = m.mins ? "mv_q4_m" : "mv_q4";
         l.x = std::min(runs, 2 * cus);
         l.y = (n + per - 1) / per;
         return l;
