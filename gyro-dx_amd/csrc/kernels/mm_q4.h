@@ -1,10 +1,13 @@
 // Products of many tokens with a 4-bit matrix in the layout of q4_repack (q4.h).
 //
 // A group of four waves takes 16 tiles (256 weight rows), four to a wave, and 16 T tokens. Chunks of 128 columns of the
-// tokens go through LDS as operands, two buffers in turn, one being filled while the other is multiplied;
-// weights go from memory to registers, a chunk ahead. Per group of 32 columns a wave unpacks 4 operands, each used for T
-// products, and scales 4 T sums: 28 + 16 T vector instructions beside 5 T matrix ones. bf16 and binary16 tokens are
-// operands as they are; fp32 ones go through the products three times, a part each (PARTS).
+// tokens go through LDS as operands, two buffers in turn, one being filled while the other is multiplied; weights
+// go from memory to registers, a chunk ahead. Of 32 columns a wave unpacks 4 operands, each used for T products
+// of 16 + q; a scale's products (SPAN groups of 32) add up in the matrix unit before they are scaled into the sums, 16 T /
+// SPAN vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much and the minimum,
+// (m - 16 s) sum x (or -24 s sum x), is a product of its own: of the chunk's four sums of 32 activations, which come
+// with the staging, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens are operands as they are; fp32 ones
+// go through the products three times, a part each.
 #pragma once
 #include "q4.h"
 
@@ -12,6 +15,8 @@
 #define MM_R 4
 
 typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 gd_f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 gd_bf16x2 __attribute__((ext_vector_type(2)));
 
 // c + a b of token operand a and weight operand b, both of the operand type.
 template <bool HALF>
@@ -21,14 +26,58 @@ __device__ __forceinline__ gd_f32x4 mm_mfma(gd_u32x4 a, gd_u32x4 b, gd_f32x4 c) 
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b), c, 0, 0, 0);
 }
-template <uint32_t TYPE, bool MINIMA, int T>
-__device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds) {
+// c + both values of a word of 16-bit tokens.
+template <bool HALF>
+__device__ __forceinline__ float mm_pair(uint32_t w, float c) {
+    if constexpr (HALF)
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(gd_f16x2, w), gd_f16x2{(_Float16)1.f, (_Float16)1.f}, c, false);
+    else
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(gd_bf16x2, w), gd_bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float mm_dpp(float v) {
+    return gd_bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)gd_f32_bits(v), CTRL, 0xf, 0xf, true));
+}
+
+// A chunk of a tile as a lane holds it: its 16 bytes, and its row's 4 / SPAN scales and minima, binary16 in order.
+template <int SPAN>
+struct MmChunk {
+    gd_u32x4 w;
+    uint32_t s[SPAN == 1 ? 2 : 1], m[SPAN == 1 ? 2 : 1];
+};
+template <int SPAN>
+__device__ __forceinline__ void mm_scales(uint64_t base, uint32_t row, uint32_t (&o)[SPAN == 1 ? 2 : 1]) {
+    if constexpr (SPAN == 1) {
+        const gd_u32x2 v = gd_load<gd_u32x2>(base, row * 8u);
+        o[0] = v[0];
+        o[1] = v[1];
+    } else if constexpr (SPAN == 2) {
+        o[0] = gd_load<uint32_t>(base, row * 4u);
+    } else {
+        o[0] = gd_load<uint16_t>(base, row * 2u);
+    }
+}
+
+// Asks the scheduler for `others` vector instructions spread between `products` matrix ones.
+template <int PRODUCTS, int OTHERS>
+__device__ __forceinline__ void mm_interleave() {
+#pragma unroll
+    for (int t = 0; t < PRODUCTS; ++t) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (OTHERS + PRODUCTS - 1) / PRODUCTS, 0);
+    }
+}
+
+template <uint32_t TYPE, int SPAN, int T>
+__device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float *sums) {
     constexpr bool HALF = TYPE == ROW_F16;
     constexpr int PARTS = TYPE == ROW_F32 ? 3 : 1;
     constexpr uint32_t ROWS = 16u * T, UNITS = ROWS * 16u, PER = UNITS / 256u;  // 16-byte units of a chunk, of a thread
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, col = lane & 15u, h = lane >> 4;
-    const uint64_t quants = gd_addr(a, 0), scales = gd_addr(a, 2), minima = gd_addr(a, 4);
-    const uint32_t tiles = a.c[6], chunks = a.c[7], lg = a.c[8], cols = a.c[9], outputs = a.c[10], n = a.c[17];
+    constexpr uint32_t SUMS = ROWS + 16u;  // a group's row of sums, the four groups' in different banks
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, h = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint64_t quants = gd_addr(a, 0), scales = gd_addr(a, 2), minima = gd_addr(a, 4) ? gd_addr(a, 4) : scales;
+    const uint32_t tiles = a.c[6], chunks = a.c[7], cols = a.c[9], outputs = a.c[10], n = a.c[17];
     const uint64_t X = gd_addr(a, 12), xs = gd_addr(a, 14);
     // The groups of an XCD (i % 8) take neighbouring rows, all tokens of some before the next, so that its L2 holds
     // their weights.
@@ -39,37 +88,50 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds) {
         rb = (i & 7u) * own + s / gridDim.y;
     }
     const uint32_t t0 = tb * ROWS, tile0 = (rb * MM_WAVES + wave) * MM_R;
-    const MqSpread spread = mq_spread(lg);
     const MqBits bits = mq_bits<HALF>();
-    const uint32_t b16 = HALF ? (MINIMA ? 0xcc00u : 0xce00u) : (MINIMA ? 0xc180u : 0xc1c0u), b32 = b16 | b16 << 16;  // -16, -24
-    const gd_u32x4 unbias = {b32, b32, b32, b32};
+    // The sums' coefficient of scale and minimum: m - 16 s, or -24 s (what is loaded as the minimum is the scale then).
+    const float of_scale = gd_addr(a, 4) ? -16.f : -24.f, of_minimum = gd_addr(a, 4) ? 1.f : 0.f;
     const gd_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    MqChunk cur[MM_R], next[MM_R];
-    auto load = [&](uint32_t c, MqChunk (&o)[MM_R]) {
+    MmChunk<SPAN> cur[MM_R], next[MM_R];
+    auto load = [&](uint32_t c, MmChunk<SPAN> (&o)[MM_R]) {
 #pragma unroll
         for (int r = 0; r < MM_R; ++r) {
             // Tiles past the last read the last again; their sums are dropped.
             const uint64_t unit = (uint64_t)min(tile0 + r, tiles - 1u) * chunks + c;
-            o[r].w = gd_at<const gd_u32x4>(quants)[unit * 64u + lane];
-            o[r].s = mq_scales(scales, unit * 16u + col, lg);
-            if constexpr (MINIMA) o[r].m = mq_scales(minima, unit * 16u + col, lg);
+            o[r].w = gd_load<gd_u32x4>(quants + unit * 1024u, lane * 16u);
+            mm_scales<SPAN>(scales + unit * (128u / SPAN), col, o[r].s);
+            mm_scales<SPAN>(minima + unit * (128u / SPAN), col, o[r].m);
         }
     };
     // Unit i = tid + 256 k of a chunk of the tokens: row i / 16, values 8 (i % 16) ..; rows past the last token read the
-    // last again. Held as loaded, made operands when they are stored.
+    // last again, columns past the last are zeros. Held as loaded, made operands when they are stored. A row is at most
+    // 2^24 values after the one before, so that a tile's 64 are within 32 bits of its first.
     constexpr int RAW = TYPE == ROW_F32 ? 2 : 1;
     gd_u32x4 raw[PER][RAW];
+    uint32_t from[PER];
+#pragma unroll
+    for (uint32_t k = 0; k < PER; ++k) {
+        const uint32_t i = tid + 256u * k, row = min(i >> 4, n - 1u - t0);
+        from[k] = (row * (uint32_t)xs + 8u * (i & 15u)) << row_shift(TYPE);
+    }
+    const uint64_t X0 = X + (((uint64_t)t0 * xs) << row_shift(TYPE));
     auto fetch = [&](uint32_t c) {
+        const uint64_t base = X0 + ((uint64_t)(c * 128u) << row_shift(TYPE));
+        const uint32_t left = cols - c * 128u;
+        if (left >= 128u) {
 #pragma unroll
-        for (uint32_t k = 0; k < PER; ++k) {
-            const uint32_t i = tid + 256u * k, row = min(t0 + (i >> 4), n - 1u), at = c * 128u + 8u * (i & 15u);
-            const uint64_t p = X + (((uint64_t)row * xs + at) << row_shift(TYPE));
+            for (uint32_t k = 0; k < PER; ++k)
 #pragma unroll
-            for (int q = 0; q < RAW; ++q) raw[k][q] = gd_u32x4{0u, 0u, 0u, 0u};
-            if (at < cols)  // cols is a multiple of 32
+                for (int q = 0; q < RAW; ++q) raw[k][q] = gd_load<gd_u32x4_any>(base, from[k] + 16u * q);
+        } else {
 #pragma unroll
-                for (int q = 0; q < RAW; ++q) raw[k][q] = gd_at<const gd_u32x4_any>(p)[q];
+            for (uint32_t k = 0; k < PER; ++k)
+#pragma unroll
+                for (int q = 0; q < RAW; ++q) {
+                    raw[k][q] = gd_u32x4{0u, 0u, 0u, 0u};
+                    if (8u * (tid & 15u) < left) raw[k][q] = gd_load<gd_u32x4_any>(base, from[k] + 16u * q);
+                }
         }
     };
     auto store = [&](uint32_t buffer) {
@@ -77,14 +139,23 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds) {
         for (uint32_t k = 0; k < PER; ++k) {
             const uint32_t i = tid + 256u * k, row = i >> 4, at = row * 16u + ((i & 15u) ^ (row & 15u));
             gd_u32x4 *const out = lds + buffer * (UNITS * PARTS) + at;
+            float sum = 0.f;
             if constexpr (TYPE == ROW_F32) {
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = gd_bits_f32(raw[k][e >> 2][e & 3]);
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = gd_bits_f32(raw[k][e >> 2][e & 3]);
+                    sum += v[e];
+                }
                 mq_planes(v, PARTS, [&](uint32_t p, gd_u32x4 w) { out[p * UNITS] = w; });
             } else {
                 out[0] = raw[k][0];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = mm_pair<HALF>(raw[k][0][e], sum);
             }
+            sum += mm_dpp<0xb1>(sum);  // lanes ^ 1
+            sum += mm_dpp<0x4e>(sum);  // lanes ^ 2: the group's four units
+            if ((i & 3u) == 0u) sums[(buffer * 4u + ((i & 15u) >> 2)) * SUMS + row] = sum;
         }
     };
 
@@ -103,61 +174,70 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds) {
             fetch(c + 1u);
             load(c + 1u, next);
         }
+        const uint32_t buffer = c & 1u;
+        const gd_u32x4 *const xl = lds + buffer * (UNITS * PARTS);
+        gd_u32x4 x[T][PARTS];
+        auto operand = [&](uint32_t j, int t) {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) x[t][p] = xl[p * UNITS + (t * 16u + col) * 16u + ((4u * j + h) ^ col)];
+        };
+#pragma unroll
+        for (int t = 0; t < T; ++t) operand(0, t);
+        float sum[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t) sum[t] = sums[(buffer * 4u + h) * SUMS + t * 16u + col];
 #pragma unroll
         for (int r = 0; r < MM_R; ++r) {
-            cur[r].s = mq_spread(cur[r].s, spread);
-            if constexpr (MINIMA) cur[r].m = mq_spread(cur[r].m, spread);
-        }
-        const gd_u32x4 *const xl = lds + (c & 1u) * (UNITS * PARTS);
+            // Of the scale and minimum of this lane's row and group h of 32.
+            const uint32_t g = h / SPAN, from = 16u * (g & 1u);
+            const uint32_t sw = SPAN == 1 && (g & 2u) ? cur[r].s[SPAN == 1] : cur[r].s[0];
+            const uint32_t mw = SPAN == 1 && (g & 2u) ? cur[r].m[SPAN == 1] : cur[r].m[0];
+            const float coefficient = of_scale * gd_half(sw >> from & 0xffffu) + of_minimum * gd_half(mw >> from & 0xffffu);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            __builtin_amdgcn_sched_barrier(0);  // one group at a time: four at once take more registers than there are
-            gd_u32x4 x[T][PARTS];
-            gd_f32x4 corr[T];
+            for (int t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[t], coefficient, acc[r][t], 0, 0, 0);
+        }
+        // A step is a tile's products with 32 columns. Beside them run the unpacking of the next step's weights, the scaling
+        // of the step's before and, in a column group's last step, the reads of the next operands; the empty asm
+        // statements and the barriers keep each where it is written, the group barriers between the products.
+        gd_f32x4 d[SPAN == 1 ? 2 : MM_R][T];
+        auto scale = [&](int r, uint32_t j) {
+            const uint32_t g = j / SPAN;
+            const float s = gd_half(cur[r].s[g >> 1] >> (16u * (g & 1u)) & 0xffffu);
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                corr[t] = zero;
 #pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p) {  // the smallest part first
-                    x[t][p] = xl[p * UNITS + (t * 16u + col) * 16u + ((4u * j + h) ^ col)];
-                    corr[t] = mm_mfma<HALF>(x[t][p], unbias, corr[t]);
-                }
+                for (int i = 0; i < 4; ++i) acc[r][t][i] += s * d[SPAN == 1 ? r & 1 : r][t][i];
+                asm volatile("" : "+v"(acc[r][t]));
             }
-            // A tile's sums are scaled while the next tile's products run.
-            gd_f32x4 d[2][T];
-            auto scale = [&](int r) {
-                const float s = mq_half(cur[r].s, j);
+        };
+        gd_u32x4 w = mq_weights<HALF>(cur[0].w[0], bits);
 #pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[r][t][i] += s * d[r & 1][t][i];
-                if constexpr (MINIMA) {  // m sum x, corr being -16 sum x
-                    const float m = mq_half(cur[r].m, j) * -0.0625f;
-#pragma unroll
-                    for (int t = 0; t < T; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[r][t][i] += m * corr[t][i];
-                }
-                // Now, not at the end of the chunk, which would keep the products of all its groups.
-#pragma unroll
-                for (int t = 0; t < T; ++t) asm volatile("" : "+v"(acc[r][t]));
-            };
-#pragma unroll
-            for (int r = 0; r < MM_R; ++r) {
-                uint32_t word = cur[r].w[j];
-                asm volatile("" : "+v"(word));  // unpacked here and not all of a chunk ahead
-                const gd_u32x4 w = mq_weights<HALF>(word, bits);
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    d[r & 1][t] = corr[t];
-#pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p) d[r & 1][t] = mm_mfma<HALF>(x[t][p], w, d[r & 1][t]);
-                }
-                if (r) scale(r - 1);
-                __builtin_amdgcn_sched_barrier(0);
+        for (uint32_t k = 0; k < 4u * MM_R; ++k) {
+            const uint32_t j = k / MM_R, r = k % MM_R, jn = (k + 1u) / MM_R, rn = (k + 1u) % MM_R;
+            const bool first = j % SPAN == 0;
+            const int at = SPAN == 1 ? r & 1 : r;
+            gd_u32x4 wn = w;
+            if (jn < 4u) {
+                asm volatile("" : "+v"(cur[rn].w));
+                wn = mq_weights<HALF>(cur[rn].w[jn], bits);
             }
-            scale(MM_R - 1);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                gd_f32x4 v = first ? zero : d[at][t];
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; --p) v = mm_mfma<HALF>(x[t][p], w, v);  // the smallest part first
+                d[at][t] = v;
+                if (r == MM_R - 1 && jn < 4u) operand(jn, t);
+            }
+            if (jn < 4u) asm volatile("" : "+v"(wn));
+            const bool scales_one = r ? j % SPAN == SPAN - 1 : j && j % SPAN == 0;
+            if (scales_one) scale(r ? r - 1 : MM_R - 1, r ? j : j - 1u);
+            w = wn;
+            if (scales_one) mm_interleave<T * PARTS, 8 + 4 * T>();
+            else mm_interleave<T * PARTS, 8>();
+            __builtin_amdgcn_sched_barrier(0);
         }
+        scale(MM_R - 1, 3u);
         if (more) {
             store((c + 1u) & 1u);  // its readers passed the barrier above
 #pragma unroll
@@ -193,14 +273,15 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds) {
     }
 }
 
-template <uint32_t TYPE, bool MINIMA>
+template <uint32_t TYPE, int SPAN>
 __device__ __forceinline__ void mm_q4_body(const GdArgs &a) {
     constexpr int MOST = TYPE == ROW_F32 ? 3 : 4;  // two groups share a CU's LDS and registers
     __shared__ __align__(16) gd_u32x4 lds[2 * 16 * MOST * 16 * (TYPE == ROW_F32 ? 3 : 1)];
+    __shared__ float sums[2 * 4 * (16 * MOST + 16)];
     switch (a.c[26]) {
-        case 1: return mm_q4_tile<TYPE, MINIMA, 1>(a, lds);
-        case 2: return mm_q4_tile<TYPE, MINIMA, 2>(a, lds);
-        case 3: return mm_q4_tile<TYPE, MINIMA, 3>(a, lds);
-        default: return mm_q4_tile<TYPE, MINIMA, MOST>(a, lds);
+        case 1: return mm_q4_tile<TYPE, SPAN, 1>(a, lds, sums);
+        case 2: return mm_q4_tile<TYPE, SPAN, 2>(a, lds, sums);
+        case 3: return mm_q4_tile<TYPE, SPAN, 3>(a, lds, sums);
+        default: return mm_q4_tile<TYPE, SPAN, MOST>(a, lds, sums);
     }
 }

@@ -1,0 +1,3 @@
+// 4-bit products of many bf16 tokens, groups of 64 (mm_q4.h).
+#include "mm_q4.h"
+GD_PIPELINE_NAMED_OCC(mm_q4_b64, 256, 2) { mm_q4_body<ROW_BF16, 2>(a); }

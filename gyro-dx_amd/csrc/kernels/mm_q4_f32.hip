@@ -1,0 +1,3 @@
+// 4-bit products of many fp32 tokens, groups of 32 (mm_q4.h).
+#include "mm_q4.h"
+GD_PIPELINE_NAMED_OCC(mm_q4_f32, 256, 2) { mm_q4_body<ROW_F32, 1>(a); }

@@ -47,9 +47,9 @@ __device__ __forceinline__ void mv_q4_body(const GdArgs &a) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const uint64_t unit = (uint64_t)min((run * WR + rg) * R + r, tiles - 1u) * chunks + c;
-            o[r].w = gd_at<const gd_u32x4>(quants)[unit * 64u + lane];
-            o[r].s = mq_scales(scales, unit * 16u + col, lg);
-            if constexpr (MINIMA) o[r].m = mq_scales(minima, unit * 16u + col, lg);
+            o[r].w = gd_load<gd_u32x4>(quants + unit * 1024u, lane * 16u);
+            o[r].s = mq_scales(scales + (unit << (12u - lg)), col, lg);
+            if constexpr (MINIMA) o[r].m = mq_scales(minima + (unit << (12u - lg)), col, lg);
         }
     };
     // The next chunk of this wave, of this run or the next, is in flight while one is multiplied; the first while

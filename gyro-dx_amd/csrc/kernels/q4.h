@@ -6,7 +6,8 @@
 // operand, itself the product of the activations with a constant matrix, so nothing of the group's sum is kept
 // apart, and it is at most five times what the group's own product rounds at. Group sums are scaled and added
 // in fp32. Activations are exact: an fp32 value is the sum of three bf16 values (its 24 bits cut in eights).
-// A token with an infinity or NaN gets NaN in every output.
+// Of a token with an infinity or NaN no output is finite: every group's product and sum with it are not, and no scale
+// makes them so.
 //
 // Constants: 0 quants 2 scales 4 minima (0: none) 6 tiles 7 chunks 8 log2(group) 9 cols 10 outputs per token
 // 11 gated pair 12 x 14 x stride 16 x type 17 tokens 18 y 20 y stride 22 y type 23 act (0 none, 1 silu, 2
@@ -64,8 +65,8 @@ struct MqChunk {
 };
 typedef gd_u32x2 gd_u32x2_any __attribute__((aligned(2)));
 // The 8 bytes at a row's scales of a chunk: 4, 2 or 1 of them are its own (128 / group), the buffer has room for the rest.
-__device__ __forceinline__ gd_u32x2 mq_scales(uint64_t base, uint64_t row, uint32_t lg) {
-    return gd_at<const gd_u32x2_any>(base + (row << (8u - lg)))[0];
+__device__ __forceinline__ gd_u32x2 mq_scales(uint64_t base, uint32_t row, uint32_t lg) {
+    return gd_load<gd_u32x2_any>(base, row << (8u - lg));
 }
 // Of those, the scale of each group of 32, by the bytes that `even` and `odd` choose.
 struct MqSpread {

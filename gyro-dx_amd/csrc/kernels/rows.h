@@ -16,6 +16,12 @@ __device__ __forceinline__ uint64_t gd_addr(const GdArgs &a, int w) { return (ui
 template <typename T>
 __device__ __forceinline__ gd_gptr<T> gd_at(uint64_t address) { return (gd_gptr<T>)(uintptr_t)address; }
 
+// The T at `offset` bytes past a wave-uniform address: scalar base, 32-bit vector offset.
+template <typename T>
+__device__ __forceinline__ T gd_load(uint64_t base, uint32_t offset) {
+    return *(gd_gptr<const T>)(gd_at<const char>(base) + offset);
+}
+
 __device__ __forceinline__ uint32_t row_shift(uint32_t type) { return type == ROW_F32 ? 2u : 1u; }
 
 // fp32 bits of the 16-bit value h of type bf16 or binary16.

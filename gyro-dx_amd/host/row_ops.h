@@ -135,6 +135,7 @@ class RowOps {
         if (!n) return l;  // of no rows there may be no memory
         check_rows(x, n, m.cols, false, "gm_linear: x");
         check_rows(y, n, m.rows, true, "gm_linear: y");
+        require(x.stride <= 1u << 24, "gm_linear: x's rows are at most 2^24 values apart");
         require(act <= GM_ACT_SIGMOID && (!m.gated || act == GM_ACT_NONE), "gm_linear: act");
         require(n <= 1u << 18, "gm_linear takes at most 2^18 tokens");
         Constants &c = l.c;
@@ -160,7 +161,9 @@ class RowOps {
         const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u;
         const char *em = getenv("MM"); 
         if (em ? em[0] == '1' : n > per) {
-            static const char *const names[2][3] = {{"mm_q4_f", "mm_q4_b", "mm_q4_h"}, {"mm_q4_fm", "mm_q4_bm", "mm_q4_hm"}};
+            static const char *const names[3][3] = {{"mm_q4_f32", "mm_q4_f64", "mm_q4_f128"},
+                                                    {"mm_q4_b32", "mm_q4_b64", "mm_q4_b128"},
+                                                    {"mm_q4_h32", "mm_q4_h64", "mm_q4_h128"}};
             uint32_t best = 1, cost = ~0u;
             for (uint32_t t = 1; t <= (x.type == GM_F32 ? 3u : 4u); ++t) {
                 const uint32_t k = (n + 16 * t - 1) / (16 * t) * (28 + 16 * t);
@@ -171,7 +174,7 @@ class RowOps {
             }
             const char *et = getenv("MMT"); if (et) best = atoi(et);
             c.set(26, best);
-            l.kernel = names[m.mins ? 1 : 0][x.type];
+            l.kernel = names[x.type][m.lg - 5];
             l.x = (m.tiles + 15) / 16;
             l.y = (n + 16 * best - 1) / (16 * best);
             return l;

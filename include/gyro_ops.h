@@ -54,8 +54,9 @@ GM_API int gm_add_matrix(gm_engine *e, const gm_matrix_desc *desc, uint32_t *out
 GM_API int gm_release_matrix(gm_engine *e, uint32_t matrix);
 /* y[t] = act(scale W x[t]) for n tokens, x [n][cols], y [n][rows]; with accumulate, the sum is added to y
  * (after act, in fp32). A gated pair: y[t] = scale silu(G x[t]) * (U x[t]), act GM_ACT_NONE. Activations and sums
- * are fp32 whatever the types (products are exact in them); y is rounded once. A token with an activation that is
- * not finite gets NaN in all its outputs. y must not overlap x. */
+ * are fp32 whatever the types (products are exact in them); y is rounded once. Of a token with an
+ * activation that is not finite no output is (a NaN or an infinity). x's rows are at most 2^24
+ * values apart, n at most 2^18; y must not overlap x. */
 enum { GM_ACT_NONE = 0, GM_ACT_SILU = 1, GM_ACT_SIGMOID = 2 };
 GM_API int gm_linear(gm_engine *e, uint32_t matrix, const gm_rows *x, uint32_t n, const gm_rows *y, uint32_t act,
                      uint32_t accumulate, float scale, void *stream);

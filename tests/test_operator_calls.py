@@ -122,7 +122,7 @@ def test_linear_refusals(shim):
     assert ok(x=rows(stride=0))[0] == 0 and ok(y=rows(stride=0), n=1)[0] == 0
     for bad in (dict(x=rows(data=None)), dict(y=rows(data=None)), dict(x=rows(type=3)), dict(y=rows(type=7)),
                 dict(x=rows(data=A + 2)), dict(y=rows(type=1, data=A + 1)), dict(y=rows(stride=63)), dict(act=3),
-                dict(d=g, act=1), dict(n=(1 << 18) + 1), dict(x=rows(stride=1 << 41))):
+                dict(d=g, act=1), dict(n=(1 << 18) + 1), dict(x=rows(stride=1 << 41)), dict(x=rows(stride=(1 << 24) + 1)), dict(y=rows(stride=1 << 41))):
         rc, why, *_ = ok(**bad)
         assert rc < 0 and why, bad
 
