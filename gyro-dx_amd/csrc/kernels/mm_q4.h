@@ -3,8 +3,8 @@
 // A group of four waves takes 16 tiles (256 weight rows), four to a wave, and 16 T tokens. Chunks of 128 columns of the
 // tokens go through LDS as operands, two buffers in turn, one being filled while the other is multiplied; weights
 // go from memory to registers, a chunk ahead. Of 32 columns a wave unpacks 4 operands, each used for T products
-// of 16 + q; a scale's products (SPAN groups of 32) add up in the matrix unit before they are scaled into the sums, 16 T /
-// SPAN vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much and the minimum,
+// of 16 + q; where two groups of 32 share a scale their products add up in the matrix unit before they are scaled into
+// the sums, 16 T (or 8 T) vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much and the minimum,
 // (m - 16 s) sum x (or -24 s sum x), is a product of its own: of the chunk's four sums of 32 activations, which come
 // with the staging, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens are operands as they are; fp32 ones
 // go through the products three times, a part each.
@@ -72,6 +72,8 @@ template <uint32_t TYPE, int SPAN, int T>
 __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float *sums) {
     constexpr bool HALF = TYPE == ROW_F16;
     constexpr int PARTS = TYPE == ROW_F32 ? 3 : 1;
+    // Groups of 32 that are scaled together (fp32 tokens' operands leave no registers for a second one's).
+    constexpr uint32_t PAIR = SPAN == 1 || PARTS > 1 ? 1u : 2u;
     constexpr uint32_t ROWS = 16u * T, UNITS = ROWS * 16u, PER = UNITS / 256u;  // 16-byte units of a chunk, of a thread
     constexpr uint32_t SUMS = ROWS + 16u;  // a group's row of sums, the four groups' in different banks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, h = lane >> 4;
@@ -176,13 +178,15 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
         }
         const uint32_t buffer = c & 1u;
         const gd_u32x4 *const xl = lds + buffer * (UNITS * PARTS);
-        gd_u32x4 x[T][PARTS];
+        gd_u32x4 x[PAIR][T][PARTS];
         auto operand = [&](uint32_t j, int t) {
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) x[t][p] = xl[p * UNITS + (t * 16u + col) * 16u + ((4u * j + h) ^ col)];
+            for (int p = 0; p < PARTS; ++p) x[j % PAIR][t][p] = xl[p * UNITS + (t * 16u + col) * 16u + ((4u * j + h) ^ col)];
         };
 #pragma unroll
-        for (int t = 0; t < T; ++t) operand(0, t);
+        for (uint32_t j = 0; j < PAIR; ++j)
+#pragma unroll
+            for (int t = 0; t < T; ++t) operand(j, t);
         float sum[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) sum[t] = sums[(buffer * 4u + h) * SUMS + t * 16u + col];
@@ -196,26 +200,26 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
 #pragma unroll
             for (int t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[t], coefficient, acc[r][t], 0, 0, 0);
         }
-        // A step is a tile's products with 32 columns. Beside them run the unpacking of the next step's weights, the scaling
-        // of the step's before and, in a column group's last step, the reads of the next operands; the empty asm
-        // statements and the barriers keep each where it is written, the group barriers between the products.
-        gd_f32x4 d[SPAN == 1 ? 2 : MM_R][T];
+        // A step is a tile's products with 32 columns; a tile takes PAIR of them, whose sums are scaled together, before
+        // the next tile. Beside a step run the unpacking of the next one's weights, the scaling of the tile before and,
+        // in the last tile's, the reads of the next operands; the empty asm statements and the barriers keep each where
+        // it is written, the group barriers between the products.
+        gd_f32x4 d[2][T];
         auto scale = [&](int r, uint32_t j) {
             const uint32_t g = j / SPAN;
             const float s = gd_half(cur[r].s[g >> 1] >> (16u * (g & 1u)) & 0xffffu);
 #pragma unroll
             for (int t = 0; t < T; ++t) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[r][t][i] += s * d[SPAN == 1 ? r & 1 : r][t][i];
+                for (int i = 0; i < 4; ++i) acc[r][t][i] += s * d[r & 1][t][i];
                 asm volatile("" : "+v"(acc[r][t]));
             }
         };
         gd_u32x4 w = mq_weights<HALF>(cur[0].w[0], bits);
 #pragma unroll
         for (uint32_t k = 0; k < 4u * MM_R; ++k) {
-            const uint32_t j = k / MM_R, r = k % MM_R, jn = (k + 1u) / MM_R, rn = (k + 1u) % MM_R;
-            const bool first = j % SPAN == 0;
-            const int at = SPAN == 1 ? r & 1 : r;
+            const uint32_t g = k / (PAIR * MM_R), r = k / PAIR % MM_R, e = k % PAIR, j = g * PAIR + e;
+            const uint32_t gn = (k + 1u) / (PAIR * MM_R), rn = (k + 1u) / PAIR % MM_R, jn = gn * PAIR + (k + 1u) % PAIR;
             gd_u32x4 wn = w;
             if (jn < 4u) {
                 asm volatile("" : "+v"(cur[rn].w));
@@ -223,14 +227,14 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
             }
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                gd_f32x4 v = first ? zero : d[at][t];
+                gd_f32x4 v = e ? d[r & 1][t] : zero;
 #pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p) v = mm_mfma<HALF>(x[t][p], w, v);  // the smallest part first
-                d[at][t] = v;
-                if (r == MM_R - 1 && jn < 4u) operand(jn, t);
+                for (int p = PARTS - 1; p >= 0; --p) v = mm_mfma<HALF>(x[e][t][p], w, v);  // the smallest part first
+                d[r & 1][t] = v;
+                if (r == MM_R - 1 && j + PAIR < 4u) operand(j + PAIR, t);
             }
             if (jn < 4u) asm volatile("" : "+v"(wn));
-            const bool scales_one = r ? j % SPAN == SPAN - 1 : j && j % SPAN == 0;
+            const bool scales_one = e == 0 && k;
             if (scales_one) scale(r ? r - 1 : MM_R - 1, r ? j : j - 1u);
             w = wn;
             if (scales_one) mm_interleave<T * PARTS, 8 + 4 * T>();
@@ -244,39 +248,39 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
             for (int r = 0; r < MM_R; ++r) cur[r] = next[r];
         }
     }
-    // Sums go out through LDS, 16 tokens at a time, as runs of 64 neighbouring outputs (32 of a gated pair): row r of
-    // token k at k * 68 + r (the four tokens of a lane's quarter write to different banks).
+    // Sums go out through LDS as runs of 64 neighbouring outputs (32 of a gated pair), four to a lane: row r of token k at
+    // k * 68 + r (the four tokens of a lane's quarter write to different banks).
     __syncthreads();
-    const MqOut y = mq_out(a);
-    float *const out = reinterpret_cast<float *>(lds) + wave * (16u * 68u);
-    const uint32_t width = y.gated ? 32u : 64u, orow = lane & (width - 1u);
-    const uint64_t first = (uint64_t)tile0 * 16u / (64u / width);
+    float *const out = reinterpret_cast<float *>(lds) + wave * (ROWS * 68u);
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int r = 0; r < MM_R; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[(4u * h + i) * 68u + 16u * r + col] = acc[r][t][i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+            for (int i = 0; i < 4; ++i) out[(16u * t + 4u * h + i) * 68u + 16u * r + col] = acc[r][t][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const MqOut y = mq_out(a);
+    const uint32_t lanes = y.gated ? 8u : 16u, o4 = (lane & (lanes - 1u)) * 4u;  // lanes of a token's run
+    const uint64_t first = (uint64_t)tile0 * 16u / (y.gated ? 2u : 1u) + o4;
+    if (first >= outputs) return;
+    const uint32_t count = (uint32_t)min((uint64_t)outputs - first, (uint64_t)4u);
+    // A gated pair's rows: 16 of gate, then 16 of up, and so on.
+    const float *const mine = out + (y.gated ? (o4 & 15u) + 32u * (o4 >> 4) : o4);
 #pragma unroll 1
-        for (uint32_t k = lane / width; k < 16u; k += 64u / width) {
-            const uint32_t token = t0 + 16u * t + k;
-            if (token >= n) break;
-            if (first + orow >= outputs) continue;
-            // A gated pair's rows: 16 of gate, then 16 of up, and so on.
-            const float *const at = out + k * 68u + (y.gated ? (orow & 15u) + 32u * (orow >> 4) : orow);
-            mq_store(y, token, first + orow, at[0], at[y.gated ? 16 : 0]);
-        }
+    for (uint32_t k = lane / lanes; k < min(ROWS, n - t0); k += 64u / lanes) {
+        const gd_f32x4 v = *reinterpret_cast<const gd_f32x4 *>(mine + k * 68u);
+        const gd_f32x4 up = *reinterpret_cast<const gd_f32x4 *>(mine + k * 68u + (y.gated ? 16 : 0));
+        mq_store4(y, t0 + k, first, count, v, up);
     }
 }
 
 template <uint32_t TYPE, int SPAN>
 __device__ __forceinline__ void mm_q4_body(const GdArgs &a) {
-    constexpr int MOST = TYPE == ROW_F32 ? 3 : 4;  // two groups share a CU's LDS and registers
-    __shared__ __align__(16) gd_u32x4 lds[2 * 16 * MOST * 16 * (TYPE == ROW_F32 ? 3 : 1)];
+    // Two groups share a CU's registers and LDS: two buffers of a chunk's operands, then the sums of four waves.
+    constexpr int MOST = TYPE == ROW_F32 ? 3 : 4;
+    constexpr uint32_t OPERANDS = 2 * 16 * MOST * 16 * (TYPE == ROW_F32 ? 3 : 1), OUT = MM_WAVES * 16 * MOST * 68 / 4;
+    __shared__ __align__(16) gd_u32x4 lds[OPERANDS > OUT ? OPERANDS : OUT];
     __shared__ float sums[2 * 4 * (16 * MOST + 16)];
     switch (a.c[26]) {
         case 1: return mm_q4_tile<TYPE, SPAN, 1>(a, lds, sums);

@@ -89,16 +89,37 @@ struct MqOut {
 __device__ __forceinline__ MqOut mq_out(const GdArgs &a) {
     return {gd_addr(a, 18), gd_addr(a, 20), a.c[22], a.c[23], a.c[24], a.c[11], gd_bits_f32(a.c[25])};
 }
+__device__ __forceinline__ float mq_value(const MqOut &o, float sum, float up) {
+    // x rcp(1 + e^-x): within two units of the last place of the division's result.
+    if (o.gated) return o.scale * (sum * __builtin_amdgcn_rcpf(1.0f + expf(-sum)) * up);
+    float v = o.scale * sum;
+    if (o.act == 1u) v = v * __builtin_amdgcn_rcpf(1.0f + expf(-v));
+    else if (o.act == 2u) v = __builtin_amdgcn_rcpf(1.0f + expf(-v));
+    return v;
+}
 __device__ __forceinline__ void mq_store(const MqOut &o, uint32_t t, uint64_t out, float sum, float up) {
-    float v;
-    if (o.gated) {
-        v = o.scale * (gd_silu_accurate(sum) * up);
-    } else {
-        v = o.scale * sum;
-        if (o.act == 1u) v = gd_silu_accurate(v);
-        else if (o.act == 2u) v = gd_sigmoid_accurate(v);
-    }
+    float v = mq_value(o, sum, up);
     const uint64_t at = (uint64_t)t * o.stride + out;
     if (o.add) v += row_load(o.y, at, o.type);
     row_store(o.y, at, o.type, v);
+}
+// Four neighbouring outputs, the first `count` of them.
+__device__ __forceinline__ void mq_store4(const MqOut &o, uint32_t t, uint64_t out, uint32_t count, gd_f32x4 sum, gd_f32x4 up) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mq_value(o, sum[i], up[i]);
+    const uint64_t at = (uint64_t)t * o.stride + out;
+    if (o.add)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] += i < count ? row_load(o.y, at + i, o.type) : 0.f;
+    if (count < 4u) {
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i)
+            if (i < count) row_store(o.y, at + i, o.type, v[i]);
+    } else if (o.type == ROW_F32) {
+        gd_at<gd_f32x4_any>(o.y + 4u * at)[0] = gd_f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+        gd_at<gd_u32x2_any>(o.y + 2u * at)[0] = gd_u32x2{row_bits16(v[0], o.type) | row_bits16(v[1], o.type) << 16,
+                                                         row_bits16(v[2], o.type) | row_bits16(v[3], o.type) << 16};
+    }
 }

@@ -1,5 +1,6 @@
 // The operators around the MoE layers (gm_linear, gm_block_norm, gm_logprobs): argument checks, the choice of a
-// build, its constants and grid. The engine launches what they return. Their kernels (csrc/kernels/mv_q4.h, block_norm.h, logprobs.hip) take every address
+// build, its constants and grid. The engine launches what they return. Their kernels (csrc/kernels/q4.h, block_norm.h,
+// logprobs.h) take every address
 // in the launch's constants, so a call needs no table entry and may be captured.
 #pragma once
 #include <algorithm>
@@ -158,35 +159,43 @@ class RowOps {
         c.set(23, act);
         c.set(24, accumulate ? 1u : 0u);
         c.set(25, scale);
-        const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u;
-        const char *em = getenv("MM"); 
-        if (em ? em[0] == '1' : n > per) {
+        // Tokens that share a pass of mv_q4 over the weights.
+        const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u, passes = (n + per - 1) / per;
+        // mm_q4's few large groups take 1.0 to 1.3 us a chunk however little there is to do; mv_q4's time grows with tiles
+        // and passes. They meet near (fp32, binary16, bf16) 14, 11 and 9 tile passes per compute unit. us at 2048
+        // columns, mv / mm: 2048 rows of 64 and 512 fp32 tokens 16.1 / 26.4 and 88.0 / 29.9, 8192 rows of 17 and 64
+        // 16.2 / 26.0 and 46.7 / 27.2, 8192 rows of 64 and 128 bf16 tokens 20.5 / 22.3 and 37.0 / 23.6.
+        static const uint32_t meet[] = {14, 9, 11};
+        if (passes > 1 && (uint64_t)m.tiles * passes > (uint64_t)meet[x.type] * cus) {
             static const char *const names[3][3] = {{"mm_q4_f32", "mm_q4_f64", "mm_q4_f128"},
                                                     {"mm_q4_b32", "mm_q4_b64", "mm_q4_b128"},
                                                     {"mm_q4_h32", "mm_q4_h64", "mm_q4_h128"}};
-            uint32_t best = 1, cost = ~0u;
+            // 16 T tokens to a group: the fewest rounds of two groups per unit, by a step's vector instructions.
+            uint32_t tokens = 16;
+            uint64_t cost = ~0ull;
+            const uint32_t blocks = (m.tiles + 15) / 16;
             for (uint32_t t = 1; t <= (x.type == GM_F32 ? 3u : 4u); ++t) {
-                const uint32_t k = (n + 16 * t - 1) / (16 * t) * (28 + 16 * t);
+                const uint64_t groups = (uint64_t)blocks * ((n + 16 * t - 1) / (16 * t));
+                const uint64_t k = (groups + 2 * cus - 1) / (2 * cus) * (28 + 16 * t);
                 if (k <= cost) {
                     cost = k;
-                    best = t;
+                    tokens = 16 * t;
                 }
             }
-            const char *et = getenv("MMT"); if (et) best = atoi(et);
-            c.set(26, best);
+            c.set(26, tokens / 16);
             l.kernel = names[x.type][m.lg - 5];
-            l.x = (m.tiles + 15) / 16;
-            l.y = (n + 16 * best - 1) / (16 * best);
+            l.x = blocks;
+            l.y = (n + tokens - 1) / tokens;
             return l;
         }
+        // Waves that share a tile's columns: as few as leave every unit its 16 waves.
         uint32_t wk = 1;
         while (wk < 8 && wk * 2 <= m.chunks && m.tiles / 2 * wk < 16 * cus) wk *= 2;
         c.set(26, wk);
-        const char *ew = getenv("MQW"); if (ew) { wk = atoi(ew); c.set(26, wk); }
         const uint32_t run = 2 * (8 / wk), runs = (m.tiles + run - 1) / run;
         l.kernel = m.mins ? "mv_q4_m" : "mv_q4";
         l.x = std::min(runs, 2 * cus);
-        l.y = (n + per - 1) / per;
+        l.y = passes;
         return l;
     }
 

@@ -6,7 +6,8 @@ Tolerances. linear: with small integers as activations, powers of two as scales 
 partial sum is a multiple of 1/4 below 2^22, so the result is exact in fp32 whatever the order. Otherwise a product goes
 through at most 32 + 32 roundings in a group's two matrix products, one per group after that and 12 where slices and
 parts meet, each of at most a unit of fp32's last place of a partial sum of at most 55 |s| sum |x| + |m| sum |x| (q + 16
-plus 24): (76 + groups) 2^-23 of their total. block_norm: a sum of at most 16384 squares (64 adds
+plus 24): (76 + groups) 2^-23 of their total. Where the corrections are added to the sums, in fours, that is at most
+two more a group, for roundings of half as much: within the same. block_norm: a sum of at most 16384 squares (64 adds
 per lane and 10 across them, halved by the root) and at most 24 roundings: 64 2^-24 of each term. logprobs: S sums V
 positive terms, at most V / 256 + 32 in a row, each term within 4 2^-24 (1 + |d|); z, m and log S round once each.
 Outputs in 16 bits add half a step of their type."""
@@ -109,6 +110,60 @@ def test_linear(eng, rows, cols, n, fmt, group, mins, xt, yt, gated):
     eng.release_matrix(index)
 
 
+# Shapes whose products take the many-token kernels, by 16, 32, 48 and 64 tokens a group (test_operator_calls.py).
+MANY = [(40000, 1, 12), (100003, 1, 30), (100003, 1, 45), (100003, 1, 64), (8000, 3, 1000), (8000, 5, 500), (8000, 3, 700)]
+
+
+@pytest.mark.parametrize("fmt,group,mins", FORMATS)
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+def test_linear_many_tokens_exact(eng, fmt, group, mins, x):
+    rng = np.random.default_rng(7 * group + len(fmt) + ord(x[0]))
+    for rows, groups, n in MANY:
+        n += 8 * (x == "bf16" and n == 12)
+        cols = groups * group
+        print(f"many tokens exact {fmt} group {group} mins {mins} x {x}: {rows} x {cols}, {n} tokens", flush=True)
+        index, ((_, W, _, _),) = add(eng, rng, fmt, rows, cols, group, mins, False, True)
+        xs = integers(rng, n, cols, x)
+        xd, _ = ref.wide_rows(xs, ref.DTYPES[x], pad=3, shift=1)
+        yd, buf = ref.wide_rows(torch.zeros(n, rows), torch.float32, pad=5, shift=3, fill=7.0)
+        eng.linear(index, xd, yd, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(yd.cpu().double(), xs @ W.T)
+        assert ref.untouched(buf, yd, 7.0)
+        eng.release_matrix(index)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "f16"), ("f16", "bf16")])
+@pytest.mark.parametrize("rows,cols,n,fmt,group,mins", [(20001, 640, 50, "q4_0", 32, False), (20001, 384, 70, "q4", 128, True),
+                                                        (6007, 1088, 200, "q4", 64, False), (30010, 96, 20, "q4_1", 32, True)])
+def test_linear_many_tokens(eng, rows, cols, n, fmt, group, mins, xt, yt, gated):
+    test_linear(eng, rows, cols, n, fmt, group, mins, xt, yt, gated)
+
+
+@pytest.mark.parametrize("yt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act", ["none", "silu", "sigmoid"])
+def test_linear_many_tokens_epilogue(eng, act, yt):
+    """Activation, scale and accumulation of the many-token kernels, rows not in fours, added to what y held."""
+    rng = np.random.default_rng(15)
+    rows, cols, n = 40003, 64, 33
+    index, ((_, W, _, _),) = add(eng, rng, "q4_0", rows, cols, 32, False, False, True)
+    xs = integers(rng, n, cols)
+    y0 = torch.from_numpy(rng.standard_normal((n, rows)))
+    for accumulate in (False, True):
+        yd, buf = ref.wide_rows(y0, ref.DTYPES[yt], pad=1, shift=1, fill=2.0)
+        held = yd.cpu().double()
+        eng.linear(index, xs.bfloat16().cuda(), yd, act=act, accumulate=accumulate, scale=0.03125, stream=stream())
+        z = 0.03125 * (xs @ W.T)
+        want = {"none": z, "silu": ref.silu(z), "sigmoid": torch.sigmoid(z)}[act]
+        part = want.abs() + z.abs() + 1
+        want = want + held if accumulate else want
+        err = (yd.cpu().double() - want).abs()
+        assert (err <= 8 * ULP * (part + want.abs()) + half_step(ref.DTYPES[yt]) * (want.abs() + 1e-6) + 1e-7 * (yt == "f16")).all()
+        assert ref.untouched(buf, yd, 2.0)
+    eng.release_matrix(index)
+
+
 @pytest.mark.parametrize("act", ["none", "silu", "sigmoid"])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_linear_epilogue(eng, act, accumulate):
@@ -153,14 +208,14 @@ def test_linear_broadcast_and_empty(eng):
     eng.release_matrix(index)
 
 
-@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("n,rows", [(3, 200), (40, 200), (40, 20000)])
 @pytest.mark.parametrize("xt", ["f32", "bf16", "f16"])
-def test_linear_nonfinite_token(eng, xt, n):
+def test_linear_nonfinite_token(eng, xt, n, rows):
     """Of a token with an infinity or a NaN no output is finite; the others keep their bits."""
     rng = np.random.default_rng(2)
-    index, _ = add(eng, rng, "q4", 200, 640, 64, True, False, False)
+    index, _ = add(eng, rng, "q4", rows, 640, 64, True, False, False)
     xs = torch.from_numpy(rng.standard_normal((n, 640))).to(ref.DTYPES[xt]).cuda()
-    clean, dirty = torch.zeros(n, 200, device="cuda"), torch.zeros(n, 200, device="cuda")
+    clean, dirty = torch.zeros(n, rows, device="cuda"), torch.zeros(n, rows, device="cuda")
     eng.linear(index, xs, clean, stream=stream())
     for value in (float("inf"), float("-inf"), float("nan")):
         xs[1, 333] = value
@@ -171,16 +226,16 @@ def test_linear_nonfinite_token(eng, xt, n):
     eng.release_matrix(index)
 
 
-@pytest.mark.parametrize("n", [4, 50])
+@pytest.mark.parametrize("n,rows", [(4, 64), (50, 64), (50, 20000)])
 @pytest.mark.parametrize("xt,sizes", [("f32", (1e-30, 1e-5, 1.0, 1e20)), ("bf16", (1e-30, 1e-5, 1e20)),
                                       ("f16", (1e-7, 1e-5, 1.0, 5000.0))])
-def test_linear_wide_range(eng, xt, sizes, n):
+def test_linear_wide_range(eng, xt, sizes, n, rows):
     """Activations keep all their bits, at any size: fp32's 24, binary16's below its normal range."""
     rng = np.random.default_rng(3)
-    index, (mats,) = add(eng, rng, "q4_0", 64, 256, 32, False, False, False)
+    index, (mats,) = add(eng, rng, "q4_0", rows, 256, 32, False, False, False)
     for size in sizes:
         x = torch.from_numpy(rng.standard_normal((n, 256)) * size).to(ref.DTYPES[xt])
-        yd = torch.zeros(n, 64, device="cuda")
+        yd = torch.zeros(n, rows, device="cuda")
         eng.linear(index, x.cuda(), yd, stream=stream())
         y = x.double() @ mats[1].T
         assert ((yd.cpu().double() - y).abs() <= linear_bound(mats, x.double(), 256, 32) + ULP * y.abs()).all()

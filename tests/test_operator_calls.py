@@ -136,6 +136,30 @@ def test_linear_grids(shim):
                 assert rc == 0 and 1 <= x <= 65535 and 1 <= y <= 65535, (r, c, type, n, why, x, y)
 
 
+def test_linear_builds(shim):
+    """Few tokens or few rows take mv_q4, many mm_q4 by 16 to 64 tokens a group (16 to 48 of fp32 ones)."""
+    def plan(r, c, type, n, fmt=0, group=32):
+        rc, why, x, y = call(shim.plan_linear, matrix(fmt, r, c, group), rows(type), n, rows(stride=r), 0, 0, 1.0)
+        out, why = (C.c_uint32 * 62)(), C.create_string_buffer(200)
+        m, a, b = matrix(fmt, r, c, group), rows(type), rows(stride=r)
+        assert shim.plan_linear(C.byref(m), C.byref(a), n, C.byref(b), 0, 0, 1.0, out, why) == 0
+        return why.value.decode(), out[2 + 26], x, y
+    assert plan(2048, 512, 0, 1)[0] == "mv_q4" and plan(2048, 512, 0, 1, 2, 128)[0] == "mv_q4"
+    for type in (0, 1, 2):
+        assert plan(131072, 2048, type, 1)[0] == "mv_q4" and plan(512, 2048, type, 64)[0] == "mv_q4"
+        for n in (12, 20, 30, 45, 64, 150, 1023):
+            name, t, x, y = plan(40000, 128, type, n, 2, 64)
+            if n > (5, 16, 8)[type]:
+                assert name == "mm_q4_" + "fbh"[type] + "64" and 1 <= t <= (3, 4, 4)[type]
+                assert x == 157 and y * 16 * t >= n > (y - 1) * 16 * t
+    tokens = [[plan(r, g, type, n, 2 if g > 32 else 0, g)[1] for r, n in
+               ((100003, 30), (100003, 45), (100003, 64), (8000, 1000), (8000, 500), (8000, 700))]
+              for type in (1, 2) for g in (32, 64, 128)]
+    assert all(t == [2, 3, 4, 4, 2, 3] for t in tokens), tokens
+    assert [plan(r, 64, 0, n)[1] for r, n in ((40000, 12), (100003, 30), (100003, 45), (8000, 1000), (8000, 700))] == [1, 2, 3, 2, 3]
+    assert plan(40000, 64, 1, 20)[0] == "mm_q4_b32" and plan(40000, 64, 2, 12)[0] == "mm_q4_h32"
+
+
 def norm(**kw):
     d = BlockNormDesc(E=100, post=0, h=rows(), x=rows(), out=rows(), normed=rows(), post_eps=1e-6, pre_eps=1e-6, scale=1.0)
     for k, v in kw.items():
