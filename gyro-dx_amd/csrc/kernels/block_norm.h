@@ -33,7 +33,7 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
     const float scale = gd_bits_f32(a.c[30]);
     const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.c[31]) return;
-    float v[STEPS][8], x[STEPS][8];
+    float v[STEPS][8], x[STEPS][8], w[STEPS][8];
     float ss = 0.f;
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
@@ -44,36 +44,52 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[k][j] = 0.f;
     }
+    // The factors of a beside its root: the post weight times the gate, while the sum of squares waits for h.
+    float factor = scale;
+    if (G && !channel) {
+        const float g = row_load(G, row * gs, gt);
+        factor *= sigmoid ? gd_sigmoid_accurate(g) : g;
+    }
+    auto factors = [&](int k) {
+        const uint32_t i = (k * 256u + threadIdx.x) * 8u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[k][j] = 1.f;
+        if (PW) row_load8(PW, i, E, ROW_F32, w[k]);
+        if (G && channel) {
+            float g[8];
+            row_load8(G + ((row * gs) << row_shift(gt)), i, E, gt, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[k][j] *= sigmoid ? gd_sigmoid_accurate(g[j]) : g[j];
+        }
+    };
+    auto pre_weights = [&](int k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[k][j] = 1.f;
+        if (NW) row_load8(NW, (k * 256u + threadIdx.x) * 8u, E, ROW_F32, w[k]);
+    };
+    constexpr bool AHEAD = STEPS <= 2;  // weights asked for before the sums they wait for, where registers allow it
     if (H) {
-        float r = scale;
+        if (AHEAD)
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) factors(k);
+        float r = factor;
         if (post) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss += v[k][j] * v[k][j];
-            r = scale / sqrtf(bn_group_sum(ss, part[0]) / (float)E + gd_bits_f32(a.c[28]));
-        }
-        if (G && !channel) {
-            const float g = row_load(G, row * gs, gt);
-            r *= sigmoid ? gd_sigmoid_accurate(g) : g;
+            r = factor / sqrtf(bn_group_sum(ss, part[0]) / (float)E + gd_bits_f32(a.c[28]));
         }
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
-            const uint32_t i = (k * 256u + threadIdx.x) * 8u;
-            float w[8], g[8];
+            if (!AHEAD) factors(k);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = g[j] = 1.f;
-            if (PW) row_load8(PW, i, E, ROW_F32, w);
-            if (G && channel) {
-                row_load8(G + ((row * gs) << row_shift(gt)), i, E, gt, g);
-                if (sigmoid)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] = gd_sigmoid_accurate(g[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[k][j] += v[k][j] * r * w[j] * g[j];
+            for (int j = 0; j < 8; ++j) x[k][j] += v[k][j] * r * w[k][j];
         }
     }
+    if (AHEAD && N)
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) pre_weights(k);
     if (O)
 #pragma unroll
         for (int k = 0; k < STEPS; ++k)
@@ -87,13 +103,9 @@ __device__ __forceinline__ void block_norm_body(const GdArgs &a) {
     const float r = 1.0f / sqrtf(bn_group_sum(ss, part[1]) / (float)E + gd_bits_f32(a.c[29]));
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
-        const uint32_t i = (k * 256u + threadIdx.x) * 8u;
-        float w[8];
+        if (!AHEAD) pre_weights(k);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = 1.f;
-        if (NW) row_load8(NW, i, E, ROW_F32, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] *= x[k][j] * r;
-        row_store8(N + ((row * ns) << row_shift(nt)), i, E, nt, w);
+        for (int j = 0; j < 8; ++j) w[k][j] *= x[k][j] * r;
+        row_store8(N + ((row * ns) << row_shift(nt)), (k * 256u + threadIdx.x) * 8u, E, nt, w[k]);
     }
 }

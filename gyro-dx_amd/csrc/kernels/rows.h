@@ -66,12 +66,24 @@ __device__ __forceinline__ void row_load8(uint64_t row, uint32_t i, float (&v)[8
         }
     }
 }
-// As before, of a type known at run time, those from `n` on as zeros.
+// As before, of a type known at run time, those from `n` on as zeros: a lane that reaches past the end reads the row's
+// last eight and moves them down.
 __device__ __forceinline__ void row_load8(uint64_t row, uint32_t i, uint32_t n, uint32_t type, float (&v)[8]) {
-    if (i + 8u <= n) {
-        if (type == ROW_F32) row_load8<ROW_F32>(row, i, v);
-        else if (type == ROW_BF16) row_load8<ROW_BF16>(row, i, v);
-        else row_load8<ROW_F16>(row, i, v);
+    if (n >= 8u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        if (i >= n) return;
+        const uint32_t at = min(i, n - 8u), past = i - at;
+        if (type == ROW_F32) row_load8<ROW_F32>(row, at, v);
+        else if (type == ROW_BF16) row_load8<ROW_BF16>(row, at, v);
+        else row_load8<ROW_F16>(row, at, v);
+        if (past) {
+#pragma unroll
+            for (uint32_t step = 4; step > 0; step >>= 1)
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j)
+                    if (past & step) v[j] = j + step < 8u ? v[(j + step) & 7u] : 0.f;
+        }
         return;
     }
 #pragma unroll

@@ -238,7 +238,7 @@ class RowOps {
         c.set(29, d.pre_eps);
         c.set(30, d.scale);
         c.set(31, n);
-        l.kernel = d.E <= 4096 ? "block_norm" : "block_norm_l";
+        l.kernel = d.E <= 2048 ? "block_norm_s" : d.E <= 4096 ? "block_norm" : "block_norm_l";
         l.x = std::min(n, 65535u);
         l.y = (uint32_t)(((uint64_t)n + 65534) / 65535);
         return l;
