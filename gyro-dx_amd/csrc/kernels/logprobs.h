@@ -56,6 +56,50 @@ __device__ __forceinline__ LpSums lp_wave_join(LpSums p, float scale) {
     return {p.m, gd_wave_sum_dpp(p.s), gd_wave_sum_dpp(p.t)};
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lp_dpp_max_step_u32(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
+}
+// The wave's largest, a scalar.
+__device__ __forceinline__ uint32_t lp_wave_max_u32(uint32_t v) {
+    v = lp_dpp_max_step_u32<0x111, 0xf>(v);
+    v = lp_dpp_max_step_u32<0x112, 0xf>(v);
+    v = lp_dpp_max_step_u32<0x114, 0xf>(v);
+    v = lp_dpp_max_step_u32<0x118, 0xf>(v);
+    v = lp_dpp_max_step_u32<0x142, 0xa>(v);
+    v = lp_dpp_max_step_u32<0x143, 0xc>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// The largest order u with reached(u) >= top, by its bits from the highest down to `lowest`, until reached(u) <= enough;
+// `count` becomes reached(u) (from `all`, of 0), and `above` what reaches more where the search went to the last bit.
+// The top of a row mostly lie within a factor of two, so the search starts below the exponent of the largest, `most`,
+// where `top` reach that.
+template <typename F>
+__device__ __forceinline__ uint32_t lp_search(F &&reached, uint32_t most, uint32_t top, uint32_t enough, uint32_t lowest,
+                                              uint32_t all, uint32_t &count, uint32_t &above) {
+    uint32_t at = most & 0xff800000u, bit = 0x00400000u;
+    count = reached(at);
+    above = 0;
+    if (count < top) {
+        above = count;
+        at = 0;
+        bit = 0x80000000u;
+        count = all;
+    }
+#pragma unroll 1
+    for (; bit >= lowest && count > enough; bit >>= 1) {
+        const uint32_t n = reached(at | bit);
+        if (n >= top) {
+            at |= bit;
+            count = n;
+        } else {
+            above = n;
+        }
+    }
+    return at;
+}
+
 // Order of a value: falling with it, NaNs above all, both zeros alike; never 0 nor ~0.
 __device__ __forceinline__ uint32_t lp_order(float x) {
     const uint32_t u = gd_f32_bits(x + 0.0f);
@@ -100,22 +144,20 @@ __device__ __forceinline__ uint32_t lp_cut(const uint64_t *list, uint32_t c, uin
     }
     lp_wave_sync();
     // The largest order that `top` reach, then, of those that equal it, the largest low word that the rest reach.
-    uint32_t at = 0, low = 0, count = c, above = 0;
-    for (uint32_t bit = 0x80000000u; bit && count != top; bit >>= 1) {
-        const uint32_t probe = at | bit;
-        uint32_t n = 0;
+    uint32_t low = 0, count, above, most = 0;
 #pragma unroll
-        for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
-            if (64u * r >= c) break;
-            n += __popcll(__ballot(hi[r] >= probe));
-        }
-        if (n >= top) {
-            at = probe;
-            count = n;
-        } else {
-            above = n;  // at the end, what is above `at`
-        }
-    }
+    for (uint32_t r = 0; r < LP_LIST / 64; ++r) most = max(most, hi[r]);
+    const uint32_t at = lp_search(
+        [&](uint32_t probe) {
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < LP_LIST / 64; ++r) {
+                if (64u * r >= c) break;
+                n += __popcll(__ballot(hi[r] >= probe));
+            }
+            return n;
+        },
+        lp_wave_max_u32(most), top, top, 1u, c, count, above);
     for (uint32_t bit = 0x80000000u; bit && count != top; bit >>= 1) {
         const uint32_t probe = low | bit;
         uint32_t n = above;
@@ -179,27 +221,33 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
         }
         // A lower bound of the batch's top-th value from the maxima of 8, by their leading bits: up to 16, fewer where
         // no more than 8 maxima too many reach it.
-        uint32_t order[4], leading = 0, count = 256;
+        uint32_t order[4], count, above, top = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) order[j] = lp_order(group[j]);
-#pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit >= 0x10000u && count > l.top + 8u; bit >>= 1) {
-            uint32_t reached = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) reached += __popcll(__ballot(order[j] >= (leading | bit)));
-            if (reached >= l.top) {
-                leading |= bit;
-                count = reached;
-            }
+        for (uint32_t j = 0; j < 4; ++j) {
+            order[j] = lp_order(group[j]);
+            top = max(top, order[j]);
         }
+        const uint32_t leading = lp_search(
+            [&](uint32_t probe) {
+                uint32_t reached = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) reached += __popcll(__ballot(order[j] >= probe));
+                return reached;
+            },
+            lp_wave_max_u32(top), l.top, l.top + 8u, 0x10000u, 256u, count, above);
         if (leading > lp_order(-INFINITY)) {
             const float low = lp_bound(leading - 1u);
             if (!(low <= bound)) bound = low;
         }
-        n = 0;
-        const float b = gd_rounded(bound);
+        n = nan ? 256u : groups(bound);
+        if (l.c + 8u * n > LP_LIST) {
+            n = 0;
+            const float b = gd_rounded(bound);
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) n += __popcll(__ballot(!(x[i] <= b)));
+            for (uint32_t i = 0; i < 32; ++i) n += __popcll(__ballot(!(x[i] <= b)));
+        } else {
+            n = 0;  // fits, however many of them pass
+        }
         if (l.c + n > LP_LIST) {
             // The batch's own top, exactly: the largest order that `top` of its values reach, what is above it, and of
             // those that equal it the first.
@@ -248,18 +296,24 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
             return;
         }
     }
+    // Few lanes have any: a bit for each value that passes, then a round of the wave for the first of each lane's.
+    uint32_t passing = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-        if (!nan && !__any(!(group[j] <= bound))) continue;
+    for (int i = 31; i >= 0; --i)  // passing = 2 passing + !(x[i] <= bound); the compiler would keep 32 comparisons apart
+        asm("v_cmp_nle_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(passing) : "v"(x[i]), "v"(bound) : "vcc");
+    for (uint64_t mask = __ballot(passing != 0u); mask; mask = __ballot(passing != 0u)) {
+        const uint32_t i = (uint32_t)__builtin_ctz(passing | 0x80000000u);
+        float v[16];
+        auto choose = [](bool upper, float hi, float lo) { return upper ? hi : lo; };
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            const float v = x[8 * j + e];
-            const bool take = !(v <= bound);
-            const uint64_t mask = __ballot(take);
-            if (!mask) continue;
-            if (take) l.list[l.c + lp_before(mask)] = lp_place(v, at(j) + e);
-            l.c += __popcll(mask);
-        }
+        for (int k = 0; k < 16; ++k) v[k] = choose(i & 16u, x[16 + k], x[k]);
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; ++k) v[k] = choose(i & (uint32_t)w, v[w + k], v[k]);
+        if (passing) l.list[l.c + lp_before(mask)] = lp_place(v[0], at(i >> 3) + (i & 7u));
+        l.c += __popcll(mask);
+        passing &= passing - 1u;
     }
     lp_wave_sync();
     if (l.c >= l.top && !(bound <= l.bound)) l.bound = bound;
@@ -334,7 +388,8 @@ __device__ __forceinline__ void logprobs_body(const GdArgs &a) {
     __shared__ uint64_t merged[LP_LIST];
     __shared__ LpSums sums[LP_WAVES];
     __shared__ uint32_t counts[LP_WAVES];
-    const uint32_t V = a.c[5], top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t V = a.c[5], top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: branches and loops by it are scalar
     const uint32_t part = blockIdx.y % parts;
     const uint64_t row = (uint64_t)(blockIdx.y / parts) * gridDim.x + blockIdx.x;
     if (row >= a.c[26]) return;

@@ -5,7 +5,8 @@
 GD_PIPELINE_NAMED(logprobs_join, 256) {
     __shared__ uint64_t lists[LP_WAVES * LP_LIST];
     __shared__ uint64_t merged[LP_WAVES * LP_TOP];
-    const uint32_t top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t top = a.c[7], parts = a.c[27], lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: branches and loops by it are scalar
     const uint64_t row = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x;
     if (row >= a.c[26]) return;
     const float scale = gd_bits_f32(a.c[6]);
