@@ -299,8 +299,10 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
     // Few lanes have any: a bit for each value that passes, then a round of the wave for the first of each lane's.
     uint32_t passing = 0;
 #pragma unroll
-    for (int i = 31; i >= 0; --i)  // passing = 2 passing + !(x[i] <= bound); the compiler would keep 32 comparisons apart
-        asm("v_cmp_nle_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc" : "+v"(passing) : "v"(x[i]), "v"(bound) : "vcc");
+    for (int i = 0; i < 32; ++i) {
+        passing |= !(x[i] <= bound) ? 1u << i : 0u;
+        asm("" : "+v"(passing));  // one comparison at a time, not 32 kept apart
+    }
     for (uint64_t mask = __ballot(passing != 0u); mask; mask = __ballot(passing != 0u)) {
         const uint32_t i = (uint32_t)__builtin_ctz(passing | 0x80000000u);
         float v[16];
