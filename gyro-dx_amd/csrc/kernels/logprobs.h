@@ -3,14 +3,19 @@
 // of range), S = sum exp(d), T = sum d exp(d):
 //   logprob[j] = d[token j] - log S,   entropy = log S - T / S,   the `top` largest x, equal ones by id.
 //
-// A row goes in batches of 2048 values, 32 to a lane of one wave, held in registers for all uses: the lane's
+// A row goes in batches of 1024 values, 16 to a lane of one wave, held in registers for all uses: the lane's
 // maximum, which rescales its running S and T once per batch, the exponentials, and the choice of the top.
 // The top are kept as a superset, a list in LDS of 64-bit places in the order (lp_place). The first batch's list
-// takes what is above a lower bound of its top-th value: the top-th largest of the wave's 256 maxima of 8 values,
-// by its leading 16 bits (16 rounds of ballots). Later batches add what is above the bound, usually a few values or
-// none: one comparison per lane. A list that would run over is cut to its top and the bound raised to the last of
-// them; a batch that by itself runs over the list (ties, values in step with the lanes) goes through an exact
+// takes what is above a lower bound of its top-th value: the top-th largest of the wave's 128 maxima of 8 values,
+// by its leading bits. Later batches add what is above the bound, usually a few values or
+// none: one comparison per lane. A list that grows is cut to its top and the bound raised to the last of them; a batch
+// that by itself runs over the list (ties, values in step with the lanes) goes through an exact
 // selection. The result depends on none of this: places are unique, and the final order is by place.
+//
+// What bounds it: of many rows the reads (1023 fp32 rows of 131072: 96 us, 5.5 TB/s, 99 with the top 20); of few rows the
+// launches and one batch's chain of dependent steps (one such row: 5.6 us without a top, 14.9 with the top 20, of which the
+// join's launch and kernel take 6). Batches of 2048 took 101 to 121 us for the first and 6.1 to 14.2 for the second: half
+// the waves per SIMD, and 1023 rows in one round and a third instead of one.
 //
 // Rows shared by several groups (`parts`) leave their sums and lists in the workspace for logprobs_join.
 // Constants: 0 x 2 x stride 4 type 5 V 6 scale (fp32 bits) 7 top 8 tokens 10 tokens' stride 12 given 13 token type
@@ -20,7 +25,9 @@
 #include "rows.h"
 
 #define LP_WAVES 4u
-#define LP_BATCH 2048u
+#define LP_VALUES 16u                 // a lane's of a batch
+#define LP_EIGHTS (LP_VALUES / 8u)
+#define LP_BATCH (64u * LP_VALUES)
 #define LP_LIST 512u
 #define LP_TOP 64u
 
@@ -193,14 +200,14 @@ struct LpTop {
     float bound;
 };
 
-// Adds to the list what may be among the top of the 32 values of a lane, x[8 j + e] being value at(j) + e of the row
+// Adds to the list what may be among the top of the LP_VALUES values of a lane, x[8 j + e] being value at(j) + e of the row
 // (-infinity outside it). gd_rounded: the compiler makes ballots and orders again where they are used again, instead
-// of keeping 32 of them.
+// of keeping all of them.
 template <typename F>
-__device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, bool nan) {
-    float group[4];  // maxima of 8
+__device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[LP_VALUES], F &&at, bool nan) {
+    float group[LP_EIGHTS];  // maxima of 8
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < LP_EIGHTS; ++j) {
         group[j] = x[8 * j];
 #pragma unroll
         for (uint32_t e = 1; e < 8; ++e) group[j] = fmaxf(group[j], x[8 * j + e]);
@@ -208,22 +215,25 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
     auto groups = [&](float bound) {
         uint32_t n = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) n += __popcll(__ballot(!(group[j] <= bound)));
+        for (uint32_t j = 0; j < LP_EIGHTS; ++j) n += __popcll(__ballot(!(group[j] <= bound)));
         return n;
     };
     float bound = l.bound;
-    uint32_t n = nan ? 256u : groups(bound);  // a maximum leaves out NaNs
+    uint32_t n = nan ? 64u * LP_EIGHTS : groups(bound);  // a maximum leaves out NaNs
     if (!n) return;
+    // Cut once a wave's worth more than the top have come, which keeps the bound near the top of what was read.
+    if (l.c > l.top && (l.c >= l.top + 64u || l.c + 8u * n > LP_LIST)) {
+        bound = l.bound = lp_bound(lp_cut(l.list, l.c, l.top, l.list));
+        l.c = l.top;
+        if (!nan) n = groups(bound);
+        if (!n) return;
+    }
     if (l.c + 8u * n > LP_LIST) {
-        if (l.c > l.top) {
-            bound = l.bound = lp_bound(lp_cut(l.list, l.c, l.top, l.list));
-            l.c = l.top;
-        }
         // A lower bound of the batch's top-th value from the maxima of 8, by their leading bits: up to 16, fewer where
         // no more than 8 maxima too many reach it.
-        uint32_t order[4], count, above, top = 0;
+        uint32_t order[LP_EIGHTS], count, above, top = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
+        for (uint32_t j = 0; j < LP_EIGHTS; ++j) {
             order[j] = lp_order(group[j]);
             top = max(top, order[j]);
         }
@@ -231,20 +241,20 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
             [&](uint32_t probe) {
                 uint32_t reached = 0;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) reached += __popcll(__ballot(order[j] >= probe));
+                for (uint32_t j = 0; j < LP_EIGHTS; ++j) reached += __popcll(__ballot(order[j] >= probe));
                 return reached;
             },
-            lp_wave_max_u32(top), l.top, l.top + 8u, 0x10000u, 256u, count, above);
+            lp_wave_max_u32(top), l.top, l.top + 8u, 0x10000u, 64u * LP_EIGHTS, count, above);
         if (leading > lp_order(-INFINITY)) {
             const float low = lp_bound(leading - 1u);
             if (!(low <= bound)) bound = low;
         }
-        n = nan ? 256u : groups(bound);
+        n = nan ? 64u * LP_EIGHTS : groups(bound);
         if (l.c + 8u * n > LP_LIST) {
             n = 0;
             const float b = gd_rounded(bound);
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) n += __popcll(__ballot(!(x[i] <= b)));
+            for (uint32_t i = 0; i < LP_VALUES; ++i) n += __popcll(__ballot(!(x[i] <= b)));
         } else {
             n = 0;  // fits, however many of them pass
         }
@@ -260,11 +270,11 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
             for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
                 uint32_t reached = 0;
 #pragma unroll
-                for (uint32_t i = 0; i < 32; ++i) reached += __popcll(__ballot(exact(x[i]) >= (last | bit)));
+                for (uint32_t i = 0; i < LP_VALUES; ++i) reached += __popcll(__ballot(exact(x[i]) >= (last | bit)));
                 if (reached >= l.top) last |= bit;
             }
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) {
+            for (uint32_t i = 0; i < LP_VALUES; ++i) {
                 const bool take = exact(x[i]) > last;
                 const uint64_t mask = __ballot(take);
                 if (!mask) continue;
@@ -272,9 +282,9 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
                 l.c += __popcll(mask);
                 left -= __popcll(mask);  // fewer than `top` are above
             }
-            // 512 values of a step in order: by lane, then within its 8.
+            // The 512 values of a step in order: by lane, then within its 8.
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
+            for (uint32_t j = 0; j < LP_EIGHTS; ++j) {
                 if (!left) break;
                 uint32_t mine = 0;
 #pragma unroll
@@ -299,20 +309,20 @@ __device__ __forceinline__ void lp_add(LpTop &l, const float (&x)[32], F &&at, b
     // Few lanes have any: a bit for each value that passes, then a round of the wave for the first of each lane's.
     uint32_t passing = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (uint32_t i = 0; i < LP_VALUES; ++i) {
         passing |= !(x[i] <= bound) ? 1u << i : 0u;
-        asm("" : "+v"(passing));  // one comparison at a time, not 32 kept apart
+        asm("" : "+v"(passing));  // one comparison at a time, not all kept apart
     }
     for (uint64_t mask = __ballot(passing != 0u); mask; mask = __ballot(passing != 0u)) {
         const uint32_t i = (uint32_t)__builtin_ctz(passing | 0x80000000u);
-        float v[16];
+        float v[LP_VALUES / 2];
         auto choose = [](bool upper, float hi, float lo) { return upper ? hi : lo; };
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = choose(i & 16u, x[16 + k], x[k]);
+        for (uint32_t k = 0; k < LP_VALUES / 2; ++k) v[k] = choose(i & (LP_VALUES / 2), x[LP_VALUES / 2 + k], x[k]);
 #pragma unroll
-        for (int w = 8; w > 0; w >>= 1)
+        for (uint32_t w = LP_VALUES / 4; w > 0; w >>= 1)
 #pragma unroll
-            for (int k = 0; k < w; ++k) v[k] = choose(i & (uint32_t)w, v[w + k], v[k]);
+            for (uint32_t k = 0; k < w; ++k) v[k] = choose(i & w, v[w + k], v[k]);
         if (passing) l.list[l.c + lp_before(mask)] = lp_place(v[0], at(i >> 3) + (i & 7u));
         l.c += __popcll(mask);
         passing &= passing - 1u;
@@ -405,13 +415,13 @@ __device__ __forceinline__ void logprobs_body(const GdArgs &a) {
     LpSums p = {-INFINITY, 0.f, 0.f};
     for (uint32_t b = b0 + wave; b < b1; b += LP_WAVES) {
         const uint32_t first = b * LP_BATCH + 8u * lane;
-        float x[32];
+        float x[LP_VALUES];
         // Eight values at a time; a lane that reaches past the row reads the row's last eight and leaves out (as
         // -infinity) those before its own. A row of fewer than eight is one lane's.
         auto at = [&](uint32_t j) { return V < 8u ? first + 512u * j : min(first + 512u * j, V - 8u); };
         if (V >= 8u) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
+            for (uint32_t j = 0; j < LP_EIGHTS; ++j) {
                 float v[8];
                 row_load8<TYPE>(X, at(j), v);
 #pragma unroll
@@ -419,21 +429,21 @@ __device__ __forceinline__ void logprobs_body(const GdArgs &a) {
             }
             if (b + 1u == batches) {
 #pragma unroll
-                for (uint32_t i = 0; i < 32; ++i)
+                for (uint32_t i = 0; i < LP_VALUES; ++i)
                     if (at(i >> 3) + (i & 7u) < first + 512u * (i >> 3)) x[i] = -INFINITY;
             }
         } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) x[i] = i < 8u && first + i < V ? row_load(X, first + i, TYPE) : -INFINITY;
+            for (uint32_t i = 0; i < LP_VALUES; ++i) x[i] = i < 8u && first + i < V ? row_load(X, first + i, TYPE) : -INFINITY;
         }
         float most = x[0];
 #pragma unroll
-        for (uint32_t i = 1; i < 32; ++i) most = fmaxf(most, x[i]);
+        for (uint32_t i = 1; i < LP_VALUES; ++i) most = fmaxf(most, x[i]);
         lp_move(p, fmaxf(p.m, most), scale);
         const float ref = p.m == -INFINITY ? 0.f : p.m;
         float s = 0.f, t = 0.f;
 #pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
+        for (uint32_t i = 0; i < LP_VALUES; ++i) {
             const float d = scale * (x[i] - ref), e = __expf(d);
             s += e;
             t += e * fmaxf(d, -1e30f);

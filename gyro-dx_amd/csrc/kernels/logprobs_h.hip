@@ -1,3 +1,3 @@
 // Log probabilities, entropy and top alternatives of rows of binary16 logits (logprobs.h).
 #include "logprobs.h"
-GD_PIPELINE_NAMED_OCC(logprobs_h, 256, 3) { logprobs_body<ROW_F16>(a); }
+GD_PIPELINE_NAMED(logprobs_h, 256) { logprobs_body<ROW_F16>(a); }

@@ -246,12 +246,12 @@ class RowOps {
 
     // ---- log probabilities ----
 
-    // Groups that share a row: three for each of 256 compute units, each of a group's four waves with a batch of 2048
-    // logits at least. Fewer leave units idle, more pay for their lists twice (131072 logits, top 5, us at 1 / 3 / 6 / 12
-    // groups a row: one row 31.1 / 18.0 / 13.3 / 11.8, 128 rows 36.8 / 25.7 / 21.5 / 25.6, 512 rows 55.7 / 60.3 / 61.9 / 77.3).
+    // Groups that share a row: four for each of 256 compute units, each of a group's four waves with a batch of 1024 logits
+    // at least. Fewer leave units idle, more pay for their lists twice (131072 logits, top 5, us at 1 / 2 / 4 / 8 / 16 groups
+    // a row: one row 37 / 25 / 17 / 13 / 11, 128 rows 45 / 31 / 25 / 22 / 25, 512 rows 61 / 57 / 62 / 63 / 73).
     static uint32_t logprobs_parts(uint32_t n, uint32_t V) {
-        const uint32_t batches = (V + 2047) / 2048;
-        return std::max(1u, std::min({32u, (batches + 3) / 4, 768 / std::max(1u, n)}));
+        const uint32_t batches = (V + 1023) / 1024;
+        return std::max(1u, std::min({32u, (batches + 3) / 4, 1024 / std::max(1u, n)}));
     }
     static uint64_t logprobs_workspace(uint32_t n, uint32_t V, uint32_t top) {
         const uint32_t parts = logprobs_parts(n, V);
