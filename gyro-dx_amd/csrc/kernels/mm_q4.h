@@ -4,10 +4,10 @@
 // tokens go through LDS as operands, two buffers in turn, one being filled while the other is multiplied; weights
 // go from memory to registers, a chunk ahead. Of 32 columns a wave unpacks 4 operands, each used for T products
 // of 16 + q; where two groups of 32 share a scale their products add up in the matrix unit before they are scaled into
-// the sums, 16 T (or 8 T) vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much and the minimum,
-// (m - 16 s) sum x (or -24 s sum x), is a product of its own: of the chunk's four sums of 32 activations, which come
-// with the staging, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens are operands as they are; fp32 ones
-// go through the products three times, a part each.
+// the sums, 16 T (or 8 T) vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much starts
+// each sum, as in mv_q4, so that sums are rounded at their own size. Minima times the chunk's four sums of 32 activations,
+// which come with the staging, are a product of their own, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens
+// are operands as they are; fp32 ones go through the products three times, a part each.
 #pragma once
 #include "q4.h"
 
@@ -39,11 +39,12 @@ __device__ __forceinline__ float mm_dpp(float v) {
     return gd_bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)gd_f32_bits(v), CTRL, 0xf, 0xf, true));
 }
 
-// A chunk of a tile as a lane holds it: its 16 bytes, and its row's 4 / SPAN scales and minima, binary16 in order.
+// A chunk of a tile as a lane holds it: its 16 bytes, its row's 4 / SPAN scales, binary16 in order, and the minimum of
+// group lane / 16 of 32 (where there are minima).
 template <int SPAN>
 struct MmChunk {
     gd_u32x4 w;
-    uint32_t s[SPAN == 1 ? 2 : 1], m[SPAN == 1 ? 2 : 1];
+    uint32_t s[SPAN == 1 ? 2 : 1], m;
 };
 template <int SPAN>
 __device__ __forceinline__ void mm_scales(uint64_t base, uint32_t row, uint32_t (&o)[SPAN == 1 ? 2 : 1]) {
@@ -78,7 +79,7 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
     constexpr uint32_t SUMS = ROWS + 16u;  // a group's row of sums, the four groups' in different banks
     const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, h = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint64_t quants = gd_addr(a, 0), scales = gd_addr(a, 2), minima = gd_addr(a, 4) ? gd_addr(a, 4) : scales;
+    const uint64_t quants = gd_addr(a, 0), scales = gd_addr(a, 2), minima = gd_addr(a, 4);
     const uint32_t tiles = a.c[6], chunks = a.c[7], cols = a.c[9], outputs = a.c[10], n = a.c[17];
     const uint64_t X = gd_addr(a, 12), xs = gd_addr(a, 14);
     // The groups of an XCD (i % 8) take neighbouring rows, all tokens of some before the next, so that its L2 holds
@@ -91,8 +92,9 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
     }
     const uint32_t t0 = tb * ROWS, tile0 = (rb * MM_WAVES + wave) * MM_R;
     const MqBits bits = mq_bits<HALF>();
-    // The sums' coefficient of scale and minimum: m - 16 s, or -24 s (what is loaded as the minimum is the scale then).
-    const float of_scale = gd_addr(a, 4) ? -16.f : -24.f, of_minimum = gd_addr(a, 4) ? 1.f : 0.f;
+    // What the products' 16 is too much, and the 8 of weights without a minimum, as an operand of its own.
+    const uint32_t bias = HALF ? (minima ? 0xcc00u : 0xce00u) : (minima ? 0xc180u : 0xc1c0u), bias2 = bias | bias << 16;  // -16, -24
+    const gd_u32x4 unbias = {bias2, bias2, bias2, bias2};
     const gd_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
     MmChunk<SPAN> cur[MM_R], next[MM_R];
@@ -103,7 +105,7 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
             const uint64_t unit = (uint64_t)min(tile0 + r, tiles - 1u) * chunks + c;
             o[r].w = gd_load<gd_u32x4>(quants + unit * 1024u, lane * 16u);
             mm_scales<SPAN>(scales + unit * (128u / SPAN), col, o[r].s);
-            mm_scales<SPAN>(minima + unit * (128u / SPAN), col, o[r].m);
+            if (minima) o[r].m = gd_load<uint16_t>(minima + unit * (128u / SPAN), (col * (4u / SPAN) + h / SPAN) * 2u);
         }
     };
     // Unit i = tid + 256 k of a chunk of the tokens: row i / 16, values 8 (i % 16) ..; rows past the last token read the
@@ -141,23 +143,30 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
         for (uint32_t k = 0; k < PER; ++k) {
             const uint32_t i = tid + 256u * k, row = i >> 4, at = row * 16u + ((i & 15u) ^ (row & 15u));
             gd_u32x4 *const out = lds + buffer * (UNITS * PARTS) + at;
-            float sum = 0.f;
             if constexpr (TYPE == ROW_F32) {
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[e] = gd_bits_f32(raw[k][e >> 2][e & 3]);
-                    sum += v[e];
-                }
+                for (int e = 0; e < 8; ++e) v[e] = gd_bits_f32(raw[k][e >> 2][e & 3]);
                 mq_planes(v, PARTS, [&](uint32_t p, gd_u32x4 w) { out[p * UNITS] = w; });
             } else {
                 out[0] = raw[k][0];
+            }
+        }
+        if (!minima) return;
+#pragma unroll
+        for (uint32_t k = 0; k < PER; ++k) {
+            const uint32_t i = tid + 256u * k;
+            float sum = 0.f;
+            if constexpr (TYPE == ROW_F32) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += gd_bits_f32(raw[k][e >> 2][e & 3]);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum = mm_pair<HALF>(raw[k][0][e], sum);
             }
             sum += mm_dpp<0xb1>(sum);  // lanes ^ 1
             sum += mm_dpp<0x4e>(sum);  // lanes ^ 2: the group's four units
-            if ((i & 3u) == 0u) sums[(buffer * 4u + ((i & 15u) >> 2)) * SUMS + row] = sum;
+            if ((i & 3u) == 0u) sums[(buffer * 4u + ((i & 15u) >> 2)) * SUMS + (i >> 4)] = sum;
         }
     };
 
@@ -187,19 +196,23 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
         for (uint32_t j = 0; j < PAIR; ++j)
 #pragma unroll
             for (int t = 0; t < T; ++t) operand(j, t);
-        float sum[T];
+        if (minima) {
 #pragma unroll
-        for (int t = 0; t < T; ++t) sum[t] = sums[(buffer * 4u + h) * SUMS + t * 16u + col];
+            for (int t = 0; t < T; ++t) {
+                const float sum = sums[(buffer * 4u + h) * SUMS + t * 16u + col];
 #pragma unroll
-        for (int r = 0; r < MM_R; ++r) {
-            // Of the scale and minimum of this lane's row and group h of 32.
-            const uint32_t g = h / SPAN, from = 16u * (g & 1u);
-            const uint32_t sw = SPAN == 1 && (g & 2u) ? cur[r].s[SPAN == 1] : cur[r].s[0];
-            const uint32_t mw = SPAN == 1 && (g & 2u) ? cur[r].m[SPAN == 1] : cur[r].m[0];
-            const float coefficient = of_scale * gd_half(sw >> from & 0xffffu) + of_minimum * gd_half(mw >> from & 0xffffu);
-#pragma unroll
-            for (int t = 0; t < T; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[t], coefficient, acc[r][t], 0, 0, 0);
+                for (int r = 0; r < MM_R; ++r)
+                    acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum, gd_half(cur[r].m), acc[r][t], 0, 0, 0);
+            }
         }
+        gd_f32x4 corr[T];
+        auto correct = [&](int t) {
+            corr[t] = zero;
+#pragma unroll
+            for (uint32_t e = 0; e < PAIR; ++e)
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; --p) corr[t] = mm_mfma<HALF>(x[e][t][p], unbias, corr[t]);
+        };
         // A step is a tile's products with 32 columns; a tile takes PAIR of them, whose sums are scaled together, before
         // the next tile. Beside a step run the unpacking of the next one's weights, the scaling of the tile before and,
         // in the last tile's, the reads of the next operands; the empty asm statements and the barriers keep each where
@@ -221,15 +234,18 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
             const uint32_t g = k / (PAIR * MM_R), r = k / PAIR % MM_R, e = k % PAIR, j = g * PAIR + e;
             const uint32_t gn = (k + 1u) / (PAIR * MM_R), rn = (k + 1u) / PAIR % MM_R, jn = gn * PAIR + (k + 1u) % PAIR;
             gd_u32x4 wn = w;
+            if (r == 0 && e == 0)
+#pragma unroll
+                for (int t = 0; t < T; ++t) correct(t);
             if (jn < 4u) {
                 asm volatile("" : "+v"(cur[rn].w));
                 wn = mq_weights<HALF>(cur[rn].w[jn], bits);
             }
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                gd_f32x4 v = e ? d[r & 1][t] : zero;
+                gd_f32x4 v = e ? d[r & 1][t] : corr[t];
 #pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p) v = mm_mfma<HALF>(x[e][t][p], w, v);  // the smallest part first
+                for (int p = 0; p < PARTS; ++p) v = mm_mfma<HALF>(x[e][t][p], w, v);  // the largest part first: it takes the correction away
                 d[r & 1][t] = v;
                 if (r == MM_R - 1 && j + PAIR < 4u) operand(j + PAIR, t);
             }
@@ -278,14 +294,14 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
 template <uint32_t TYPE, int SPAN>
 __device__ __forceinline__ void mm_q4_body(const GdArgs &a) {
     // Two groups share a CU's registers and LDS: two buffers of a chunk's operands, then the sums of four waves.
-    constexpr int MOST = TYPE == ROW_F32 ? 3 : 4;
+    constexpr int MOST = TYPE == ROW_F32 ? (SPAN == 1 ? 2 : 3) : 4;
     constexpr uint32_t OPERANDS = 2 * 16 * MOST * 16 * (TYPE == ROW_F32 ? 3 : 1), OUT = MM_WAVES * 16 * MOST * 68 / 4;
     __shared__ __align__(16) gd_u32x4 lds[OPERANDS > OUT ? OPERANDS : OUT];
     __shared__ float sums[2 * 4 * (16 * MOST + 16)];
     switch (a.c[26]) {
         case 1: return mm_q4_tile<TYPE, SPAN, 1>(a, lds, sums);
         case 2: return mm_q4_tile<TYPE, SPAN, 2>(a, lds, sums);
-        case 3: return mm_q4_tile<TYPE, SPAN, 3>(a, lds, sums);
+        case 3: return mm_q4_tile<TYPE, SPAN, MOST < 3 ? MOST : 3>(a, lds, sums);
         default: return mm_q4_tile<TYPE, SPAN, MOST>(a, lds, sums);
     }
 }

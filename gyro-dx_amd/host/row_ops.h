@@ -174,7 +174,8 @@ class RowOps {
             uint32_t tokens = 16;
             uint64_t cost = ~0ull;
             const uint32_t blocks = (m.tiles + 15) / 16;
-            for (uint32_t t = 1; t <= (x.type == GM_F32 ? 3u : 4u); ++t) {
+            const uint32_t most = x.type != GM_F32 ? 4 : m.lg == 5 ? 2 : 3;  // mm_q4_body's
+            for (uint32_t t = 1; t <= most; ++t) {
                 const uint64_t groups = (uint64_t)blocks * ((n + 16 * t - 1) / (16 * t));
                 const uint64_t k = (groups + 2 * cus - 1) / (2 * cus) * (28 + 16 * t);
                 if (k <= cost) {
@@ -188,8 +189,10 @@ class RowOps {
             l.y = (n + tokens - 1) / tokens;
             return l;
         }
-        // Waves that share a tile's columns: as few as leave every unit its 16 waves.
-        uint32_t wk = 1;
+        // Waves that share a tile's columns: two, or as few as leave every unit its 16 waves (one fp32 token at 2048 columns,
+        // us at 1 / 2 / 4 / 8: 131072 rows 35.8 / 35.0 / 35.6 / 41.7, 32768 rows 18.2 / 12.3 / 11.3 / 12.9, 2048 rows 14.9 /
+        // 9.6 / 7.0 / 6.2).
+        uint32_t wk = m.chunks > 1 ? 2 : 1;
         while (wk < 8 && wk * 2 <= m.chunks && m.tiles / 2 * wk < 16 * cus) wk *= 2;
         c.set(26, wk);
         const uint32_t run = 2 * (8 / wk), runs = (m.tiles + run - 1) / run;

@@ -156,7 +156,9 @@ def test_linear_builds(shim):
                ((100003, 30), (100003, 45), (100003, 64), (8000, 1000), (8000, 500), (8000, 700))]
               for type in (1, 2) for g in (32, 64, 128)]
     assert all(t == [2, 3, 4, 4, 2, 3] for t in tokens), tokens
-    assert [plan(r, 64, 0, n)[1] for r, n in ((40000, 12), (100003, 30), (100003, 45), (8000, 1000), (8000, 700))] == [1, 2, 3, 2, 3]
+    for g, want in ((32, [1, 2, 2, 2, 2]), (64, [1, 2, 3, 2, 3]), (128, [1, 2, 3, 2, 3])):
+        assert [plan(r, 128, 0, n, 2 if g > 32 else 0, g)[1] for r, n in
+                ((40000, 12), (100003, 30), (100003, 45), (8000, 1000), (8000, 700))] == want
     assert plan(40000, 64, 1, 20)[0] == "mm_q4_b32" and plan(40000, 64, 2, 12)[0] == "mm_q4_h32"
 
 
