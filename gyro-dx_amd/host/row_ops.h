@@ -1,7 +1,6 @@
 // The operators around the MoE layers (gm_linear, gm_block_norm, gm_logprobs): argument checks, the choice of a
 // build, its constants and grid. The engine launches what they return. Their kernels (csrc/kernels/q4.h, block_norm.h,
-// logprobs.h) take every address
-// in the launch's constants, so a call needs no table entry and may be captured.
+// logprobs.h) take every address in the launch's constants, so a call needs no table entry and may be captured.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -53,8 +52,9 @@ class RowOps {
     std::vector<Matrix> matrices;
 
     static bool owns(const std::string &kernel) {
-        return kernel.rfind("mv_q4", 0) == 0 || kernel.rfind("mm_q4", 0) == 0 || kernel == "q4_repack" || kernel.rfind("block_norm", 0) == 0 ||
-               kernel.rfind("logprobs", 0) == 0;
+        for (const char *prefix : {"mv_q4", "mm_q4", "q4_repack", "block_norm", "logprobs"})
+            if (kernel.rfind(prefix, 0) == 0) return true;
+        return false;
     }
     using Loader = std::function<gd_pipeline *(const std::string &file)>;
     Loader loader;
@@ -136,7 +136,7 @@ class RowOps {
         if (!n) return l;  // of no rows there may be no memory
         check_rows(x, n, m.cols, false, "gm_linear: x");
         check_rows(y, n, m.rows, true, "gm_linear: y");
-        require(x.stride <= 1u << 24, "gm_linear: x's rows are at most 2^24 values apart");
+        require(n == 1 || x.stride <= 1u << 24, "gm_linear: x's rows are at most 2^24 values apart");
         require(act <= GM_ACT_SIGMOID && (!m.gated || act == GM_ACT_NONE), "gm_linear: act");
         require(n <= 1u << 18, "gm_linear takes at most 2^18 tokens");
         Constants &c = l.c;
@@ -165,15 +165,16 @@ class RowOps {
         // and passes. They meet near (fp32, binary16, bf16) 14, 11 and 9 tile passes per compute unit. us at 2048
         // columns, mv / mm: 2048 rows of 64 and 512 fp32 tokens 16.1 / 26.4 and 88.0 / 29.9, 8192 rows of 17 and 64
         // 16.2 / 26.0 and 46.7 / 27.2, 8192 rows of 64 and 128 bf16 tokens 20.5 / 22.3 and 37.0 / 23.6.
+        // (The grid of more than 2^20 tiles would be too wide for mm_q4.)
         static const uint32_t meet[] = {14, 9, 11};
-        if (passes > 1 && (uint64_t)m.tiles * passes > (uint64_t)meet[x.type] * cus) {
+        const uint32_t blocks = (m.tiles + 15) / 16;
+        if (passes > 1 && blocks <= 65535 && (uint64_t)m.tiles * passes > (uint64_t)meet[x.type] * cus) {
             static const char *const names[3][3] = {{"mm_q4_f32", "mm_q4_f64", "mm_q4_f128"},
                                                     {"mm_q4_b32", "mm_q4_b64", "mm_q4_b128"},
                                                     {"mm_q4_h32", "mm_q4_h64", "mm_q4_h128"}};
             // 16 T tokens to a group: the fewest rounds of two groups per unit, by a step's vector instructions.
             uint32_t tokens = 16;
             uint64_t cost = ~0ull;
-            const uint32_t blocks = (m.tiles + 15) / 16;
             const uint32_t most = x.type != GM_F32 ? 4 : m.lg == 5 ? 2 : 3;  // mm_q4_body's
             for (uint32_t t = 1; t <= most; ++t) {
                 const uint64_t groups = (uint64_t)blocks * ((n + 16 * t - 1) / (16 * t));

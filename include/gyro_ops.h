@@ -5,8 +5,9 @@
  * probabilities of an answer, on rows in device memory of the engine's GPU. They need no layer. A call queues its
  * launches on `stream` and does not wait, allocate or copy; `stream` is a hipStream_t of the engine's
  * device as HIP means it (NULL: the device's null stream, unlike gm_forward_decode_noalloc's), and the caller's
- * current device is left as it was. All may be captured into a HIP graph; a kernel that no call has used yet is loaded
- * by its first call, which a capture refuses, so call once (or gm_load_operators) before. n = 0 does nothing. Calls on
+ * current device is left as it was. gm_linear, gm_block_norm and gm_logprobs may be captured into a HIP graph; a kernel
+ * that no call has used yet is loaded by its first call, which a capture refuses, so call once (or gm_load_operators)
+ * before. The calls that load, add or release wait and allocate, and belong outside captures. n = 0 does nothing. Calls on
  * one engine are serialised by the caller, as all of gyro_moe.h's; what they queue may overlap where its outputs and
  * workspaces are apart. All return 0 or a negative code; gm_last_error describes the failure.
  */
@@ -50,12 +51,14 @@ typedef struct gm_matrix_desc {
 /* Uploads a matrix (at most 4 GiB in the device's layout: half a byte per value and the scales, of rows in
  * sixteens and columns in 128s) and returns its index. */
 GM_API int gm_add_matrix(gm_engine *e, const gm_matrix_desc *desc, uint32_t *out_index);
-/* Frees a matrix once the device's work is done; its index may come again. */
+/* Frees a matrix once the device's work is done; its index may come again. A graph captured with it may not be
+ * replayed any more. */
 GM_API int gm_release_matrix(gm_engine *e, uint32_t matrix);
 /* y[t] = act(scale W x[t]) for n tokens, x [n][cols], y [n][rows]; with accumulate, the sum is added to y
  * (after act, in fp32). A gated pair: y[t] = scale silu(G x[t]) * (U x[t]), act GM_ACT_NONE. Activations and sums
- * are fp32 whatever the types (products are exact in them); y is rounded once. Of a token with an
- * activation that is not finite no output is (a NaN or an infinity). x's rows are at most 2^24
+ * are fp32 whatever the types (products are exact in them); y is rounded once. Activations
+ * are below 2^116 in magnitude (a group's sums of products with 0 .. 31 stay in range then). Of a token with an
+ * activation that is not finite no output is (a NaN or an infinity). Two or more rows of x are at most 2^24
  * values apart, n at most 2^18; y must not overlap x. */
 enum { GM_ACT_NONE = 0, GM_ACT_SILU = 1, GM_ACT_SIGMOID = 2 };
 GM_API int gm_linear(gm_engine *e, uint32_t matrix, const gm_rows *x, uint32_t n, const gm_rows *y, uint32_t act,

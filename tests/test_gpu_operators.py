@@ -242,6 +242,60 @@ def test_linear_wide_range(eng, xt, sizes, n, rows):
     eng.release_matrix(index)
 
 
+@pytest.mark.parametrize("n,rows", [(4, 64), (50, 64), (50, 20000)])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("xt,sizes", [("f32", (1e-30, 1.0, 1e20)), ("bf16", (1e-30, 1e20)), ("f16", (1e-7, 1e-5, 5000.0))])
+def test_linear_minima_wide_range(eng, xt, sizes, group, n, rows):
+    """The sums that minima multiply keep all bits as well."""
+    rng = np.random.default_rng(5)
+    index, (mats,) = add(eng, rng, "q4", rows, 384, group, True, False, False)
+    for size in sizes:
+        x = torch.from_numpy(rng.standard_normal((n, 384)) * size).to(ref.DTYPES[xt])
+        yd = torch.zeros(n, rows, device="cuda")
+        eng.linear(index, x.cuda(), yd, stream=stream())
+        y = x.double() @ mats[1].T
+        assert ((yd.cpu().double() - y).abs() <= linear_bound(mats, x.double(), 384, group) + ULP * y.abs()).all()
+    eng.release_matrix(index)
+
+
+def far_rows(n, width, stride, dtype):
+    """[n, width] zeros whose rows are `stride` values apart (memory between them untouched)."""
+    view = torch.empty((n - 1) * stride + width, dtype=dtype, device="cuda").as_strided((n, width), (stride, 1))
+    view.zero_()
+    return view
+
+
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+@pytest.mark.parametrize("n,rows", [(70, 40), (70, 20000)])
+def test_linear_far_rows(eng, xt, n, rows):
+    """Inputs and outputs whose offsets pass 32 bits, in few and in many tokens' kernels."""
+    rng = np.random.default_rng(6)
+    index, ((_, W, _, _),) = add(eng, rng, "q4_0", rows, 160, 32, False, False, True)
+    xs = integers(rng, n, 160)
+    x = far_rows(n, 160, 1 << 24, ref.DTYPES[xt])
+    x.copy_(xs)
+    y = far_rows(n, rows, (1 << 25) + 3, torch.bfloat16)
+    eng.linear(index, x, y, stream=stream())
+    assert torch.equal(y.cpu(), (xs @ W.T).bfloat16())
+    eng.release_matrix(index)
+
+
+def test_norm_and_logprobs_far_rows(eng):
+    n, stride = 20, (1 << 28) + 1
+    x, out = far_rows(n, 100, stride, torch.bfloat16), far_rows(n, 100, stride, torch.bfloat16)
+    xs = torch.randn(n, 100, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x.copy_(xs)
+    near = torch.zeros(n, 100, dtype=torch.bfloat16, device="cuda")
+    eng.block_norm(None, xs.cuda(), None, near, stream=stream())
+    eng.block_norm(None, x, None, out, stream=stream())
+    assert torch.equal(out, near) and near.abs().sum() > 0
+    a, b = ([torch.zeros(n, 3, dtype=torch.int32, device="cuda"), torch.zeros(n, 3, device="cuda"), torch.zeros(n, device="cuda")]
+            for _ in range(2))
+    for t, (ids, top, entropy) in ((xs.cuda(), a), (x, b)):
+        eng.logprobs(t, top_ids=ids, top_logprobs=top, entropy=entropy, stream=stream())
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and a[2].min() > 0
+
+
 def test_matrix_indices(eng):
     rng = np.random.default_rng(4)
     first, ((_, W, _, _),) = add(eng, rng, "q4_0", 32, 64, 32, False, False, True)

@@ -119,6 +119,7 @@ def test_linear_refusals(shim):
     ok = lambda d=m, x=rows(), n=4, y=rows(), act=0, acc=0, scale=1.0: call(shim.plan_linear, d, x, n, y, act, acc, scale)  # noqa: E731
     assert ok()[0] == 0 and ok()[2] >= 1
     assert ok(n=0)[0] == 0 and ok(n=0)[2] == 0
+    assert ok(x=rows(stride=1 << 30), n=1)[0] == 0  # one row's stride is not used
     assert ok(x=rows(stride=0))[0] == 0 and ok(y=rows(stride=0), n=1)[0] == 0
     for bad in (dict(x=rows(data=None)), dict(y=rows(data=None)), dict(x=rows(type=3)), dict(y=rows(type=7)),
                 dict(x=rows(data=A + 2)), dict(y=rows(type=1, data=A + 1)), dict(y=rows(stride=63)), dict(act=3),
@@ -129,7 +130,8 @@ def test_linear_refusals(shim):
 
 def test_linear_grids(shim):
     """Any token count and matrix fits the grid's 65535 groups a dimension."""
-    for fmt, r, c in ((0, 1, 32), (0, 131072, 2048), (2, 100003, 2560), (0, 1 << 22, 1024)):
+    for fmt, r, c in ((0, 1, 32), (0, 131072, 2048), (2, 100003, 2560), (0, 1 << 22, 1024), (0, (1 << 24) - 240, 128),
+                      (0, 1 << 24, 32), (0, 50 << 20, 32)):
         for type in (0, 1, 2):
             for n in (1, 5, 6, 64, 1023, 1 << 18):
                 rc, why, x, y = call(shim.plan_linear, matrix(fmt, r, c), rows(type), n, rows(stride=r), 0, 0, 1.0)
