@@ -6,6 +6,13 @@
 // sum to `normed`; out and normed are rounded once. A group of 256 threads takes a token's row, 8 neighbouring
 // values per thread and step, all of them in registers between the two sums of squares, whose partial sums meet
 // in fixed order. out may be x, and normed h, in place.
+//
+// What bounds it: of many rows the bytes (4096 rows of 2048, fp32 stream, bf16 in and out, 101 MB: 23 to 26 us, 3.9 to 4.4
+// TB/s; a large copy moves 5.1). Of few, one row's chain of loads, two sums and stores: 3.6 us at 2048 values, 4.9 at 2560.
+// One row to a group rather than to a wave: a wave would hold a row of 2048 in 100 registers and leave a single row to
+// one unit's fourth part. The builds differ in the steps of 2048 values that registers hold (1, 2, 8): a shorter one
+// has more waves in flight and less to skip (block_norm_s against the two-step build: one row of 2048 3.8 against 4.9 us, 4096
+// rows 25.5 against 26.8).
 // Constants: 0 h (0: none, v = x) 2 h stride 4 x 6 x stride 8 out (0: none) 10 out stride 12 normed (0: none)
 // 14 normed stride 16 post weight (0: none) 18 pre weight (0: none) 20 gate (0: none) 22 gate's token stride
 // 24 gate's channel step (0 or 1) 25 types (h | x << 4 | out << 8 | normed << 12 | gate << 16) 26 flags (1 post norm,

@@ -8,6 +8,15 @@
 // each sum, as in mv_q4, so that sums are rounded at their own size. Minima times the chunk's four sums of 32 activations,
 // which come with the staging, are a product of their own, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens
 // are operands as they are; fp32 ones go through the products three times, a part each.
+//
+// What bounds it: issue. 8192 x 2048 on 1023 bf16 tokens takes 60 us with groups of 32 (570 TFLOP/s) and 51 with groups of
+// 128 (670), half of a large matrix product's 1200; in fp32 118 us (290). Of a gated 4096 x 2048 in groups of 64 with
+// minima on 1023 binary16 tokens (58 to 66 us, box to box) the matrix unit is busy 36% of the cycles (two fifths of that
+// corrections and minima), the vector unit 41%, and two waves a SIMD, which is what registers and LDS hold, wait for one
+// another's results the rest. Few tokens are bound by the waves' waits for
+// chunks and by groups that do not divide among the units (100003 x 2560 on 37 tokens: 391 groups, 52 to 57 us, 2.7 TB/s):
+// weights or tokens two chunks ahead gained 0 to 4%. Minima as exact bf16 parts in one 16x16x32 product, half the
+// matrix cycles, gained nothing either.
 #pragma once
 #include "q4.h"
 

@@ -11,7 +11,8 @@
 // Source (kind): 0 GGUF Q4_0 (18-byte blocks: binary16 scale, 16 bytes whose low bits hold values 0 .. 15
 // and high bits 16 .. 31), 1 Q4_1 (20 bytes: scale, minimum, as before), 2 arrays: quants [rows][cols / 2]
 // with value 2 i in byte i's low bits, scales and minima [rows][cols / group] binary16.
-// One thread per 16 output bytes. Constants: 0 kind 1 rows 2 cols 3 chunks 4 log2(group) 5 tiles 6 tile step
+// One thread per 16 output bytes, which reads its bytes one by one: 0.5 ms for 131072 x 2048 Q4_0 (151 MB in, as much out),
+// beside 4 ms for the upload before it. Constants: 0 kind 1 rows 2 cols 3 chunks 4 log2(group) 5 tiles 6 tile step
 // (2 in a gated pair) 7 first tile 8 quants 10 scales 12 minima (0: none) 14 output quants 16 output scales
 // 18 output minima (64-bit addresses). 32-bit thread index: tiles * chunks * 64 < 2^32.
 #include "rows.h"

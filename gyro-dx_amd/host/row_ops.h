@@ -161,12 +161,13 @@ class RowOps {
         c.set(25, scale);
         // Tokens that share a pass of mv_q4 over the weights.
         const uint32_t per = x.type == GM_F32 ? 5u : x.type == GM_F16 ? 8u : 16u, passes = (n + per - 1) / per;
-        // mm_q4's few large groups take 1.0 to 1.3 us a chunk however little there is to do; mv_q4's time grows with tiles
-        // and passes. They meet near (fp32, binary16, bf16) 14, 11 and 9 tile passes per compute unit. us at 2048
-        // columns, mv / mm: 2048 rows of 64 and 512 fp32 tokens 16.1 / 26.4 and 88.0 / 29.9, 8192 rows of 17 and 64
-        // 16.2 / 26.0 and 46.7 / 27.2, 8192 rows of 64 and 128 bf16 tokens 20.5 / 22.3 and 37.0 / 23.6.
+        // mm_q4's few large groups take 1.1 to 1.4 us a chunk however little there is to do; mv_q4's time grows with tiles
+        // and passes. They meet near (fp32, bf16, binary16) 12, 7 and 8 tile passes per compute unit. us at 2048
+        // columns, mv / mm: 2048 rows of 64, 128 and 512 fp32 tokens 16.6 / 23.4, 28.1 / 23.6 and 90.3 / 25.3; 8192 rows of
+        // 17 and 32 16.3 / 23.4 and 26.8 / 23.6; of 32 and 64 bf16 tokens 12.2 / 18.6 and 21.4 / 19.2, binary16 18.4 / 18.9
+        // and 33.5 / 19.4.
         // (The grid of more than 2^20 tiles would be too wide for mm_q4.)
-        static const uint32_t meet[] = {14, 9, 11};
+        static const uint32_t meet[] = {12, 7, 8};
         const uint32_t blocks = (m.tiles + 15) / 16;
         if (passes > 1 && blocks <= 65535 && (uint64_t)m.tiles * passes > (uint64_t)meet[x.type] * cus) {
             static const char *const names[3][3] = {{"mm_q4_f32", "mm_q4_f64", "mm_q4_f128"},
