@@ -2,7 +2,7 @@
 //
 // A group of four waves takes 16 tiles (256 weight rows), four to a wave, and 16 T tokens. Chunks of 128 columns of the
 // tokens go through LDS as operands, two buffers in turn, one being filled while the other is multiplied; weights
-// go from memory to registers, a chunk ahead. Of 32 columns a wave unpacks 4 operands, each used for T products
+// go from memory to registers, one or two chunks ahead. Of 32 columns a wave unpacks 4 operands, each used for T products
 // of 16 + q; where two groups of 32 share a scale their products add up in the matrix unit before they are scaled into
 // the sums, 16 T (or 8 T) vector instructions per 32 columns beside 28 for unpacking. What the 16 is too much starts
 // each sum, as in mv_q4, so that sums are rounded at their own size. Minima times the chunk's four sums of 32 activations,
@@ -13,10 +13,10 @@
 // 128 (670), half of a large matrix product's 1200; in fp32 118 us (290). Of a gated 4096 x 2048 in groups of 64 with
 // minima on 1023 binary16 tokens (58 to 66 us, box to box) the matrix unit is busy 36% of the cycles (two fifths of that
 // corrections and minima), the vector unit 41%, and two waves a SIMD, which is what registers and LDS hold, wait for one
-// another's results the rest. Few tokens are bound by the waves' waits for
-// chunks and by groups that do not divide among the units (100003 x 2560 on 37 tokens: 391 groups, 52 to 57 us, 2.7 TB/s):
-// weights or tokens two chunks ahead gained 0 to 4%. Minima as exact bf16 parts in one 16x16x32 product, half the
-// matrix cycles, gained nothing either.
+// another's results the rest. Few tokens are bound by the chain of a chunk (load, store to LDS, barrier, products: 1.1 us)
+// and by groups that do not divide among the units (100003 x 2560 on 37 tokens: 391 groups, 51 to 55 us, 2.8 TB/s). Groups
+// that start at different chunks gained nothing, nor did minima as exact bf16 parts in one 16x16x32 product, half the
+// matrix cycles.
 #pragma once
 #include "q4.h"
 
@@ -106,7 +106,11 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
     const gd_u32x4 unbias = {bias2, bias2, bias2, bias2};
     const gd_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    MmChunk<SPAN> cur[MM_R], next[MM_R];
+    // Chunks asked for ahead: two where few tokens leave the registers and a chunk's products are shorter than a load takes (us
+    // with one / two: 32768 x 2048 on 32 tokens 22.4 / 18.2, 131072 x 2048 on 12 fp32 tokens 48.5 / 43.2 and on 48 bf16 ones
+    // 54.2 / 51.5, but 51.7 / 54.8 for 48 tokens a group of 100003 x 2560 in groups of 64).
+    constexpr int AHEAD = T <= (PARTS > 1 ? 1 : SPAN == 4 ? 3 : 2) ? 2 : 1;
+    MmChunk<SPAN> held[AHEAD + 1][MM_R];
     auto load = [&](uint32_t c, MmChunk<SPAN> (&o)[MM_R]) {
 #pragma unroll
         for (int r = 0; r < MM_R; ++r) {
@@ -121,7 +125,7 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
     // last again, columns past the last are zeros. Held as loaded, made operands when they are stored. A row is at most
     // 2^24 values after the one before, so that a tile's 64 are within 32 bits of its first.
     constexpr int RAW = TYPE == ROW_F32 ? 2 : 1;
-    gd_u32x4 raw[PER][RAW];
+    gd_u32x4 raws[AHEAD == 1 ? 1 : 3][PER][RAW];
     uint32_t from[PER];
 #pragma unroll
     for (uint32_t k = 0; k < PER; ++k) {
@@ -129,14 +133,17 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
         from[k] = (row * (uint32_t)xs + 8u * (i & 15u)) << row_shift(TYPE);
     }
     const uint64_t X0 = X + (((uint64_t)t0 * xs) << row_shift(TYPE));
-    auto fetch = [&](uint32_t c) {
+    auto fetch = [&](uint32_t c, gd_u32x4 (&raw)[PER][RAW]) {
         const uint64_t base = X0 + ((uint64_t)(c * 128u) << row_shift(TYPE));
         const uint32_t left = cols - c * 128u;
-        if (left >= 128u) {
+        // (Where chunks are asked for two ahead, no branch may make their number uncertain: the last one's missing columns
+        // read its first, and store() drops them.)
+        const uint32_t back = AHEAD > 1 && 8u * (tid & 15u) >= left ? (8u * (tid & 15u)) << row_shift(TYPE) : 0u;
+        if (AHEAD > 1 || left >= 128u) {
 #pragma unroll
             for (uint32_t k = 0; k < PER; ++k)
 #pragma unroll
-                for (int q = 0; q < RAW; ++q) raw[k][q] = gd_load<gd_u32x4_any>(base, from[k] + 16u * q);
+                for (int q = 0; q < RAW; ++q) raw[k][q] = gd_load<gd_u32x4_any>(base, from[k] - back + 16u * q);
         } else {
 #pragma unroll
             for (uint32_t k = 0; k < PER; ++k)
@@ -147,7 +154,14 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
                 }
         }
     };
-    auto store = [&](uint32_t buffer) {
+    auto store = [&](uint32_t c, gd_u32x4 (&raw)[PER][RAW]) {
+        const uint32_t buffer = c & 1u;
+        if (AHEAD > 1 && 8u * (tid & 15u) >= cols - c * 128u) {
+#pragma unroll
+            for (uint32_t k = 0; k < PER; ++k)
+#pragma unroll
+                for (int q = 0; q < RAW; ++q) raw[k][q] = gd_u32x4{0u, 0u, 0u, 0u};
+        }
 #pragma unroll
         for (uint32_t k = 0; k < PER; ++k) {
             const uint32_t i = tid + 256u * k, row = i >> 4, at = row * 16u + ((i & 15u) ^ (row & 15u));
@@ -184,16 +198,16 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
     for (int r = 0; r < MM_R; ++r)
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[r][t] = zero;
-    load(0, cur);
-    fetch(0);
-    store(0);
-    for (uint32_t c = 0; c < chunks; ++c) {
-        __syncthreads();
-        const bool more = c + 1u < chunks;
-        if (more) {
-            fetch(c + 1u);
-            load(c + 1u, next);
-        }
+    load(0, held[0]);
+    fetch(0, raws[0]);
+    store(0, raws[0]);
+    const uint32_t last = chunks - 1u;
+    if constexpr (AHEAD > 1) {
+        fetch(min(1u, last), raws[1]);
+        load(min(1u, last), held[1]);
+    }
+    // The products of chunk c.
+    auto multiply = [&](uint32_t c, MmChunk<SPAN> (&cur)[MM_R]) {
         const uint32_t buffer = c & 1u;
         const gd_u32x4 *const xl = lds + buffer * (UNITS * PARTS);
         gd_u32x4 x[PAIR][T][PARTS];
@@ -267,10 +281,39 @@ __device__ __forceinline__ void mm_q4_tile(const GdArgs &a, gd_u32x4 *lds, float
             __builtin_amdgcn_sched_barrier(0);
         }
         scale(MM_R - 1, 3u);
-        if (more) {
-            store((c + 1u) & 1u);  // its readers passed the barrier above
+    };
+    if constexpr (AHEAD > 1) {
+        // Three sets of registers in turn: a copy of what is on its way would wait for it.
+        auto step = [&](uint32_t c, MmChunk<SPAN> (&cur)[MM_R], MmChunk<SPAN> (&second)[MM_R], gd_u32x4 (&raw)[PER][RAW],
+                        gd_u32x4 (&raw2)[PER][RAW]) {
+            __syncthreads();
+            fetch(min(c + 2u, last), raw2);
+            load(min(c + 2u, last), second);
+            multiply(c, cur);
+            if (c < last) store(c + 1u, raw);  // its buffer's readers passed the barrier above
+        };
+#pragma unroll 1
+        for (uint32_t c = 0;; c += 3u) {
+            step(c, held[0], held[2], raws[1], raws[2]);
+            if (c + 1u > last) break;
+            step(c + 1u, held[1], held[0], raws[2], raws[0]);
+            if (c + 2u > last) break;
+            step(c + 2u, held[2], held[1], raws[0], raws[1]);
+            if (c + 3u > last) break;
+        }
+    } else {
+        for (uint32_t c = 0; c < chunks; ++c) {
+            __syncthreads();
+            if (c < last) {
+                fetch(c + 1u, raws[0]);
+                load(c + 1u, held[1]);
+            }
+            multiply(c, held[0]);
+            if (c < last) {
+                store(c + 1u, raws[0]);  // its buffer's readers passed the barrier above
 #pragma unroll
-            for (int r = 0; r < MM_R; ++r) cur[r] = next[r];
+                for (int r = 0; r < MM_R; ++r) held[0][r] = held[1][r];
+            }
         }
     }
     // Sums go out through LDS as runs of 64 neighbouring outputs (32 of a gated pair), four to a lane: row r of token k at
