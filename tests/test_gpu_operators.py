@@ -133,6 +133,41 @@ def test_linear_many_tokens_exact(eng, fmt, group, mins, x):
         eng.release_matrix(index)
 
 
+@pytest.mark.parametrize("group,mins", [(32, False), (64, True), (128, False)])
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+def test_linear_many_tokens_chunks(eng, group, mins, x):
+    """One to eight chunks of 128 columns, the last one whole or not, by 16 to 64 tokens a group."""
+    rng = np.random.default_rng(group + ord(x[0]))
+    for chunks in range(1, 9):
+        for cols in {128 * chunks, 128 * chunks - (96 if group == 32 else 64 if group == 64 else 0)}:
+            index, ((_, W, _, _),) = add(eng, rng, "q4", 30001, cols, group, mins, False, True)
+            for n in (17, 30, 47, 60):
+                print(f"chunks, group {group} mins {mins} x {x}: {cols} columns, {n} tokens", flush=True)
+                xs = integers(rng, n, cols)
+                yd = torch.zeros(n, 30001, device="cuda")
+                eng.linear(index, xs.to(ref.DTYPES[x]).cuda(), yd, stream=stream())
+                assert torch.equal(yd.cpu().double(), xs @ W.T)
+            eng.release_matrix(index)
+
+
+def test_linear_many_tokens_graph(eng):
+    """A captured product of many tokens, replayed with eager ones of other inputs between."""
+    rng = np.random.default_rng(12)
+    index, ((_, W, _, _),) = add(eng, rng, "q4_0", 20000, 640, 32, False, False, True)
+    xs = [integers(rng, 40, 640) for _ in range(4)]
+    x, y, other = torch.zeros(40, 640, device="cuda"), torch.zeros(40, 20000, device="cuda"), torch.zeros(40, 20000, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        eng.linear(index, x, y, stream=stream())
+    for i in range(4):
+        x.copy_(xs[i])
+        g.replay()
+        eng.linear(index, xs[i - 1].float().cuda(), other, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(y.cpu().double(), xs[i] @ W.T) and torch.equal(other.cpu().double(), xs[i - 1] @ W.T)
+    eng.release_matrix(index)
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "f16"), ("f16", "bf16")])
 @pytest.mark.parametrize("rows,cols,n,fmt,group,mins", [(20001, 640, 50, "q4_0", 32, False), (20001, 384, 70, "q4", 128, True),
