@@ -36,8 +36,11 @@ struct LpSums {
     float m, s, t;
 };
 
-// scale (a - b), at least -1e30 so that an exp of 0 times it is 0.
-__device__ __forceinline__ float lp_diff(float a, float b, float scale) { return fmaxf(scale * (a - b), -1e30f); }
+// A distance whose exp is 0, and which a sum of up to 2^31 terms may be multiplied by within fp32's range: 0 times either is 0.
+#define LP_FAR -1e28f
+
+// scale (a - b), LP_FAR at least.
+__device__ __forceinline__ float lp_diff(float a, float b, float scale) { return fmaxf(scale * (a - b), LP_FAR); }
 
 // Moves p's sums to the maximum m >= p.m (-infinity: there is no term yet, and any reference will do).
 __device__ __forceinline__ void lp_move(LpSums &p, float m, float scale) {
@@ -446,7 +449,7 @@ __device__ __forceinline__ void logprobs_body(const GdArgs &a) {
         for (uint32_t i = 0; i < LP_VALUES; ++i) {
             const float d = scale * (x[i] - ref), e = __expf(d);
             s += e;
-            t += e * fmaxf(d, -1e30f);
+            t += e * fmaxf(d, LP_FAR);
         }
         p.s += s;
         p.t += t;

@@ -1,0 +1,46 @@
+"""Log probabilities at the far ends of what the call takes, against 64 bits."""
+import pytest
+import torch
+
+from gyrodx.engine import Engine
+
+pytestmark = pytest.mark.gpu
+ULP = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def eng():
+    e = Engine(max_tok=8)
+    yield e
+    e.close()
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def test_masked_part_of_a_long_row(eng):
+    """A part of a row that holds nothing but 3.6e8 masked logits of the type's lowest value: joined with the other part
+    it adds nothing, though its sum times the distance of the maxima is past fp32's range. 512 rows take two parts each;
+    they are one row in memory.
+
+    The other part has 1000 logits that count, each within 4 2^-24 (1 + |d|), summed in at most 64 steps."""
+    n, V, kept = 512, 720_000_000, 1000
+    print(f"{n} rows of {V} logits, {V - kept} masked", flush=True)
+    row = torch.full((1, V), torch.finfo(torch.bfloat16).min, dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(kept, generator=torch.Generator().manual_seed(3)).bfloat16()
+    at = torch.arange(kept) * 13 + V - 20_000
+    row[0, at.cuda()] = x.cuda()
+    tokens = torch.tensor([[int(at[7]), 5]], device="cuda").expand(n, 2).contiguous()
+    lp, H = torch.full((n, 2), 7.0, device="cuda"), torch.full((n,), 7.0, device="cuda")
+    ws = torch.empty(eng.logprobs_workspace(n, V), dtype=torch.uint8, device="cuda")
+    eng.logprobs(row.expand(n, V), ws, tokens=tokens, logprob=lp, entropy=H, stream=stream())
+    torch.cuda.synchronize()
+    d = x.double() - x.double().max()
+    S, T = d.exp().sum(), (d * d.exp()).sum()
+    logs, ts = float(S.log()), float((T / S).abs())
+    rel = (64 + 4 * (1 + float(d.abs().max()))) * ULP
+    entropy, own = float((H.cpu().double() - (logs + ts)).abs().max()), float((lp[:, 0].cpu().double() - (float(d[7]) - logs)).abs().max())
+    assert entropy <= rel * (2 + 2 * ts) + 4 * ULP * (logs + 1)
+    assert own <= rel + 4 * ULP * (abs(float(d[7])) + logs + 1)
+    assert bool((lp[:, 1] < -3e38).all())
