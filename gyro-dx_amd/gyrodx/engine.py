@@ -367,7 +367,7 @@ class Engine:
 
     @staticmethod
     def logprobs_workspace(n: int, V: int, top: int = 0) -> int:
-        """Bytes of the workspace that logprobs() of n rows of V logits takes."""
+        """Bytes of a workspace that suffices for logprobs() of up to n rows of V logits."""
         return lib().gm_logprobs_workspace(n, V, top)
 
     def logprobs(self, logits, workspace=None, tokens=None, logprob=None, entropy=None, top_ids=None,

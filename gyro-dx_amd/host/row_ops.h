@@ -258,9 +258,13 @@ class RowOps {
         const uint32_t batches = (V + 1023) / 1024;
         return std::max(1u, std::min({32u, (batches + 3) / 4, 1024 / std::max(1u, n)}));
     }
+    static uint64_t logprobs_part_bytes(uint32_t top) { return 16 + 8ull * ((top + 1) & ~1u); }
+    // Bytes that every call of up to n rows finds enough: the most parts of any such call, p to each of the most rows that
+    // are split into p (so at most 1024 parts).
     static uint64_t logprobs_workspace(uint32_t n, uint32_t V, uint32_t top) {
-        const uint32_t parts = logprobs_parts(n, V);
-        return parts == 1 ? 0 : (uint64_t)n * parts * (16 + 8ull * ((top + 1) & ~1u));
+        uint64_t most = 0;
+        for (uint32_t p = logprobs_parts(1, V); p > 1; --p) most = std::max(most, (uint64_t)p * std::min(n, 1024 / p));
+        return most * logprobs_part_bytes(top);
     }
 
     static Launch logprobs(const gm_logprobs_desc &d, uint32_t n) {
@@ -277,7 +281,8 @@ class RowOps {
                            (uintptr_t)d.top_logprobs % 4 == 0 && (n <= 1 || d.top_stride >= d.top)),
                 "gm_logprobs: top_ids and top_logprobs");
         require((uintptr_t)d.entropy % 4 == 0 && (d.given || d.entropy || d.top), "gm_logprobs: no output");
-        const uint64_t need = logprobs_workspace(n, d.V, d.top);
+        const uint32_t parts = logprobs_parts(n, d.V);
+        const uint64_t need = parts == 1 ? 0 : (uint64_t)n * parts * logprobs_part_bytes(d.top);
         require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0),
                 "gm_logprobs: workspace");
         Constants &c = l.c;
@@ -298,7 +303,6 @@ class RowOps {
         c.set(22, d.top_logprobs);
         c.set64(24, d.top_stride);
         c.set(26, n);
-        const uint32_t parts = logprobs_parts(n, d.V);
         c.set(27, parts);
         c.set(28, d.workspace);
         l.kernel = d.logits.type == GM_F32 ? "logprobs" : d.logits.type == GM_BF16 ? "logprobs_b" : "logprobs_h";

@@ -88,8 +88,8 @@ GM_API int gm_block_norm(gm_engine *e, const gm_block_norm_desc *desc, uint32_t 
  *   top_ids[t][k], top_logprobs[t][k]  the `top` <= 64 largest logits, equal ones by id, and their log p
  * A logit of -infinity has p = 0. A row of nothing but those has log p -infinity everywhere and entropy 0; one with a NaN or
  * +infinity has NaN for both (top_ids still order the logits, NaNs first). Strides count values. The
- * workspace (gm_logprobs_workspace bytes, 256-byte aligned; may be NULL where that is 0) holds nothing between calls;
- * calls that may overlap, replayed graphs among them, take one each. */
+ * workspace (256-byte aligned; may be NULL where gm_logprobs_workspace is 0) holds nothing between calls; calls that may
+ * overlap, replayed graphs among them, take one each. */
 typedef struct gm_logprobs_desc {
     gm_rows logits;
     uint32_t V, given, top, tokens_64;
@@ -106,6 +106,8 @@ typedef struct gm_logprobs_desc {
     void *workspace;
     uint64_t workspace_bytes;
 } gm_logprobs_desc;
+/* Bytes that suffice for every call of up to n rows (few rows are split over more groups than many, and take more of them
+ * than n rows may). */
 GM_API uint64_t gm_logprobs_workspace(uint32_t n, uint32_t V, uint32_t top);
 GM_API int gm_logprobs(gm_engine *e, const gm_logprobs_desc *desc, uint32_t n, void *stream);
 

@@ -44,3 +44,20 @@ def test_masked_part_of_a_long_row(eng):
     assert entropy <= rel * (2 + 2 * ts) + 4 * ULP * (logs + 1)
     assert own <= rel + 4 * ULP * (abs(float(d[7])) + logs + 1)
     assert bool((lp[:, 1] < -3e38).all())
+
+
+def test_one_workspace_for_every_batch(eng):
+    """A workspace taken for 1024 rows serves the smaller batches, which are split over more groups a row; S sums 20000
+    terms, each within 4 2^-24 (1 + |d|) and |d| < 25, at most 20000 / 256 + 32 in a row."""
+    V, top = 20_000, 5
+    ws = torch.full((eng.logprobs_workspace(1024, V, top),), 0xA5, dtype=torch.uint8, device="cuda")
+    x = torch.randn(1024, V, generator=torch.Generator().manual_seed(4)) * 2.5
+    want = torch.log_softmax(x.double(), -1)
+    xd, tol = x.cuda(), (V / 256 + 32 + 4 * 26) * ULP + 8 * ULP * 25
+    for n in (1024, 1, 64, 513, 300, 37, 512):
+        print(f"{n} rows in the workspace of 1024", flush=True)
+        ids, lp = torch.full((n, top), -1, dtype=torch.int32, device="cuda"), torch.zeros(n, top, device="cuda")
+        eng.logprobs(xd[:n], ws, top_ids=ids, top_logprobs=lp, stream=stream())
+        best = torch.sort(x[:n], dim=-1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(ids.cpu().long(), best)
+        assert float((lp.cpu().double() - want[:n].gather(1, best)).abs().max()) <= tol

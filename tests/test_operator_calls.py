@@ -282,3 +282,20 @@ def test_workspace_sizes():
     for n in (1, 5, 64, 1023, 70000):
         for V in (1, 50, 4096, 131072):
             assert f(n, V, 0) <= f(n, V, min(V, 64)) < 1 << 40
+
+
+@pytest.mark.parametrize("V", [1000, 4097, 9000, 40000, 131072, (1 << 31) - 1])
+@pytest.mark.parametrize("top", [0, 5, 64])
+def test_workspace_serves_smaller_batches(shim, V, top):
+    """The workspace of the largest batch is enough for every smaller one, and no more than some batch needs."""
+    f = engine.lib().gm_logprobs_workspace
+    sizes = [*range(70), 85, 86, 127, 128, 129, 204, 205, 255, 256, 257, 341, 342, 511, 512, 513, 700, 1024, 1025, 70000]
+
+    def taken(n, bytes):
+        return call(shim.plan_logprobs, lp(V=V, top=top, top_stride=top, workspace_bytes=bytes), n)[0] == 0
+
+    for i, n in enumerate(sizes):
+        assert all(taken(m, f(n, V, top)) for m in sizes[:i + 1]), n
+    most = f(70000, V, top)
+    assert most <= 1024 * (16 + 8 * (top + 1))
+    assert most == 0 or any(not taken(m, most - 1) for m in range(1, 1025))
