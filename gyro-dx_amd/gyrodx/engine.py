@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import sys
 
 import numpy as np
 
@@ -265,7 +266,13 @@ class Engine:
     # ---- operators around the layers, on device tensors ------------------------------------------
     # Tensors are torch tensors (or objects with their shape, dtype, stride(), data_ptr() and get_device()) on the
     # engine's GPU; `stream` is a hipStream_t as torch gives it (torch.cuda.current_stream().cuda_stream; 0 is the
-    # default stream). Each call queues its work and returns. include/gyro_ops.h states the formulas.
+    # default stream; None torch's current stream on the engine's GPU, which takes 3 us to look up). Each call queues its
+    # work and returns. include/gyro_ops.h states the formulas.
+
+    def _stream(self):
+        """Torch's current stream on the engine's GPU, or the default one where torch does not use the GPU."""
+        torch = sys.modules.get("torch")
+        return torch.cuda.current_stream(self.adapter).cuda_stream if torch and torch.cuda.is_initialized() else 0
 
     def load_operators(self):
         """Loads the operators' kernels, so that first calls may be captured into a graph."""
@@ -330,20 +337,21 @@ class Engine:
         return t.data_ptr()
 
     def linear(self, matrix: int, x, y, act: str = "none", accumulate: bool = False, scale: float = 1.0,
-               stream: int = 0):
+               stream: int | None = None):
         """y = act(scale W x) per row (+ y with accumulate), or scale silu(G x) * (U x) of a gated pair."""
         if matrix not in self._matrices:
             raise ValueError(f"no matrix {matrix}")
         rows, cols = self._matrices[matrix]
         n = x.shape[0]
         rc = lib().gm_linear(self._h, matrix, _PACK_ROWS(*self._rows(x, (n, cols), "x"), 0), n,
-                             _PACK_ROWS(*self._rows(y, (n, rows), "y"), 0), ACTS[act], accumulate, scale, stream)
+                             _PACK_ROWS(*self._rows(y, (n, rows), "y"), 0), ACTS[act], accumulate, scale,
+                             self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_linear")
 
     def block_norm(self, h, x, out=None, normed=None, post: bool = False, post_weight=None, post_eps: float = 1e-6,
                    gate=None, gate_act: str = "none", scale: float = 1.0, pre_weight=None, pre_eps: float = 1e-6,
-                   stream: int = 0):
+                   stream: int | None = None):
         """out = v = x + scale * gate * a with a = RMSNorm(h) (post) or h, normed = RMSNorm(v). `gate` is [n, 1] (per
         token), [1, E] (per channel) or [n, E]; weights are fp32 [E]. h None: v = x."""
         shape = tuple(x.shape)
@@ -361,7 +369,7 @@ class Engine:
                        self._flat(post_weight, E, _FLOAT, "post_weight") if post_weight is not None else 0,
                        self._flat(pre_weight, E, _FLOAT, "pre_weight") if pre_weight is not None else 0,
                        post_eps, pre_eps, scale, 0)
-        rc = lib().gm_block_norm(self._h, d, n, stream)
+        rc = lib().gm_block_norm(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_block_norm")
 
@@ -371,7 +379,7 @@ class Engine:
         return lib().gm_logprobs_workspace(n, V, top)
 
     def logprobs(self, logits, workspace=None, tokens=None, logprob=None, entropy=None, top_ids=None,
-                 top_logprobs=None, scale: float = 1.0, stream: int = 0):
+                 top_logprobs=None, scale: float = 1.0, stream: int | None = None):
         """Log probabilities of `tokens` (int32 or int64 [n, given]) under softmax(scale * logits) into logprob (fp32
         [n, given]), the entropy (fp32 [n]), and the largest logits' ids (int32 [n, top]) and log probabilities.
         workspace: a uint8 tensor of at least logprobs_workspace() bytes, not shared with calls that may overlap."""
@@ -398,6 +406,6 @@ class Engine:
             ws = self._flat(workspace, ws_bytes, _UINT8, "workspace")
         d = _PACK_LOGPROBS(*x, 0, V, given, top, wide, scale, 0, tp, given, lp, given,
                            self._flat(entropy, n, _FLOAT, "entropy") if entropy is not None else 0, ip, kp, top, ws, ws_bytes)
-        rc = lib().gm_logprobs(self._h, d, n, stream)
+        rc = lib().gm_logprobs(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_logprobs")

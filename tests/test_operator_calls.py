@@ -299,3 +299,29 @@ def test_workspace_serves_smaller_batches(shim, V, top):
     most = f(70000, V, top)
     assert most <= 1024 * (16 + 8 * (top + 1))
     assert most == 0 or any(not taken(m, most - 1) for m in range(1, 1025))
+
+
+def test_default_stream_is_torchs_current(eng, monkeypatch):
+    """A call without a stream goes to torch's current one on the engine's GPU, one with a stream to that."""
+    queued = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: queued.append((name, args[-1])) or 0
+
+    class Stream:
+        cuda_stream = 0x5150
+
+    monkeypatch.setattr(engine, "lib", Library)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: Stream if device == -1 else None)
+    x, y = torch.zeros(3, 96), torch.zeros(3, 64)
+    for kw, want in (({}, 0x5150), (dict(stream=0), 0), (dict(stream=7), 7)):
+        eng.linear(0, x, y, **kw)
+        eng.block_norm(None, x, x, **kw)
+        eng.logprobs(x, entropy=torch.zeros(3), **kw)
+        assert queued == [("gm_linear", want), ("gm_block_norm", want), ("gm_logprobs", want)]
+        queued.clear()
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: False)
+    eng.linear(0, x, y)
+    assert queued == [("gm_linear", 0)]
