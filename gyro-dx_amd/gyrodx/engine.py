@@ -63,6 +63,13 @@ _PACK_LOGPROBS = struct.Struct("@PQII4IfIPQPQPPPQPQ").pack
 _NO_ROWS = (0, 0, 0)
 
 
+def _count(n, what):
+    """n, which the library takes in 32 bits (ctypes would drop the rest)."""
+    if not 0 <= n <= 0xffffffff:
+        raise ValueError(f"{what}: {n} is not a 32-bit count")
+    return n
+
+
 def _type(t, allowed, what):
     code = _type_codes.get(t.dtype)
     if code is None:
@@ -284,6 +291,8 @@ class Engine:
         cols / group], mins float16 or None)."""
         if fmt not in MATRIX_FORMATS:
             raise ValueError(f"matrix format {fmt!r} is none of {sorted(MATRIX_FORMATS)}")
+        for value, what in ((rows, "rows"), (cols, "cols"), (group, "group")):
+            _count(value, what)
         keep = []
 
         def parts(m):
@@ -312,6 +321,7 @@ class Engine:
         return idx.value
 
     def release_matrix(self, matrix: int):
+        _count(matrix, "matrix")
         if self._h:
             self._check(lib().gm_release_matrix(self._h, matrix), "gm_release_matrix")
             self._matrices.pop(matrix, None)
@@ -342,7 +352,7 @@ class Engine:
         if matrix not in self._matrices:
             raise ValueError(f"no matrix {matrix}")
         rows, cols = self._matrices[matrix]
-        n = x.shape[0]
+        n = _count(x.shape[0], "rows of x")
         rc = lib().gm_linear(self._h, matrix, _PACK_ROWS(*self._rows(x, (n, cols), "x"), 0), n,
                              _PACK_ROWS(*self._rows(y, (n, rows), "y"), 0), ACTS[act], accumulate, scale,
                              self._stream() if stream is None else stream)
@@ -356,6 +366,8 @@ class Engine:
         token), [1, E] (per channel) or [n, E]; weights are fp32 [E]. h None: v = x."""
         shape = tuple(x.shape)
         n, E = shape
+        _count(n, "rows of x")
+        _count(E, "values of a row")
         kind, g = 0, _NO_ROWS
         if gate is not None:
             gs = tuple(gate.shape)
@@ -376,7 +388,7 @@ class Engine:
     @staticmethod
     def logprobs_workspace(n: int, V: int, top: int = 0) -> int:
         """Bytes of a workspace that suffices for logprobs() of up to n rows of V logits."""
-        return lib().gm_logprobs_workspace(n, V, top)
+        return lib().gm_logprobs_workspace(_count(n, "n"), _count(V, "V"), _count(top, "top"))
 
     def logprobs(self, logits, workspace=None, tokens=None, logprob=None, entropy=None, top_ids=None,
                  top_logprobs=None, scale: float = 1.0, stream: int | None = None):
@@ -384,6 +396,8 @@ class Engine:
         [n, given]), the entropy (fp32 [n]), and the largest logits' ids (int32 [n, top]) and log probabilities.
         workspace: a uint8 tensor of at least logprobs_workspace() bytes, not shared with calls that may overlap."""
         n, V = logits.shape
+        _count(n, "rows of logits")
+        _count(V, "logits of a row")
         x = self._rows(logits, (n, V), "logits")
         given = top = wide = ws_bytes = tp = lp = ip = kp = ws = 0
         if tokens is not None:

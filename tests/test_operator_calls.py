@@ -325,3 +325,18 @@ def test_default_stream_is_torchs_current(eng, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_initialized", lambda: False)
     eng.linear(0, x, y)
     assert queued == [("gm_linear", 0)]
+
+
+def test_counts_past_32_bits(eng):
+    """Rows, sizes and indices that the library's 32-bit counts cannot hold are refused, not cut to their low bits."""
+    many, row = (1 << 32) + 1, torch.zeros(1, 96)
+    x, y = row.expand(many, 96), torch.zeros(1, 64).expand(many, 64)
+    long = torch.zeros(1).expand(1, (1 << 32) + 8)
+    refused(eng.linear, 0, x, y)
+    refused(eng.block_norm, None, x, x)
+    refused(eng.logprobs, x, entropy=torch.zeros(1).expand(many))
+    for f, args in ((eng.block_norm, (None, long, long)), (eng.logprobs, (long,)), (eng.release_matrix, (1 << 32,)),
+                    (eng.release_matrix, (-1,)), (Engine.logprobs_workspace, (1 << 32, 1000)), (Engine.logprobs_workspace, (-1, 1000)),
+                    (Engine.logprobs_workspace, (4, (1 << 32) + 1000, 5)), (eng.add_matrix, ("q4_0", (1 << 32) + 4, 64, None))):
+        with pytest.raises(ValueError, match="32-bit"):
+            f(*args)
