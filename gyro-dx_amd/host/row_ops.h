@@ -215,6 +215,11 @@ class RowOps {
         if (d.h.data) check_rows(d.h, n, d.E, false, "gm_block_norm: h");
         if (d.out.data) check_rows(d.out, n, d.E, true, "gm_block_norm: out");
         if (d.normed.data) check_rows(d.normed, n, d.E, true, "gm_block_norm: normed");
+        // In place a thread writes where it has read; rows of another layout would reach into its neighbours'.
+        for (const gm_rows *in : {&d.x, &d.h})
+            for (const gm_rows *to : {&d.out, &d.normed})
+                require(!in->data || in->data != to->data || (in->type == to->type && (n == 1 || in->stride == to->stride)),
+                        "gm_block_norm: rows in place have one type and stride");
         require(d.gate_kind <= GM_GATE_VALUE && (d.gate_act == GM_ACT_NONE || d.gate_act == GM_ACT_SIGMOID), "gm_block_norm: gate");
         const bool gate = d.gate_kind != GM_GATE_NONE;
         require(d.h.data || (!gate && !d.post), "gm_block_norm: a gate or a post norm without h");

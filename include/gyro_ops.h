@@ -70,7 +70,8 @@ GM_API int gm_linear(gm_engine *e, uint32_t matrix, const gm_rows *x, uint32_t n
  *   out = v;  normed = v / sqrt(mean(v^2) + pre_eps) * pre_weight
  * in fp32, normed from the unrounded v. gate: GM_GATE_NONE; one value per token (value t at t * stride), per
  * channel [E], or per value; through a sigmoid with gate_act GM_ACT_SIGMOID. out or normed may be absent (data NULL),
- * not both. out may be x's rows, normed h's. Weights fp32 [E], on the device. */
+ * not both. out may be x's rows, normed h's, of the same type and stride (another layout at the same address is refused);
+ * outputs overlap nothing else. Weights fp32 [E], on the device. */
 enum { GM_GATE_NONE = 0, GM_GATE_TOKEN = 1, GM_GATE_CHANNEL = 2, GM_GATE_VALUE = 3 };
 typedef struct gm_block_norm_desc {
     uint32_t E, post, gate_kind, gate_act;

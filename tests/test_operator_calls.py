@@ -340,3 +340,17 @@ def test_counts_past_32_bits(eng):
                     (Engine.logprobs_workspace, (4, (1 << 32) + 1000, 5)), (eng.add_matrix, ("q4_0", (1 << 32) + 4, 64, None))):
         with pytest.raises(ValueError, match="32-bit"):
             f(*args)
+
+
+def test_block_norm_in_place_layouts(shim):
+    """Outputs at an input's address have its type and stride; one row has no stride."""
+    def takes(n, **kw):
+        apart = dict(h=rows(data=A), x=rows(data=2 * A), out=rows(data=3 * A), normed=rows(data=4 * A))
+        return call(shim.plan_norm, norm(**{**apart, **kw}), n)[0] == 0
+
+    for to, at in (("out", 2 * A), ("normed", A), ("out", A), ("normed", 2 * A)):
+        assert takes(3, **{to: rows(data=at)}) and takes(1, **{to: rows(data=at, stride=100)})
+        assert not takes(3, **{to: rows(data=at, stride=100)})
+        assert not takes(3, **{to: rows(1, data=at)}) and not takes(1, **{to: rows(2, data=at)})
+    assert takes(3, out=rows(1, data=3 * A, stride=100))
+    assert takes(3, h=Rows(), out=Rows()) and takes(3, h=Rows(), normed=Rows())
