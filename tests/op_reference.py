@@ -102,3 +102,20 @@ def logprobs(x, tokens, scale):
     given = lp.gather(1, torch.where(inside, tokens, 0).long())
     given = torch.where(inside, given, torch.where(tokens < 0, 0.0, np.nan))
     return given, H, lp, m, logs, T / S
+
+
+# Products for which a group of the few-token kernel takes a second run of rows: (rows, cols, fmt, group, mins, gated, x,
+# tokens, whether its LDS holds all columns of the tokens).
+SECOND_RUNS = [
+    (66001, 256, "q4_0", 32, False, False, "f32", 1, True), (66001, 256, "q4", 64, True, False, "f32", 5, True),
+    (100003, 384, "q4_1", 32, True, False, "bf16", 16, True), (66001, 256, "q4", 128, False, False, "f16", 8, True),
+    (40009, 256, "q4_0", 32, False, True, "f32", 3, True), (40009, 256, "q4", 64, True, True, "bf16", 1, True),
+    (132001, 96, "q4_0", 32, False, False, "f32", 1, True),
+    (66001, 2304, "q4_0", 32, False, False, "bf16", 16, False), (66001, 2400, "q4_1", 32, True, False, "f32", 5, False),
+    (33001, 2304, "q4", 128, True, True, "f16", 8, False)]
+
+
+def repeated(data, times, rows):
+    """A matrix's data (random_matrix) repeated and cut to `rows` rows."""
+    cut = lambda a: None if a is None else np.tile(a, (times, 1))[:rows]  # noqa: E731
+    return tuple(cut(a) for a in data) if isinstance(data, tuple) else cut(data)

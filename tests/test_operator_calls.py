@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import op_reference as ref
 from gyrodx import engine
 from gyrodx.engine import BlockNormDesc, Engine, LogprobsDesc, MatrixDesc, Rows
 from test_abi import declared, exported
@@ -354,3 +355,20 @@ def test_block_norm_in_place_layouts(shim):
         assert not takes(3, **{to: rows(1, data=at)}) and not takes(1, **{to: rows(2, data=at)})
     assert takes(3, out=rows(1, data=3 * A, stride=100))
     assert takes(3, h=Rows(), out=Rows()) and takes(3, h=Rows(), normed=Rows())
+
+
+@pytest.mark.parametrize("case", ref.SECOND_RUNS)
+def test_second_runs(shim, case):
+    """The products that tests run for it do take the few-token kernel with more runs of rows than groups."""
+    r, cols, fmt, group, mins, gated, x, n, whole = case
+    d = matrix(engine.MATRIX_FORMATS[fmt], r, cols, group, mins=A if mins and fmt == "q4" else None)
+    if gated:
+        d.up_quants = A
+        d.up_scales, d.up_mins = d.scales, d.mins
+    type, out, why = ("f32", "bf16", "f16").index(x), (C.c_uint32 * 62)(), C.create_string_buffer(200)
+    a, b = rows(type, 1 << 12), rows(stride=r)
+    assert shim.plan_linear(C.byref(d), C.byref(a), n, C.byref(b), 0, 0, 1.0, out, why) == 0
+    tiles, chunks, wk = out[2 + 6], out[2 + 7], out[2 + 26]
+    runs, operands = -(-tiles // (2 * (8 // wk))), n * (3, 1, 2)[type]
+    assert why.value.decode() == ("mv_q4_m" if mins else "mv_q4") and out[1] == 1 and runs > out[0]
+    assert whole == ((81920 - 8 * 2 * operands * 64) // (operands * 256) >= chunks)
