@@ -5,7 +5,8 @@
 // exactly. Those extra 16 (24 where W = s (q - 8)) times the group's sum of activations go in as the product's C
 // operand, itself the product of the activations with a constant matrix, so nothing of the group's sum is kept
 // apart, and it is at most five times what the group's own product rounds at. Group sums are scaled and added
-// in fp32. Activations are exact: an fp32 value is the sum of three bf16 values (its 24 bits cut in eights).
+// in fp32. Activations are exact: an fp32 value is the sum of three bf16 values (its 24 bits cut in eights). The matrix unit
+// takes bf16 values below 2^-126 as zero, so from 2^-103 on an activation keeps all its bits.
 // Of a token with an infinity or NaN no output is finite: every group's product and sum with it are not, and no scale
 // makes them so.
 //

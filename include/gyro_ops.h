@@ -57,9 +57,9 @@ GM_API int gm_release_matrix(gm_engine *e, uint32_t matrix);
 /* y[t] = act(scale W x[t]) for n tokens, x [n][cols], y [n][rows]; with accumulate, the sum is added to y
  * (after act, in fp32). A gated pair: y[t] = scale silu(G x[t]) * (U x[t]), act GM_ACT_NONE. Activations and sums
  * are fp32 whatever the types (products are exact in them); y is rounded once. Activations
- * are below 2^116 in magnitude (a group's sums of products with 0 .. 31 stay in range then). Of a token with an
- * activation that is not finite no output is (a NaN or an infinity). Two or more rows of x are at most 2^24
- * values apart, n at most 2^18; y must not overlap x. */
+ * are below 2^116 in magnitude (a group's sums of products with 0 .. 31 stay in range then); of fp32 and bf16 ones below
+ * 2^-103 what is below 2^-126 counts as zero. Of a token with an activation that is not finite no output is (a NaN or an
+ * infinity). Two or more rows of x are at most 2^24 values apart, n at most 2^18; y must not overlap x. */
 enum { GM_ACT_NONE = 0, GM_ACT_SILU = 1, GM_ACT_SIGMOID = 2 };
 GM_API int gm_linear(gm_engine *e, uint32_t matrix, const gm_rows *x, uint32_t n, const gm_rows *y, uint32_t act,
                      uint32_t accumulate, float scale, void *stream);

@@ -140,3 +140,22 @@ def test_few_token_epilogue_in_16_bits(eng, yt, act):
     assert ((yd.cpu().double() - want).abs() <= tol + half_step(ref.DTYPES[yt]) * (want.abs() + tol) + 2.0 ** -25 * (yt == "f16")).all()
     assert ref.untouched(buf, yd, 2.0)
     eng.release_matrix(index)
+
+
+@pytest.mark.parametrize("n,rows", [(4, 64), (50, 20000)])
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("size", [1e-31, 1e-34, 1e-36])
+def test_smallest_activations(eng, size, mins, n, rows):
+    """Of an fp32 activation below 2^-103 what is below 2^-126 counts as zero, and no more: 2^-126 sum |W| beside the roundings of
+    (76 + groups) 2^-23 of 55 |s| sum |x| + |m| sum |x|; the minimum and the 16 that go through other sums may keep it, 2^-126
+    of the sum of both at most."""
+    rng = np.random.default_rng(9)
+    data, W, s, m = ref.random_matrix(rng, "q4", rows, 256, 64, mins, True)
+    index = eng.add_matrix("q4", rows, 256, data, group=64)
+    x = torch.from_numpy(rng.standard_normal((n, 256)) * size).float()
+    yd = torch.zeros(n, rows, device="cuda")
+    eng.linear(index, x.cuda(), yd, stream=stream())
+    x = x.double()
+    bound = (76 + 4) * 2 * ULP * (x.abs() @ (55 * s + m).T) + 2.0 ** -126 * (16 * s + m + W.abs()).sum(1)
+    assert ((yd.cpu().double() - x @ W.T).abs() <= bound).all()
+    eng.release_matrix(index)
