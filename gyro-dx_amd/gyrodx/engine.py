@@ -260,8 +260,8 @@ class Engine:
 
     def forward_decode_noalloc(self, layer: int, x_ptr: int, n: int, out_ptr: int, stream: int = 0):
         """Decode-path forward of n <= 8 tokens between device buffers (addresses x_ptr, out_ptr),
-        queued on the hipStream_t `stream` (0: the engine's compute stream); allocates nothing and
-        does not wait."""
+        queued on the hipStream_t `stream` (0: the engine's compute stream; 1, hipStreamLegacy: the
+        default stream, which torch calls 0); allocates nothing and does not wait."""
         self._check(lib().gm_forward_decode_noalloc(self._h, layer, x_ptr, n, out_ptr, stream or None),
                     "gm_forward_decode_noalloc")
 

@@ -3,12 +3,13 @@
  *
  * No counterpart in the reference: products with 4-bit matrices, the residual step's norms and the log
  * probabilities of an answer, on rows in device memory of the engine's GPU. They need no layer. A call queues its
- * launches on `stream` and does not wait, allocate or copy; `stream` is a hipStream_t of the engine's
- * device as HIP means it (NULL: the device's null stream, unlike gm_forward_decode_noalloc's), and the caller's
- * current device is left as it was. gm_linear, gm_block_norm and gm_logprobs may be captured into a HIP graph; a kernel
- * that no call has used yet is loaded by its first call, which a capture refuses, so call once (or gm_load_operators)
- * before. The calls that load, add or release wait and allocate, and belong outside captures. n = 0 does nothing. Calls on
- * one engine are serialised by the caller, as all of gyro_moe.h's; what they queue may overlap where its outputs and
+ * launches on `stream` and does not wait, allocate or copy; `stream` is a hipStream_t of the engine's device as HIP
+ * means it, and the caller's current device is left as it was. NULL is the device's null stream. (To
+ * gm_forward_decode_noalloc NULL is the engine's compute stream, which is not ordered with the null stream, and the
+ * null stream hipStreamLegacy.) gm_linear, gm_block_norm and gm_logprobs may be captured into a HIP graph; a kernel that no
+ * call has used yet is loaded by its first call, which a capture refuses, so call once (or gm_load_operators) before.
+ * The calls that load, add or release wait and allocate, and belong outside captures. n = 0 does nothing. Calls on one
+ * engine are serialised by the caller, as all of gyro_moe.h's; what they queue may overlap where its outputs and
  * workspaces are apart. All return 0 or a negative code; gm_last_error describes the failure.
  */
 #ifndef GYRO_OPS_H
