@@ -7,8 +7,12 @@
 // values per thread and step, all of them in registers between the two sums of squares, whose partial sums meet
 // in fixed order. out may be x, and normed h, in place.
 //
-// What bounds it: of many rows the bytes (4096 rows of 2048, fp32 stream, bf16 in and out, 101 MB: 23 to 26 us, 3.9 to 4.4
-// TB/s; a large copy moves 5.1). Of few, one row's chain of loads, two sums and stores: 3.6 us at 2048 values, 4.9 at 2560.
+// What bounds it: of many rows the bytes (4096 rows of 2048, fp32 stream, bf16 in and out, 101 MB: median 26 us of kernel, 3.9
+// TB/s, 24 in a loop; a large copy moves 5.1). Rows of 2560 take 28.5 us in a loop (4.4 TB/s), of 16384 192 (4.2), but of 8192
+// 131 (3.1): half the steps of the longest build are empty, and its 221 registers leave two waves a SIMD. Of few rows, one
+// row's chain of loads, two sums and stores: median 3.8 us at 2048 values, 5.3 at 2560. The chain waits for each input in turn:
+// row_load8 converts inside the branch on the type, so the next input's load is asked for after the one before has come. 777
+// rows with a gate per value, all binary16, take 9.3 us of kernel for 3.1 us of bytes, at odd addresses or not.
 // One row to a group rather than to a wave: a wave would hold a row of 2048 in 100 registers and leave a single row to
 // one unit's fourth part. The builds differ in the steps of 2048 values that registers hold (1, 2, 8): a shorter one
 // has more waves in flight and less to skip (block_norm_s against the two-step build: one row of 2048 3.8 against 4.9 us, 4096

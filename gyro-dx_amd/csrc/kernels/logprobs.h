@@ -12,9 +12,10 @@
 // that by itself runs over the list (ties, values in step with the lanes) goes through an exact
 // selection. The result depends on none of this: places are unique, and the final order is by place.
 //
-// What bounds it: of many rows the reads (1023 fp32 rows of 131072: 96 us, 5.5 TB/s, 99 with the top 20); of few rows the
-// launches and one batch's chain of dependent steps (one such row: 5.6 us without a top, 14.9 with the top 20, of which the
-// join's launch and kernel take 6). Batches of 2048 took 101 to 121 us for the first and 6.1 to 14.2 for the second: half
+// What bounds it: of many rows the reads (1023 fp32 rows of 131072: 96 us in a loop, 5.6 TB/s, 99 with the top 20; median 102 of
+// kernel); of few rows the launches and one batch's chain of dependent steps, the bit searches for the top among them (one such
+// row: 5.5 us without a top, 14.6 with the top 20, of which the join's kernel, 7.8 by itself, is half; 64 bf16 rows of
+// 100003 with the top 5 20). Batches of 2048 took 101 to 121 us for the first and 6.1 to 14.2 for the second: half
 // the waves per SIMD, and 1023 rows in one round and a third instead of one.
 //
 // Rows shared by several groups (`parts`) leave their sums and lists in the workspace for logprobs_join.

@@ -9,14 +9,16 @@
 // which come with the staging, are a product of their own, in fp32 on v_mfma_f32_16x16x4_f32. bf16 and binary16 tokens
 // are operands as they are; fp32 ones go through the products three times, a part each.
 //
-// What bounds it: issue. 8192 x 2048 on 1023 bf16 tokens takes 60 us with groups of 32 (570 TFLOP/s) and 51 with groups of
-// 128 (670), half of a large matrix product's 1200; in fp32 118 us (290). Of a gated 4096 x 2048 in groups of 64 with
-// minima on 1023 binary16 tokens (58 to 66 us, box to box) the matrix unit is busy 36% of the cycles (two fifths of that
-// corrections and minima), the vector unit 41%, and two waves a SIMD, which is what registers and LDS hold, wait for one
-// another's results the rest. Few tokens are bound by the chain of a chunk (load, store to LDS, barrier, products: 1.1 us)
-// and by groups that do not divide among the units (100003 x 2560 on 37 tokens: 391 groups, 51 to 55 us, 2.8 TB/s). Groups
-// that start at different chunks gained nothing, nor did minima as exact bf16 parts in one 16x16x32 product, half the
-// matrix cycles.
+// What bounds it: dependent results at two waves a SIMD, which is what registers (208 to 256) and LDS hold. 8192 x 2048 on
+// 1023 bf16 tokens takes 56 to 60 us with groups of 32 (570 TFLOP/s) and 51 with groups of 128 (670), half of a large matrix
+// product's 1200; in fp32 111 to 118 us (300), of which three products of each operand explain 86. Of a gated 4096 x 2048
+// in groups of 64 with minima on 1023 binary16 tokens (58 to 66 us, box to box) neither unit is full: the matrix unit is busy
+// 36% of the cycles (two fifths of that corrections and minima), the vector unit 41%. Fewer tokens are bound by the chain
+// of a chunk (load, store to LDS, barrier, products: 1.1 us), which one group goes through for all columns however few
+// tokens there are: 8192 x 2048 on 64 bf16 tokens 18 us, 2048 x 2048 on 512 19, five to eight times their floors.
+// 391 groups that do not divide among 256 units add a quarter at most (100003 x 2560 on 37 tokens: 49 to 55 us, 2.8 TB/s).
+// Groups that start at different chunks gained nothing, nor did minima as exact bf16 parts in one 16x16x32 product, half
+// the matrix cycles.
 #pragma once
 #include "q4.h"
 

@@ -91,7 +91,8 @@ __device__ __forceinline__ MqOut mq_out(const GdArgs &a) {
     return {gd_addr(a, 18), gd_addr(a, 20), a.c[22], a.c[23], a.c[24], a.c[11], gd_bits_f32(a.c[25])};
 }
 __device__ __forceinline__ float mq_value(const MqOut &o, float sum, float up) {
-    // x rcp(1 + e^-x): within two units of the last place of the division's result.
+    // x rcp(1 + e^-x): within two units of the last place of the division's result. expf's own relative error grows with |x|
+    // to |x| 2^-24 (its argument times log2 e is rounded); e^-x counts in the result where x is negative.
     if (o.gated) return o.scale * (sum * __builtin_amdgcn_rcpf(1.0f + expf(-sum)) * up);
     float v = o.scale * sum;
     if (o.act == 1u) v = v * __builtin_amdgcn_rcpf(1.0f + expf(-v));

@@ -165,7 +165,8 @@ class RowOps {
         // and passes. They meet near (fp32, bf16, binary16) 12, 7 and 8 tile passes per compute unit. us at 2048
         // columns, mv / mm: 2048 rows of 64, 128 and 512 fp32 tokens 16.6 / 23.4, 28.1 / 23.6 and 90.3 / 25.3; 8192 rows of
         // 17 and 32 16.3 / 23.4 and 26.8 / 23.6; of 32 and 64 bf16 tokens 12.2 / 18.6 and 21.4 / 19.2, binary16 18.4 / 18.9
-        // and 33.5 / 19.4.
+        // and 33.5 / 19.4. Measured at 512 to 32768 rows of 2048 columns and 2048 rows of 512, on 6 to 512 tokens; the worst
+        // choice there is mm_q4 for 32768 rows and 6 fp32 tokens (21.8 / 23.8). Longer rows were not measured.
         // (The grid of more than 2^20 tiles would be too wide for mm_q4.)
         static const uint32_t meet[] = {12, 7, 8};
         const uint32_t blocks = (m.tiles + 15) / 16;
