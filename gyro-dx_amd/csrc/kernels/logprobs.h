@@ -37,7 +37,7 @@ struct LpSums {
     float m, s, t;
 };
 
-// A distance whose exp is 0, and which a sum of up to 2^31 terms may be multiplied by within fp32's range: 0 times either is 0.
+// A distance whose exp is 0, and that times a sum of up to 2^31 terms is within fp32's range, so that 0 times either is 0.
 #define LP_FAR -1e28f
 
 // scale (a - b), LP_FAR at least.

@@ -11,9 +11,10 @@
 // kernel, 32.1 in a loop, 4.7 TB/s of 151 MB; a large copy moves 5.1). Of a small one the chain of a launch, staging, one
 // chunk's loads and the join: 2048 x 512 median 5.2 us, a gated 1024 x 2048 with minima on 3 tokens 8.2. binary16 tokens go as
 // two rows each, so that 9 to 16 of them read the weights twice (8192 x 2048 on 32 18.4 us, bf16 12.2). Every
-// pass reads and unpacks all weights again: 2048 x 8192 on 128 bf16 tokens, 8 passes, 35 us for a floor of 3.6. The matrix unit is busy an eighth of the first
-// one's time, so that fp32 activations as three planes cost nothing; vector instructions would need a product and a
-// conversion per value beside the unpacking. Two tiles a wave (R) share its reads of the operand rows.
+// pass reads and unpacks all weights again: 2048 x 8192 on 128 bf16 tokens, 8 passes, 35 us for a floor of 3.6. The matrix
+// unit is busy an eighth of the output head's time, so that fp32 activations as three planes cost nothing; vector
+// instructions would need a product and a conversion per value beside the unpacking. Two tiles a wave (R) share its
+// reads of the operand rows.
 #pragma once
 #include "q4.h"
 

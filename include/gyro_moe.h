@@ -135,10 +135,10 @@ GM_API int gm_read_outputs(gm_engine *e, float *out, uint32_t n_total);
  * HIP graph capture, serving loops, harnesses that forbid hipMalloc). The GM_PATH_DECODE forward
  * of gm_forward on n <= 8 tokens, with x[n][E] and out[n][E] in device memory, queued on
  * `stream` (a hipStream_t of the engine's device; NULL: the engine's compute stream;
- * hipStreamLegacy: the device's null stream) without waiting for it. It calls no hipMalloc / hipFree and no memset or copy: router logits, routes,
- * the rotated input, the gate/up partials and the shared expert's rows live in a fixed device
- * array of GM_NOALLOC_SCRATCH_BYTES per GPU, and the launches carry the addresses of x and out in
- * their constants. A layer shape whose buffers exceed that array is refused with an error. Every call on one
+ * hipStreamLegacy: the device's null stream) without waiting for it. It calls no hipMalloc /
+ * hipFree and no memset or copy: router logits, routes, the rotated input, the gate/up partials and
+ * the shared expert's rows live in a fixed device array of GM_NOALLOC_SCRATCH_BYTES per GPU, and the
+ * launches carry the addresses of x and out in their constants. A layer shape whose buffers exceed that array is refused with an error. Every call on one
  * GPU shares the array: calls that overlap on one GPU race, so a caller
  * serialises them (one stream, or its own ordering). Results equal gm_forward's bit for bit: the
  * decode path keeps its activations in fp32, so no call of it is ever recomputed on another path
