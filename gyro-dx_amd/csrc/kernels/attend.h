@@ -1,0 +1,193 @@
+// Attention of new tokens over a paged cache: what every build of it shares. The tokens of a sequence that read one of the
+// cache's heads, `group` = heads / kv_heads queries' heads each, are its rows: row r is head r % group of token r / group, so
+// that a page read once serves them all. A launch's groups take (sequence, cache head, tile of rows, part of the keys); where
+// the keys are split, attend_join puts the parts together.
+//
+// Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table
+// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 workspace 28 heads 29 group 30 D 31 kv heads
+// 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 causal 39 window 40 scale times log2(e)
+// 41 parts 42 tiles of rows per sequence 43 type 44 rows of a tile 45 keys of a tile 46 tiles that make a part worth its join
+#pragma once
+#include "rows.h"
+
+// What a group that shares its rows' keys keeps in the workspace: the maximum and the sum of each row, then the rows.
+__device__ __forceinline__ uint64_t at_part(const GdArgs &a, uint64_t item, uint32_t part, uint32_t rows) {
+    return gd_addr(a, 26) + (item * a.c[41] + part) * (uint64_t)(rows * 4u) * (a.c[30] + 2u);
+}
+
+// A tile of rows of a sequence and cache head, and the keys that any of them sees.
+struct AtItem {
+    uint32_t seq, head, token0, ql, rows, row0;  // rows: of the sequence and head; row0: the tile's first
+    int32_t kl, first, end;       // keys first .. end - 1 are seen by some row of the tile,
+    int32_t all_first, all_end;   // all_first .. all_end - 1 by each
+};
+
+__device__ __forceinline__ bool at_item(const GdArgs &a, uint32_t item, uint32_t tile_rows, AtItem &o) {
+    const uint32_t KVH = a.c[31], S = a.c[32], longest = a.c[33], n = a.c[34], group = a.c[29], tiles = a.c[42];
+    const uint32_t rest = item / KVH;
+    o.head = item - rest * KVH;
+    o.seq = rest / tiles;
+    o.row0 = (rest - o.seq * tiles) * tile_rows;
+    if (o.seq >= S) return false;
+    const int32_t most = (int32_t)(a.c[37] * a.c[36]);
+    o.kl = min(max(gd_at<const int32_t>(gd_addr(a, 22))[o.seq], 0), most);
+    if (gd_addr(a, 24)) {
+        const gd_gptr<const int32_t> starts = gd_at<const int32_t>(gd_addr(a, 24)) + o.seq;
+        const int32_t from = min(max(starts[0], 0), (int32_t)n), to = min(max(starts[1], from), (int32_t)n);
+        o.token0 = from;
+        o.ql = to - from;
+    } else {
+        o.token0 = o.seq * longest;
+        o.ql = longest;
+    }
+    o.rows = o.ql * group;
+    if (o.row0 >= o.rows) return false;
+    // Positions of the tile's first and last token.
+    const int32_t base = o.kl - (int32_t)o.ql, p0 = base + (int32_t)(o.row0 / group),
+                  p1 = base + (int32_t)((min(o.row0 + tile_rows, o.rows) - 1u) / group), window = (int32_t)a.c[39];
+    const bool causal = a.c[38] != 0u;
+    o.first = window ? max(0, p0 - window + 1) : 0;
+    o.end = causal ? max(0, p1 + 1) : o.kl;
+    o.all_first = window ? max(0, p1 - window + 1) : 0;
+    o.all_end = causal ? p0 + 1 : o.kl;
+    return true;
+}
+// Tiles of `keys` keys of an item, the first's number, and how many of the launch's parts share them: as many as leave each
+// `least` tiles.
+__device__ __forceinline__ uint32_t at_tiles(const AtItem &o, uint32_t keys, uint32_t &tile0) {
+    tile0 = (uint32_t)o.first / keys;
+    return o.end > o.first ? ((uint32_t)o.end + keys - 1u) / keys - tile0 : 0u;
+}
+__device__ __forceinline__ uint32_t at_parts(const GdArgs &a, uint32_t tiles, uint32_t least) {
+    return max(1u, min(a.c[41], (tiles + least - 1u) / least));
+}
+
+// The offset in the cache, in bytes, of key j of a sequence; -1: on a page outside it (or past `end`).
+__device__ __forceinline__ int64_t at_key(const GdArgs &a, uint32_t seq, uint32_t head, int32_t j, int32_t end) {
+    if (j >= end) return -1;
+    const uint32_t page_size = a.c[36], slot = (uint32_t)j / page_size;
+    const uint32_t page = (uint32_t)gd_at<const int32_t>(gd_addr(a, 18))[seq * gd_addr(a, 20) + slot];
+    if (page >= a.c[35]) return -1;
+    return page * gd_addr(a, 12) + ((uint32_t)j - slot * page_size) * gd_addr(a, 16) + head * gd_addr(a, 14);
+}
+
+// The larger of a value and lane ^ 32's.
+__device__ __forceinline__ float at_max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(gd_f32_bits(v), gd_f32_bits(v), false, false);
+    return fmaxf(gd_bits_f32(r[0]), gd_bits_f32(r[1]));
+}
+__device__ __forceinline__ float at_sum_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(gd_f32_bits(v), gd_f32_bits(v), false, false);
+    return gd_bits_f32(r[0]) + gd_bits_f32(r[1]);
+}
+__device__ __forceinline__ float at_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// Four values of a row from d on, times `by`; zeros where nothing was seen.
+typedef gd_u32x2 at_u32x2_any __attribute__((aligned(2)));
+template <uint32_t TYPE>
+__device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, float by, bool none) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = none ? 0.f : x[i] * by;
+    if constexpr (TYPE == ROW_F32)
+        *gd_at<gd_f32x4_any>(row + 4ull * d) = x;
+    else
+        *gd_at<at_u32x2_any>(row + 2ull * d) = gd_u32x2{row_bits16(x[0], TYPE) | row_bits16(x[1], TYPE) << 16,
+                                                        row_bits16(x[2], TYPE) | row_bits16(x[3], TYPE) << 16};
+}
+
+// Below every score that counts, and finite: the difference of two such is zero, not NaN.
+#define AT_LOWEST -1e30f
+
+// Few rows (attend_few.h, attend_f32.h): a group of four waves takes a tile of 16 rows and a part of the keys.
+#define AF_WAVES 4u
+#define AF_ROWS 16u
+
+// The larger (the sum) of the four lanes that hold a row's keys, 16 lanes apart.
+__device__ __forceinline__ float af_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(gd_f32_bits(v), gd_f32_bits(v), false, false);
+    return at_max_halves(fmaxf(gd_bits_f32(r[0]), gd_bits_f32(r[1])));
+}
+__device__ __forceinline__ float af_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(gd_f32_bits(v), gd_f32_bits(v), false, false);
+    return at_sum_halves(gd_bits_f32(r[0]) + gd_bits_f32(r[1]));
+}
+
+// A group's tile, its part of the keys' tiles, and what a lane knows of its row: lane l has row l % 16 (rows past the last are
+// the last again), and of the scores the keys 4 (l / 16) + i.
+struct AfWork {
+    AtItem o;
+    uint32_t item, part, shared, from, to;
+    uint64_t q;           // offset of the row in q, in values
+    int32_t first, last;  // keys that the row sees
+};
+__device__ __forceinline__ bool af_work(const GdArgs &a, AfWork &w) {
+    const uint32_t parts = a.c[41], id = blockIdx.y * gridDim.x + blockIdx.x, group = a.c[29];
+    w.item = id / parts;
+    w.part = id - w.item * parts;
+    if (!at_item(a, w.item, AF_ROWS, w.o)) return false;
+    uint32_t tile0;
+    const uint32_t tiles = at_tiles(w.o, a.c[45], tile0);
+    w.shared = at_parts(a, tiles, a.c[46]);
+    if (w.part >= w.shared) return false;
+    w.from = tile0 + (uint32_t)((uint64_t)tiles * w.part / w.shared);
+    w.to = tile0 + (uint32_t)((uint64_t)tiles * (w.part + 1u) / w.shared);
+    const uint32_t row = min(w.o.row0 + (threadIdx.x & 15u), w.o.rows - 1u), token = row / group;
+    w.q = (uint64_t)(w.o.token0 + token) * gd_addr(a, 2) + (uint64_t)(w.o.head * group + row - token * group) * a.c[30];
+    const int32_t p = w.o.kl - (int32_t)w.o.ql + (int32_t)token, window = (int32_t)a.c[39];
+    w.last = a.c[38] ? p : w.o.kl - 1;
+    w.first = window ? p - window + 1 : 0;
+    return true;
+}
+
+// Joins the waves' parts in LDS and writes the rows, or the group's part of them. A lane holds channels 16 d + 4 (l / 16) + i
+// of its row; a wave's room in lds, EACH values, holds its 16 rows of DT + 4.
+template <uint32_t TYPE, uint32_t DT, uint32_t EACH>
+__device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, const gd_f32x4 (&acc)[DT / 16u], float top, float sum, float *lds) {
+    constexpr uint32_t WIDE = DT + 4u;
+    static_assert(EACH >= AF_ROWS * WIDE, "a wave's rows");
+    __shared__ float stats[AF_WAVES][2][AF_ROWS];
+    const AtItem &o = k.o;
+    const uint32_t lane = threadIdx.x & 63u, col = lane & 15u, h = lane >> 4, wave = threadIdx.x >> 6, D = a.c[30], group = a.c[29];
+    sum = af_sum(sum);
+    if (h == 0u) {
+        stats[wave][0][col] = top;
+        stats[wave][1][col] = sum;
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < DT / 16u; ++d) *reinterpret_cast<gd_f32x4 *>(lds + wave * EACH + col * WIDE + 16u * d + 4u * h) = acc[d];
+    __syncthreads();
+    const uint32_t r = threadIdx.x >> 4, c = threadIdx.x & 15u;  // 16 threads a row
+    if (o.row0 + r >= o.rows) return;
+    float most = stats[0][0][r], total = 0.f, shrink[AF_WAVES];
+#pragma unroll
+    for (uint32_t w = 1; w < AF_WAVES; ++w) most = fmaxf(most, stats[w][0][r]);
+#pragma unroll
+    for (uint32_t w = 0; w < AF_WAVES; ++w) {
+        shrink[w] = at_exp2(stats[w][0][r] - most);
+        total += stats[w][1][r] * shrink[w];
+    }
+    const bool alone = k.shared == 1u;
+    const uint64_t to_part = at_part(a, k.item, k.part, AF_ROWS);
+    if (!alone && c == 0u) {
+        gd_at<float>(to_part)[r] = most;
+        gd_at<float>(to_part)[AF_ROWS + r] = total;
+    }
+    const uint32_t token = (o.row0 + r) / group;
+    const uint64_t out = gd_addr(a, 4) + (((uint64_t)(o.token0 + token) * gd_addr(a, 6) + (uint64_t)(o.head * group + o.row0 + r - token * group) * D)
+                                          << row_shift(TYPE));
+    const float by = 1.f / total;
+#pragma unroll
+    for (uint32_t e = 0; e < (DT + 63u) / 64u; ++e) {
+        const uint32_t d = 64u * e + 4u * c;
+        if (d >= D) continue;
+        gd_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t w = 0; w < AF_WAVES; ++w) {
+            const gd_f32x4 y = *reinterpret_cast<const gd_f32x4 *>(lds + w * EACH + r * WIDE + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] += y[i] * shrink[w];
+        }
+        if (alone) at_store4<TYPE>(out, d, x, by, total == 0.f);
+        else *gd_at<gd_f32x4>(to_part + 8u * AF_ROWS + ((uint64_t)r * D + d) * 4u) = x;
+    }
+}

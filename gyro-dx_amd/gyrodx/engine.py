@@ -1,4 +1,5 @@
-"""ctypes binding of the C++ MoE layer engine (include/gyro_moe.h) and its operators (include/gyro_ops.h)."""
+"""ctypes binding of the C++ MoE layer engine (include/gyro_moe.h) and its operators (include/gyro_ops.h,
+include/gyro_attention.h)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -47,9 +48,36 @@ class LogprobsDesc(C.Structure):
                 ("top_stride", C.c_uint64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
+class Cache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_uint32), ("pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("reserved", C.c_uint32), ("page_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("token_stride", C.c_uint64)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("rotary", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("positions_64", C.c_uint32),
+                ("x", Rows), ("y", Rows), ("positions", C.c_void_p)]
+
+
+class CacheAppendDesc(C.Structure):
+    _fields_ = [("cache", Cache), ("rotary", C.c_uint32), ("heads", C.c_uint32), ("slots_64", C.c_uint32),
+                ("positions_64", C.c_uint32), ("k", Rows), ("v", Rows), ("q", Rows), ("q_out", Rows), ("slots", C.c_void_p),
+                ("positions", C.c_void_p)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("cache", Cache), ("q", Rows), ("out", Rows), ("heads", C.c_uint32), ("sequences", C.c_uint32),
+                ("longest", C.c_uint32), ("causal", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float),
+                ("table", C.c_void_p), ("table_stride", C.c_uint64), ("lengths", C.c_void_p), ("starts", C.c_void_p),
+                ("table_width", C.c_uint32), ("reserved", C.c_uint32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
 # 4-bit matrix formats (gm_matrix_desc) and the operators' activations and element types.
 MATRIX_FORMATS = {"q4_0": 0, "q4_1": 1, "q4": 2}
 ACTS = {"none": 0, "silu": 1, "sigmoid": 2}
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+NO_ROTARY = 0xffffffff
 GATE_TOKEN, GATE_CHANNEL, GATE_VALUE = 1, 2, 3
 _TYPE_NAMES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2, "torch.int32": 3, "torch.int64": 4,
                "torch.uint8": 5}
@@ -60,6 +88,10 @@ _ROW_TYPES, _FLOAT, _INT32, _INTS, _UINT8 = (0, 1, 2), (0,), (3,), (3, 4), (5,)
 _PACK_ROWS = struct.Struct("@PQII").pack
 _PACK_NORM = struct.Struct("@4I" + 5 * "PQII" + "PP4f").pack
 _PACK_LOGPROBS = struct.Struct("@PQII4IfIPQPQPPPQPQ").pack
+_CACHE = "PP6I3Q"
+_PACK_ROTARY = struct.Struct("@4I" + 2 * "PQII" + "P").pack
+_PACK_APPEND = struct.Struct("@" + _CACHE + "4I" + 4 * "PQII" + "PP").pack
+_PACK_ATTENTION = struct.Struct("@" + _CACHE + 2 * "PQII" + "5IfPQPPIIPQ").pack
 _NO_ROWS = (0, 0, 0)
 
 
@@ -123,6 +155,13 @@ def lib() -> C.CDLL:
         L.gm_logprobs_workspace.argtypes = [u32, u32, u32]
         L.gm_logprobs_workspace.restype = C.c_uint64
         L.gm_logprobs.argtypes = [vp, vp, u32, vp]
+        L.gm_add_rotary.argtypes = [vp, vp, u32, u32, C.c_float, C.POINTER(u32)]
+        L.gm_release_rotary.argtypes = [vp, u32]
+        L.gm_rotary.argtypes = [vp, vp, u32, vp]
+        L.gm_cache_append.argtypes = [vp, vp, u32, vp]
+        L.gm_attention_workspace.argtypes = [u32, u32, u32]
+        L.gm_attention_workspace.restype = C.c_uint64
+        L.gm_attention.argtypes = [vp, vp, u32, vp]
         _lib = L
     return _lib
 
@@ -423,3 +462,130 @@ class Engine:
         rc = lib().gm_logprobs(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_logprobs")
+
+    # ---- positions, the paged cache and attention (include/gyro_attention.h) ------------------------
+
+    def add_rotary(self, frequencies, layout: str = "half", scale: float = 1.0) -> int:
+        """Uploads the frequencies of a head's pairs (float64, radians per position: rotary.frequencies()) and returns their
+        index. layout "half": pair j is values j and pairs + j; "interleaved": 2 j and 2 j + 1."""
+        if layout not in ROTARY_LAYOUTS:
+            raise ValueError(f"rotary layout {layout!r} is none of {sorted(ROTARY_LAYOUTS)}")
+        f = np.ascontiguousarray(frequencies, np.float64)
+        if f.ndim != 1:
+            raise ValueError("frequencies: one per pair")
+        idx = C.c_uint32()
+        self._check(lib().gm_add_rotary(self._h, f.ctypes.data, _count(f.size, "pairs"), ROTARY_LAYOUTS[layout], scale,
+                                        C.byref(idx)), "gm_add_rotary")
+        return idx.value
+
+    def release_rotary(self, rotary: int):
+        _count(rotary, "rotary")
+        if self._h:
+            self._check(lib().gm_release_rotary(self._h, rotary), "gm_release_rotary")
+
+    def rotary(self, rotary: int, x, positions, y, heads: int, stream: int | None = None):
+        """y = the heads of x (rows of `heads` heads) turned by positions (int32 or int64 [n]); y may be x."""
+        n, values = x.shape
+        _count(n, "rows of x")
+        if heads <= 0 or values % heads:
+            raise ValueError(f"x: {values} values are not {heads} heads")
+        shape = (n, values)
+        p = self._flat(positions, n, _INTS, "positions")
+        d = _PACK_ROTARY(_count(rotary, "rotary"), _count(heads, "heads"), _count(values // heads, "values of a head"),
+                         _type_codes[positions.dtype] == 4, *self._rows(x, shape, "x"), 0, *self._rows(y, shape, "y"), 0, p)
+        rc = lib().gm_rotary(self._h, d, n, self._stream() if stream is None else stream)
+        if rc:
+            self._check(rc, "gm_rotary")
+
+    def _cache(self, k_cache, v_cache):
+        """The fields of a gm_cache, of two tensors [pages, kv_heads, page_size, head_dim] of the same strides."""
+        shape, strides = k_cache.shape, k_cache.stride()
+        if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides or v_cache.dtype != k_cache.dtype:
+            raise ValueError("k_cache and v_cache: [pages, kv_heads, page_size, head_dim] of one type and the same strides")
+        if strides[3] != 1 and shape[3] > 1:
+            raise ValueError("k_cache: the values of a head are not neighbours")
+        if k_cache.get_device() != self.adapter or v_cache.get_device() != self.adapter:
+            raise ValueError("k_cache and v_cache: not on the engine's GPU")
+        pages, heads, size, dim = shape
+        if max(shape) > 0xffffffff:
+            raise ValueError("k_cache: not 32-bit counts")
+        return (k_cache.data_ptr(), v_cache.data_ptr(), _type(k_cache, _ROW_TYPES, "k_cache"), pages, size, heads, dim, 0,
+                strides[0], strides[1], strides[2])
+
+    def cache_append(self, k, v, k_cache, v_cache, slots, rotary: int | None = None, positions=None, q=None, q_out=None,
+                     stream: int | None = None):
+        """New tokens' keys and values (rows of kv_heads heads) into the slots (int32 or int64 [n]; page * page_size + place,
+        negative: skipped) of a cache [pages, kv_heads, page_size, head_dim], the keys turned by their positions; with q
+        (rows of any number of heads) also q_out = q turned."""
+        c = self._cache(k_cache, v_cache)
+        n, dim = k.shape[0], c[6]
+        _count(n, "rows of k")
+        shape = (n, c[5] * dim)
+        s = self._flat(slots, n, _INTS, "slots")
+        p = wide = heads = 0
+        if rotary is not None:
+            if positions is None:
+                raise ValueError("a rotary without positions")
+            p = self._flat(positions, n, _INTS, "positions")
+            wide = _type_codes[positions.dtype] == 4
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out go together")
+        qr = qo = _NO_ROWS
+        if q is not None:
+            values = q.shape[1]
+            if not dim or not values or values % dim:
+                raise ValueError(f"q: {values} values are not heads of {dim}")
+            heads = _count(values // dim, "heads of q")
+            qr, qo = self._rows(q, (n, values), "q"), self._rows(q_out, (n, values), "q_out")
+        d = _PACK_APPEND(*c, NO_ROTARY if rotary is None else _count(rotary, "rotary"), heads, _type_codes[slots.dtype] == 4, wide,
+                         *self._rows(k, shape, "k"), 0, *self._rows(v, shape, "v"), 0, *qr, 0, *qo, 0, s, p)
+        rc = lib().gm_cache_append(self._h, d, n, self._stream() if stream is None else stream)
+        if rc:
+            self._check(rc, "gm_cache_append")
+
+    @staticmethod
+    def attention_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
+        """Bytes of a workspace that suffices for every attention() of such heads."""
+        return lib().gm_attention_workspace(_count(heads, "heads"), _count(kv_heads, "kv_heads"), _count(head_dim, "head_dim"))
+
+    def attention(self, q, k_cache, v_cache, table, lengths, out, workspace=None, starts=None, longest: int | None = None,
+                  scale: float | None = None, causal: bool = True, window: int = 0, stream: int | None = None):
+        """out = the attention of q's tokens (rows of heads) over the pages table[b] (int32 [sequences, width]) of each
+        sequence's first lengths[b] keys (int32 [sequences]), the tokens' own among them. The sequences have equally many
+        tokens, or tokens starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1]) and at most `longest` of them. Without `causal`
+        every token sees all keys; a window limits it to the last `window` up to its own. scale: 1 / sqrt(head_dim).
+        workspace: a uint8 tensor of attention_workspace() bytes, not shared with calls that may overlap."""
+        c = self._cache(k_cache, v_cache)
+        n, values = q.shape
+        _count(n, "rows of q")
+        dim = c[6]
+        if not dim or not values or values % dim:
+            raise ValueError(f"q: {values} values are not heads of {dim}")
+        sequences, width = table.shape
+        _type(table, _INT32, "table")
+        if table.get_device() != self.adapter:
+            raise ValueError("table: not on the engine's GPU")
+        row, step = table.stride()
+        if step != 1 and width > 1:
+            raise ValueError("table: the pages of a sequence are not neighbours")
+        lp = self._flat(lengths, sequences, _INT32, "lengths")
+        sp = ws = ws_bytes = 0
+        if starts is not None:
+            sp = self._flat(starts, sequences + 1, _INT32, "starts")
+            if longest is None:
+                raise ValueError("starts without the longest sequence's count")
+        elif longest is None:
+            if not sequences or n % sequences:
+                raise ValueError(f"q: {n} tokens are not of {sequences} equal sequences")
+            longest = n // sequences
+        if workspace is not None:
+            ws_bytes = workspace.numel()
+            ws = self._flat(workspace, ws_bytes, _UINT8, "workspace")
+        shape = (n, values)
+        d = _PACK_ATTENTION(*c, *self._rows(q, shape, "q"), 0, *self._rows(out, shape, "out"), 0, _count(values // dim, "heads"),
+                            _count(sequences, "sequences"), _count(longest, "longest"), causal, _count(window, "window"),
+                            dim ** -0.5 if scale is None else scale, table.data_ptr(), row, lp, sp, _count(width, "table"), 0,
+                            ws, ws_bytes)
+        rc = lib().gm_attention(self._h, d, n, self._stream() if stream is None else stream)
+        if rc:
+            self._check(rc, "gm_attention")

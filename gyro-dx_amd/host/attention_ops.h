@@ -1,0 +1,272 @@
+// Rotary positions, the paged cache's appending and the attention over it (gm_rotary, gm_cache_append, gm_attention): argument
+// checks, the choice of a build, its constants and grid, as row_ops.h has them for the other operators. Their kernels are
+// csrc/kernels/rotary.h and attend*.h.
+#pragma once
+#include "gyro_attention.h"
+#include "row_ops.h"
+
+namespace gyro {
+
+struct Rotary {
+    Buffer table;  // per pair the fraction of a turn of one position, of 2^64
+    uint32_t pairs = 0, layout = 0;
+    float scale = 1;
+};
+
+class AttentionOps {
+  public:
+    std::vector<Rotary> rotaries;
+
+    // ---- rotary positions ----
+
+    static Rotary describe(const double *frequencies, uint32_t pairs, uint32_t layout, float scale, std::vector<uint64_t> &table) {
+        require(frequencies && pairs && pairs <= 512, "a rotary has 1 to 512 pairs");
+        require(layout <= GM_ROTARY_INTERLEAVED, "unknown rotary layout");
+        require(std::isfinite(scale), "a rotary's scale is finite");
+        table.resize(pairs);
+        for (uint32_t i = 0; i < pairs; ++i) {
+            require(std::fabs(frequencies[i]) < 2147483648.0, "a rotary's frequencies are below 2^31 in magnitude");
+            // x87's 64-bit mantissa keeps the fraction's last places.
+            const long double turns = (long double)frequencies[i] / 6.283185307179586476925286766559L;
+            const long double scaled = std::floor((turns - std::floor(turns)) * 18446744073709551616.0L + 0.5L);
+            table[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
+        }
+        Rotary r;
+        r.pairs = pairs;
+        r.layout = layout;
+        r.scale = scale;
+        return r;
+    }
+    const Rotary &rotary(uint32_t i) const {
+        require(i < rotaries.size() && rotaries[i].table.handle, "no such rotary");
+        return rotaries[i];
+    }
+    uint32_t keep(Rotary &&r) {
+        for (uint32_t i = 0; i < rotaries.size(); ++i)
+            if (!rotaries[i].table.handle) {
+                rotaries[i] = std::move(r);
+                return i;
+            }
+        rotaries.push_back(std::move(r));
+        return (uint32_t)rotaries.size() - 1;
+    }
+
+    // Rows of `heads` heads and what becomes of them: in place, of one type and stride.
+    static void check_pair(const gm_rows &x, const gm_rows &y, uint32_t n, uint32_t values, const char *what) {
+        RowOps::check_rows(x, n, values, false, what);
+        RowOps::check_rows(y, n, values, true, what);
+        require(x.data != y.data || (x.type == y.type && (n == 1 || x.stride == y.stride)), what);
+    }
+
+    // The launch of queries (heads of them), keys and values (kv_heads of each) of n tokens, D values a head.
+    static void turn(Launch &l, const Rotary *r, const gm_rows *q, const gm_rows *q_out, uint32_t heads, const gm_rows *k, const gm_rows *v,
+                     uint32_t kv_heads, uint32_t D, uint32_t n) {
+        Constants &c = l.c;
+        const gm_rows &x = q ? *q : *k;
+        if (q) {
+            c.set(0, q->data);
+            c.set64(2, q->stride);
+            c.set(4, q_out->data);
+            c.set64(6, q_out->stride);
+        }
+        if (k) {
+            c.set(8, k->data);
+            c.set64(10, k->stride);
+            c.set(12, v->data);
+            c.set64(14, v->stride);
+        }
+        const uint32_t pairs = r ? r->pairs : 0, all = heads + 2 * kv_heads;
+        if (r) {
+            c.set64(26, r->table.gpu);
+            c.set(39, r->scale);
+        }
+        c.set(32, D);
+        c.set(33, pairs);
+        c.set(34, heads);
+        c.set(35, kv_heads);
+        c.set(36, n);
+        const uint32_t units = std::max((pairs + 7) / 8 + (D - 2 * pairs + 15) / 16, (D + 15) / 16);
+        // Heads of a thread, which form its angles once: as many as leave 2^16 threads, at most 8.
+        uint32_t per = 1;
+        while (per < 8 && per * 2 <= all && (uint64_t)n * ((all + 2 * per - 1) / (2 * per)) * units >= 1u << 16) per *= 2;
+        const uint32_t groups = (all + per - 1) / per, at_once = 256 / units;
+        c.set(42, per);
+        c.set(43, groups);
+        c.set(44, units);
+        const uint64_t blocks = ((uint64_t)n * groups + at_once - 1) / at_once;
+        l.kernel = x.type == GM_F32 ? "rotary_f" : x.type == GM_BF16 ? "rotary_b" : "rotary_h";
+        l.x = (uint32_t)std::min<uint64_t>(blocks, 65535);
+        l.y = (uint32_t)((blocks + 65534) / 65535);
+    }
+
+    Launch turned(const gm_rotary_desc &d, uint32_t n) const {
+        Launch l;
+        const Rotary &r = rotary(d.rotary);
+        if (!n) return l;  // of no rows there may be no memory
+        require(d.heads && d.head_dim && d.head_dim <= 1024 && 2 * r.pairs <= d.head_dim, "gm_rotary: heads of up to 1024 values, all pairs in them");
+        require((uint64_t)n * d.heads < 1u << 31 && d.heads <= 1u << 20, "gm_rotary: n * heads is below 2^31");
+        check_pair(d.x, d.y, n, d.heads * d.head_dim, "gm_rotary: x and y");
+        require(d.positions && (uintptr_t)d.positions % (d.positions_64 ? 8 : 4) == 0, "gm_rotary: positions");
+        turn(l, &r, &d.x, &d.y, d.heads, nullptr, nullptr, 0, d.head_dim, n);
+        l.c.set(28, d.positions);
+        l.c.set(37, d.y.type);
+        l.c.set(38, (r.layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u));
+        return l;
+    }
+
+    // ---- the cache ----
+
+    static void check_cache(const gm_cache &c, const char *what) {
+        require(c.k && c.v && c.type <= GM_F16, what);
+        const uint64_t size = c.type == GM_F32 ? 4 : 2;
+        require((uintptr_t)c.k % size == 0 && (uintptr_t)c.v % size == 0, what);
+        require(c.pages && c.page_size && (uint64_t)c.pages * c.page_size < 1u << 31, what);
+        require(c.kv_heads && c.kv_heads <= 1u << 20 && c.head_dim, what);
+        const uint64_t most = uint64_t(1) << 40;
+        require(c.page_stride <= most && c.head_stride <= most && c.token_stride <= most, what);
+    }
+    // Strides in bytes, at constant `at`.
+    static void set_cache(Constants &c, const gm_cache &cache, int at) {
+        const uint64_t size = cache.type == GM_F32 ? 4 : 2;
+        c.set64(at, cache.page_stride * size);
+        c.set64(at + 2, cache.head_stride * size);
+        c.set64(at + 4, cache.token_stride * size);
+    }
+
+    Launch append(const gm_cache_append_desc &d, uint32_t n) const {
+        Launch l;
+        const Rotary *const r = d.rotary == GM_NO_ROTARY ? nullptr : &rotary(d.rotary);
+        if (!n) return l;  // of no rows there may be no memory
+        const uint32_t D = d.cache.head_dim, G = d.cache.kv_heads;
+        check_cache(d.cache, "gm_cache_append: cache");
+        require(D <= 1024 && (!r || 2 * r->pairs <= D), "gm_cache_append: heads of up to 1024 values, all pairs in them");
+        require(d.heads <= 1u << 20 && (uint64_t)n * (d.heads + 2ull * G) < 1u << 31, "gm_cache_append: n times the heads is below 2^31");
+        RowOps::check_rows(d.k, n, G * D, false, "gm_cache_append: k");
+        RowOps::check_rows(d.v, n, G * D, false, "gm_cache_append: v");
+        require(d.k.type == d.v.type, "gm_cache_append: k and v have one type");
+        require(!d.heads == !d.q.data && !d.heads == !d.q_out.data, "gm_cache_append: q, q_out and its heads go together");
+        if (d.heads) {
+            check_pair(d.q, d.q_out, n, d.heads * D, "gm_cache_append: q and q_out");
+            require(d.q.type == d.k.type, "gm_cache_append: q has the type of k");
+        }
+        require(d.slots && (uintptr_t)d.slots % (d.slots_64 ? 8 : 4) == 0, "gm_cache_append: slots");
+        require(!r || (d.positions && (uintptr_t)d.positions % (d.positions_64 ? 8 : 4) == 0), "gm_cache_append: positions");
+        // No two (page, head, token) may share an element: of two dimensions one's stride spans the other's extent.
+        check_apart(d.cache);
+        turn(l, r, d.heads ? &d.q : nullptr, &d.q_out, d.heads, &d.k, &d.v, G, D, n);
+        Constants &c = l.c;
+        c.set(16, d.cache.k);
+        c.set(18, d.cache.v);
+        set_cache(c, d.cache, 20);
+        if (r) c.set(28, d.positions);
+        c.set(30, d.slots);
+        c.set(37, (d.heads ? d.q_out.type : 0u) | d.cache.type << 4);
+        c.set(38, (r && r->layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u) | (d.slots_64 ? 4u : 0u));
+        c.set(40, d.cache.page_size);
+        c.set(41, d.cache.pages * d.cache.page_size);
+        return l;
+    }
+    static void check_apart(const gm_cache &c) {
+        struct Dim {
+            uint64_t stride, count;
+        } dims[3] = {{c.page_stride, c.pages}, {c.head_stride, c.kv_heads}, {c.token_stride, c.page_size}};
+        std::sort(dims, dims + 3, [](const Dim &a, const Dim &b) { return a.stride < b.stride; });
+        uint64_t extent = c.head_dim;
+        for (const Dim &d : dims) {
+            if (d.count == 1) continue;
+            require(d.stride >= extent, "gm_cache_append: the cache's heads overlap");
+            extent = d.stride * (d.count - 1) + extent;
+        }
+    }
+
+    // ---- attention ----
+
+    // Groups that a launch's keys are split for, and rows that a group takes: the workspace holds that many groups' rows.
+    static constexpr uint32_t kGroups = 1024, kParts = 256;
+    static uint64_t workspace(uint32_t heads, uint32_t kv_heads, uint32_t D) {
+        if (!heads || !kv_heads || heads % kv_heads || !D || D > 256) return 0;
+        return (uint64_t)kGroups * 16 * 4 * (D + 2);
+    }
+
+    static Launch attention(const gm_attention_desc &d, uint32_t n) {
+        Launch l;
+        if (!n) return l;  // of no rows there may be no memory
+        const uint32_t D = d.cache.head_dim, G = d.cache.kv_heads, H = d.heads;
+        check_cache(d.cache, "gm_attention: cache");
+        require(D % 8 == 0 && D <= 256, "gm_attention takes heads of a multiple of 8 values up to 256");
+        require(H && H % G == 0 && H <= 1u << 20, "gm_attention: heads are a multiple of kv_heads");
+        require((uint64_t)n * H <= 1u << 30, "gm_attention: n * heads is at most 2^30");
+        RowOps::check_rows(d.q, n, H * D, false, "gm_attention: q");
+        RowOps::check_rows(d.out, n, H * D, true, "gm_attention: out");
+        require(d.q.type == d.cache.type && d.out.type == d.cache.type, "gm_attention: q, out and the cache have one type");
+        require(d.q.data != d.out.data || n == 1 || d.q.stride == d.out.stride, "gm_attention: rows in place have one stride");
+        require(d.sequences && d.longest && d.longest <= n, "gm_attention: sequences, longest");
+        require(d.starts || (uint64_t)d.sequences * d.longest == n, "gm_attention: without starts n is sequences * longest");
+        require(d.lengths && (uintptr_t)d.lengths % 4 == 0 && (uintptr_t)d.starts % 4 == 0, "gm_attention: lengths and starts");
+        require(d.table && (uintptr_t)d.table % 4 == 0 && d.table_width && d.table_stride <= uint64_t(1) << 40, "gm_attention: table");
+        const uint64_t capacity = (uint64_t)d.table_width * d.cache.page_size;
+        require(capacity < 1u << 31, "gm_attention: table_width * page_size is below 2^31");
+        require(d.causal || !d.window, "gm_attention: a window without the causal mask");
+        require(d.scale > 0 && std::isfinite(d.scale), "gm_attention: scale");
+        const bool wide = d.cache.type == GM_F32;
+        const uint32_t tile_rows = 16, keys = wide ? 16 : 32, least = 4;
+        const uint32_t group = H / G, tiles = (uint32_t)(((uint64_t)d.longest * group + tile_rows - 1) / tile_rows);
+        const uint64_t items = (uint64_t)d.sequences * G * tiles;
+        require(items < 1u << 31, "gm_attention: too many sequences");
+        // Parts of the keys, while the groups are fewer than those the GPU holds.
+        const uint64_t key_tiles = (capacity + keys - 1) / keys;
+        const uint32_t parts = (uint32_t)std::max<uint64_t>(1, std::min({(uint64_t)kParts, kGroups / items, (key_tiles + least - 1) / least}));
+        const uint64_t need = parts == 1 ? 0 : items * parts * tile_rows * 4 * (D + 2);
+        require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0), "gm_attention: workspace");
+        Constants &c = l.c;
+        c.set(0, d.q.data);
+        c.set64(2, d.q.stride);
+        c.set(4, d.out.data);
+        c.set64(6, d.out.stride);
+        c.set(8, d.cache.k);
+        c.set(10, d.cache.v);
+        set_cache(c, d.cache, 12);
+        c.set(18, d.table);
+        c.set64(20, d.table_stride);
+        c.set(22, d.lengths);
+        c.set(24, d.starts);
+        c.set(26, d.workspace);
+        c.set(28, H);
+        c.set(29, group);
+        c.set(30, D);
+        c.set(31, G);
+        c.set(32, d.sequences);
+        c.set(33, d.longest);
+        c.set(34, n);
+        c.set(35, d.cache.pages);
+        c.set(36, d.cache.page_size);
+        c.set(37, d.table_width);
+        c.set(38, d.causal ? 1u : 0u);
+        c.set(39, std::min(d.window, 1u << 30));
+        c.set(40, d.scale * 1.44269504088896341f);
+        c.set(41, parts);
+        c.set(42, tiles);
+        c.set(43, d.cache.type);
+        c.set(44, tile_rows);
+        c.set(45, keys);
+        c.set(46, least);
+        const int size = D <= 64 ? 0 : D <= 128 ? 1 : 2;
+        static const char *const names[3][3] = {{"attend_f32_64", "attend_f32_128", "attend_f32_256"},
+                                                {"attend_few_b64", "attend_few_b128", "attend_few_b256"},
+                                                {"attend_few_h64", "attend_few_h128", "attend_few_h256"}};
+        l.kernel = names[d.cache.type][size];
+        grid(items * parts, l.x, l.y);
+        if (parts > 1) {
+            l.next = "attend_join";
+            grid((items * tile_rows + 3) / 4, l.next_x, l.next_y);
+        }
+        return l;
+    }
+    // A grid of at least `groups` groups.
+    static void grid(uint64_t groups, uint32_t &x, uint32_t &y) {
+        x = (uint32_t)std::min<uint64_t>(groups, 65535);
+        y = (uint32_t)((groups + x - 1) / x);
+    }
+};
+
+}  // namespace gyro

@@ -26,6 +26,7 @@
 #include "decode_split.h"
 #include "device.h"
 #include "gyro_moe.h"
+#include "attention_ops.h"
 #include "row_ops.h"
 
 // Intermediate buffers of gm_forward_decode_noalloc: router logits, routes, the rotated input,
@@ -480,6 +481,23 @@ class Engine {
         m.data = out.b;
         out.b = Buffer{};
         return ops.keep(std::move(m));
+    }
+    AttentionOps attention;
+    // Uploads the frequencies of rotary positions.
+    uint32_t add_rotary(const double *frequencies, uint32_t pairs, uint32_t layout, float scale) {
+        std::vector<uint64_t> table;
+        Rotary r = AttentionOps::describe(frequencies, pairs, layout, scale, table);
+        struct Held {
+            Device &dev;
+            Buffer b;
+            ~Held() { dev.release(b); }
+        } out{dev, {}};
+        out.b = dev.buffer(table.size() * 8, Kind::device);
+        upload_bytes(out.b, 0, table.data(), table.size() * 8);
+        r.table = out.b;
+        const uint32_t index = attention.keep(std::move(r));
+        out.b = Buffer{};
+        return index;
     }
     // The operator's kernel, loaded if this is its first call: which may allocate, and a capture does not take.
     gd_pipeline *op_kernel(const char *name, void *stream) {
@@ -1862,5 +1880,54 @@ extern "C" int gm_logprobs(gm_engine *g, const gm_logprobs_desc *d, uint32_t n, 
     return guarded(g, [&] {
         KeepDevice keep;
         g->e.launch(gyro::RowOps::logprobs(*d, n), stream);
+    });
+}
+
+// ---- positions, the paged cache and attention (attention_ops.h) ----
+
+extern "C" int gm_add_rotary(gm_engine *g, const double *frequencies, uint32_t pairs, uint32_t layout, float scale, uint32_t *out_index) {
+    if (!out_index) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        *out_index = g->e.add_rotary(frequencies, pairs, layout, scale);
+    });
+}
+
+extern "C" int gm_release_rotary(gm_engine *g, uint32_t rotary) {
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.attention.rotary(rotary);
+        // Its readers are on the callers' streams.
+        if (hipSetDevice((int)g->e.adapter) != hipSuccess || hipDeviceSynchronize() != hipSuccess)
+            throw gyro::NativeError(-1, "gm_release_rotary: the device's work did not finish");
+        g->e.dev.release(g->e.attention.rotaries[rotary].table);
+    });
+}
+
+extern "C" int gm_rotary(gm_engine *g, const gm_rotary_desc *d, uint32_t n, void *stream) {
+    if (!d) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(g->e.attention.turned(*d, n), stream);
+    });
+}
+
+extern "C" int gm_cache_append(gm_engine *g, const gm_cache_append_desc *d, uint32_t n, void *stream) {
+    if (!d) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(g->e.attention.append(*d, n), stream);
+    });
+}
+
+extern "C" uint64_t gm_attention_workspace(uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+    return gyro::AttentionOps::workspace(heads, kv_heads, head_dim);
+}
+
+extern "C" int gm_attention(gm_engine *g, const gm_attention_desc *d, uint32_t n, void *stream) {
+    if (!d) return -1;
+    return guarded(g, [&] {
+        KeepDevice keep;
+        g->e.launch(gyro::AttentionOps::attention(*d, n), stream);
     });
 }

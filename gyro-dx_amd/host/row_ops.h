@@ -52,7 +52,7 @@ class RowOps {
     std::vector<Matrix> matrices;
 
     static bool owns(const std::string &kernel) {
-        for (const char *prefix : {"mv_q4", "mm_q4", "q4_repack", "block_norm", "logprobs"})
+        for (const char *prefix : {"mv_q4", "mm_q4", "q4_repack", "block_norm", "logprobs", "rotary", "attend"})
             if (kernel.rfind(prefix, 0) == 0) return true;
         return false;
     }
