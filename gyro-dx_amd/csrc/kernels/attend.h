@@ -1,71 +1,111 @@
 // Attention of new tokens over a paged cache: what every build of it shares. The tokens of a sequence that read one of the
 // cache's heads, `group` = heads / kv_heads queries' heads each, are its rows: row r is head r % group of token r / group, so
-// that a page read once serves them all. A launch's groups take (sequence, cache head, tile of rows, part of the keys); where
-// the keys are split, attend_join puts the parts together.
+// that a page read once serves them all.
+//
+// Sequences of few rows (attend_few.h, fp32 in attend_f32.h): a launch's groups take (sequence, cache head, tile of 16 rows, part
+// of the keys). Those of more (attend_tile.h): attend_plan cuts them into units, a tile of 128 rows and a run of its keys
+// each, which the groups take, every head's. Where keys are split, attend_join puts the parts together.
 //
 // Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table
-// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 workspace 28 heads 29 group 30 D 31 kv heads
+// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 heads 29 group 30 D 31 kv heads
 // 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 causal 39 window 40 scale times log2(e)
-// 41 parts 42 tiles of rows per sequence 43 type 44 rows of a tile 45 keys of a tile 46 tiles that make a part worth its join
+// 41 parts 42 tiles of rows per sequence 43 type 44 keys of a tile 45 tiles that make a part worth its join 46 rows of a
+// sequence that units take it from (0: none) 47 groups of attend_join for the few rows 48 units' list 50 units' parts 52 page
+// size's shift plus one (0: no power of two) 53 units that the list holds 54 parts that the workspace holds, per head
+// 55 keys of a tile of units
 #pragma once
 #include "rows.h"
 
 // What a group that shares its rows' keys keeps in the workspace: the maximum and the sum of each row, then the rows.
-__device__ __forceinline__ uint64_t at_part(const GdArgs &a, uint64_t item, uint32_t part, uint32_t rows) {
-    return gd_addr(a, 26) + (item * a.c[41] + part) * (uint64_t)(rows * 4u) * (a.c[30] + 2u);
+__device__ __forceinline__ uint64_t at_part_bytes(const GdArgs &a, uint32_t rows) { return (uint64_t)(rows * 4u) * (a.c[30] + 2u); }
+
+// Of few rows: AF_ROWS a group.
+#define AF_WAVES 4u
+#define AF_ROWS 16u
+__device__ __forceinline__ uint64_t af_part(const GdArgs &a, uint64_t item, uint32_t part) {
+    return gd_addr(a, 26) + (item * a.c[41] + part) * at_part_bytes(a, AF_ROWS);
+}
+
+// Of many rows: AT_ROWS a group. The list of units that attend_plan makes.
+#define AT_ROWS 128u
+#define AT_SPLITS 1024u
+struct AtUnit {
+    uint32_t seq, tile, from, to;       // tile of rows, tiles of keys
+    uint32_t slot, part, parts, none;  // parts of one tile of rows have neighbouring slots
+};
+struct AtPlan {
+    uint32_t units, splits, none[62];
+    uint32_t split[AT_SPLITS];  // units that are the first of several parts
+};
+__device__ __forceinline__ gd_gptr<AtPlan> at_plan(const GdArgs &a) { return gd_at<AtPlan>(gd_addr(a, 48)); }
+__device__ __forceinline__ gd_gptr<AtUnit> at_units(const GdArgs &a) { return gd_at<AtUnit>(gd_addr(a, 48) + sizeof(AtPlan)); }
+__device__ __forceinline__ uint64_t at_slot(const GdArgs &a, uint32_t slot, uint32_t head) {
+    return gd_addr(a, 50) + ((uint64_t)slot * a.c[31] + head) * at_part_bytes(a, AT_ROWS);
 }
 
 // A tile of rows of a sequence and cache head, and the keys that any of them sees.
 struct AtItem {
     uint32_t seq, head, token0, ql, rows, row0;  // rows: of the sequence and head; row0: the tile's first
-    int32_t kl, first, end;       // keys first .. end - 1 are seen by some row of the tile,
-    int32_t all_first, all_end;   // all_first .. all_end - 1 by each
+    int32_t kl, first, end;      // keys first .. end - 1 are seen by some row of the tile,
+    int32_t all_first, all_end;  // all_first .. all_end - 1 by each
 };
 
-__device__ __forceinline__ bool at_item(const GdArgs &a, uint32_t item, uint32_t tile_rows, AtItem &o) {
-    const uint32_t KVH = a.c[31], S = a.c[32], longest = a.c[33], n = a.c[34], group = a.c[29], tiles = a.c[42];
-    const uint32_t rest = item / KVH;
-    o.head = item - rest * KVH;
-    o.seq = rest / tiles;
-    o.row0 = (rest - o.seq * tiles) * tile_rows;
-    if (o.seq >= S) return false;
+// A sequence's tokens and keys, as the tables say and the call's bounds allow.
+__device__ __forceinline__ void at_sequence(const GdArgs &a, uint32_t seq, AtItem &o) {
+    const uint32_t longest = a.c[33], n = a.c[34];
     const int32_t most = (int32_t)(a.c[37] * a.c[36]);
-    o.kl = min(max(gd_at<const int32_t>(gd_addr(a, 22))[o.seq], 0), most);
+    o.seq = seq;
+    o.kl = min(max(gd_at<const int32_t>(gd_addr(a, 22))[seq], 0), most);
     if (gd_addr(a, 24)) {
-        const gd_gptr<const int32_t> starts = gd_at<const int32_t>(gd_addr(a, 24)) + o.seq;
+        const gd_gptr<const int32_t> starts = gd_at<const int32_t>(gd_addr(a, 24)) + seq;
         const int32_t from = min(max(starts[0], 0), (int32_t)n), to = min(max(starts[1], from), (int32_t)n);
         o.token0 = from;
         o.ql = to - from;
     } else {
-        o.token0 = o.seq * longest;
+        o.token0 = seq * longest;
         o.ql = longest;
     }
-    o.rows = o.ql * group;
-    if (o.row0 >= o.rows) return false;
-    // Positions of the tile's first and last token.
-    const int32_t base = o.kl - (int32_t)o.ql, p0 = base + (int32_t)(o.row0 / group),
-                  p1 = base + (int32_t)((min(o.row0 + tile_rows, o.rows) - 1u) / group), window = (int32_t)a.c[39];
+    o.rows = o.ql * a.c[29];
+}
+// The keys that rows row0 .. row0 + rows - 1 (as far as there are) of a sequence see.
+__device__ __forceinline__ void at_keys(const GdArgs &a, uint32_t row0, uint32_t rows, AtItem &o) {
+    const uint32_t group = a.c[29];
+    const int32_t window = (int32_t)a.c[39];
     const bool causal = a.c[38] != 0u;
+    o.row0 = row0;
+    // Positions of the tile's first and last token.
+    const int32_t base = o.kl - (int32_t)o.ql, p0 = base + (int32_t)(row0 / group),
+                  p1 = base + (int32_t)((min(row0 + rows, o.rows) - 1u) / group);
     o.first = window ? max(0, p0 - window + 1) : 0;
     o.end = causal ? max(0, p1 + 1) : o.kl;
     o.all_first = window ? max(0, p1 - window + 1) : 0;
     o.all_end = causal ? p0 + 1 : o.kl;
+}
+// A tile of few rows.
+__device__ __forceinline__ bool af_item(const GdArgs &a, uint32_t item, AtItem &o) {
+    const uint32_t KVH = a.c[31], tiles = a.c[42];
+    const uint32_t rest = item / KVH, seq = rest / tiles, row0 = (rest - seq * tiles) * AF_ROWS;
+    if (seq >= a.c[32]) return false;
+    o.head = item - rest * KVH;
+    at_sequence(a, seq, o);
+    if (row0 >= o.rows || (a.c[46] && o.rows >= a.c[46])) return false;
+    at_keys(a, row0, AF_ROWS, o);
     return true;
 }
-// Tiles of `keys` keys of an item, the first's number, and how many of the launch's parts share them: as many as leave each
-// `least` tiles.
+// Tiles of `keys` keys of an item and the first's number; and how many of the launch's parts share them: as many as leave each
+// enough of them.
 __device__ __forceinline__ uint32_t at_tiles(const AtItem &o, uint32_t keys, uint32_t &tile0) {
     tile0 = (uint32_t)o.first / keys;
     return o.end > o.first ? ((uint32_t)o.end + keys - 1u) / keys - tile0 : 0u;
 }
-__device__ __forceinline__ uint32_t at_parts(const GdArgs &a, uint32_t tiles, uint32_t least) {
-    return max(1u, min(a.c[41], (tiles + least - 1u) / least));
+__device__ __forceinline__ uint32_t at_parts(const GdArgs &a, uint32_t tiles) {
+    return max(1u, min(a.c[41], (tiles + a.c[45] - 1u) / a.c[45]));
 }
 
 // The offset in the cache, in bytes, of key j of a sequence; -1: on a page outside it (or past `end`).
 __device__ __forceinline__ int64_t at_key(const GdArgs &a, uint32_t seq, uint32_t head, int32_t j, int32_t end) {
     if (j >= end) return -1;
-    const uint32_t page_size = a.c[36], slot = (uint32_t)j / page_size;
+    const uint32_t page_size = a.c[36], slot = a.c[52] ? (uint32_t)j >> (a.c[52] - 1u) : (uint32_t)j / page_size;
     const uint32_t page = (uint32_t)gd_at<const int32_t>(gd_addr(a, 18))[seq * gd_addr(a, 20) + slot];
     if (page >= a.c[35]) return -1;
     return page * gd_addr(a, 12) + ((uint32_t)j - slot * page_size) * gd_addr(a, 16) + head * gd_addr(a, 14);
@@ -98,9 +138,7 @@ __device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, 
 // Below every score that counts, and finite: the difference of two such is zero, not NaN.
 #define AT_LOWEST -1e30f
 
-// Few rows (attend_few.h, attend_f32.h): a group of four waves takes a tile of 16 rows and a part of the keys.
-#define AF_WAVES 4u
-#define AF_ROWS 16u
+// Few rows (attend_few.h, attend_f32.h).
 
 // The larger (the sum) of the four lanes that hold a row's keys, 16 lanes apart.
 __device__ __forceinline__ float af_max(float v) {
@@ -124,10 +162,10 @@ __device__ __forceinline__ bool af_work(const GdArgs &a, AfWork &w) {
     const uint32_t parts = a.c[41], id = blockIdx.y * gridDim.x + blockIdx.x, group = a.c[29];
     w.item = id / parts;
     w.part = id - w.item * parts;
-    if (!at_item(a, w.item, AF_ROWS, w.o)) return false;
+    if (!af_item(a, w.item, w.o)) return false;
     uint32_t tile0;
-    const uint32_t tiles = at_tiles(w.o, a.c[45], tile0);
-    w.shared = at_parts(a, tiles, a.c[46]);
+    const uint32_t tiles = at_tiles(w.o, a.c[44], tile0);
+    w.shared = at_parts(a, tiles);
     if (w.part >= w.shared) return false;
     w.from = tile0 + (uint32_t)((uint64_t)tiles * w.part / w.shared);
     w.to = tile0 + (uint32_t)((uint64_t)tiles * (w.part + 1u) / w.shared);
@@ -167,7 +205,7 @@ __device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, cons
         total += stats[w][1][r] * shrink[w];
     }
     const bool alone = k.shared == 1u;
-    const uint64_t to_part = at_part(a, k.item, k.part, AF_ROWS);
+    const uint64_t to_part = af_part(a, k.item, k.part);
     if (!alone && c == 0u) {
         gd_at<float>(to_part)[r] = most;
         gd_at<float>(to_part)[AF_ROWS + r] = total;

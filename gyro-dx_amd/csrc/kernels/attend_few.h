@@ -10,12 +10,9 @@
 // The weights are the sum of two 16-bit parts, so that they lose nothing: these rows are bound by memory, and the second
 // products run in its shadow.
 #pragma once
-#include "attend.h"
+#include "attend16.h"
 
 #define AF_KEYS 32u
-
-typedef _Float16 at_f16x8 __attribute__((ext_vector_type(8)));
-typedef short at_s16x4 __attribute__((ext_vector_type(4)));
 
 template <uint32_t TYPE>
 __device__ __forceinline__ gd_f32x4 af_mfma(gd_u32x4 a, gd_u32x4 b, gd_f32x4 c) {
@@ -24,26 +21,6 @@ __device__ __forceinline__ gd_f32x4 af_mfma(gd_u32x4 a, gd_u32x4 b, gd_f32x4 c) 
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b), c, 0, 0, 0);
 }
-template <uint32_t TYPE>
-__device__ __forceinline__ uint32_t at_pair(float lo, float hi) {
-    return row_bits16(lo, TYPE) | row_bits16(hi, TYPE) << 16;
-}
-// The larger magnitudes of two words' values, as bits; and whether one of them is not finite.
-typedef uint16_t at_u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t at_larger(uint32_t a, uint32_t w) {
-    const at_u16x2 r = __builtin_elementwise_max(__builtin_bit_cast(at_u16x2, a), __builtin_bit_cast(at_u16x2, w & 0x7fff7fffu));
-    return __builtin_bit_cast(uint32_t, r);
-}
-template <uint32_t TYPE>
-__device__ __forceinline__ bool at_not_finite(uint32_t a) {
-    constexpr uint32_t e = TYPE == ROW_BF16 ? 0x7f80u : 0x7c00u;
-    return (a & 0xffffu) >= e || a >> 16 >= e;
-}
-// Of 4 rows of 16 neighbouring 16-bit values in LDS, lane l of 16 names values 4 (l % 4) .. of row l / 4 and gets column l.
-__device__ __forceinline__ gd_u32x2 at_transposed(const char *p) {
-    return __builtin_bit_cast(gd_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s16x4 *)(uintptr_t)p));
-}
-
 template <uint32_t TYPE, uint32_t DT>
 __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
     // VROW: 16 rows' neighbouring 32 bytes in all banks.
@@ -65,7 +42,7 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
     }
     const float scale = gd_bits_f32(a.c[40]);
     const uint64_t K = gd_addr(a, 8), V = gd_addr(a, 10);
-    char *const mine = lds + wave * VTILE;
+    const uint32_t mine = at_lds(lds) + wave * VTILE;
     gd_f32x4 acc[DIMS];
 #pragma unroll
     for (uint32_t d = 0; d < DIMS; ++d) acc[d] = none;
@@ -105,7 +82,7 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
                 for (uint32_t i = 0; i < 4; ++i) {
                     const uint32_t key = 16u * b + 4u * h + i;
                     const int32_t j = (int32_t)(32u * t + key);
-                    if (!(valid >> key & 1u) || j > work.last || j < work.first) s[b][i] = -INFINITY;
+                    s[b][i] = !(valid >> key & 1u) | (j > work.last) | (j < work.first) ? -INFINITY : s[b][i];
                 }
         }
         // Keys whose values are not all finite.
@@ -155,14 +132,14 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
 #pragma unroll
             for (uint32_t j = 0; j < AF_KEYS / PER; ++j) {
                 const uint32_t key = PER * j + lane / CHUNKS;
-                *reinterpret_cast<gd_u32x4 *>(mine + key * VROW + (lane % CHUNKS) * 16u) = keys >> key & 1u ? v[j] : empty;
+                at_lds_store(mine + key * VROW + (lane % CHUNKS) * 16u, keys >> key & 1u ? v[j] : empty);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
         // V^T of 16 channels and the keys 4 h .. and 16 + 4 h .., in the order of the weights.
         auto values = [&](uint32_t d) {
-            const char *const p = mine + (4u * h + (col >> 2)) * VROW + 32u * d + 8u * (col & 3u);
+            const uint32_t p = mine + (4u * h + (col >> 2)) * VROW + 32u * d + 8u * (col & 3u);
             const gd_u32x2 x = at_transposed(p), y = at_transposed(p + 16u * VROW);
             return gd_u32x4{x[0], x[1], y[0], y[1]};
         };
@@ -186,7 +163,7 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
                 const gd_f32x4 one = af_mfma<TYPE>(values(d), large, none);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (seen) acc[d][i] += one[i];
+                    acc[d][i] += seen ? one[i] : 0.f;
             }
         }
     }

@@ -1,0 +1,3 @@
+// Attention of many rows, bf16 heads of up to 128 values (attend_tile.h).
+#include "attend_tile.h"
+GD_PIPELINE_NAMED_OCC(attend_tile_b128, 256, 2) { attend_tile_body<ROW_BF16, 128, 64>(a); }

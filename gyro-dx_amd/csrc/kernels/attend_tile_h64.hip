@@ -1,0 +1,3 @@
+// Attention of many rows, binary16 heads of up to 64 values (attend_tile.h).
+#include "attend_tile.h"
+GD_PIPELINE_NAMED_OCC(attend_tile_h64, 256, 2) { attend_tile_body<ROW_F16, 64, 64>(a); }

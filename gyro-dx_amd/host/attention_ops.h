@@ -7,6 +7,21 @@
 
 namespace gyro {
 
+// Launches of the same constants, one after another.
+struct Launches {
+    Constants c;
+    struct Step {
+        const char *kernel;
+        uint32_t x, y;
+    } step[4] = {};
+    int count = 0;
+    // A grid of at least `groups` groups (a kernel's own check drops the others).
+    void add(const char *kernel, uint64_t groups) {
+        const uint32_t x = (uint32_t)std::min<uint64_t>(groups, 65535);
+        step[count++] = {kernel, x, (uint32_t)((groups + x - 1) / x)};
+    }
+};
+
 struct Rotary {
     Buffer table;  // per pair the fraction of a turn of one position, of 2^64
     uint32_t pairs = 0, layout = 0;
@@ -181,15 +196,21 @@ class AttentionOps {
 
     // ---- attention ----
 
-    // Groups that a launch's keys are split for, and rows that a group takes: the workspace holds that many groups' rows.
-    static constexpr uint32_t kGroups = 1024, kParts = 256;
+    // Few rows: groups that a launch's keys are split for at most. Many: parts of 128 rows that the workspace holds (attend_plan
+    // makes them of tiles with more keys than a 512th of all, twice 512 at most), and units.
+    static constexpr uint32_t kGroups = 1024, kParts = 256, kSlots = 1024, kUnits = 1u << 18, kPlanBytes = 256 + 4 * 1024, kUnitBytes = 32;
+    static constexpr uint32_t kFewRows = 16, kTileRows = 128;
+    static uint64_t part_bytes(uint32_t rows, uint32_t D) { return (uint64_t)rows * 4 * (D + 2); }
+    // The workspace: the few rows' parts, the plan with its units, the units' parts.
+    static uint64_t plan_at(uint32_t D) { return kGroups * part_bytes(kFewRows, D); }
+    static uint64_t slots_at(uint32_t D) { return plan_at(D) + kPlanBytes + (uint64_t)kUnits * kUnitBytes; }
     static uint64_t workspace(uint32_t heads, uint32_t kv_heads, uint32_t D) {
         if (!heads || !kv_heads || heads % kv_heads || !D || D > 256) return 0;
-        return (uint64_t)kGroups * 16 * 4 * (D + 2);
+        return slots_at(D) + kSlots * part_bytes(kTileRows, D);
     }
 
-    static Launch attention(const gm_attention_desc &d, uint32_t n) {
-        Launch l;
+    static Launches attention(const gm_attention_desc &d, uint32_t n) {
+        Launches l;
         if (!n) return l;  // of no rows there may be no memory
         const uint32_t D = d.cache.head_dim, G = d.cache.kv_heads, H = d.heads;
         check_cache(d.cache, "gm_attention: cache");
@@ -209,15 +230,10 @@ class AttentionOps {
         require(d.causal || !d.window, "gm_attention: a window without the causal mask");
         require(d.scale > 0 && std::isfinite(d.scale), "gm_attention: scale");
         const bool wide = d.cache.type == GM_F32;
-        const uint32_t tile_rows = 16, keys = wide ? 16 : 32, least = 4;
-        const uint32_t group = H / G, tiles = (uint32_t)(((uint64_t)d.longest * group + tile_rows - 1) / tile_rows);
-        const uint64_t items = (uint64_t)d.sequences * G * tiles;
-        require(items < 1u << 31, "gm_attention: too many sequences");
-        // Parts of the keys, while the groups are fewer than those the GPU holds.
-        const uint64_t key_tiles = (capacity + keys - 1) / keys;
-        const uint32_t parts = (uint32_t)std::max<uint64_t>(1, std::min({(uint64_t)kParts, kGroups / items, (key_tiles + least - 1) / least}));
-        const uint64_t need = parts == 1 ? 0 : items * parts * tile_rows * 4 * (D + 2);
-        require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0), "gm_attention: workspace");
+        const uint32_t group = H / G;
+        const uint64_t rows = (uint64_t)d.longest * group;
+        // Sequences of more than 16 rows go to attend_tile, the others, and all of fp32, to the kernels of few rows.
+        const bool many = !wide && rows > kFewRows, few = !many || d.starts;
         Constants &c = l.c;
         c.set(0, d.q.data);
         c.set64(2, d.q.stride);
@@ -230,7 +246,6 @@ class AttentionOps {
         c.set64(20, d.table_stride);
         c.set(22, d.lengths);
         c.set(24, d.starts);
-        c.set(26, d.workspace);
         c.set(28, H);
         c.set(29, group);
         c.set(30, D);
@@ -244,29 +259,59 @@ class AttentionOps {
         c.set(38, d.causal ? 1u : 0u);
         c.set(39, std::min(d.window, 1u << 30));
         c.set(40, d.scale * 1.44269504088896341f);
-        c.set(41, parts);
-        c.set(42, tiles);
         c.set(43, d.cache.type);
-        c.set(44, tile_rows);
-        c.set(45, keys);
-        c.set(46, least);
-        const int size = D <= 64 ? 0 : D <= 128 ? 1 : 2;
-        static const char *const names[3][3] = {{"attend_f32_64", "attend_f32_128", "attend_f32_256"},
-                                                {"attend_few_b64", "attend_few_b128", "attend_few_b256"},
-                                                {"attend_few_h64", "attend_few_h128", "attend_few_h256"}};
-        l.kernel = names[d.cache.type][size];
-        grid(items * parts, l.x, l.y);
-        if (parts > 1) {
-            l.next = "attend_join";
-            grid((items * tile_rows + 3) / 4, l.next_x, l.next_y);
+        c.set(45, kLeast);
+        c.set(46, many ? kFewRows + 1 : 0u);
+        for (uint32_t shift = 0; shift < 31; ++shift)
+            if (d.cache.page_size == 1u << shift) c.set(52, shift + 1);
+        const int size = D <= 64 ? 0 : D <= 128 ? 1 : 2, type = d.cache.type;
+        uint64_t need = 0, join = 0;
+        uint32_t parts = 1;
+        uint64_t items = 0;
+        if (few) {
+            const uint32_t keys = wide ? 16 : 32, tiles = wide ? (uint32_t)((rows + kFewRows - 1) / kFewRows) : 1;
+            items = (uint64_t)d.sequences * G * tiles;
+            require(items < 1u << 31, "gm_attention: too many sequences");
+            // Parts of the keys, while the groups are fewer than those the GPU holds.
+            const uint64_t key_tiles = (capacity + keys - 1) / keys;
+            parts = (uint32_t)std::max<uint64_t>(1, std::min({(uint64_t)kParts, kGroups / items, (key_tiles + kLeast - 1) / kLeast}));
+            c.set(41, parts);
+            c.set(42, tiles);
+            c.set(44, keys);
+            if (parts > 1) {
+                need = items * parts * part_bytes(kFewRows, D);
+                join = (items * kFewRows + 3) / 4;
+            }
         }
+        c.set(47, (uint32_t)join);
+        uint64_t units = 0;
+        if (many) {
+            // Whole tiles of rows, one more for each sequence, and the parts of those that are split.
+            units = (uint64_t)n * group / kTileRows + std::min<uint64_t>(d.sequences, (uint64_t)n * group / (kFewRows + 1)) + 512 / G + 1;
+            require(units <= kUnits && units * G < 1u << 31, "gm_attention: n * heads / kv_heads / 128 + sequences is at most 2^18 - 1024");
+            need = workspace(H, G, D);
+            join += 512;
+            c.set64(48, (uint64_t)(uintptr_t)d.workspace + plan_at(D));
+            c.set64(50, (uint64_t)(uintptr_t)d.workspace + slots_at(D));
+            c.set(53, (uint32_t)units);
+            c.set(54, kSlots / G);
+            c.set(55, D > 128 ? 32u : 64u);
+            l.add("attend_plan", 1);
+        }
+        require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0), "gm_attention: workspace");
+        c.set(26, d.workspace);
+        static const char *const few_names[3][3] = {{"attend_f32_64", "attend_f32_128", "attend_f32_256"},
+                                                    {"attend_few_b64", "attend_few_b128", "attend_few_b256"},
+                                                    {"attend_few_h64", "attend_few_h128", "attend_few_h256"}};
+        static const char *const tile_names[3][3] = {{}, {"attend_tile_b64", "attend_tile_b128", "attend_tile_b256"},
+                                                     {"attend_tile_h64", "attend_tile_h128", "attend_tile_h256"}};
+        if (few) l.add(few_names[type][size], items * parts);
+        if (many) l.add(tile_names[type][size], units * G);
+        if (join) l.add("attend_join", join);
         return l;
     }
-    // A grid of at least `groups` groups.
-    static void grid(uint64_t groups, uint32_t &x, uint32_t &y) {
-        x = (uint32_t)std::min<uint64_t>(groups, 65535);
-        y = (uint32_t)((groups + x - 1) / x);
-    }
+    // Tiles of keys that make a part worth its join.
+    static constexpr uint32_t kLeast = 4;
 };
 
 }  // namespace gyro

@@ -518,6 +518,12 @@ class Engine {
         check(gd_dispatch_on(dev.ctx, first, l.c.w, 60, l.x, l.y, 1, on), "gd_dispatch_on");
         if (next) check(gd_dispatch_on(dev.ctx, next, l.c.w, 60, l.next_x, l.next_y, 1, on), "gd_dispatch_on");
     }
+    void launch(const Launches &l, void *stream) {
+        gd_pipeline *pipes[4] = {};
+        for (int i = 0; i < l.count; ++i) pipes[i] = op_kernel(l.step[i].kernel, stream);
+        for (int i = 0; i < l.count; ++i)
+            check(gd_dispatch_on(dev.ctx, pipes[i], l.c.w, 60, l.step[i].x, l.step[i].y, 1, stream ? stream : GD_STREAM_DEFAULT), "gd_dispatch_on");
+    }
     // upload() of any number of bytes: the last word is filled up with zeros (the buffer has room).
     void upload_bytes(const Buffer &dst, uint64_t off, const void *src, uint64_t bytes) {
         const uint64_t whole = bytes & ~uint64_t(3);

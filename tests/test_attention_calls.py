@@ -46,8 +46,20 @@ extern "C" int plan_rotary(const gm_rotary_desc *d, uint32_t n, uint32_t pairs, 
 extern "C" int plan_append(const gm_cache_append_desc *d, uint32_t n, uint32_t pairs, uint32_t *out, char *why) {
     return run(why, [&] { tell(ops(pairs).append(*d, n), out, why); });
 }
+// The launches' grids, then the constants; their names, one after another.
 extern "C" int plan_attention(const gm_attention_desc *d, uint32_t n, uint32_t, uint32_t *out, char *why) {
-    return run(why, [&] { tell(AttentionOps::attention(*d, n), out, why); });
+    return run(why, [&] {
+        const Launches l = AttentionOps::attention(*d, n);
+        std::string names;
+        out[0] = l.count;
+        for (int i = 0; i < l.count; ++i) {
+            out[1 + 2 * i] = l.step[i].x;
+            out[2 + 2 * i] = l.step[i].y;
+            names += std::string(l.step[i].kernel) + " ";
+        }
+        std::memcpy(out + 9, l.c.w, sizeof(l.c.w));
+        std::strncpy(why, names.c_str(), 199);
+    });
 }
 """
 
@@ -79,7 +91,7 @@ def cache(**kw):
 
 
 def call(f, d, n, pairs=16):
-    why, out = C.create_string_buffer(200), (C.c_uint32 * 64)()
+    why, out = C.create_string_buffer(200), (C.c_uint32 * 70)()
     rc = f(C.byref(d), n, pairs, out, why)
     return rc, why.value.decode(), list(out)
 
@@ -255,31 +267,68 @@ def test_attention_refusals(shim):
                   attention(table_width=0), attention(table_width=1 << 27), attention(table_stride=1 << 41), attention(causal=0, window=4),
                   attention(scale=0.0), attention(scale=-1.0), attention(scale=float("nan")), attention(scale=float("inf")),
                   attention(table_width=1000, workspace=None), attention(table_width=1000, workspace=A + 128),
-                  attention(table_width=1000, workspace_bytes=4096), attention(cache=cache(pages=0)), attention(cache=cache(type=3)),
+                  attention(table_width=1000, workspace_bytes=4096), attention(heads=64, table_width=1, workspace=None),
+                  attention(heads=64, table_width=1, workspace_bytes=1 << 20), attention(cache=cache(pages=0)), attention(cache=cache(type=3)),
                   attention(cache=cache(pages=1 << 27)), (attention(sequences=1 << 28, longest=1), 1 << 28)])
     assert call(shim.plan_attention, attention(), 0)[2][0] == 0
 
 
 @pytest.mark.parametrize("type", [0, 1, 2])
-@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (1, 1, 8), (64, 1, 256), (32, 8, 128), (40, 40, 72)])
-def test_attention_workspace(shim, type, heads, kv, dim):
-    """The workspace serves every call, and the grid covers every row and part."""
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (1, 1, 8), (64, 1, 256), (32, 8, 128), (40, 40, 72), (700, 700, 64)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_launches(shim, type, heads, kv, dim, ragged):
+    """Sequences of few rows and of many go to their kernels, the grids cover every row and part, and the workspace serves
+    every call."""
     most = engine.lib().gm_attention_workspace(heads, kv, dim)
-    c = cache(type=type, kv_heads=kv, head_dim=dim)
+    c, group = cache(type=type, kv_heads=kv, head_dim=dim), heads // kv
+    few_bytes, part = 1024 * 16 * 4 * (dim + 2), 128 * 4 * (dim + 2)
+    assert most == few_bytes + 4352 + (32 << 18) + 1024 * part
     for sequences, longest in ((1, 1), (1, 5), (1, 4096), (3, 1), (64, 1), (64, 7), (300, 100), (5000, 1), (2, 100000)):
+        if sequences * longest * group > 128 * 250000 or sequences * longest * heads > 1 << 30:
+            continue
         for width in (1, 3, 60, 1000, 60000000):
             d = attention(cache=c, q=rows(type), out=rows(type, data=3 * A), heads=heads, sequences=sequences, longest=longest, table_width=width,
-                          workspace_bytes=most)
-            rc, why, out = call(shim.plan_attention, d, sequences * longest)
-            assert rc == 0, why
-            w = out[4:]
-            parts, tiles, tile_rows, keys, least = w[41], w[42], w[44], w[45], w[46]
-            assert tiles * tile_rows >= longest * heads // kv > (tiles - 1) * tile_rows
-            assert 1 <= parts <= 256 and (parts == 1 or (parts - 1) * least * keys < width * 16)
-            assert 1 <= out[0] <= 65535 and 1 <= out[1] <= 65535 and out[0] * out[1] >= sequences * kv * tiles * parts
-            if parts > 1:
-                assert 4 * out[2] * out[3] >= sequences * kv * tiles * tile_rows and out[3] <= 65535
-                assert sequences * kv * tiles * parts * tile_rows * 4 * (dim + 2) <= most
+                          workspace_bytes=most, starts=A if ragged else None)
+            rc, names, out = call(shim.plan_attention, d, sequences * longest)
+            assert rc == 0, names
+            names, w = names.split(), out[9:]
+            grids = {name: out[1 + 2 * i] * out[2 + 2 * i] for i, name in enumerate(names)}
+            assert len(names) == out[0] and all(1 <= v <= 65535 for v in out[1:1 + 2 * out[0]])
+            many = type and longest * group > 16
+            size = 64 if dim <= 64 else 128 if dim <= 128 else 256
+            few = "attend_f32_%d" % size if not type else "attend_few_%s%d" % ("?bh"[type], size)
+            tile = "attend_tile_%s%d" % ("?bh"[type], size)
+            assert names[:1] == ["attend_plan"] if many else "attend_plan" not in names
+            assert (few in names) == (not many or ragged) and (tile in names) == bool(many)
+            assert w[46] == (17 if many else 0) and w[52] == 5  # pages of 16
+            join = 0
+            if few in names:
+                parts, tiles, keys, least = w[41], w[42], w[44], w[45]
+                assert keys == (32 if type else 16)
+                assert tiles == 1 if type else tiles * 16 >= longest * group > (tiles - 1) * 16
+                assert 1 <= parts <= 256 and (parts == 1 or (parts - 1) * least * keys < width * 16)
+                assert grids[few] >= sequences * kv * tiles * parts
+                if parts > 1:
+                    assert sequences * kv * tiles * parts * 16 * 4 * (dim + 2) <= few_bytes
+                    join = w[47]
+                    assert 4 * join >= sequences * kv * tiles * 16
+            assert w[47] == join
+            if many:
+                units = w[53]
+                assert grids["attend_plan"] == 1 and grids[tile] >= units * kv and units <= 1 << 18
+                # Tiles of rows, the most there are if every sequence has one that is not whole, and what splits add.
+                assert units > -(-sequences * longest * group // 128) + 512 // kv
+                assert w[48] | w[49] << 32 == A + few_bytes and w[50] | w[51] << 32 == A + few_bytes + 4352 + (32 << 18)
+                assert w[54] * kv * part <= 1024 * part and w[55] == (32 if dim > 128 else 64)
+                assert grids["attend_join"] >= join + 512
+            else:
+                assert ("attend_join" in names) == bool(join) and (not join or grids["attend_join"] >= join)
+
+
+def test_page_shifts(shim):
+    for size, want in ((1, 1), (2, 2), (3, 0), (16, 5), (100, 0), (256, 9), (1 << 20, 21)):
+        c = cache(page_size=size, token_stride=64, head_stride=size * 64, page_stride=size * 128)
+        assert call(shim.plan_attention, attention(cache=c), 3)[2][9 + 52] == want
 
 
 def test_workspace_of_no_shape():

@@ -350,6 +350,32 @@ def test_attention_long(eng):
         assert all(torch.equal(first, x) for x in again)
 
 
+@pytest.mark.parametrize("type,dim", [("bf16", 128), ("f16", 64), ("bf16", 256), ("f16", 200)])
+def test_attention_split_tiles(eng, type, dim):
+    """Rows of one or a few tiles whose keys many groups share, beside sequences of few rows; the same results every time."""
+    for counts, lengths, kw in (([20], [9001], {}), ([50, 1, 5, 40], [4000, 5000, 77, 30], dict(window=1000)), ([70, 17], [1500, 3000], dict(causal=False))):
+        print(f"split tiles {type} {dim} {counts} {kw}", flush=True)
+        b = Batch(eng, type, 2, 1, dim, 16, counts, lengths, seed=16)
+        b.run(**kw)
+        b.check(**kw)
+        first = b.out.clone()
+        for _ in range(3):
+            b.run(**kw)
+        torch.cuda.synchronize()
+        assert torch.equal(first, b.out)
+
+
+def test_attention_many_sequences(eng):
+    """More sequences than the plan looks at in one go, of few rows, many, none."""
+    rng = np.random.default_rng(61)
+    counts = [int(c) for c in rng.choice([0, 1, 2, 9, 20, 40, 150], 1300, p=[0.1, 0.3, 0.2, 0.2, 0.1, 0.09, 0.01])]
+    lengths = [c + int(rng.integers(0, 30)) for c in counts]
+    b = Batch(eng, "bf16", 2, 1, 64, 16, counts, lengths, seed=17)
+    print(f"{len(counts)} sequences, {b.n} tokens", flush=True)
+    b.run()
+    b.check()
+
+
 @pytest.mark.parametrize("type", ["bf16", "f16"])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 1]])
 def test_offsets_past_32_bits(eng, type, counts):
