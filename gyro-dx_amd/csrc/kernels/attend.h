@@ -2,17 +2,19 @@
 // cache's heads, `group` = heads / kv_heads queries' heads each, are its rows: row r is head r % group of token r / group, so
 // that a page read once serves them all.
 //
-// Sequences of few rows (attend_few.h, fp32 in attend_f32.h): a launch's groups take (sequence, cache head, tile of 16 rows, part
-// of the keys). Those of more (attend_tile.h): attend_plan cuts them into units, a tile of 128 rows and a run of its keys
-// each, which the groups take, every head's. Where keys are split, attend_join puts the parts together.
+// Sequences of few rows (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and cache head and a
+// part of its keys, and finds out by itself which (af_share). Those of more (attend_tile.h): attend_plan cuts them into units, a
+// tile of 128 rows and a run of its keys each, which the groups take, every head's. Where keys are split, attend_join puts the
+// parts together.
 //
 // Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table
 // 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 heads 29 group 30 D 31 kv heads
 // 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 causal 39 window 40 scale times log2(e)
-// 41 parts 42 tiles of rows per sequence 43 type 44 keys of a tile 45 tiles that make a part worth its join 46 rows of a
-// sequence that units take it from (0: none) 47 groups of attend_join for the few rows 48 units' list 50 units' parts 52 page
-// size's shift plus one (0: no power of two) 53 units that the list holds 54 parts that the workspace holds, per head
-// 55 keys of a tile of units
+// 41 groups that few rows' keys are split for (0: they are not) 42 tiles of few rows per sequence 43 type 44 keys of a tile
+// 45 tiles that make a part 46 rows of a sequence that units take it from (0: none) 47 groups of attend_join for
+// the few rows 48 units' list 50 units' parts 52 page size's shift plus one (0: no power of two) 53 units that the list holds
+// 54 parts that the workspace holds, per head 55 keys of a tile of units 56 rows that attend_join takes of a few rows' tile
+// 57 tiles of keys up to which few rows' are not split 58 tiles that make a unit
 #pragma once
 #include "rows.h"
 
@@ -20,10 +22,9 @@
 __device__ __forceinline__ uint64_t at_part_bytes(const GdArgs &a, uint32_t rows) { return (uint64_t)(rows * 4u) * (a.c[30] + 2u); }
 
 // Of few rows: AF_ROWS a group.
-#define AF_WAVES 4u
 #define AF_ROWS 16u
-__device__ __forceinline__ uint64_t af_part(const GdArgs &a, uint64_t item, uint32_t part) {
-    return gd_addr(a, 26) + (item * a.c[41] + part) * at_part_bytes(a, AF_ROWS);
+__device__ __forceinline__ uint64_t af_part(const GdArgs &a, uint32_t slot, uint32_t head) {
+    return gd_addr(a, 26) + ((uint64_t)slot * a.c[31] + head) * at_part_bytes(a, AF_ROWS);
 }
 
 // Of many rows: AT_ROWS a group. The list of units that attend_plan makes.
@@ -81,34 +82,23 @@ __device__ __forceinline__ void at_keys(const GdArgs &a, uint32_t row0, uint32_t
     o.all_first = window ? max(0, p1 - window + 1) : 0;
     o.all_end = causal ? p0 + 1 : o.kl;
 }
-// A tile of few rows.
-__device__ __forceinline__ bool af_item(const GdArgs &a, uint32_t item, AtItem &o) {
-    const uint32_t KVH = a.c[31], tiles = a.c[42];
-    const uint32_t rest = item / KVH, seq = rest / tiles, row0 = (rest - seq * tiles) * AF_ROWS;
-    if (seq >= a.c[32]) return false;
-    o.head = item - rest * KVH;
-    at_sequence(a, seq, o);
-    if (row0 >= o.rows || (a.c[46] && o.rows >= a.c[46])) return false;
-    at_keys(a, row0, AF_ROWS, o);
-    return true;
-}
-// Tiles of `keys` keys of an item and the first's number; and how many of the launch's parts share them: as many as leave each
-// enough of them.
+// Tiles of `keys` keys of an item and the first's number.
 __device__ __forceinline__ uint32_t at_tiles(const AtItem &o, uint32_t keys, uint32_t &tile0) {
     tile0 = (uint32_t)o.first / keys;
     return o.end > o.first ? ((uint32_t)o.end + keys - 1u) / keys - tile0 : 0u;
 }
-__device__ __forceinline__ uint32_t at_parts(const GdArgs &a, uint32_t tiles) {
-    return max(1u, min(a.c[41], (tiles + a.c[45] - 1u) / a.c[45]));
-}
 
-// The offset in the cache, in bytes, of key j of a sequence; -1: on a page outside it (or past `end`).
-__device__ __forceinline__ int64_t at_key(const GdArgs &a, uint32_t seq, uint32_t head, int32_t j, int32_t end) {
-    if (j >= end) return -1;
-    const uint32_t page_size = a.c[36], slot = a.c[52] ? (uint32_t)j >> (a.c[52] - 1u) : (uint32_t)j / page_size;
-    const uint32_t page = (uint32_t)gd_at<const int32_t>(gd_addr(a, 18))[seq * gd_addr(a, 20) + slot];
-    if (page >= a.c[35]) return -1;
-    return page * gd_addr(a, 12) + ((uint32_t)j - slot * page_size) * gd_addr(a, 16) + head * gd_addr(a, 14);
+// The page of key j of a sequence, and the key's offset in the cache, in bytes; -1: on a page outside it (or past `end`). Apart,
+// so that the page's load can be far ahead of its use. No load is conditional: the compiler counts the loads that are on their
+// way, and would wait for all of them where it is not certain of their number.
+__device__ __forceinline__ uint32_t at_slot_of(const GdArgs &a, uint32_t i) { return a.c[52] ? i >> (a.c[52] - 1u) : i / a.c[36]; }
+__device__ __forceinline__ uint32_t at_page(const GdArgs &a, uint32_t seq, int32_t j, int32_t end) {
+    return (uint32_t)gd_at<const int32_t>(gd_addr(a, 18))[seq * gd_addr(a, 20) + at_slot_of(a, j < end ? (uint32_t)j : 0u)];
+}
+__device__ __forceinline__ int64_t at_key(const GdArgs &a, uint32_t page, uint32_t head, int32_t j, int32_t end) {
+    const uint32_t place = (uint32_t)j - at_slot_of(a, (uint32_t)j) * a.c[36];
+    const int64_t at = page * gd_addr(a, 12) + place * gd_addr(a, 16) + head * gd_addr(a, 14);
+    return (j < end) & (page < a.c[35]) ? at : -1;
 }
 
 // The larger of a value and lane ^ 32's.
@@ -150,25 +140,101 @@ __device__ __forceinline__ float af_sum(float v) {
     return at_sum_halves(gd_bits_f32(r[0]) + gd_bits_f32(r[1]));
 }
 
+// How the few rows' keys are shared out: entry e is tile e % tiles of sequence e / tiles. One of more tiles of keys than a constant is
+// split into as many parts as leave none more than `share` tiles, a fair part of all entries' and heads' among the groups. The
+// split entries' parts come first, then the whole ones. Every wave works this out by itself, 64 entries at a time.
+struct AfEntry {
+    uint32_t rows, keys;  // of the sequence (0: none for this launch), tiles of keys
+};
+__device__ __forceinline__ AfEntry af_entry(const GdArgs &a, uint32_t e, AtItem &o, uint32_t &tile0) {
+    const uint32_t tiles = a.c[42], seq = tiles == 1u ? e : e / tiles, row0 = (e - seq * tiles) * AF_ROWS;
+    o.rows = 0u;
+    if (seq >= a.c[32]) return {0u, 0u};
+    at_sequence(a, seq, o);
+    if (row0 >= o.rows || (a.c[46] && o.rows >= a.c[46])) {
+        o.rows = 0u;
+        return {0u, 0u};
+    }
+    at_keys(a, row0, AF_ROWS, o);
+    return {o.rows, at_tiles(o, a.c[44], tile0)};
+}
+__device__ __forceinline__ uint32_t af_last(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+
+struct AfShare {
+    AfEntry first;  // the lane's of the first 64
+    uint32_t share;
+};
+__device__ __forceinline__ AfEntry af_mine(const GdArgs &a, const AfShare &s, uint32_t e0) {
+    AtItem o;
+    uint32_t tile0;
+    return e0 ? af_entry(a, e0 + (threadIdx.x & 63u), o, tile0) : s.first;
+}
+__device__ __forceinline__ AfShare af_share(const GdArgs &a) {
+    const uint32_t entries = a.c[32] * a.c[42];
+    AfShare s;
+    AtItem o;
+    uint32_t tile0;
+    s.first = af_entry(a, threadIdx.x & 63u, o, tile0);
+    uint64_t all = 0;
+    for (uint32_t e0 = 0; e0 < entries; e0 += 64u) all += af_last(gd_wave_scan_u32(af_mine(a, s, e0).keys));  // at most 2^25 each
+    s.share = (uint32_t)max((uint64_t)a.c[45], (all * a.c[31] + a.c[41] - 1u) / a.c[41]);
+    return s;
+}
+// The entry of number `wanted` among the split ones, counting parts (or entries), or the whole ones; false: there are fewer.
+// `wanted` becomes the part's number in it, `slot` the number of its first part among all split ones'.
+enum { AF_PARTS, AF_SPLITS, AF_WHOLE };
+template <int WHAT>
+__device__ __forceinline__ bool af_find(const GdArgs &a, const AfShare &s, uint32_t &wanted, uint32_t &entry, uint32_t &parts, uint32_t &slot) {
+    const uint32_t entries = a.c[32] * a.c[42];
+    slot = 0;
+    for (uint32_t e0 = 0; e0 < entries; e0 += 64u) {
+        const AfEntry mine = af_mine(a, s, e0);
+        const uint32_t split = mine.keys > max(s.share, a.c[57]) ? (mine.keys + s.share - 1u) / s.share : 0u;
+        const uint32_t count = WHAT == AF_PARTS ? split : WHAT == AF_SPLITS ? (split ? 1u : 0u) : mine.rows && !split ? 1u : 0u;
+        const uint32_t upto = gd_wave_scan_u32(count), total = af_last(upto), slots = gd_wave_scan_u32(split);
+        if (wanted < total) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(__ballot(upto > wanted));  // the first lane past it
+            auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)at); };
+            entry = e0 + at;
+            parts = max(1u, of(split));
+            slot += of(slots) - of(split);
+            wanted -= of(upto) - of(count);
+            return true;
+        }
+        wanted -= total;
+        slot += af_last(slots);
+    }
+    return false;
+}
+
 // A group's tile, its part of the keys' tiles, and what a lane knows of its row: lane l has row l % 16 (rows past the last are
 // the last again), and of the scores the keys 4 (l / 16) + i.
 struct AfWork {
     AtItem o;
-    uint32_t item, part, shared, from, to;
+    uint32_t slot, parts, from, to;
     uint64_t q;           // offset of the row in q, in values
     int32_t first, last;  // keys that the row sees
 };
 __device__ __forceinline__ bool af_work(const GdArgs &a, AfWork &w) {
-    const uint32_t parts = a.c[41], id = blockIdx.y * gridDim.x + blockIdx.x, group = a.c[29];
-    w.item = id / parts;
-    w.part = id - w.item * parts;
-    if (!af_item(a, w.item, w.o)) return false;
-    uint32_t tile0;
-    const uint32_t tiles = at_tiles(w.o, a.c[44], tile0);
-    w.shared = at_parts(a, tiles);
-    if (w.part >= w.shared) return false;
-    w.from = tile0 + (uint32_t)((uint64_t)tiles * w.part / w.shared);
-    w.to = tile0 + (uint32_t)((uint64_t)tiles * (w.part + 1u) / w.shared);
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, group = a.c[29], KVH = a.c[31], unit = id / KVH;
+    uint32_t part = 0, entry = unit, tile0;
+    w.parts = 1;
+    w.slot = 0;
+    if (a.c[41]) {
+        const AfShare share = af_share(a);
+        part = unit;
+        if (!af_find<AF_PARTS>(a, share, part, entry, w.parts, w.slot)) {
+            uint32_t none;
+            if (!af_find<AF_WHOLE>(a, share, part, entry, w.parts, none)) return false;
+        }
+    }
+    const AfEntry own = af_entry(a, entry, w.o, tile0);
+    const uint32_t tiles = own.keys;
+    if (!own.rows) return false;
+    w.o.head = id - unit * KVH;
+    w.slot += part;
+    w.from = tile0 + (uint32_t)((uint64_t)tiles * part / w.parts);
+    w.to = tile0 + (uint32_t)((uint64_t)tiles * (part + 1u) / w.parts);
     const uint32_t row = min(w.o.row0 + (threadIdx.x & 15u), w.o.rows - 1u), token = row / group;
     w.q = (uint64_t)(w.o.token0 + token) * gd_addr(a, 2) + (uint64_t)(w.o.head * group + row - token * group) * a.c[30];
     const int32_t p = w.o.kl - (int32_t)w.o.ql + (int32_t)token, window = (int32_t)a.c[39];
@@ -177,35 +243,34 @@ __device__ __forceinline__ bool af_work(const GdArgs &a, AfWork &w) {
     return true;
 }
 
-// Joins the waves' parts in LDS and writes the rows, or the group's part of them. A lane holds channels 16 d + 4 (l / 16) + i
-// of its row; a wave's room in lds, EACH values, holds its 16 rows of DT + 4.
-template <uint32_t TYPE, uint32_t DT, uint32_t EACH>
-__device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, const gd_f32x4 (&acc)[DT / 16u], float top, float sum, float *lds) {
+// Joins the waves' parts and writes the rows, or the group's part of them. The waves have put their rows into LDS, DT + 4 values
+// each, EACH values a wave.
+template <uint32_t TYPE, uint32_t DT, uint32_t EACH, uint32_t WAVES>
+__device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, float top, float sum, float *lds) {
     constexpr uint32_t WIDE = DT + 4u;
     static_assert(EACH >= AF_ROWS * WIDE, "a wave's rows");
-    __shared__ float stats[AF_WAVES][2][AF_ROWS];
+    __shared__ float stats[WAVES][2][AF_ROWS];
     const AtItem &o = k.o;
-    const uint32_t lane = threadIdx.x & 63u, col = lane & 15u, h = lane >> 4, wave = threadIdx.x >> 6, D = a.c[30], group = a.c[29];
+    const uint32_t lane = threadIdx.x & 63u, col = lane & 15u, wave = threadIdx.x >> 6, D = a.c[30], group = a.c[29];
     sum = af_sum(sum);
-    if (h == 0u) {
+    if (lane < 16u) {
         stats[wave][0][col] = top;
         stats[wave][1][col] = sum;
     }
-#pragma unroll
-    for (uint32_t d = 0; d < DT / 16u; ++d) *reinterpret_cast<gd_f32x4 *>(lds + wave * EACH + col * WIDE + 16u * d + 4u * h) = acc[d];
     __syncthreads();
-    const uint32_t r = threadIdx.x >> 4, c = threadIdx.x & 15u;  // 16 threads a row
+    constexpr uint32_t THREADS = 4u * WAVES;  // of a row
+    const uint32_t r = threadIdx.x / THREADS, c = threadIdx.x % THREADS;
     if (o.row0 + r >= o.rows) return;
-    float most = stats[0][0][r], total = 0.f, shrink[AF_WAVES];
+    float most = stats[0][0][r], total = 0.f, shrink[WAVES];
 #pragma unroll
-    for (uint32_t w = 1; w < AF_WAVES; ++w) most = fmaxf(most, stats[w][0][r]);
+    for (uint32_t w = 1; w < WAVES; ++w) most = fmaxf(most, stats[w][0][r]);
 #pragma unroll
-    for (uint32_t w = 0; w < AF_WAVES; ++w) {
+    for (uint32_t w = 0; w < WAVES; ++w) {
         shrink[w] = at_exp2(stats[w][0][r] - most);
         total += stats[w][1][r] * shrink[w];
     }
-    const bool alone = k.shared == 1u;
-    const uint64_t to_part = af_part(a, k.item, k.part);
+    const bool alone = k.parts == 1u;
+    const uint64_t to_part = af_part(a, k.slot, o.head);
     if (!alone && c == 0u) {
         gd_at<float>(to_part)[r] = most;
         gd_at<float>(to_part)[AF_ROWS + r] = total;
@@ -215,12 +280,12 @@ __device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, cons
                                           << row_shift(TYPE));
     const float by = 1.f / total;
 #pragma unroll
-    for (uint32_t e = 0; e < (DT + 63u) / 64u; ++e) {
-        const uint32_t d = 64u * e + 4u * c;
+    for (uint32_t e = 0; e < (DT + 4u * THREADS - 1u) / (4u * THREADS); ++e) {
+        const uint32_t d = 4u * THREADS * e + 4u * c;
         if (d >= D) continue;
         gd_f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (uint32_t w = 0; w < AF_WAVES; ++w) {
+        for (uint32_t w = 0; w < WAVES; ++w) {
             const gd_f32x4 y = *reinterpret_cast<const gd_f32x4 *>(lds + w * EACH + r * WIDE + d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] += y[i] * shrink[w];

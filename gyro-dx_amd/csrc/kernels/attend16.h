@@ -6,21 +6,24 @@ typedef _Float16 at_f16x8 __attribute__((ext_vector_type(8)));
 typedef float at_f32x16 __attribute__((ext_vector_type(16)));
 typedef short at_s16x4 __attribute__((ext_vector_type(4)));
 
+// Two values rounded to the type, to nearest even, as a word.
+typedef __bf16 at_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 at_f16x2 __attribute__((ext_vector_type(2)));
+typedef float at_f32x2 __attribute__((ext_vector_type(2)));
 template <uint32_t TYPE>
 __device__ __forceinline__ uint32_t at_pair(float lo, float hi) {
-    return row_bits16(lo, TYPE) | row_bits16(hi, TYPE) << 16;
+    if constexpr (TYPE == ROW_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f32x2{lo, hi}), at_bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f32x2{lo, hi}), at_f16x2));
 }
-// The larger magnitudes of two words' values, as bits; and whether one of them is not finite.
-typedef uint16_t at_u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t at_larger(uint32_t a, uint32_t w) {
-    const at_u16x2 r = __builtin_elementwise_max(__builtin_bit_cast(at_u16x2, a), __builtin_bit_cast(at_u16x2, w & 0x7fff7fffu));
-    return __builtin_bit_cast(uint32_t, r);
-}
+// c while a word's values are finite, from then on NaN (0 times the others is).
 template <uint32_t TYPE>
-__device__ __forceinline__ bool at_not_finite(uint32_t a) {
-    constexpr uint32_t e = TYPE == ROW_BF16 ? 0x7f80u : 0x7c00u;
-    return (a & 0xffffu) >= e || a >> 16 >= e;
+__device__ __forceinline__ float at_finite(uint32_t w, float c) {
+    if constexpr (TYPE == ROW_BF16)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(at_bf16x2, w), at_bf16x2{(__bf16)0.f, (__bf16)0.f}, c, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(at_f16x2, w), at_f16x2{(_Float16)0.f, (_Float16)0.f}, c, false);
 }
+
 // LDS by its 32-bit addresses.
 template <typename T>
 using at_lptr = __attribute__((address_space(3))) T *;

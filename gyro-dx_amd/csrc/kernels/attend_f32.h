@@ -1,66 +1,97 @@
-// Attention of fp32 rows (attend.h): a group of four waves takes up to 16 rows and a part of the keys, its waves every
-// fourth tile of 16 keys.
+// Attention of fp32 rows (attend.h): a group takes up to 16 rows and a part of the keys, its waves tiles of 16 keys in turn.
 //
 // As attend_few.h, by v_mfma_f32_16x16x4_f32: a lane holds 4 keys of one row, which are the second product's operand as they
-// lie, and the values' operand is one value of a key, so that both cache arrays go from memory straight to operands.
+// lie. Of the values a lane loads 4 neighbouring channels of a key, one for each of 4 products, whose rows are then channels 4
+// apart: both cache arrays go from memory straight to operands, 16 bytes a lane.
 #pragma once
 #include "attend.h"
 
-#define AS_KEYS 16u
-
-template <uint32_t DT>
+template <uint32_t DT, uint32_t WAVES>
 __device__ __forceinline__ void attend_f32_body(const GdArgs &a) {
-    constexpr uint32_t STEPS = DT / 16u;
-    __shared__ __align__(16) float lds[AF_WAVES * AF_ROWS * (DT + 4u)];
+    constexpr uint32_t STEPS = DT / 16u, WIDE = DT + 4u, EACH = AF_ROWS * WIDE;
+    __shared__ __align__(16) float lds[WAVES * EACH];
     const uint32_t lane = threadIdx.x & 63u, col = lane & 15u, h = lane >> 4, D = a.c[30];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    AfWork k;
-    if (!af_work(a, k)) return;
-    const AtItem &o = k.o;
+    AfWork work;
+    if (!af_work(a, work)) return;
+    const AtItem &o = work.o;
     const gd_f32x4 none = {0.f, 0.f, 0.f, 0.f};
     gd_f32x4 q[STEPS], acc[STEPS];
 #pragma unroll
     for (uint32_t s = 0; s < STEPS; ++s) {
         q[s] = acc[s] = none;
-        if (16u * s + 4u * h < D) q[s] = *gd_at<const gd_f32x4_any>(gd_addr(a, 0) + 4u * k.q + 64u * s + 16u * h);
+        if (16u * s + 4u * h < D) q[s] = *gd_at<const gd_f32x4_any>(gd_addr(a, 0) + 4u * work.q + 64u * s + 16u * h);
     }
     const float scale = gd_bits_f32(a.c[40]);
     const uint64_t K = gd_addr(a, 8), V = gd_addr(a, 10);
     float top = AT_LOWEST, sum = 0.f;
 
-    for (uint32_t t = k.from + wave; t < k.to; t += AF_WAVES) {
-        const int64_t at = at_key(a, o.seq, o.head, (int32_t)(16u * t + col), o.end);
-        const uint32_t valid = (uint32_t)__ballot(at >= 0) & 0xffffu;  // the wave's quarters hold the same keys
+    // A tile's keys, as in attend_few.h: lane l knows the place in the cache of key l % 16; k and v are on their way from when
+    // their registers are free again.
+    gd_f32x4 k[STEPS], v[4][STEPS / 4u];
+    auto key_of = [&](uint32_t t) { return (int32_t)(16u * t + col); };
+    auto page = [&](uint32_t t) { return at_page(a, o.seq, key_of(t), t < work.to ? o.end : 0); };
+    auto locate = [&](uint32_t t, uint32_t page) { return at_key(a, page, o.head, key_of(t), t < work.to ? o.end : 0); };
+    auto place = [&](int64_t at, uint32_t key) {
         const uint64_t offset = at < 0 ? 0ull : (uint64_t)at;
-        gd_f32x4 s = none;
+        return (uint64_t)__shfl((uint32_t)offset, key, 64) | (uint64_t)__shfl((uint32_t)(offset >> 32), key, 64) << 32;
+    };
+    auto head_end = [&] {
+        uint32_t d = D;
+        asm volatile("" : "+s"(d));
+        return d;
+    };
+    auto load_k = [&](int64_t at) {
+        const uint64_t from = K + (at < 0 ? 0ull : (uint64_t)at) + 16u * h;
+        if (D == DT) {
 #pragma unroll
-        for (uint32_t e = 0; e < STEPS; ++e) {
-            gd_f32x4 x = none;
-            if (16u * e + 4u * h < D) x = *gd_at<const gd_f32x4_any>(K + offset + 64u * e + 16u * h);
+            for (uint32_t s = 0; s < STEPS; ++s) k[s] = gd_at<const gd_f32x4_any>(from)[4u * s];
+        } else {
+            const uint32_t d = head_end();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], q[e][i], s, 0, 0, 0);
+            for (uint32_t s = 0; s < STEPS; ++s) k[s] = *gd_at<const gd_f32x4_any>(16u * s + 4u * h < d ? from + 64u * s : from - 16u * h);
         }
-        float v[4][STEPS];
-        bool odd = false;
+    };
+    auto load_v = [&](int64_t at) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t key = 4u * h + i;
-            const uint32_t lo = __shfl((uint32_t)offset, key, 64), hi = __shfl((uint32_t)(offset >> 32), key, 64);
+            const uint64_t from = V + place(at, 4u * h + i) + 16u * col;
+            if (D == DT) {
 #pragma unroll
-            for (uint32_t d = 0; d < STEPS; ++d) {
-                v[i][d] = 0.f;
-                if (16u * d + col < D && (valid >> key & 1u))
-                    v[i][d] = *gd_at<const float>(V + ((uint64_t)lo | (uint64_t)hi << 32) + 64u * d + 4u * col);
-                odd |= !(__builtin_fabsf(v[i][d]) < INFINITY);
+                for (uint32_t g = 0; g < STEPS / 4u; ++g) v[i][g] = gd_at<const gd_f32x4_any>(from)[16u * g];
+            } else {
+                const uint32_t d = head_end();
+#pragma unroll
+                for (uint32_t g = 0; g < STEPS / 4u; ++g) v[i][g] = *gd_at<const gd_f32x4_any>(64u * g + 4u * col < d ? from + 256u * g : from - 16u * col);
             }
         }
+    };
+    uint32_t soon = page(work.from + wave + WAVES);
+    int64_t here = locate(work.from + wave, page(work.from + wave));
+    load_k(here);
+    __builtin_amdgcn_sched_barrier(0);  // keys first, as in the loop: the waits count what came after them
+    load_v(here);
+    for (uint32_t t = work.from + wave; t < work.to; t += WAVES) {
+        const uint32_t later = page(t + 2u * WAVES);
+        const uint32_t valid = (uint32_t)__ballot(here >= 0) & 0xffffu;  // the wave's quarters hold the same keys
+        if (D != DT)
+#pragma unroll
+            for (uint32_t e = 0; e < STEPS; ++e)
+                if (16u * e + 4u * h >= head_end()) k[e] = none;  // (q is zero there, but 0 times NaN is not)
+        gd_f32x4 s = none;
+#pragma unroll
+        for (uint32_t e = 0; e < STEPS; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e][i], q[e][i], s, 0, 0, 0);
+        const int64_t next = locate(t + WAVES, soon);
+        load_k(next);
         // Tiles that not every row sees whole.
         if (valid != 0xffffu || (int32_t)(16u * t) < o.all_first || (int32_t)(16u * t + 16u) > o.all_end) {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t key = 4u * h + i;
                 const int32_t j = (int32_t)(16u * t + key);
-                if (!(valid >> key & 1u) || j > k.last || j < k.first) s[i] = -INFINITY;
+                s[i] = !(valid >> key & 1u) | (j > work.last) | (j < work.first) ? -INFINITY : s[i];
             }
         }
         const float most = fmaxf(top, af_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * scale);
@@ -73,6 +104,19 @@ __device__ __forceinline__ void attend_f32_body(const GdArgs &a) {
         for (uint32_t d = 0; d < STEPS; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[d][i] *= shrink;
+        if (valid != 0xffffu || D != DT)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+                for (uint32_t g = 0; g < STEPS / 4u; ++g)
+                    if ((64u * g + 4u * col >= head_end()) | !(valid >> (4u * h + i) & 1u)) v[i][g] = none;
+        bool odd = false;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+            for (uint32_t g = 0; g < STEPS / 4u; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= !(__builtin_fabsf(v[i][g][e]) < INFINITY);
         if (__ballot(odd)) {
             // A value that is not finite reaches the rows that see its key, and no other (0 times it is NaN): one key
             // after another.
@@ -81,21 +125,30 @@ __device__ __forceinline__ void attend_f32_body(const GdArgs &a) {
 #pragma unroll 1
                 for (uint32_t w = 0; w < 4; ++w) {
                     const int32_t j = (int32_t)(16u * t + 4u * w + i);
-                    const bool seen = j <= k.last && j >= k.first;
+                    const bool seen = j <= work.last && j >= work.first;
 #pragma unroll
                     for (uint32_t d = 0; d < STEPS; ++d) {
-                        const gd_f32x4 one = __builtin_amdgcn_mfma_f32_16x16x4f32(h == w ? v[i][d] : 0.f, s[i], none, 0, 0, 0);
+                        const gd_f32x4 one = __builtin_amdgcn_mfma_f32_16x16x4f32(h == w ? v[i][d >> 2][d & 3u] : 0.f, s[i], none, 0, 0, 0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (seen) acc[d][e] += one[e];
+                        for (int e = 0; e < 4; ++e) acc[d][e] += seen ? one[e] : 0.f;
                     }
                 }
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
 #pragma unroll
-                for (uint32_t d = 0; d < STEPS; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], s[i], acc[d], 0, 0, 0);
+                for (uint32_t d = 0; d < STEPS; ++d) acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d >> 2][d & 3u], s[i], acc[d], 0, 0, 0);
         }
+        load_v(next);
+        here = next;
+        soon = later;
     }
-    af_finish<ROW_F32, DT, AF_ROWS * (DT + 4u)>(a, k, acc, top, sum, lds);
+    // Row 4 h + i of product 4 g + e is channel 64 g + 16 h + 4 i + e.
+#pragma unroll
+    for (uint32_t g = 0; g < STEPS / 4u; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<gd_f32x4 *>(lds + wave * EACH + col * WIDE + 64u * g + 16u * h + 4 * i) =
+                gd_f32x4{acc[4 * g][i], acc[4 * g + 1][i], acc[4 * g + 2][i], acc[4 * g + 3][i]};
+    af_finish<ROW_F32, DT, EACH, WAVES>(a, work, top, sum, lds);
 }

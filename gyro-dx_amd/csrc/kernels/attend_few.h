@@ -1,11 +1,14 @@
-// Attention of few rows (attend.h), 16-bit types: a group of four waves takes up to 16 rows and a part of the keys, its waves
-// every fourth tile of 32 keys.
+// Attention of few rows (attend.h), 16-bit types: a group takes up to 16 rows and a part of the keys, its waves tiles of 32 keys
+// in turn.
 //
 // A tile's scores are K Q^T by two v_mfma_f32_16x16x32 a step: a lane then holds 8 keys of one row, the others are 16, 32 and 48
 // lanes away, so that the running maximum needs two exchanges per tile, the sum none until the end, and the weights are the
 // second product's operand as they lie: O^T += V^T P^T, contracted over keys in the order in which lanes hold them. Keys go
 // from memory straight to operands. Values go through LDS, a wave's tile its own, and come back transposed
 // (ds_read_b64_tr_b16).
+//
+// The maximum that weights are relative to follows the running one only when that has grown by more than 2^8, so that the sums
+// are rarely rescaled; weights are at most 2^8 then, and as precise.
 //
 // The weights are the sum of two 16-bit parts, so that they lose nothing: these rows are bound by memory, and the second
 // products run in its shadow.
@@ -21,12 +24,12 @@ __device__ __forceinline__ gd_f32x4 af_mfma(gd_u32x4 a, gd_u32x4 b, gd_f32x4 c) 
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b), c, 0, 0, 0);
 }
-template <uint32_t TYPE, uint32_t DT>
+template <uint32_t TYPE, uint32_t DT, uint32_t WAVES>
 __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
     // VROW: 16 rows' neighbouring 32 bytes in all banks.
     constexpr uint32_t STEPS = DT / 32u, DIMS = DT / 16u, VROW = DT * 2u + 32u, CHUNKS = DT / 8u, PER = 64u / CHUNKS;
     constexpr uint32_t VTILE = AF_KEYS * VROW;
-    __shared__ __align__(16) char lds[AF_WAVES * VTILE];
+    __shared__ __align__(16) char lds[WAVES * VTILE];
     const uint32_t lane = threadIdx.x & 63u, col = lane & 15u, h = lane >> 4, D = a.c[30];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     AfWork work;
@@ -48,32 +51,65 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
     for (uint32_t d = 0; d < DIMS; ++d) acc[d] = none;
     float top = AT_LOWEST, sum = 0.f;
 
-    for (uint32_t t = work.from + wave; t < work.to; t += AF_WAVES) {
-        const int64_t at = at_key(a, o.seq, o.head, (int32_t)(32u * t + (lane & 31u)), o.end);
-        const uint32_t valid = (uint32_t)__ballot(at >= 0);  // both halves of the wave hold the same keys
+    // A tile's keys: a lane knows the place in the cache of key l % 32; k and v are on their way from when their registers are
+    // free again, a tile ahead of their use. (Where there is none, the cache's first are loaded, and dropped later: at_key says
+    // why.)
+    gd_u32x4 k[2][STEPS], v[AF_KEYS / PER];
+    const uint32_t chunk = lane % CHUNKS, of_key = lane / CHUNKS;
+    const bool beyond = 8u * chunk >= D;
+    auto key_of = [&](uint32_t t) { return (int32_t)(32u * t + (lane & 31u)); };
+    auto page = [&](uint32_t t) { return at_page(a, o.seq, key_of(t), t < work.to ? o.end : 0); };
+    auto locate = [&](uint32_t t, uint32_t page) { return at_key(a, page, o.head, key_of(t), t < work.to ? o.end : 0); };
+    auto place = [&](int64_t at, uint32_t key) {
         const uint64_t offset = at < 0 ? 0ull : (uint64_t)at;
-        gd_u32x4 k[2][STEPS], v[AF_KEYS / PER];
+        return (uint64_t)__shfl((uint32_t)offset, key, 64) | (uint64_t)__shfl((uint32_t)(offset >> 32), key, 64) << 32;
+    };
+    // (D as the compiler sees it anew in each tile: it would hold the clamped offsets in registers through the loop.)
+    auto head_end = [&] {
+        uint32_t d = D;
+        asm volatile("" : "+s"(d));
+        return d;
+    };
+    auto load_k = [&](int64_t at) {
+        const uint64_t from[2] = {K + place(at, col) + 16u * h, K + place(at, 16u + col) + 16u * h};
+        if (D == DT) {
 #pragma unroll
-        for (uint32_t b = 0; b < 2; ++b) {
-            const uint32_t lo = __shfl((uint32_t)offset, 16u * b + col, 64), hi = __shfl((uint32_t)(offset >> 32), 16u * b + col, 64);
+            for (uint32_t b = 0; b < 2; ++b)
 #pragma unroll
-            for (uint32_t s = 0; s < STEPS; ++s) {
-                k[b][s] = empty;
-                if (32u * s + 8u * h < D) k[b][s] = *gd_at<const gd_u32x4_any>(K + ((uint64_t)lo | (uint64_t)hi << 32) + 64u * s + 16u * h);
-            }
+                for (uint32_t s = 0; s < STEPS; ++s) k[b][s] = gd_at<const gd_u32x4_any>(from[b])[4u * s];
+        } else {
+            const uint32_t d = head_end();
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b)
+#pragma unroll
+                for (uint32_t s = 0; s < STEPS; ++s) k[b][s] = *gd_at<const gd_u32x4_any>(32u * s + 8u * h < d ? from[b] + 64u * s : from[b] - 16u * h);
         }
+    };
+    auto load_v = [&](int64_t at) {
 #pragma unroll
-        for (uint32_t j = 0; j < AF_KEYS / PER; ++j) {
-            const uint32_t key = PER * j + lane / CHUNKS, chunk = lane % CHUNKS;
-            const uint32_t lo = __shfl((uint32_t)offset, key, 64), hi = __shfl((uint32_t)(offset >> 32), key, 64);
-            v[j] = empty;
-            if (8u * chunk < D && (valid >> key & 1u)) v[j] = *gd_at<const gd_u32x4_any>(V + ((uint64_t)lo | (uint64_t)hi << 32) + 16u * chunk);
-        }
+        for (uint32_t j = 0; j < AF_KEYS / PER; ++j) v[j] = *gd_at<const gd_u32x4_any>(V + place(at, PER * j + of_key) + (beyond ? 0u : 16u * chunk));
+    };
+    uint32_t soon = page(work.from + wave + WAVES);
+    int64_t here = locate(work.from + wave, page(work.from + wave));
+    load_k(here);
+    __builtin_amdgcn_sched_barrier(0);  // keys first, as in the loop: the waits count what came after them
+    load_v(here);
+    for (uint32_t t = work.from + wave; t < work.to; t += WAVES) {
+        const uint32_t later = page(t + 2u * WAVES);
+        const uint32_t valid = (uint32_t)__ballot(here >= 0);  // both halves of the wave hold the same keys
+        if (D != DT)
+#pragma unroll
+            for (uint32_t b = 0; b < 2; ++b)
+#pragma unroll
+                for (uint32_t s = 0; s < STEPS; ++s)
+                    if (32u * s + 8u * h >= head_end()) k[b][s] = empty;  // (q is zero there, but 0 times NaN is not)
         gd_f32x4 s[2] = {none, none};
 #pragma unroll
         for (uint32_t e = 0; e < STEPS; ++e)
 #pragma unroll
             for (uint32_t b = 0; b < 2; ++b) s[b] = af_mfma<TYPE>(k[b][e], q[e], s[b]);
+        const int64_t next = locate(t + WAVES, soon);
+        load_k(next);
         // Tiles that not every row sees whole.
         if (valid != ~0u || (int32_t)(32u * t) < o.all_first || (int32_t)(32u * t + 32u) > o.all_end) {
 #pragma unroll
@@ -85,41 +121,49 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
                     s[b][i] = !(valid >> key & 1u) | (j > work.last) | (j < work.first) ? -INFINITY : s[b][i];
                 }
         }
-        // Keys whose values are not all finite.
-        uint32_t bad = 0, largest = 0;
+        if (valid != ~0u || D != DT)
+#pragma unroll
+            for (uint32_t j = 0; j < AF_KEYS / PER; ++j)
+                if (beyond | !(valid >> (PER * j + of_key) & 1u)) v[j] = empty;
+        // Keys whose values are not all finite: taken out here, they come back one by one below.
+        uint32_t bad = 0;
+        float finite[2] = {0.f, 0.f};
 #pragma unroll
         for (uint32_t j = 0; j < AF_KEYS / PER; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) largest = at_larger(largest, v[j][i]);
-        if (__ballot(at_not_finite<TYPE>(largest))) {
+            for (int i = 0; i < 4; ++i) finite[i & 1] = at_finite<TYPE>(v[j][i], finite[i & 1]);
+        if (__ballot(!(finite[0] + finite[1] == 0.f))) {
 #pragma unroll
             for (uint32_t j = 0; j < AF_KEYS / PER; ++j) {
-                largest = 0;
+                float c = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) largest = at_larger(largest, v[j][i]);
-                const uint64_t lanes = __ballot(at_not_finite<TYPE>(largest));
+                for (int i = 0; i < 4; ++i) c = at_finite<TYPE>(v[j][i], c);
+                const uint64_t lanes = __ballot(!(c == 0.f));
 #pragma unroll
                 for (uint32_t e = 0; e < PER; ++e)
                     if (lanes >> (e * CHUNKS) & ((1ull << CHUNKS) - 1u)) bad |= 1u << (PER * j + e);
+                if (bad >> (PER * j + of_key) & 1u) v[j] = empty;
             }
         }
         float most = s[0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, s[i >> 2][i & 3]);
-        most = fmaxf(top, af_max(most) * scale);
-        const float shrink = at_exp2(top - most);
-        top = most;
-        float of_tile = 0.f;
+        most = af_max(most) * scale;
+        if (__ballot(most > top + 8.f)) {
+            most = fmaxf(most, top);
+            const float shrink = at_exp2(top - most);
+            top = most;
+            sum *= shrink;
+#pragma unroll
+            for (uint32_t d = 0; d < DIMS; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[d][i] *= shrink;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            s[i >> 2][i & 3] = at_exp2(fmaf(s[i >> 2][i & 3], scale, -most));
-            of_tile += s[i >> 2][i & 3];
+            s[i >> 2][i & 3] = at_exp2(fmaf(s[i >> 2][i & 3], scale, -top));
+            sum += s[i >> 2][i & 3];
         }
-        sum = sum * shrink + of_tile;
-#pragma unroll
-        for (uint32_t d = 0; d < DIMS; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[d][i] *= shrink;
         gd_u32x4 large, small;  // the weights' parts
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -127,23 +171,21 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
             large[i] = at_pair<TYPE>(x, y);
             small[i] = at_pair<TYPE>(x - row_value16(large[i] & 0xffffu, TYPE), y - row_value16(large[i] >> 16, TYPE));
         }
-        auto stage = [&](uint32_t keys) {
-            __builtin_amdgcn_wave_barrier();  // after the reads of what is there
+        __builtin_amdgcn_wave_barrier();  // after the reads of what is there
 #pragma unroll
-            for (uint32_t j = 0; j < AF_KEYS / PER; ++j) {
-                const uint32_t key = PER * j + lane / CHUNKS;
-                at_lds_store(mine + key * VROW + (lane % CHUNKS) * 16u, keys >> key & 1u ? v[j] : empty);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        };
+        for (uint32_t j = 0; j < AF_KEYS / PER; ++j) {
+            const uint32_t key = PER * j + of_key;
+            at_lds_store(mine + key * VROW + chunk * 16u, v[j]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        load_v(next);
         // V^T of 16 channels and the keys 4 h .. and 16 + 4 h .., in the order of the weights.
         auto values = [&](uint32_t d) {
             const uint32_t p = mine + (4u * h + (col >> 2)) * VROW + 32u * d + 8u * (col & 3u);
             const gd_u32x2 x = at_transposed(p), y = at_transposed(p + 16u * VROW);
             return gd_u32x4{x[0], x[1], y[0], y[1]};
         };
-        stage(~bad);
 #pragma unroll
         for (uint32_t d = 0; d < DIMS; ++d) {
             const gd_u32x4 x = values(d);
@@ -157,15 +199,27 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
             bad &= bad - 1u;
             const int32_t j = (int32_t)(32u * t + key);
             const bool seen = j <= work.last && j >= work.first;
-            stage(1u << key);
+            const uint64_t from = V + place(here, key);
+            // The key's weight is in the lanes of quarter key / 4 % 4, one of a pair in a word.
+            uint32_t pair = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                if ((key >> 4) * 2u + (key >> 1 & 1u) == i) pair = large[i];
+            pair = __shfl(key & 1u ? pair >> 16 : pair & 0xffffu, col + 16u * (key >> 2 & 3u), 64);
+            const float weight = row_value16(pair, TYPE);
 #pragma unroll
             for (uint32_t d = 0; d < DIMS; ++d) {
-                const gd_f32x4 one = af_mfma<TYPE>(values(d), large, none);
+                const uint32_t dim = 16u * d + 4u * h;
+                const gd_u32x2 x = *gd_at<const at_u32x2_any>(from + 2u * (dim < D ? dim : 0u));
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[d][i] += seen ? one[i] : 0.f;
+                for (int i = 0; i < 4; ++i) acc[d][i] += seen ? weight * row_value16(x[i >> 1] >> (16 * (i & 1)) & 0xffffu, TYPE) : 0.f;
             }
         }
+        here = next;
+        soon = later;
     }
-    af_finish<TYPE, DT, VTILE / 4u>(a, work, acc, top, sum, reinterpret_cast<float *>(lds));
+    float *const rows = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (uint32_t d = 0; d < DIMS; ++d) *reinterpret_cast<gd_f32x4 *>(rows + wave * (VTILE / 4u) + col * (DT + 4u) + 16u * d + 4u * h) = acc[d];
+    af_finish<TYPE, DT, VTILE / 4u, WAVES>(a, work, top, sum, rows);
 }

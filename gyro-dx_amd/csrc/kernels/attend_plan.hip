@@ -55,7 +55,7 @@ GD_PIPELINE_NAMED(attend_plan, 1024) {
     each([&](uint32_t, uint32_t, uint32_t keys, uint32_t) { sum += keys; });
     if (sum) atomicAdd((unsigned long long *)&total, (unsigned long long)sum);
     __syncthreads();
-    const uint32_t share = (uint32_t)max((uint64_t)a.c[45], (total * KVH + 511u) / 512u);
+    const uint32_t share = (uint32_t)max((uint64_t)a.c[58], (total * KVH + 511u) / 512u);
     auto parts_of = [&](uint32_t keys) { return max(1u, (uint32_t)(((uint64_t)keys + share - 1u) / share)); };
     auto class_of = [&](uint32_t keys, uint32_t parts) {
         return AP_CLASSES - 1u - min(AP_CLASSES - 1u, (uint32_t)((uint64_t)(keys / parts) * AP_CLASSES / ((uint64_t)share + 1u)));

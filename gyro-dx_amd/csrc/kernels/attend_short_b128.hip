@@ -1,0 +1,3 @@
+// Attention of few rows over short contexts, bf16 heads of up to 128 values (attend_few.h).
+#include "attend_few.h"
+GD_PIPELINE_NAMED(attend_short_b128, 512) { attend_few_body<ROW_BF16, 128, 8>(a); }

@@ -83,8 +83,10 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
     // Where a lane's operands begin: its key of 32 and 8 of its channels, its 4 of 16 keys and 4 of its 32 channels.
     const uint32_t from_k = at_lds(lds_k) + col * KROW + 16u * h;
     const uint32_t from_v = at_lds(lds_v) + (4u * h + ((lane & 15u) >> 2)) * VROW + 32u * (lane >> 4 & 1u) + 8u * (lane & 3u);
-    auto locate = [&](uint32_t t) { return at_key(a, seq, head, (int32_t)(KEYS * t + lane % KEYS), t < unit_to ? end : 0); };
-    auto load = [&](int64_t where) {
+    auto key_of = [&](uint32_t t) { return (int32_t)(KEYS * t + lane % KEYS); };
+    auto page = [&](uint32_t t) { return at_page(a, seq, key_of(t), t < unit_to ? end : 0); };
+    auto load = [&](uint32_t t, uint32_t page) {
+        const int64_t where = at_key(a, page, head, key_of(t), t < unit_to ? end : 0);
         valid_next = __ballot(where >= 0);  // (32 keys: twice)
         const uint64_t offset = where < 0 ? 0ull : (uint64_t)where;
 #pragma unroll
@@ -109,13 +111,13 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
             // taken out here and come back one by one below.
 #pragma unroll
             for (uint32_t i = 0; i < PASSES; ++i) {
-                uint32_t largest = 0;
+                float finite = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) largest = at_larger(largest, v_next[i][e]);
-                const uint64_t odd = __ballot(at_not_finite<TYPE>(largest));
+                for (int e = 0; e < 4; ++e) finite = at_finite<TYPE>(v_next[i][e], finite);
+                const uint64_t odd = __ballot(!(finite == 0.f));
                 if (odd) {
                     const uint32_t key = PASS * i + mine;
-                    if (at_not_finite<TYPE>(largest)) atomicOr(&lds_bad[marks][key >> 5], 1u << (key & 31u));
+                    if (!(finite == 0.f)) atomicOr(&lds_bad[marks][key >> 5], 1u << (key & 31u));
                     if (odd >> (lane - lane % CHUNKS) & ((1ull << CHUNKS) - 1u)) v_next[i] = empty;
                 }
             }
@@ -129,17 +131,17 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
 
     if (tid < 6u) lds_bad[tid >> 1][tid & 1u] = 0u;
     __syncthreads();
-    int64_t next = locate(unit_from);
-    load(next);
-    next = locate(unit_from + 1u);
+    uint32_t soon = page(unit_from + 1u);
+    load(unit_from, page(unit_from));
     if (unit_from < unit_to) store(unit_from, 0u, 0u);
     valid = valid_next;
     __syncthreads();
     uint32_t marks = 0;
     for (uint32_t t = unit_from; t < unit_to; ++t) {
         const uint32_t buffer = (t - unit_from) & 1u, marks_next = marks == 2u ? 0u : marks + 1u;
-        if (t + 1u < unit_to) load(next);
-        next = locate(t + 2u);
+        const uint32_t later = page(t + 2u);
+        load(t + 1u, soon);  // behind the last as well: at_page says why
+        soon = later;
         const uint32_t kl = from_k + buffer * (KEYS * KROW), vl = from_v + buffer * (KEYS * VROW);
         if (!idle) {
             at_f32x16 s[BLOCKS];
@@ -207,7 +209,7 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
                 const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(bad));
                 bad &= bad - 1u;
                 const int32_t j = (int32_t)(KEYS * t + key);
-                const int64_t where = at_key(a, seq, head, j, end);
+                const int64_t where = at_key(a, at_page(a, seq, j, end), head, j, end);
                 const bool seen = j <= last && j >= first;
                 // The key's weight is in the lanes of half key / 4 % 2, one of a pair in a word.
                 uint32_t pair = 0;

@@ -196,13 +196,14 @@ class AttentionOps {
 
     // ---- attention ----
 
-    // Few rows: groups that a launch's keys are split for at most. Many: parts of 128 rows that the workspace holds (attend_plan
-    // makes them of tiles with more keys than a 512th of all, twice 512 at most), and units.
-    static constexpr uint32_t kGroups = 1024, kParts = 256, kSlots = 1024, kUnits = 1u << 18, kPlanBytes = 256 + 4 * 1024, kUnitBytes = 32;
+    // Few rows: groups that their keys are split for, the workspace holds twice as many parts (an entry of more than a fair part
+    // is split into less than twice as many), and entries whose shares every group works out. Many: parts of 128 rows that the
+    // workspace holds (attend_plan splits tiles of more than a 512th of all keys: twice 512 at most), and units.
+    static constexpr uint32_t kGroups = 1024, kEntries = 1024, kSlots = 1024, kUnits = 1u << 18, kPlanBytes = 256 + 4 * 1024, kUnitBytes = 32;
     static constexpr uint32_t kFewRows = 16, kTileRows = 128;
     static uint64_t part_bytes(uint32_t rows, uint32_t D) { return (uint64_t)rows * 4 * (D + 2); }
     // The workspace: the few rows' parts, the plan with its units, the units' parts.
-    static uint64_t plan_at(uint32_t D) { return kGroups * part_bytes(kFewRows, D); }
+    static uint64_t plan_at(uint32_t D) { return 2 * kGroups * part_bytes(kFewRows, D); }
     static uint64_t slots_at(uint32_t D) { return plan_at(D) + kPlanBytes + (uint64_t)kUnits * kUnitBytes; }
     static uint64_t workspace(uint32_t heads, uint32_t kv_heads, uint32_t D) {
         if (!heads || !kv_heads || heads % kv_heads || !D || D > 256) return 0;
@@ -226,7 +227,7 @@ class AttentionOps {
         require(d.lengths && (uintptr_t)d.lengths % 4 == 0 && (uintptr_t)d.starts % 4 == 0, "gm_attention: lengths and starts");
         require(d.table && (uintptr_t)d.table % 4 == 0 && d.table_width && d.table_stride <= uint64_t(1) << 40, "gm_attention: table");
         const uint64_t capacity = (uint64_t)d.table_width * d.cache.page_size;
-        require(capacity < 1u << 31, "gm_attention: table_width * page_size is below 2^31");
+        require(capacity < 1u << 29, "gm_attention: table_width * page_size is below 2^29");  // 2^25 tiles of 16 keys, 64 of them in 32 bits
         require(d.causal || !d.window, "gm_attention: a window without the causal mask");
         require(d.scale > 0 && std::isfinite(d.scale), "gm_attention: scale");
         const bool wide = d.cache.type == GM_F32;
@@ -260,27 +261,32 @@ class AttentionOps {
         c.set(39, std::min(d.window, 1u << 30));
         c.set(40, d.scale * 1.44269504088896341f);
         c.set(43, d.cache.type);
-        c.set(45, kLeast);
         c.set(46, many ? kFewRows + 1 : 0u);
         for (uint32_t shift = 0; shift < 31; ++shift)
             if (d.cache.page_size == 1u << shift) c.set(52, shift + 1);
         const int size = D <= 64 ? 0 : D <= 128 ? 1 : 2, type = d.cache.type;
-        uint64_t need = 0, join = 0;
-        uint32_t parts = 1;
-        uint64_t items = 0;
+        uint64_t need = 0, join = 0, groups = 0;
+        bool short_keys = false;
         if (few) {
             const uint32_t keys = wide ? 16 : 32, tiles = wide ? (uint32_t)((rows + kFewRows - 1) / kFewRows) : 1;
-            items = (uint64_t)d.sequences * G * tiles;
-            require(items < 1u << 31, "gm_attention: too many sequences");
-            // Parts of the keys, while the groups are fewer than those the GPU holds.
-            const uint64_t key_tiles = (capacity + keys - 1) / keys;
-            parts = (uint32_t)std::max<uint64_t>(1, std::min({(uint64_t)kParts, kGroups / items, (key_tiles + kLeast - 1) / kLeast}));
-            c.set(41, parts);
+            const uint64_t entries = (uint64_t)d.sequences * tiles;
+            require(entries * G < 1u << 31, "gm_attention: too many sequences");
+            groups = entries * G;
             c.set(42, tiles);
             c.set(44, keys);
-            if (parts > 1) {
-                need = items * parts * part_bytes(kFewRows, D);
-                join = (items * kFewRows + 3) / 4;
+            // Split where there may be keys for it, and entries enough to fill the GPU are not there anyway. Keys that one
+            // group takes may be taken by one of eight waves.
+            const uint32_t resident = (wide ? 256 : kResident[size]) * (d.sequences > 1 ? kPerGroup : 1);
+            short_keys = capacity <= kAlone;
+            if (entries <= kEntries && entries * G < 2 * resident && !short_keys) {
+                groups += resident;
+                c.set(41, resident);
+                c.set(45, kLeast / keys);
+                c.set(57, kAlone / keys);
+                need = plan_at(D);
+                const uint32_t most = (uint32_t)std::min<uint64_t>(kFewRows, rows);
+                c.set(56, most);
+                join = std::min<uint64_t>(entries, resident / G) * G * most;
             }
         }
         c.set(47, (uint32_t)join);
@@ -290,9 +296,10 @@ class AttentionOps {
             units = (uint64_t)n * group / kTileRows + std::min<uint64_t>(d.sequences, (uint64_t)n * group / (kFewRows + 1)) + 512 / G + 1;
             require(units <= kUnits && units * G < 1u << 31, "gm_attention: n * heads / kv_heads / 128 + sequences is at most 2^18 - 1024");
             need = workspace(H, G, D);
-            join += 512;
+            join += 2048;
             c.set64(48, (uint64_t)(uintptr_t)d.workspace + plan_at(D));
             c.set64(50, (uint64_t)(uintptr_t)d.workspace + slots_at(D));
+            c.set(58, kTileLeast);
             c.set(53, (uint32_t)units);
             c.set(54, kSlots / G);
             c.set(55, D > 128 ? 32u : 64u);
@@ -305,13 +312,18 @@ class AttentionOps {
                                                     {"attend_few_h64", "attend_few_h128", "attend_few_h256"}};
         static const char *const tile_names[3][3] = {{}, {"attend_tile_b64", "attend_tile_b128", "attend_tile_b256"},
                                                      {"attend_tile_h64", "attend_tile_h128", "attend_tile_h256"}};
-        if (few) l.add(few_names[type][size], items * parts);
+        static const char *const short_names[3][3] = {{"attend_f32_64", "attend_f32_128", "attend_f32_256"},
+                                                      {"attend_short_b64", "attend_short_b128", "attend_few_b256"},
+                                                      {"attend_short_h64", "attend_short_h128", "attend_few_h256"}};
+        if (few) l.add((short_keys ? short_names : few_names)[type][size], groups);
         if (many) l.add(tile_names[type][size], units * G);
         if (join) l.add("attend_join", join);
         return l;
     }
-    // Tiles of keys that make a part worth its join.
-    static constexpr uint32_t kLeast = 4;
+    // Few rows' keys: groups that the GPU holds, by the heads' size; parts for each of them where sequences differ; keys that
+    // make a part; and those that one group takes without a join.
+    static constexpr uint32_t kResident[3] = {512, 512, 256}, kPerGroup = 2, kLeast = 256, kAlone = 1024;
+    static constexpr uint32_t kTileLeast = 4;  // tiles that make a part of many rows' keys
 };
 
 }  // namespace gyro

@@ -69,7 +69,7 @@ GM_API int gm_cache_append(gm_engine *e, const gm_cache_append_desc *desc, uint3
  * with starts NULL, `longest` tokens from b * longest on (then n = sequences * longest); `longest` is at least every
  * sequence's count of tokens (of more, the first `longest` are certain to be computed, the rest may be left). Its keys are
  * the first lengths[b] places (int32, the new tokens' own among them) of the pages table[b * table_stride + i],
- * i < table_width (int32; cut to table_width * page_size, which is below 2^31).
+ * i < table_width (int32; cut to table_width * page_size, which is below 2^29).
  * Token i of q tokens stands at p = lengths[b] - q + i and sees the keys j <= p with `causal`, else all of its sequence's;
  * with a window w > 0 (and causal) only j > p - w. A key on a page outside the cache is seen by no token.
  *   out = sum_j softmax_j(scale q . k_j) v_j   (scale > 0)

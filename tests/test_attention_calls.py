@@ -281,12 +281,12 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
     every call."""
     most = engine.lib().gm_attention_workspace(heads, kv, dim)
     c, group = cache(type=type, kv_heads=kv, head_dim=dim), heads // kv
-    few_bytes, part = 1024 * 16 * 4 * (dim + 2), 128 * 4 * (dim + 2)
+    few_bytes, part = 2048 * 16 * 4 * (dim + 2), 128 * 4 * (dim + 2)
     assert most == few_bytes + 4352 + (32 << 18) + 1024 * part
     for sequences, longest in ((1, 1), (1, 5), (1, 4096), (3, 1), (64, 1), (64, 7), (300, 100), (5000, 1), (2, 100000)):
         if sequences * longest * group > 128 * 250000 or sequences * longest * heads > 1 << 30:
             continue
-        for width in (1, 3, 60, 1000, 60000000):
+        for width in (1, 3, 60, 1000, 30000000):
             d = attention(cache=c, q=rows(type), out=rows(type, data=3 * A), heads=heads, sequences=sequences, longest=longest, table_width=width,
                           workspace_bytes=most, starts=A if ragged else None)
             rc, names, out = call(shim.plan_attention, d, sequences * longest)
@@ -296,22 +296,25 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
             assert len(names) == out[0] and all(1 <= v <= 65535 for v in out[1:1 + 2 * out[0]])
             many = type and longest * group > 16
             size = 64 if dim <= 64 else 128 if dim <= 128 else 256
-            few = "attend_f32_%d" % size if not type else "attend_few_%s%d" % ("?bh"[type], size)
+            build = "f32_" if not type else ("short_" if width * 16 <= 1024 and size < 256 else "few_") + "?bh"[type]
+            few = f"attend_{build}{size}"
             tile = "attend_tile_%s%d" % ("?bh"[type], size)
             assert names[:1] == ["attend_plan"] if many else "attend_plan" not in names
             assert (few in names) == (not many or ragged) and (tile in names) == bool(many)
             assert w[46] == (17 if many else 0) and w[52] == 5  # pages of 16
             join = 0
             if few in names:
-                parts, tiles, keys, least = w[41], w[42], w[44], w[45]
+                split, tiles, keys, least = w[41], w[42], w[44], w[45]
                 assert keys == (32 if type else 16)
                 assert tiles == 1 if type else tiles * 16 >= longest * group > (tiles - 1) * 16
-                assert 1 <= parts <= 256 and (parts == 1 or (parts - 1) * least * keys < width * 16)
-                assert grids[few] >= sequences * kv * tiles * parts
-                if parts > 1:
-                    assert sequences * kv * tiles * parts * 16 * 4 * (dim + 2) <= few_bytes
+                # A group for every entry and head, and for what splits add: of each entry less than its share of `split`.
+                assert split in (0, 256, 512, 1024) and grids[few] >= sequences * tiles * kv + split
+                assert not split or (sequences * tiles <= 1024 and width * 16 > w[57] * keys and least >= 1)
+                if split:
+                    most_rows = min(16, longest * group)
+                    assert w[56] == most_rows
                     join = w[47]
-                    assert 4 * join >= sequences * kv * tiles * 16
+                    assert join >= min(sequences * tiles, split // kv) * kv * most_rows
             assert w[47] == join
             if many:
                 units = w[53]
@@ -320,7 +323,7 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
                 assert units > -(-sequences * longest * group // 128) + 512 // kv
                 assert w[48] | w[49] << 32 == A + few_bytes and w[50] | w[51] << 32 == A + few_bytes + 4352 + (32 << 18)
                 assert w[54] * kv * part <= 1024 * part and w[55] == (32 if dim > 128 else 64)
-                assert grids["attend_join"] >= join + 512
+                assert grids["attend_join"] >= join + 2048
             else:
                 assert ("attend_join" in names) == bool(join) and (not join or grids["attend_join"] >= join)
 

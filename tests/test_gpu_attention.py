@@ -365,6 +365,15 @@ def test_attention_split_tiles(eng, type, dim):
         assert torch.equal(first, b.out)
 
 
+def test_attention_most_parts(eng):
+    """One cache head's keys in as many parts as there are: of 16 rows, and of 128."""
+    for type, counts, length in (("f16", [2], 140001), ("bf16", [17], 200003)):
+        print(f"most parts {type} {counts} {length}", flush=True)
+        b = Batch(eng, type, 1, 1, 16, 256, counts, [length], seed=18)
+        b.run()
+        b.check()
+
+
 def test_attention_many_sequences(eng):
     """More sequences than the plan looks at in one go, of few rows, many, none."""
     rng = np.random.default_rng(61)
