@@ -15,6 +15,7 @@
 // the few rows 48 units' list 50 units' parts 52 page size's shift plus one (0: no power of two) 53 units that the list holds
 // 54 parts that the workspace holds, per head 55 keys of a tile of units 56 rows that attend_join takes of a few rows' tile
 // 57 tiles of keys up to which few rows' are not split 58 tiles that make a unit
+// 59 whether 32 bits span the cache
 #pragma once
 #include "rows.h"
 
@@ -99,6 +100,13 @@ __device__ __forceinline__ int64_t at_key(const GdArgs &a, uint32_t page, uint32
     const uint32_t place = (uint32_t)j - at_slot_of(a, (uint32_t)j) * a.c[36];
     const int64_t at = page * gd_addr(a, 12) + place * gd_addr(a, 16) + head * gd_addr(a, 14);
     return (j < end) & (page < a.c[35]) ? at : -1;
+}
+
+// As at_key, of a cache that 32 bits span, without the head (its offset is the wave's).
+__device__ __forceinline__ uint32_t at_key_small(const GdArgs &a, uint32_t page, int32_t j, int32_t end, bool &there) {
+    const uint32_t place = (uint32_t)j - at_slot_of(a, (uint32_t)j) * a.c[36];
+    there = (j < end) & (page < a.c[35]);
+    return there ? page * a.c[12] + place * a.c[16] : 0u;
 }
 
 // The larger of a value and lane ^ 32's.

@@ -15,6 +15,14 @@ __device__ __forceinline__ uint32_t at_pair(float lo, float hi) {
     if constexpr (TYPE == ROW_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f32x2{lo, hi}), at_bf16x2));
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f32x2{lo, hi}), at_f16x2));
 }
+// c and both values of a word.
+template <uint32_t TYPE>
+__device__ __forceinline__ float at_add_pair(uint32_t w, float c) {
+    if constexpr (TYPE == ROW_BF16)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(at_bf16x2, w), at_bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(at_f16x2, w), at_f16x2{(_Float16)1.f, (_Float16)1.f}, c, false);
+}
 // c while a word's values are finite, from then on NaN (0 times the others is).
 template <uint32_t TYPE>
 __device__ __forceinline__ float at_finite(uint32_t w, float c) {

@@ -1,13 +1,19 @@
-// Attention of many rows (attend.h), 16-bit types: a group of four waves takes 128 rows, 32 a wave, and a run of tiles of 64 or 32 keys
-// (attend_plan says which), keys and values of a tile in LDS, the next one on its way in registers.
+// Attention of many rows (attend.h), 16-bit types: a group of four waves takes 128 rows, 32 a wave, and a run of tiles of 64 or 32
+// keys (attend_plan says which), which go from memory straight to LDS, two buffers of keys and of values in turn.
 //
 // Scores are K Q^T by v_mfma_f32_32x32x16: a lane holds half the keys of one row, the other half is lane ^ 32's, so the
 // running maximum needs one exchange per tile, the sum none until the end, and the weights are the second product's operand
 // as they lie: O^T += V^T P^T, contracted over keys in the order in which lanes hold them; values come out of LDS transposed
-// (ds_read_b64_tr_b16). The maximum that weights are relative to follows the running one only when that has grown by
-// more than 2^8, so that the sums are rarely rescaled; weights are at most 2^8 then, and as precise.
+// (ds_read_b64_tr_b16). The next tile's scores are multiplied while this one's weights are worked out, which are independent: the
+// matrix unit and the vector unit work side by side within a wave. The maximum that weights are relative to follows the running
+// one only when that has grown by more than 2^8, so that the sums are rarely rescaled; weights are at most 2^8 then, and as
+// precise.
+//
+// LDS is filled 1 KB an instruction in the order of lanes, so rows cannot be padded; instead their 16-byte pieces are swapped
+// by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v).
 #pragma once
 #include "attend16.h"
+#include <type_traits>
 
 template <uint32_t TYPE>
 __device__ __forceinline__ at_f32x16 at_mfma(gd_u32x4 a, gd_u32x4 b, at_f32x16 c) {
@@ -17,28 +23,31 @@ __device__ __forceinline__ at_f32x16 at_mfma(gd_u32x4 a, gd_u32x4 b, at_f32x16 c
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b), c, 0, 0, 0);
 }
 
-// Asks the scheduler for FIRST reads of LDS, then STEPS times MFMAS products and READS reads: operands come just ahead of their
-// products, and few registers hold them.
-template <int FIRST, int READS, int MFMAS, int STEPS>
-__device__ __forceinline__ void at_feed() {
-    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+// 16 bytes at each lane's address to LDS, from `lds` (of the wave) on in the order of lanes. Counted by vmcnt; at_landed waits.
+__device__ __forceinline__ void at_to_lds(uint32_t lds, uint64_t from) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory", "m0");
 }
+// The same at a 32-bit offset from a uniform address.
+__device__ __forceinline__ void at_to_lds(uint32_t lds, uint64_t base, uint32_t offset) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base), hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
+    const uint64_t uniform = (uint64_t)hi << 32 | (uint64_t)lo;
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(uniform)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <uint32_t TYPE, uint32_t DT, uint32_t KEYS>
-__device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
-    // Rows in LDS: keys' 16 bytes of 8 neighbouring keys, and values' 64 of 4, in all banks.
-    constexpr uint32_t KROW = DT * 2u + 16u, VROW = DT * 2u + 64u, STEPS = DT / 16u, DIMS = DT / 32u, CHUNKS = DT / 8u;
-    constexpr uint32_t PASS = 256u / CHUNKS, PASSES = KEYS / PASS, BLOCKS = KEYS / 32u;  // keys that 256 threads load at once
-    __shared__ __align__(16) char lds_k[2][KEYS * KROW];
-    __shared__ __align__(16) char lds_v[2][KEYS * VROW];
-    // Keys of a tile whose values are not all finite: of the one read, the one stored, and the one before, being cleared.
-    __shared__ uint32_t lds_bad[3][2];
+// What a 16-byte piece's number in its row is changed by (exclusive or). Keys: 8 neighbouring rows are read at once, one piece of
+// each. Values: 4 neighbouring rows, 4 pieces of each.
+template <uint32_t CHUNKS>
+__device__ __forceinline__ uint32_t at_tile_k(uint32_t row) { return row & (CHUNKS < 16u ? CHUNKS - 1u : 15u); }
+template <uint32_t CHUNKS>
+__device__ __forceinline__ uint32_t at_tile_v(uint32_t row) { return (CHUNKS < 16u ? row >> 1 & 1u : row & 3u) << 2; }
+
+template <uint32_t TYPE, uint32_t DT, uint32_t KEYS, bool SMALL>
+__device__ __forceinline__ void attend_tile_of(const GdArgs &a, char *lds_k, char *lds_v, uint32_t (*lds_bad)[2]) {
+    constexpr uint32_t ROW = DT * 2u, STEPS = DT / 16u, DIMS = DT / 32u, CHUNKS = DT / 8u, BLOCKS = KEYS / 32u;
+    constexpr uint32_t PER = 64u / CHUNKS, LOADS = KEYS / (4u * PER);  // keys of a wave's load, loads of a wave
+    using Place = std::conditional_t<SMALL, uint32_t, uint64_t>;  // of a key in the cache (in a head of it, if 32 bits span it)
     const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 31u, h = lane >> 5, D = a.c[30], group = a.c[29], KVH = a.c[31];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, index = id / KVH, head = id - index * KVH;
@@ -55,18 +64,19 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
 
     const uint32_t row = min(o.row0 + 32u * wave + col, o.rows - 1u), token = row / group;  // rows past the last are the last again
     const bool idle = o.row0 + 32u * wave >= o.rows;                                       // a wave with none but those
-    const uint64_t at = (uint64_t)(head * group + row - token * group) * D;
     const int32_t p = o.kl - (int32_t)o.ql + (int32_t)token, window = (int32_t)a.c[39];
     const int32_t last = a.c[38] ? p : o.kl - 1, first = window ? p - window + 1 : 0;
     gd_u32x4 q[STEPS];
+    {
+        const uint64_t at = (uint64_t)(o.token0 + token) * gd_addr(a, 2) + (uint64_t)(head * group + row - token * group) * D;
 #pragma unroll
-    for (uint32_t s = 0; s < STEPS; ++s) {
-        q[s] = empty;
-        if (16u * s + 8u * h < D)
-            q[s] = *gd_at<const gd_u32x4_any>(gd_addr(a, 0) + ((uint64_t)(o.token0 + token) * gd_addr(a, 2) + at) * 2u + 32u * s + 16u * h);
+        for (uint32_t s = 0; s < STEPS; ++s) {
+            q[s] = empty;
+            if (16u * s + 8u * h < D) q[s] = *gd_at<const gd_u32x4_any>(gd_addr(a, 0) + at * 2u + 32u * s + 16u * h);
+        }
     }
     const float scale = gd_bits_f32(a.c[40]);
-    const uint64_t K = gd_addr(a, 8), V = gd_addr(a, 10);
+    const uint64_t of_head = SMALL ? head * gd_addr(a, 14) : 0ull, K = gd_addr(a, 8) + of_head, V = gd_addr(a, 10) + of_head;
     at_f32x16 acc[DIMS];
 #pragma unroll
     for (uint32_t d = 0; d < DIMS; ++d)
@@ -74,88 +84,142 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
     float top = AT_LOWEST, sum = 0.f;
 
-    // Tile t's keys: a lane knows one's place in the cache, a thread loads 16 bytes of each of PASSES.
-    // (Where there is none, it loads the cache's first, and drops it when it stores.)
-    const uint32_t chunk = tid % CHUNKS, mine = tid / CHUNKS, in_head = 8u * chunk < D ? chunk : 0u;
-    gd_u32x4 k_next[PASSES], v_next[PASSES];
-    uint64_t valid_next = 0, valid = 0;
-    const uint32_t to_k = at_lds(lds_k) + mine * KROW + 16u * chunk, to_v = at_lds(lds_v) + mine * VROW + 16u * chunk;
-    // Where a lane's operands begin: its key of 32 and 8 of its channels, its 4 of 16 keys and 4 of its 32 channels.
-    const uint32_t from_k = at_lds(lds_k) + col * KROW + 16u * h;
-    const uint32_t from_v = at_lds(lds_v) + (4u * h + ((lane & 15u) >> 2)) * VROW + 32u * (lane >> 4 & 1u) + 8u * (lane & 3u);
+    // Load i of a wave brings keys 4 PER i + PER wave .. of a tile; a lane piece lane % CHUNKS of key lane / CHUNKS, which is the
+    // piece of the head that belongs there. (Of shorter heads the others stay zeros.)
+    const uint32_t of_key = PER * wave + lane / CHUNKS;  // + 4 PER i: at_tile_k and at_tile_v are the same for each i
+    const uint32_t piece_k = (lane % CHUNKS) ^ at_tile_k<CHUNKS>(of_key), piece_v = (lane % CHUNKS) ^ at_tile_v<CHUNKS>(of_key);
+    static_assert(4u * PER % 16u == 0u || CHUNKS > 16u, "a load's rows");
     auto key_of = [&](uint32_t t) { return (int32_t)(KEYS * t + lane % KEYS); };
     auto page = [&](uint32_t t) { return at_page(a, seq, key_of(t), t < unit_to ? end : 0); };
-    auto load = [&](uint32_t t, uint32_t page) {
-        const int64_t where = at_key(a, page, head, key_of(t), t < unit_to ? end : 0);
-        valid_next = __ballot(where >= 0);  // (32 keys: twice)
-        const uint64_t offset = where < 0 ? 0ull : (uint64_t)where;
+    // Where a tile's keys are in the cache (those that are not: at its start), of each load; which there are.
+    auto locate = [&](uint32_t t, uint32_t page, Place (&at)[LOADS]) {
+        bool there;
+        if constexpr (SMALL) {
+            const uint32_t offset = at_key_small(a, page, key_of(t), t < unit_to ? end : 0, there);
 #pragma unroll
-        for (uint32_t i = 0; i < PASSES; ++i) {
-            const uint32_t key = PASS * i + mine;
-            const uint32_t lo = __shfl((uint32_t)offset, key, 64), hi = __shfl((uint32_t)(offset >> 32), key, 64);
-            const uint64_t from = ((uint64_t)lo | (uint64_t)hi << 32) + 16u * in_head;
-            k_next[i] = *gd_at<const gd_u32x4_any>(K + from);
-            v_next[i] = *gd_at<const gd_u32x4_any>(V + from);
+            for (uint32_t i = 0; i < LOADS; ++i) at[i] = __shfl(offset, 4u * PER * i + of_key, 64);
+        } else {
+            const int64_t where = at_key(a, page, head, key_of(t), t < unit_to ? end : 0);
+            there = where >= 0;
+            const uint64_t offset = there ? (uint64_t)where : 0ull;
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t key = 4u * PER * i + of_key;
+                at[i] = (uint64_t)__shfl((uint32_t)offset, key, 64) | (uint64_t)__shfl((uint32_t)(offset >> 32), key, 64) << 32;
+            }
         }
+        return (uint64_t)__ballot(there);  // (32 keys: twice)
+    };
+    auto fetch = [&](uint32_t lds, uint32_t t, uint64_t cache, Place at, uint32_t i, uint32_t piece) {
+        lds += (t & 1u) * (KEYS * ROW) + (4u * PER * i + PER * wave) * ROW;
+        if (D != DT && 8u * piece >= D) return;
+        if constexpr (SMALL) at_to_lds(lds, cache, at + 16u * piece);
+        else at_to_lds(lds, cache + at + 16u * piece);
+    };
+    // Load i of tile t's keys, or values, in buffer t % 2. (Of 256 values the rows of a load number are not those of the first.)
+    auto fetch_k = [&](uint32_t t, Place at, uint32_t i) {
+        fetch(at_lds(lds_k), t, K, at, i, CHUNKS > 16u ? (lane % CHUNKS) ^ at_tile_k<CHUNKS>(4u * PER * i + of_key) : piece_k);
+    };
+    auto fetch_v = [&](uint32_t t, Place at, uint32_t i) { fetch(at_lds(lds_v), t, V, at, i, piece_v); };
+
+    // Where a lane's operands begin: its key of 32 and 8 of its channels; its 4 of 16 keys and 4 of 32 channels.
+    const uint32_t from_k = at_lds(lds_k) + col * ROW + ((h ^ at_tile_k<CHUNKS>(col)) * 16u);
+    const uint32_t of_v = (lane & 15u) >> 2, from_v = at_lds(lds_v) + (4u * h + of_v) * ROW + 32u * (lane >> 4 & 1u) + 8u * (lane & 3u);
+    auto keys = [&](uint32_t base, uint32_t b, uint32_t e) { return at_lds_load((base ^ (32u * e)) + 32u * b * ROW); };
+    auto values = [&](uint32_t t, uint32_t j, uint32_t d) {
+        const uint32_t at = from_v + (t & 1u) * (KEYS * ROW) + 16u * j * ROW + 16u * (4u * d ^ at_tile_v<CHUNKS>(of_v));
+        const gd_u32x2 lower = at_transposed(at), upper = at_transposed(at + 8u * ROW);
+        return gd_u32x4{lower[0], lower[1], upper[0], upper[1]};
     };
     // Tiles that not every row sees whole.
     auto mixed = [&](uint32_t t) { return (int32_t)(KEYS * t) < all_first || (int32_t)(KEYS * t + KEYS) > all_end; };
-    auto store = [&](uint32_t t, uint32_t buffer, uint32_t marks) {
-        if (valid_next != ~0ull || D != DT) {
-#pragma unroll
-            for (uint32_t i = 0; i < PASSES; ++i)
-                if ((8u * chunk >= D) | !(valid_next >> (PASS * i + mine) & 1u)) k_next[i] = v_next[i] = empty;
+
+    if (D != DT)
+        for (uint32_t i = tid; i < 2u * KEYS * CHUNKS; i += 256u) {
+            at_lds_store(at_lds(lds_k) + 16u * i, empty);
+            at_lds_store(at_lds(lds_v) + 16u * i, empty);
         }
-        if (mixed(t)) {
-            // A value that is not finite must reach no row that does not see its key (0 times it is NaN): such keys are
-            // taken out here and come back one by one below.
+    if (tid < 4u) lds_bad[tid >> 1][tid & 1u] = 0u;
+    __syncthreads();
+    Place place[LOADS], place_next[LOADS];  // of the next tile's values, of the keys of the one after it
+    uint64_t valid = locate(unit_from, page(unit_from), place);
 #pragma unroll
-            for (uint32_t i = 0; i < PASSES; ++i) {
-                float finite = 0.f;
+    for (uint32_t i = 0; i < LOADS; ++i) {
+        fetch_k(unit_from, place[i], i);
+        fetch_v(unit_from, place[i], i);
+    }
+    uint64_t valid_next = locate(unit_from + 1u, page(unit_from + 1u), place);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) finite = at_finite<TYPE>(v_next[i][e], finite);
-                const uint64_t odd = __ballot(!(finite == 0.f));
-                if (odd) {
-                    const uint32_t key = PASS * i + mine;
-                    if (!(finite == 0.f)) atomicOr(&lds_bad[marks][key >> 5], 1u << (key & 31u));
-                    if (odd >> (lane - lane % CHUNKS) & ((1ull << CHUNKS) - 1u)) v_next[i] = empty;
-                }
-            }
-        }
+    for (uint32_t i = 0; i < LOADS; ++i) fetch_k(unit_from + 1u, place[i], i);
+    uint32_t soon = page(unit_from + 2u);
+    asm volatile("" : "+v"(soon));
+    at_f32x16 s[BLOCKS];
+    // A tile's scores, a product a step: its operand is read AHEAD steps before, `beside` is work to run beside it. The steps stay
+    // in this order (the scheduler would put one kind of work after the other).
+    constexpr uint32_t PRODUCTS = STEPS * BLOCKS, AHEAD = 3;
+    gd_u32x4 operand[AHEAD];
+    uint32_t base_k = 0;
+    auto scores_begin = [&](uint32_t t) {
+        base_k = from_k + (t & 1u) * (KEYS * ROW);
+        asm volatile("" : "+v"(base_k));  // (what follows from it is not to be held through the loop)
 #pragma unroll
-        for (uint32_t i = 0; i < PASSES; ++i) {
-            at_lds_store(to_k + buffer * (KEYS * KROW) + PASS * i * KROW, k_next[i]);
-            at_lds_store(to_v + buffer * (KEYS * VROW) + PASS * i * VROW, v_next[i]);
+        for (uint32_t i = 0; i < AHEAD; ++i) operand[i] = keys(base_k, i % BLOCKS, i / BLOCKS);
+    };
+    auto scores = [&](at_f32x16 (&s)[BLOCKS], auto beside) {
+#pragma unroll
+        for (uint32_t b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < PRODUCTS; ++i) {
+            s[i % BLOCKS] = at_mfma<TYPE>(operand[i % AHEAD], q[i / BLOCKS], s[i % BLOCKS]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + AHEAD < PRODUCTS) operand[i % AHEAD] = keys(base_k, (i + AHEAD) % BLOCKS, (i + AHEAD) / BLOCKS);
+            beside(i);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
+    at_landed();
+    __syncthreads();
+    if (!idle) {
+        scores_begin(unit_from);
+        scores(s, [](uint32_t) {});
+    }
+    __syncthreads();  // its buffer is filled again
 
-    if (tid < 6u) lds_bad[tid >> 1][tid & 1u] = 0u;
-    __syncthreads();
-    uint32_t soon = page(unit_from + 1u);
-    load(unit_from, page(unit_from));
-    if (unit_from < unit_to) store(unit_from, 0u, 0u);
-    valid = valid_next;
-    __syncthreads();
-    uint32_t marks = 0;
-    for (uint32_t t = unit_from; t < unit_to; ++t) {
-        const uint32_t buffer = (t - unit_from) & 1u, marks_next = marks == 2u ? 0u : marks + 1u;
-        const uint32_t later = page(t + 2u);
-        load(t + 1u, soon);  // behind the last as well: at_page says why
-        soon = later;
-        const uint32_t kl = from_k + buffer * (KEYS * KROW), vl = from_v + buffer * (KEYS * VROW);
+    auto tile = [&](uint32_t t, at_f32x16 (&s)[BLOCKS], at_f32x16 (&s_next)[BLOCKS]) {
+        const uint64_t valid_later = locate(t + 2u, soon, place_next);
+        const uint32_t later = page(t + 3u);
+        // To be on its way during this tile: the next one's values, the keys of the one after it (behind the last tile, the
+        // cache's first). Loads one behind another wait for the address unit: 8 of them took 1300 cycles of a tile's 4200.
+        auto fetch_next = [&](uint32_t i) {
+            if (i < LOADS) fetch_v(t + 1u, place[i], i);
+            else if (i < 2u * LOADS) fetch_k(t + 2u, place_next[i - LOADS], i - LOADS);
+        };
+        const bool partly = valid != ~0ull || mixed(t);
+        if (partly) {
+            // Values of keys that are not there become zeros. One that is not finite must reach no row that does not see its
+            // key (0 times it is NaN): such keys are taken out here and come back one by one below. (The empty asm keeps the
+            // addresses out of the loop's registers.)
+            uint32_t key0 = of_key;
+            asm volatile("" : "+v"(key0));
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t key = 4u * PER * i + key0, at = at_lds(lds_v) + (t & 1u) * (KEYS * ROW) + key * ROW + 16u * (lane % CHUNKS);
+                const gd_u32x4 x = at_lds_load(at);
+                float finite = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) finite = at_finite<TYPE>(x[e], finite);
+                const bool there = valid >> key & 1u, odd = there & !(finite == 0.f);
+                const uint64_t lanes = __ballot(odd);
+                if (odd) atomicOr(&lds_bad[t & 1u][key >> 5], 1u << (key & 31u));
+                if (!there | ((lanes >> (lane - lane % CHUNKS) & ((1ull << CHUNKS) - 1u)) != 0ull)) at_lds_store(at, empty);
+            }
+            __syncthreads();
+        }
+        if (tid < 2u) lds_bad[(t + 1u) & 1u][tid] = 0u;  // read a tile ago, written after the next barrier
         if (!idle) {
-            at_f32x16 s[BLOCKS];
-#pragma unroll
-            for (uint32_t b = 0; b < BLOCKS; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-            for (uint32_t e = 0; e < STEPS; ++e)
-#pragma unroll
-                for (uint32_t b = 0; b < BLOCKS; ++b)
-                    s[b] = at_mfma<TYPE>(at_lds_load(kl + 32u * b * KROW + 32u * e), q[e], s[b]);
-            at_feed<2 * BLOCKS, BLOCKS, BLOCKS, STEPS>();
-            if (valid != ~0ull || mixed(t)) {
+            if (partly) {
                 const int32_t key0 = (int32_t)(KEYS * t + 4u * h), most_key = last - key0, least_key = first - key0;
 #pragma unroll
                 for (int b = 0; b < (int)BLOCKS; ++b) {
@@ -168,6 +232,7 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
                     }
                 }
             }
+            scores_begin(t + 1u);
             float most = s[0][0];
 #pragma unroll
             for (int i = 1; i < 16 * (int)BLOCKS; ++i) most = fmaxf(most, s[i >> 4][i & 15]);
@@ -182,62 +247,81 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
             }
-            gd_u32x4 w[BLOCKS][2];
-            float part = 0.f;
+            // The weights beside the next tile's scores (of the last one's: of what is in the buffer), with the first of V^T, whose
+            // 16 keys and 32 channels an operand has in the order of the weights, behind.
+            constexpr uint32_t PAIRS = 8u * BLOCKS;
+            constexpr uint32_t SUMS = 2u * BLOCKS * DIMS, RING = 4;
+            gd_u32x4 w[BLOCKS][2], x[RING];
+            __builtin_amdgcn_s_setprio(1);  // the wave that multiplies goes first: 6% (two share a unit)
+            scores(s_next, [&](uint32_t step) {
 #pragma unroll
-            for (uint32_t b = 0; b < BLOCKS; ++b)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = at_exp2(fmaf(s[b][2 * i], scale, -top)), y = at_exp2(fmaf(s[b][2 * i + 1], scale, -top));
-                    part += x + y;
-                    w[b][i >> 2][i & 3] = at_pair<TYPE>(x, y);
+                for (uint32_t i = step * PAIRS / PRODUCTS; i < (step + 1u) * PAIRS / PRODUCTS; ++i) {
+                    const uint32_t b = i >> 3, e = i & 7u;
+                    const float x = at_exp2(fmaf(s[b][2 * e], scale, -top)), y = at_exp2(fmaf(s[b][2 * e + 1], scale, -top));
+                    w[b][e >> 2][e & 3u] = at_pair<TYPE>(x, y);
+                    sum = at_add_pair<TYPE>(w[b][e >> 2][e & 3u], sum);  // the sum of what the values are weighed with
                 }
-            sum += part;
+                if (step % 2u == 0u) fetch_next(step / 2u);
+                if (step + RING >= PRODUCTS) x[step + RING - PRODUCTS] = values(t, (step + RING - PRODUCTS) / DIMS, (step + RING - PRODUCTS) % DIMS);
+            });
 #pragma unroll
-            for (uint32_t b = 0; b < BLOCKS; ++b)
+            for (uint32_t i = 0; i < SUMS; ++i) {
+                const uint32_t d = i % DIMS, j = i / DIMS, ahead = i + RING;
+                acc[d] = at_mfma<TYPE>(x[i % RING], w[j >> 1][j & 1u], acc[d]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (ahead < SUMS) x[i % RING] = values(t, ahead / DIMS, ahead % DIMS);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (partly) {
+                uint64_t bad = (uint64_t)lds_bad[t & 1u][0] | (uint64_t)lds_bad[t & 1u][1] << 32;
+                while (bad) {
+                    const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(bad));
+                    bad &= bad - 1u;
+                    const int32_t j = (int32_t)(KEYS * t + key);
+                    const int64_t where = at_key(a, at_page(a, seq, j, end), SMALL ? 0u : head, j, end);
+                    const bool seen = j <= last && j >= first;
+                    // The key's weight is in the lanes of half key / 4 % 2, one of a pair in a word.
+                    uint32_t pair = 0;
 #pragma unroll
-                for (uint32_t e = 0; e < 2; ++e)
+                    for (uint32_t i = 0; i < 8u * BLOCKS; ++i)
+                        if (((key >> 5) * 8u + (key >> 4 & 1u) * 4u + (key >> 3 & 1u) * 2u + (key >> 1 & 1u)) == i) pair = w[i >> 3][i >> 2 & 1][i & 3];
+                    pair = __shfl(key & 1u ? pair >> 16 : pair & 0xffffu, col + 32u * (key >> 2 & 1u), 64);
+                    const float weight = row_value16(pair, TYPE);
+                    uint32_t half = h;
+                    asm volatile("" : "+v"(half));
 #pragma unroll
                     for (uint32_t d = 0; d < DIMS; ++d) {
-                        const uint32_t from = vl + (32u * b + 16u * e) * VROW + 64u * d;
-                        const gd_u32x2 x = at_transposed(from), y = at_transposed(from + 8u * VROW);
-                        acc[d] = at_mfma<TYPE>(gd_u32x4{x[0], x[1], y[0], y[1]}, w[b][e], acc[d]);
+#pragma unroll
+                        for (uint32_t b = 0; b < 4; ++b) {
+                            const uint32_t dim = 32u * d + 8u * b + 4u * half;
+                            const gd_u32x2 x = *gd_at<const at_u32x2_any>(V + (uint64_t)where + 2u * (dim < D ? dim : 0u));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                acc[d][4 * b + i] += seen ? weight * row_value16(x[i >> 1] >> (16 * (i & 1)) & 0xffffu, TYPE) : 0.f;
+                        }
+                        if constexpr (DT > 128u) asm volatile("" : "+a"(acc[d]));  // not all of them beside the others at once
                     }
-            at_feed<8, 2, 1, 2 * BLOCKS * DIMS>();
-            uint64_t bad = (uint64_t)lds_bad[marks][0] | (uint64_t)lds_bad[marks][1] << 32;
-            while (bad) {
-                const uint32_t key = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)__builtin_ctzll(bad));
-                bad &= bad - 1u;
-                const int32_t j = (int32_t)(KEYS * t + key);
-                const int64_t where = at_key(a, at_page(a, seq, j, end), head, j, end);
-                const bool seen = j <= last && j >= first;
-                // The key's weight is in the lanes of half key / 4 % 2, one of a pair in a word.
-                uint32_t pair = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < 8u * BLOCKS; ++i)
-                    if (((key >> 5) * 8u + (key >> 4 & 1u) * 4u + (key >> 3 & 1u) * 2u + (key >> 1 & 1u)) == i) pair = w[i >> 3][i >> 2 & 1][i & 3];
-                pair = key & 1u ? pair >> 16 : pair & 0xffffu;
-                pair = __shfl(pair, col + 32u * (key >> 2 & 1u), 64);
-                const float weight = row_value16(pair, TYPE);
-#pragma unroll
-                for (uint32_t d = 0; d < DIMS; ++d)
-#pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b) {
-                        const uint32_t dim = 32u * d + 8u * b + 4u * h;
-                        const gd_u32x2 x = *gd_at<const at_u32x2_any>(V + (uint64_t)where + 2u * (dim < D ? dim : 0u));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[d][4 * b + i] += seen ? weight * row_value16(x[i >> 1] >> (16 * (i & 1)) & 0xffffu, TYPE) : 0.f;
-                    }
+                }
             }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 2u * LOADS; ++i) fetch_next(i);
         }
-        if (t + 1u < unit_to) {
-            store(t + 1u, buffer ^ 1u, marks_next);
-            valid = valid_next;
-        }
-        if (tid < 2u) lds_bad[marks_next == 2u ? 0u : marks_next + 1u][tid] = 0u;  // read a tile ago, written after the barrier
-        marks = marks_next;
+        valid = valid_next;
+        valid_next = valid_later;
+        soon = later;
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) place[i] = place_next[i];
+        at_landed();
+        asm volatile("" : "+v"(soon));  // (it has landed as well: the compiler, which counts its load alone, is not to wait for others)
         __syncthreads();
+    };
+    at_f32x16 s_next[BLOCKS];
+    for (uint32_t t = unit_from; t < unit_to;) {  // the scores by turns: copying them would be a tenth of the work
+        tile(t, s, s_next);
+        if (++t == unit_to) break;
+        tile(t++, s_next, s);
     }
 
     if (o.row0 + 32u * wave + col >= o.rows) return;
@@ -263,4 +347,13 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
             if (!alone) *gd_at<gd_f32x4>(part + 8u * AT_ROWS + ((uint64_t)r * D + dim) * 4u) = x;
             else at_store4<TYPE>(out, dim, x, by, sum == 0.f);
         }
+}
+
+template <uint32_t TYPE, uint32_t DT, uint32_t KEYS>
+__device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
+    __shared__ __align__(1024) char lds_k[2 * KEYS * DT * 2];
+    __shared__ __align__(1024) char lds_v[2 * KEYS * DT * 2];
+    __shared__ uint32_t lds_bad[2][2];  // keys of a tile whose values are not all finite, by turns
+    if (a.c[59]) attend_tile_of<TYPE, DT, KEYS, true>(a, lds_k, lds_v, lds_bad);
+    else attend_tile_of<TYPE, DT, KEYS, false>(a, lds_k, lds_v, lds_bad);
 }

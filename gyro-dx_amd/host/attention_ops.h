@@ -261,6 +261,10 @@ class AttentionOps {
         c.set(39, std::min(d.window, 1u << 30));
         c.set(40, d.scale * 1.44269504088896341f);
         c.set(43, d.cache.type);
+        // Whether 32 bits span the cache: keys' offsets take half the work then.
+        const auto reach = [](uint32_t count, uint64_t stride) { return count > 1 ? (unsigned __int128)(count - 1) * stride : 0; };
+        const auto span = reach(d.cache.pages, d.cache.page_stride) + reach(G, d.cache.head_stride) + reach(d.cache.page_size, d.cache.token_stride) + D;
+        c.set(59, span <= (uint64_t(1) << 32) / (wide ? 4 : 2) ? 1u : 0u);
         c.set(46, many ? kFewRows + 1 : 0u);
         for (uint32_t shift = 0; shift < 31; ++shift)
             if (d.cache.page_size == 1u << shift) c.set(52, shift + 1);

@@ -334,6 +334,19 @@ def test_page_shifts(shim):
         assert call(shim.plan_attention, attention(cache=c), 3)[2][9 + 52] == want
 
 
+@pytest.mark.parametrize("kw,small", [
+    (dict(), 1), (dict(pages=1 << 20, page_stride=2048), 1), (dict(pages=(1 << 20) + 1, page_stride=2048), 0),
+    (dict(type=0, pages=1 << 19, page_stride=2048), 1), (dict(type=0, pages=(1 << 19) + 1, page_stride=2048), 0),
+    (dict(pages=2, page_stride=1 << 40), 0), (dict(pages=1, page_stride=1 << 40), 1), (dict(pages=1 << 26, page_stride=1 << 40), 0),
+    (dict(head_stride=(1 << 31) - 100 * 2048), 1), (dict(head_stride=1 << 31), 0), (dict(pages=1, page_size=2, token_stride=1 << 31), 0)])
+def test_cache_spans(shim, kw, small):
+    """Caches whose last byte 32 bits reach are told from larger ones, whatever the strides."""
+    c = cache(**kw)
+    t = c.type
+    rc, why, out = call(shim.plan_attention, attention(cache=c, q=rows(t), out=rows(t, data=3 * A)), 3)
+    assert rc == 0 and out[9 + 59] == small, why
+
+
 def test_workspace_of_no_shape():
     f = engine.lib().gm_attention_workspace
     assert f(0, 1, 64) == f(8, 0, 64) == f(8, 3, 64) == f(8, 8, 0) == f(8, 8, 264) == 0
