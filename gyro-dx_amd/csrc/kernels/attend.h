@@ -3,19 +3,19 @@
 // that a page read once serves them all.
 //
 // Sequences of few rows (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and cache head and a
-// part of its keys, and finds out by itself which (af_share). Those of more (attend_tile.h): attend_plan cuts them into units, a
-// tile of 128 rows and a run of its keys each, which the groups take, every head's. Where keys are split, attend_join puts the
-// parts together.
+// part of its keys, and finds out by itself which (af_share). Those of more (attend_tile.h): a group takes a unit, a tile of 128
+// rows and a run of its keys, of every head; of up to 1024 tiles it finds out by itself which (at_share), of more attend_plan
+// makes a list. Where keys are split, attend_join puts the parts together.
 //
 // Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table
-// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 heads 29 group 30 D 31 kv heads
-// 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 causal 39 window 40 scale times log2(e)
+// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 tiles of 128 rows of the longest sequence 29 group 30 D 31 kv heads
+// 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 flags (1 causal, 2 32 bits span the cache) 39 window 40 scale times log2(e)
 // 41 groups that few rows' keys are split for (0: they are not) 42 tiles of few rows per sequence 43 type 44 keys of a tile
 // 45 tiles that make a part 46 rows of a sequence that units take it from (0: none) 47 groups of attend_join for
-// the few rows 48 units' list 50 units' parts 52 page size's shift plus one (0: no power of two) 53 units that the list holds
+// the few rows 48 units' list (0: none) 50 units' parts 52 logarithm of the page size, rounded up, and 59 its reciprocal 53 units that the list holds
 // 54 parts that the workspace holds, per head 55 keys of a tile of units 56 rows that attend_join takes of a few rows' tile
 // 57 tiles of keys up to which few rows' are not split 58 tiles that make a unit
-// 59 whether 32 bits span the cache
+
 #pragma once
 #include "rows.h"
 
@@ -73,7 +73,7 @@ __device__ __forceinline__ void at_sequence(const GdArgs &a, uint32_t seq, AtIte
 __device__ __forceinline__ void at_keys(const GdArgs &a, uint32_t row0, uint32_t rows, AtItem &o) {
     const uint32_t group = a.c[29];
     const int32_t window = (int32_t)a.c[39];
-    const bool causal = a.c[38] != 0u;
+    const bool causal = a.c[38] & 1u;
     o.row0 = row0;
     // Positions of the tile's first and last token.
     const int32_t base = o.kl - (int32_t)o.ql, p0 = base + (int32_t)(row0 / group),
@@ -92,7 +92,8 @@ __device__ __forceinline__ uint32_t at_tiles(const AtItem &o, uint32_t keys, uin
 // The page of key j of a sequence, and the key's offset in the cache, in bytes; -1: on a page outside it (or past `end`). Apart,
 // so that the page's load can be far ahead of its use. No load is conditional: the compiler counts the loads that are on their
 // way, and would wait for all of them where it is not certain of their number.
-__device__ __forceinline__ uint32_t at_slot_of(const GdArgs &a, uint32_t i) { return a.c[52] ? i >> (a.c[52] - 1u) : i / a.c[36]; }
+// i / page size, of i < 2^29: the size's reciprocal in 29 bits and its logarithm.
+__device__ __forceinline__ uint32_t at_slot_of(const GdArgs &a, uint32_t i) { return __umulhi(i << 3, a.c[59]) >> a.c[52]; }
 __device__ __forceinline__ uint32_t at_page(const GdArgs &a, uint32_t seq, int32_t j, int32_t end) {
     return (uint32_t)gd_at<const int32_t>(gd_addr(a, 18))[seq * gd_addr(a, 20) + at_slot_of(a, j < end ? (uint32_t)j : 0u)];
 }
@@ -246,7 +247,7 @@ __device__ __forceinline__ bool af_work(const GdArgs &a, AfWork &w) {
     const uint32_t row = min(w.o.row0 + (threadIdx.x & 15u), w.o.rows - 1u), token = row / group;
     w.q = (uint64_t)(w.o.token0 + token) * gd_addr(a, 2) + (uint64_t)(w.o.head * group + row - token * group) * a.c[30];
     const int32_t p = w.o.kl - (int32_t)w.o.ql + (int32_t)token, window = (int32_t)a.c[39];
-    w.last = a.c[38] ? p : w.o.kl - 1;
+    w.last = a.c[38] & 1u ? p : w.o.kl - 1;
     w.first = window ? p - window + 1 : 0;
     return true;
 }
@@ -301,4 +302,90 @@ __device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, floa
         if (alone) at_store4<TYPE>(out, d, x, by, total == 0.f);
         else *gd_at<gd_f32x4>(to_part + 8u * AF_ROWS + ((uint64_t)r * D + d) * 4u) = x;
     }
+}
+
+// The tiles of keys that a unit has at most, of so many that all tiles of rows have: a 512th of every head's (two groups for each
+// compute unit) and an eighth more, so that tiles a little larger than that are not split into units that fill a second round
+// by half (40 tiles of 250 and 22 small ones, four heads: 4 parts each 288 us, 3 parts 230).
+__device__ __forceinline__ uint32_t at_fair(const GdArgs &a, uint64_t all) {
+    return (uint32_t)max((uint64_t)a.c[58], (all * a.c[31] * 9u + 4095u) / 4096u);
+}
+
+// How the many rows' keys are shared out without a list: entry e is tile tiles - 1 - e / sequences of sequence e % sequences, the
+// tiles that see most keys first. Its keys are split as attend_plan splits them. Units of half a share or more come first (the
+// parts of split entries among them, which makes their numbers slots), then the others. The 256 threads of a group work this out
+// together, four entries each at most.
+#define AT_HELD 4u
+struct AtShare {
+    uint32_t sums[AT_HELD][4], split[AT_SPLITS];  // a wave's counts; split entries: first slot << 16 | entry
+    uint32_t entry, part, parts, splits, found;
+    uint64_t all;
+};
+// The unit of number `wanted` (found 0: there is none), or the split entries, in `s`.
+__device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t wanted, bool list) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, S = a.c[32], tiles = a.c[28], entries = S * tiles;
+    if (tid == 0u) {
+        s.all = 0;
+        s.found = 0u;
+        s.splits = 0u;
+    }
+    uint32_t keys[AT_HELD], rows[AT_HELD], own = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < AT_HELD; ++k) {
+        const uint32_t e = 256u * k + tid;
+        keys[k] = rows[k] = 0u;
+        if (256u * k < entries && e < entries) {
+            AtItem o;
+            uint32_t tile0;
+            const uint32_t back = e / S, row0 = (tiles - 1u - back) * AT_ROWS;
+            at_sequence(a, e - back * S, o);
+            if (row0 < o.rows && o.rows >= a.c[46]) {
+                at_keys(a, row0, AT_ROWS, o);
+                keys[k] = at_tiles(o, a.c[55], tile0);
+                rows[k] = 1u;
+            }
+        }
+        own += keys[k];  // at most 2^24 each, 64 lanes' 4 in 32 bits
+    }
+    __syncthreads();
+    const uint32_t of_wave = (uint32_t)__builtin_amdgcn_readlane((int)gd_wave_scan_u32(own), 63);
+    if (lane == 0u && of_wave) atomicAdd((unsigned long long *)&s.all, (unsigned long long)of_wave);
+    __syncthreads();
+    const uint32_t share = at_fair(a, s.all);
+    uint32_t parts[AT_HELD], count[AT_HELD], upto[AT_HELD];  // in 16 bits: units of the first kind, of the second
+#pragma unroll
+    for (uint32_t k = 0; k < AT_HELD; ++k) {
+        parts[k] = max(1u, (keys[k] + share - 1u) / share);
+        count[k] = !rows[k] ? 0u : 2u * (keys[k] / parts[k]) >= share ? parts[k] : 1u << 16;
+        upto[k] = gd_wave_scan_u32(count[k]);
+        if (lane == 63u) s.sums[k][wave] = upto[k];
+    }
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < AT_HELD; ++k)
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) total += s.sums[k][w];
+#pragma unroll
+    for (uint32_t k = 0; k < AT_HELD; ++k) {
+#pragma unroll
+        for (uint32_t w = 0; w < 4; ++w) {
+            if (w == wave) upto[k] += before - count[k];  // units before the thread's
+            before += s.sums[k][w];
+        }
+        const uint32_t first = upto[k] & 0xffffu, small = (total & 0xffffu) + (upto[k] >> 16);
+        const bool one = count[k] >> 16;
+        if (list) {
+            if (parts[k] > 1u) {
+                const uint32_t i = atomicAdd(&s.splits, 1u);
+                if (i < AT_SPLITS) s.split[i] = first << 16 | (256u * k + tid);
+            }
+        } else if (rows[k] && (one ? wanted == small : wanted - first < parts[k])) {
+            s.entry = 256u * k + tid;
+            s.part = one ? 0u : wanted - first;
+            s.parts = one ? 1u : parts[k];
+            s.found = 1u;
+        }
+    }
+    __syncthreads();
 }

@@ -1,5 +1,5 @@
 // Joins the parts of rows whose keys several groups shared (attend.h). The first groups take the few rows' split entries, a
-// group a row, as these may have hundreds of parts; the others the plan's split tiles, a wave a row, in turn.
+// group a row, as these may have hundreds of parts; the others the many rows' split tiles, in turn.
 #include "attend.h"
 
 // Row r of a sequence and head in out.
@@ -28,14 +28,15 @@ __device__ __forceinline__ float aj_group(float v, float *waves, F join) {
     return v;
 }
 
-// A row of few rows' parts, `step` bytes apart from `at` on, by the group: slices of it take parts in turn, four channels a thread.
+// A row of parts of ROWS rows, `step` bytes apart from `at` on, by the group: slices of it take parts in turn, four channels a thread.
+template <uint32_t ROWS>
 __device__ __forceinline__ void aj_by_group(const GdArgs &a, uint64_t at, uint64_t step, uint32_t parts, uint32_t r, uint64_t out) {
     constexpr uint32_t HELD = 5, MOST = HELD * AJ_THREADS;  // few rows' keys are split for 1024 groups at most, an entry in one part more
     __shared__ float weights[MOST], waves[2][AJ_WAVES];
     __shared__ __align__(16) float sums[4u * AJ_THREADS];
     const uint32_t tid = threadIdx.x, D = a.c[30], wide = D > 128u ? 64u : D > 64u ? 32u : 16u, slices = AJ_THREADS / wide;
     const uint32_t slice = tid / wide, d = 4u * (tid - slice * wide);
-    const uint64_t from = at + 8u * AF_ROWS + ((uint64_t)r * D + (d < D ? d : 0u)) * 4u;
+    const uint64_t from = at + 8u * ROWS + ((uint64_t)r * D + (d < D ? d : 0u)) * 4u;
     gd_f32x4 y[4];  // asked for together with the statistics
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) y[i] = *gd_at<const gd_f32x4>(from + min(slice + i * slices, parts - 1u) * step);
@@ -47,7 +48,7 @@ __device__ __forceinline__ void aj_by_group(const GdArgs &a, uint64_t at, uint64
         sum[i] = 0.f;
         if (AJ_THREADS * i < parts) {
             const uint64_t own = at + min(p, parts - 1u) * step;
-            const float t = gd_at<const float>(own)[r], s = gd_at<const float>(own)[AF_ROWS + r];
+            const float t = gd_at<const float>(own)[r], s = gd_at<const float>(own)[ROWS + r];
             top[i] = p < parts ? t : AT_LOWEST;
             sum[i] = p < parts ? s : 0.f;
         }
@@ -89,48 +90,67 @@ __device__ __forceinline__ void aj_by_group(const GdArgs &a, uint64_t at, uint64
     aj_store(a, out, d, x, total);
 }
 
-// A row of many rows' parts, by a wave: four channels a lane.
-__device__ __forceinline__ void aj_by_wave(const GdArgs &a, uint64_t at, uint64_t step, uint32_t parts, uint32_t r, uint64_t out) {
-    constexpr uint32_t HELD = 8;  // a lane's parts, of 64 of them each: attend_plan splits a tile into 512 at most
-    const uint32_t lane = threadIdx.x & 63u, D = a.c[30], d = 4u * lane < D ? 4u * lane : 0u;
-    const uint64_t from = at + 8u * AT_ROWS + ((uint64_t)r * D + d) * 4u;
-    gd_f32x4 first[4];  // asked for together with the statistics
-#pragma unroll
-    for (uint32_t p = 0; p < 4; ++p) first[p] = *gd_at<const gd_f32x4>(from + min(p, parts - 1u) * step);
-    float top[HELD], sum[HELD], most = AT_LOWEST, total = 0.f;
-#pragma unroll
-    for (uint32_t k = 0; k < HELD; ++k) {
-        top[k] = AT_LOWEST;
-        sum[k] = 0.f;
-        if (64u * k < parts) {
-            const uint64_t own = at + min(64u * k + lane, parts - 1u) * step;
-            const float t = gd_at<const float>(own)[r], s = gd_at<const float>(own)[AT_ROWS + r];
-            top[k] = 64u * k + lane < parts ? t : AT_LOWEST;
-            sum[k] = 64u * k + lane < parts ? s : 0.f;
-        }
-        most = fmaxf(most, top[k]);
-    }
-    most = gd_wave_max(most);
-#pragma unroll
-    for (uint32_t k = 0; k < HELD; ++k) {
-        top[k] = at_exp2(top[k] - most);
-        total += top[k] * sum[k];
-    }
-    total = gd_wave_sum_dpp(total);
+// A row of a few parts, by as many lanes as have four channels each; the others do nothing. Every lane reads all statistics.
+__device__ __forceinline__ void aj_by_lanes(const GdArgs &a, uint64_t at, uint64_t step, uint32_t parts, uint32_t r, uint32_t d, uint64_t out) {
+    const uint32_t D = a.c[30];
+    const uint64_t from = at + 8u * AT_ROWS + ((uint64_t)r * D + (d < D ? d : 0u)) * 4u;
     gd_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](gd_f32x4 y, float of, uint32_t p) {
-        const float w = gd_bits_f32((uint32_t)__builtin_amdgcn_readlane((int)gd_f32_bits(of), (int)(p & 63u)));
+    float most = AT_LOWEST, total = 0.f;
+    for (uint32_t p = 0; p < parts; p += 4u) {
+        gd_f32x4 y[4];
+        float top[4], sum[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += w * y[i];
-    };
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint64_t off = min(p + i, parts - 1u) * step;
+            y[i] = *gd_at<const gd_f32x4>(from + off);
+            top[i] = gd_at<const float>(at + off)[r];
+            sum[i] = gd_at<const float>(at + off)[AT_ROWS + r];
+        }
+        float next = most;
 #pragma unroll
-    for (uint32_t p = 0; p < 4; ++p)
-        if (p < parts) add(first[p], top[0], p);
+        for (uint32_t i = 0; i < 4; ++i) next = fmaxf(next, top[i]);
+        const float shrink = at_exp2(most - next);
+        most = next;
+        total *= shrink;
 #pragma unroll
-    for (uint32_t k = 0; k < HELD; ++k)
-#pragma unroll 4
-        for (uint32_t p = k ? 64u * k : 4u; p < min(parts, 64u * k + 64u); ++p) add(*gd_at<const gd_f32x4>(from + p * step), top[k], p);
-    if (4u * lane < D) aj_store(a, out, d, x, total);
+        for (int e = 0; e < 4; ++e) x[e] *= shrink;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const float w = p + i < parts ? at_exp2(top[i] - most) : 0.f;
+            if (p + i < parts) total += w * sum[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (p + i < parts) x[e] += w * y[i][e];
+        }
+    }
+    if (d < D) aj_store(a, out, d, x, total);
+}
+
+// The rows of split tiles, `splits` of them, each of every head, among the groups from number `group` on. `entry` tells a split's sequence,
+// tile of rows, first slot and parts.
+template <typename F>
+__device__ __forceinline__ void aj_tiles(const GdArgs &a, uint32_t group, uint32_t groups, uint32_t splits, F entry) {
+    const uint32_t KVH = a.c[31], D = a.c[30], wide = D > 128u ? 64u : D > 64u ? 32u : 16u, at_once = AJ_THREADS / wide;
+    const uint64_t step = at_part_bytes(a, AT_ROWS) * KVH;
+    // A group's turn: at_once neighbouring rows of a split tile and head, which AT_ROWS is a multiple of.
+    const uint64_t turns = (uint64_t)splits * KVH * (AT_ROWS / at_once);
+    for (uint64_t turn = group; turn < turns; turn += groups) {
+        const uint32_t rest = (uint32_t)(turn / (AT_ROWS / at_once)), row0 = (uint32_t)(turn % (AT_ROWS / at_once)) * at_once, index = rest / KVH;
+        AtItem o;
+        uint32_t tile, slot, parts;
+        if (!entry(index, o, tile, slot, parts)) continue;
+        o.head = rest - index * KVH;
+        const uint64_t at = at_slot(a, slot, o.head);
+        if (parts <= 16u) {
+            const uint32_t r = row0 + threadIdx.x / wide;
+            if (tile * AT_ROWS + r < o.rows) aj_by_lanes(a, at, step, parts, r, 4u * (threadIdx.x % wide), aj_out(a, o, tile * AT_ROWS + r));
+        } else {
+            for (uint32_t r = row0; r < row0 + at_once && tile * AT_ROWS + r < o.rows; ++r) {
+                aj_by_group<AT_ROWS>(a, at, step, parts, r, aj_out(a, o, tile * AT_ROWS + r));
+                __syncthreads();
+            }
+        }
+    }
 }
 
 GD_PIPELINE_NAMED(attend_join, 256) {
@@ -143,20 +163,34 @@ GD_PIPELINE_NAMED(attend_join, 256) {
         af_entry(a, entry, o, tile0);
         o.head = rest - index * KVH;
         if (o.row0 + r >= o.rows) return;
-        aj_by_group(a, af_part(a, slot, o.head), at_part_bytes(a, AF_ROWS) * KVH, parts, r, aj_out(a, o, o.row0 + r));
+        aj_by_group<AF_ROWS>(a, af_part(a, slot, o.head), at_part_bytes(a, AF_ROWS) * KVH, parts, r, aj_out(a, o, o.row0 + r));
         return;
     }
-    if (!gd_addr(a, 48)) return;
     const uint32_t groups = gridDim.x * gridDim.y - few;
-    const uint64_t rows = (uint64_t)at_plan(a)->splits * KVH * AT_ROWS;
-    for (uint64_t id = (uint64_t)(group - few) * AJ_WAVES + wave; id < rows; id += groups * AJ_WAVES) {
-        const uint32_t rest = (uint32_t)(id / AT_ROWS), r = (uint32_t)id % AT_ROWS, index = rest / KVH;
-        const uint32_t at = at_plan(a)->split[index];
-        if (at == 0xffffffffu) continue;
-        const AtUnit unit = at_units(a)[at];
-        at_sequence(a, unit.seq, o);
-        o.head = rest - index * KVH;
-        if (unit.tile * AT_ROWS + r >= o.rows) continue;
-        aj_by_wave(a, at_slot(a, unit.slot, o.head), at_part_bytes(a, AT_ROWS) * KVH, unit.parts, r, aj_out(a, o, unit.tile * AT_ROWS + r));
+    if (gd_addr(a, 48)) {
+        aj_tiles(a, group - few, groups, at_plan(a)->splits, [&](uint32_t i, AtItem &o, uint32_t &tile, uint32_t &slot, uint32_t &parts) {
+            const uint32_t at = at_plan(a)->split[i];
+            if (at == 0xffffffffu) return false;
+            const AtUnit unit = at_units(a)[at];
+            at_sequence(a, unit.seq, o);
+            tile = unit.tile;
+            slot = unit.slot;
+            parts = unit.parts;
+            return true;
+        });
+    } else if (a.c[28]) {
+        __shared__ AtShare s;
+        at_share(a, s, 0u, true);
+        const uint32_t share = at_fair(a, s.all);
+        aj_tiles(a, group - few, groups, min(s.splits, AT_SPLITS), [&](uint32_t i, AtItem &o, uint32_t &tile, uint32_t &slot, uint32_t &parts) {
+            const uint32_t entry = s.split[i] & 0xffffu, S = a.c[32], back = entry / S;
+            uint32_t tile0;
+            tile = a.c[28] - 1u - back;
+            slot = s.split[i] >> 16;
+            at_sequence(a, entry - back * S, o);
+            at_keys(a, tile * AT_ROWS, AT_ROWS, o);
+            parts = (at_tiles(o, a.c[55], tile0) + share - 1u) / share;
+            return true;
+        });
     }
 }

@@ -1,6 +1,5 @@
 // Cuts the sequences of many rows into units for attend_tile (attend.h), one group for the launch: the tiles of 128 rows, whose
-// keys are split where one has more tiles of them than a 512th of all heads' (what a group at a time on every half of a
-// compute unit does on average), the units of most tiles first. Units of one size come in any order, which changes no result.
+// keys are split where one has more tiles of them than its share (at_fair), the units of most tiles first. Units of one size come in any order, which changes no result.
 #include "attend.h"
 
 #define AP_CLASSES 32u
@@ -10,7 +9,7 @@ GD_PIPELINE_NAMED(attend_plan, 1024) {
     __shared__ uint32_t waves[16];
     __shared__ uint64_t total;
     __shared__ uint32_t cursor[AP_CLASSES], slots, splits;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, S = a.c[32], KVH = a.c[31], most = a.c[53], most_slots = a.c[54];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, S = a.c[32], most = a.c[53], most_slots = a.c[54];
     const gd_gptr<AtPlan> plan = at_plan(a);
     const gd_gptr<AtUnit> units = at_units(a);
     if (tid < AP_CLASSES) cursor[tid] = 0u;
@@ -55,7 +54,7 @@ GD_PIPELINE_NAMED(attend_plan, 1024) {
     each([&](uint32_t, uint32_t, uint32_t keys, uint32_t) { sum += keys; });
     if (sum) atomicAdd((unsigned long long *)&total, (unsigned long long)sum);
     __syncthreads();
-    const uint32_t share = (uint32_t)max((uint64_t)a.c[58], (total * KVH + 511u) / 512u);
+    const uint32_t share = at_fair(a, total);
     auto parts_of = [&](uint32_t keys) { return max(1u, (uint32_t)(((uint64_t)keys + share - 1u) / share)); };
     auto class_of = [&](uint32_t keys, uint32_t parts) {
         return AP_CLASSES - 1u - min(AP_CLASSES - 1u, (uint32_t)((uint64_t)(keys / parts) * AP_CLASSES / ((uint64_t)share + 1u)));

@@ -44,28 +44,24 @@ template <uint32_t CHUNKS>
 __device__ __forceinline__ uint32_t at_tile_v(uint32_t row) { return (CHUNKS < 16u ? row >> 1 & 1u : row & 3u) << 2; }
 
 template <uint32_t TYPE, uint32_t DT, uint32_t KEYS, bool SMALL>
-__device__ __forceinline__ void attend_tile_of(const GdArgs &a, char *lds_k, char *lds_v, uint32_t (*lds_bad)[2]) {
+__device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &unit, uint32_t head, char *lds_k, char *lds_v, uint32_t (*lds_bad)[2]) {
     constexpr uint32_t ROW = DT * 2u, STEPS = DT / 16u, DIMS = DT / 32u, CHUNKS = DT / 8u, BLOCKS = KEYS / 32u;
     constexpr uint32_t PER = 64u / CHUNKS, LOADS = KEYS / (4u * PER);  // keys of a wave's load, loads of a wave
     using Place = std::conditional_t<SMALL, uint32_t, uint64_t>;  // of a key in the cache (in a head of it, if 32 bits span it)
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 31u, h = lane >> 5, D = a.c[30], group = a.c[29], KVH = a.c[31];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 31u, h = lane >> 5, D = a.c[30], group = a.c[29];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, index = id / KVH, head = id - index * KVH;
-    if (index >= at_plan(a)->units) return;
-    const gd_gptr<const AtUnit> unit = at_units(a) + index;
-    const uint32_t seq = unit->seq, unit_from = unit->from, unit_to = unit->to, slot = unit->slot + unit->part;
-    const bool alone = unit->parts == 1u;
-    if (unit->slot == 0xffffffffu) return;
+    const uint32_t seq = unit.seq, unit_from = unit.from, unit_to = unit.to, slot = unit.slot + unit.part;
+    const bool alone = unit.parts == 1u;
     AtItem o;
     at_sequence(a, seq, o);
-    at_keys(a, unit->tile * AT_ROWS, AT_ROWS, o);
+    at_keys(a, unit.tile * AT_ROWS, AT_ROWS, o);
     const int32_t end = o.end, all_first = o.all_first, all_end = o.all_end;
     const gd_u32x4 empty = {0u, 0u, 0u, 0u};
 
     const uint32_t row = min(o.row0 + 32u * wave + col, o.rows - 1u), token = row / group;  // rows past the last are the last again
     const bool idle = o.row0 + 32u * wave >= o.rows;                                       // a wave with none but those
     const int32_t p = o.kl - (int32_t)o.ql + (int32_t)token, window = (int32_t)a.c[39];
-    const int32_t last = a.c[38] ? p : o.kl - 1, first = window ? p - window + 1 : 0;
+    const int32_t last = a.c[38] & 1u ? p : o.kl - 1, first = window ? p - window + 1 : 0;
     gd_u32x4 q[STEPS];
     {
         const uint64_t at = (uint64_t)(o.token0 + token) * gd_addr(a, 2) + (uint64_t)(head * group + row - token * group) * D;
@@ -354,6 +350,33 @@ __device__ __forceinline__ void attend_tile_body(const GdArgs &a) {
     __shared__ __align__(1024) char lds_k[2 * KEYS * DT * 2];
     __shared__ __align__(1024) char lds_v[2 * KEYS * DT * 2];
     __shared__ uint32_t lds_bad[2][2];  // keys of a tile whose values are not all finite, by turns
-    if (a.c[59]) attend_tile_of<TYPE, DT, KEYS, true>(a, lds_k, lds_v, lds_bad);
-    else attend_tile_of<TYPE, DT, KEYS, false>(a, lds_k, lds_v, lds_bad);
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, KVH = a.c[31], index = id / KVH, head = id - index * KVH;
+    AtUnit unit;
+    if (gd_addr(a, 48)) {
+        if (index >= at_plan(a)->units) return;
+        const gd_gptr<const AtUnit> listed = at_units(a) + index;
+        unit = AtUnit{listed->seq, listed->tile, listed->from, listed->to, listed->slot, listed->part, listed->parts, 0u};
+        if (unit.slot == 0xffffffffu) return;
+    } else {
+        static_assert(sizeof(AtShare) <= sizeof(lds_k), "what a group works out before its first keys");
+        AtShare &s = *reinterpret_cast<AtShare *>(lds_k);
+        at_share(a, s, index, false);
+        if (!__builtin_amdgcn_readfirstlane(s.found)) return;
+        const uint32_t entry = __builtin_amdgcn_readfirstlane(s.entry), S = a.c[32], back = entry / S;
+        unit.part = __builtin_amdgcn_readfirstlane(s.part);
+        unit.parts = __builtin_amdgcn_readfirstlane(s.parts);
+        unit.seq = entry - back * S;
+        unit.tile = a.c[28] - 1u - back;
+        unit.slot = index - unit.part;
+        AtItem o;
+        uint32_t tile0;
+        at_sequence(a, unit.seq, o);
+        at_keys(a, unit.tile * AT_ROWS, AT_ROWS, o);
+        const uint32_t keys = at_tiles(o, KEYS, tile0);
+        unit.from = tile0 + (uint32_t)((uint64_t)keys * unit.part / unit.parts);
+        unit.to = tile0 + (uint32_t)((uint64_t)keys * (unit.part + 1u) / unit.parts);
+        __syncthreads();
+    }
+    if (a.c[38] & 2u) attend_tile_of<TYPE, DT, KEYS, true>(a, unit, head, lds_k, lds_v, lds_bad);
+    else attend_tile_of<TYPE, DT, KEYS, false>(a, unit, head, lds_k, lds_v, lds_bad);
 }

@@ -247,7 +247,6 @@ class AttentionOps {
         c.set64(20, d.table_stride);
         c.set(22, d.lengths);
         c.set(24, d.starts);
-        c.set(28, H);
         c.set(29, group);
         c.set(30, D);
         c.set(31, G);
@@ -257,17 +256,20 @@ class AttentionOps {
         c.set(35, d.cache.pages);
         c.set(36, d.cache.page_size);
         c.set(37, d.table_width);
-        c.set(38, d.causal ? 1u : 0u);
         c.set(39, std::min(d.window, 1u << 30));
         c.set(40, d.scale * 1.44269504088896341f);
         c.set(43, d.cache.type);
         // Whether 32 bits span the cache: keys' offsets take half the work then.
         const auto reach = [](uint32_t count, uint64_t stride) { return count > 1 ? (unsigned __int128)(count - 1) * stride : 0; };
         const auto span = reach(d.cache.pages, d.cache.page_stride) + reach(G, d.cache.head_stride) + reach(d.cache.page_size, d.cache.token_stride) + D;
-        c.set(59, span <= (uint64_t(1) << 32) / (wide ? 4 : 2) ? 1u : 0u);
+        c.set(38, (d.causal ? 1u : 0u) | (span <= (uint64_t(1) << 32) / (wide ? 4 : 2) ? 2u : 0u));
         c.set(46, many ? kFewRows + 1 : 0u);
-        for (uint32_t shift = 0; shift < 31; ++shift)
-            if (d.cache.page_size == 1u << shift) c.set(52, shift + 1);
+        // Division of key numbers below 2^29 by the page size: with 2^(s-1) < size <= 2^s the reciprocal 2^(29+s) / size, rounded
+        // up by less than one, is off by less than i / 2^(29+s) < 1 / size in i times it.
+        uint32_t shift = 0;
+        while ((uint64_t(1) << shift) < d.cache.page_size) ++shift;
+        c.set(52, shift);
+        c.set(59, (uint32_t)(((uint64_t(1) << (29 + shift)) + d.cache.page_size - 1) / d.cache.page_size));
         const int size = D <= 64 ? 0 : D <= 128 ? 1 : 2, type = d.cache.type;
         uint64_t need = 0, join = 0, groups = 0;
         bool short_keys = false;
@@ -296,18 +298,24 @@ class AttentionOps {
         c.set(47, (uint32_t)join);
         uint64_t units = 0;
         if (many) {
-            // Whole tiles of rows, one more for each sequence, and the parts of those that are split.
-            units = (uint64_t)n * group / kTileRows + std::min<uint64_t>(d.sequences, (uint64_t)n * group / (kFewRows + 1)) + 512 / G + 1;
+            // Tiles of rows: of every sequence as many as of the longest, or by their tokens, one more each; and what splits add.
+            const uint64_t tiles = (rows + kTileRows - 1) / kTileRows, entries = tiles * d.sequences;
+            units = (uint64_t)n * group / kTileRows + std::min<uint64_t>(d.sequences, (uint64_t)n * group / (kFewRows + 1));
+            units = std::min(units, entries) + 512 / G + 1;
             require(units <= kUnits && units * G < 1u << 31, "gm_attention: n * heads / kv_heads / 128 + sequences is at most 2^18 - 1024");
             need = workspace(H, G, D);
-            join += 2048;
-            c.set64(48, (uint64_t)(uintptr_t)d.workspace + plan_at(D));
             c.set64(50, (uint64_t)(uintptr_t)d.workspace + slots_at(D));
-            c.set(58, kTileLeast);
-            c.set(53, (uint32_t)units);
             c.set(54, kSlots / G);
             c.set(55, D > 128 ? 32u : 64u);
-            l.add("attend_plan", 1);
+            c.set(58, kTileLeast);
+            if (entries <= kEntries) {
+                c.set(28, (uint32_t)tiles);
+            } else {
+                c.set64(48, (uint64_t)(uintptr_t)d.workspace + plan_at(D));
+                c.set(53, (uint32_t)units);
+                l.add("attend_plan", 1);
+            }
+            join += 1024;
         }
         require(!need || (d.workspace && d.workspace_bytes >= need && (uintptr_t)d.workspace % 256 == 0), "gm_attention: workspace");
         c.set(26, d.workspace);

@@ -299,9 +299,10 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
             build = "f32_" if not type else ("short_" if width * 16 <= 1024 and size < 256 else "few_") + "?bh"[type]
             few = f"attend_{build}{size}"
             tile = "attend_tile_%s%d" % ("?bh"[type], size)
-            assert names[:1] == ["attend_plan"] if many else "attend_plan" not in names
+            listed = many and sequences * -(-longest * group // 128) > 1024
+            assert names[:1] == ["attend_plan"] if listed else "attend_plan" not in names
             assert (few in names) == (not many or ragged) and (tile in names) == bool(many)
-            assert w[46] == (17 if many else 0) and w[52] == 5  # pages of 16
+            assert w[46] == (17 if many else 0)
             join = 0
             if few in names:
                 split, tiles, keys, least = w[41], w[42], w[44], w[45]
@@ -317,21 +318,32 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
                     assert join >= min(sequences * tiles, split // kv) * kv * most_rows
             assert w[47] == join
             if many:
-                units = w[53]
-                assert grids["attend_plan"] == 1 and grids[tile] >= units * kv and units <= 1 << 18
-                # Tiles of rows, the most there are if every sequence has one that is not whole, and what splits add.
-                assert units > -(-sequences * longest * group // 128) + 512 // kv
-                assert w[48] | w[49] << 32 == A + few_bytes and w[50] | w[51] << 32 == A + few_bytes + 4352 + (32 << 18)
+                tokens = sequences * longest * group
+                units = min(sequences * -(-longest * group // 128), tokens // 128 + min(sequences, tokens // 17)) + 512 // kv
+                assert grids[tile] > units * kv and units < 1 << 18
+                assert w[50] | w[51] << 32 == A + few_bytes + 4352 + (32 << 18)
                 assert w[54] * kv * part <= 1024 * part and w[55] == (32 if dim > 128 else 64)
-                assert grids["attend_join"] >= join + 2048
+                assert grids["attend_join"] >= join + 1024
+                if listed:
+                    assert grids["attend_plan"] == 1 and w[48] | w[49] << 32 == A + few_bytes and grids[tile] >= w[53] * kv > units * kv
+                else:
+                    assert w[48] == w[49] == 0 and w[28] == -(-longest * group // 128)
             else:
                 assert ("attend_join" in names) == bool(join) and (not join or grids["attend_join"] >= join)
 
 
-def test_page_shifts(shim):
-    for size, want in ((1, 1), (2, 2), (3, 0), (16, 5), (100, 0), (256, 9), (1 << 20, 21)):
-        c = cache(page_size=size, token_stride=64, head_stride=size * 64, page_stride=size * 128)
-        assert call(shim.plan_attention, attention(cache=c), 3)[2][9 + 52] == want
+def test_page_division(shim):
+    """The kernels' division by the page size, of key numbers up to the largest."""
+    rng = np.random.default_rng(3)
+    for size in (1, 2, 3, 5, 7, 16, 24, 48, 100, 255, 256, 257, 1000, 4095, 65537, (1 << 20) - 1, 1 << 20, (1 << 29) - 1):
+        width = max(1, ((1 << 29) - 1) // size)
+        c = cache(page_size=size, pages=2, token_stride=64, head_stride=size * 64, page_stride=size * 128)
+        rc, why, out = call(shim.plan_attention, attention(cache=c, table_width=width, table_stride=width), 3)
+        assert rc == 0, why
+        shift, reciprocal = out[9 + 52], out[9 + 59]
+        i = np.concatenate([np.arange(5), rng.integers(0, 1 << 29, 100000), [(1 << 29) - 1], *(np.arange(1, 50) * size + k for k in (-1, 0, 1))])
+        i = np.unique(np.clip(i, 0, (1 << 29) - 1)).astype(object)
+        assert all(((int(v) << 3) * reciprocal >> 32) >> shift == int(v) // size for v in i), size
 
 
 @pytest.mark.parametrize("kw,small", [
@@ -344,7 +356,7 @@ def test_cache_spans(shim, kw, small):
     c = cache(**kw)
     t = c.type
     rc, why, out = call(shim.plan_attention, attention(cache=c, q=rows(t), out=rows(t, data=3 * A)), 3)
-    assert rc == 0 and out[9 + 59] == small, why
+    assert rc == 0 and out[9 + 38] == 1 + 2 * small, why
 
 
 def test_workspace_of_no_shape():
