@@ -274,7 +274,7 @@ class AttentionOps {
         uint64_t need = 0, join = 0, groups = 0;
         bool short_keys = false;
         if (few) {
-            const uint32_t keys = wide ? 16 : 32, tiles = wide ? (uint32_t)((rows + kFewRows - 1) / kFewRows) : 1;
+            const uint32_t keys = wide && D > 64 ? 16 : 32, tiles = wide ? (uint32_t)((rows + kFewRows - 1) / kFewRows) : 1;
             const uint64_t entries = (uint64_t)d.sequences * tiles;
             require(entries * G < 1u << 31, "gm_attention: too many sequences");
             groups = entries * G;
@@ -283,12 +283,12 @@ class AttentionOps {
             // Split where there may be keys for it, and entries enough to fill the GPU are not there anyway. Keys that one
             // group takes may be taken by one of eight waves.
             const uint32_t resident = (wide ? 256 : kResident[size]) * (d.sequences > 1 ? kPerGroup : 1);
-            short_keys = capacity <= kAlone;
+            short_keys = capacity <= (wide ? 2 : 1) * kAlone;
             if (entries <= kEntries && entries * G < 2 * resident && !short_keys) {
                 groups += resident;
                 c.set(41, resident);
                 c.set(45, kLeast / keys);
-                c.set(57, kAlone / keys);
+                c.set(57, (wide ? 2 * kAlone : kLeast) / keys);
                 need = plan_at(D);
                 const uint32_t most = (uint32_t)std::min<uint64_t>(kFewRows, rows);
                 c.set(56, most);
