@@ -314,7 +314,7 @@ __device__ __forceinline__ uint32_t at_fair(const GdArgs &a, uint64_t all) {
 // How the many rows' keys are shared out without a list: entry e is tile tiles - 1 - e / sequences of sequence e % sequences, the
 // tiles that see most keys first. Its keys are split as attend_plan splits them. Units of half a share or more come first (the
 // parts of split entries among them, which makes their numbers slots), then the others. The 256 threads of a group work this out
-// together, four entries each at most.
+// together, four entries each at most. Every group comes to the same numbers, those of the split entries among them.
 #define AT_HELD 4u
 struct AtShare {
     uint32_t sums[AT_HELD][4], split[AT_SPLITS];  // a wave's counts; split entries: first slot << 16 | entry
@@ -327,7 +327,6 @@ __device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t w
     if (tid == 0u) {
         s.all = 0;
         s.found = 0u;
-        s.splits = 0u;
     }
     uint32_t keys[AT_HELD], rows[AT_HELD], own = 0;
 #pragma unroll
@@ -352,11 +351,13 @@ __device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t w
     if (lane == 0u && of_wave) atomicAdd((unsigned long long *)&s.all, (unsigned long long)of_wave);
     __syncthreads();
     const uint32_t share = at_fair(a, s.all);
-    uint32_t parts[AT_HELD], count[AT_HELD], upto[AT_HELD];  // in 16 bits: units of the first kind, of the second
+    // In 11 bits each, units of the first kind and of the second, of which there are fewer than 1024 + 456 and 1025; then split
+    // entries, each of more than 9 / 4096 of all keys.
+    uint32_t parts[AT_HELD], count[AT_HELD], upto[AT_HELD];
 #pragma unroll
     for (uint32_t k = 0; k < AT_HELD; ++k) {
         parts[k] = max(1u, (keys[k] + share - 1u) / share);
-        count[k] = !rows[k] ? 0u : 2u * (keys[k] / parts[k]) >= share ? parts[k] : 1u << 16;
+        count[k] = !rows[k] ? 0u : 2u * (keys[k] / parts[k]) >= share ? parts[k] | (parts[k] > 1u ? 1u << 22 : 0u) : 1u << 11;
         upto[k] = gd_wave_scan_u32(count[k]);
         if (lane == 63u) s.sums[k][wave] = upto[k];
     }
@@ -366,6 +367,7 @@ __device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t w
     for (uint32_t k = 0; k < AT_HELD; ++k)
 #pragma unroll
         for (uint32_t w = 0; w < 4; ++w) total += s.sums[k][w];
+    if (tid == 0u) s.splits = total >> 22;
 #pragma unroll
     for (uint32_t k = 0; k < AT_HELD; ++k) {
 #pragma unroll
@@ -373,13 +375,10 @@ __device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t w
             if (w == wave) upto[k] += before - count[k];  // units before the thread's
             before += s.sums[k][w];
         }
-        const uint32_t first = upto[k] & 0xffffu, small = (total & 0xffffu) + (upto[k] >> 16);
-        const bool one = count[k] >> 16;
+        const uint32_t first = upto[k] & 2047u, small = (total & 2047u) + (upto[k] >> 11 & 2047u);
+        const bool one = count[k] == 1u << 11;
         if (list) {
-            if (parts[k] > 1u) {
-                const uint32_t i = atomicAdd(&s.splits, 1u);
-                if (i < AT_SPLITS) s.split[i] = first << 16 | (256u * k + tid);
-            }
+            if (parts[k] > 1u && upto[k] >> 22 < AT_SPLITS) s.split[upto[k] >> 22] = first << 16 | (256u * k + tid);
         } else if (rows[k] && (one ? wanted == small : wanted - first < parts[k])) {
             s.entry = 256u * k + tid;
             s.part = one ? 0u : wanted - first;

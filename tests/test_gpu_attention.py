@@ -365,6 +365,24 @@ def test_attention_split_tiles(eng, type, dim):
         assert torch.equal(first, b.out)
 
 
+@pytest.mark.parametrize("counts", [[700, 300, 20, 3, 40, 0, 130, 1, 90], [3, 200] * 20, [40] * 170 + [400]], ids=str)
+def test_attention_many_split_tiles(eng, counts):
+    """Split tiles among those that every wave of a group looks at, in every order; the same results every time."""
+    rng = np.random.default_rng(63)
+    lengths = [int(rng.integers(max(1, n), 3001)) for n in counts]
+    print(f"many split tiles {counts[:4]}", flush=True)
+    b = Batch(eng, "bf16", 5, 1, 16, 100, counts, lengths, seed=19)
+    b.out.fill_(7.0)
+    b.run()
+    b.check()
+    first = b.out.clone()
+    for _ in range(5):
+        b.out.fill_(7.0)
+        b.run()
+        torch.cuda.synchronize()
+        assert torch.equal(first, b.out)
+
+
 def test_attention_most_parts(eng):
     """One cache head's keys in as many parts as there are: of 16 rows, and of 128."""
     for type, counts, length in (("f16", [2], 140001), ("bf16", [17], 200003)):
