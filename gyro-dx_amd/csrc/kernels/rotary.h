@@ -1,8 +1,8 @@
 // Heads turned by their positions, and new tokens' keys and values on their way into a paged cache:
 //   (y1, y2) = scale (x1 cos a - x2 sin a, x1 sin a + x2 cos a),  a = position * frequency of the pair
 // Rows of up to three kinds in one launch: queries (turned, to rows), keys (turned, to the cache's slots) and values
-// (as they are, to the slots). A thread takes one unit of 8 pairs (or 16 values that do not turn) of a token and the
-// same unit of several heads, so that the angles are formed once for them.
+// (as they are, to the slots). A group takes a token, or a part of one, forms its sines and cosines once, a pair a thread, and
+// turns its heads by them: a thread takes units of 8 pairs (or 16 values that do not turn) of a head.
 //
 // Angles: a frequency is a fraction of a turn in 64 bits, whole turns dropped; its product with the position modulo 2^64 is the
 // angle's fraction of a turn, exact but for the frequency's own last place. Its top two bits, rounded, are the quadrant; what is
@@ -12,8 +12,8 @@
 // Constants: 0 q 2 q stride 4 q_out 6 q_out stride 8 k 10 k stride 12 v 14 v stride 16 cache k 18 cache v 20 page stride
 // 22 head stride 24 token stride (bytes) 26 frequencies (0: nothing turns) 28 positions 30 slots 32 D 33 pairs 34 query heads
 // 35 kv heads (0: no cache) 36 tokens 37 types (q_out | cache << 4) 38 flags (1 interleaved, 2 positions in 64 bits, 4 slots
-// in 64 bits) 39 scale 40 page size 41 pages * page size 42 heads per thread 43 threads' groups of heads per token 44 units per
-// head
+// in 64 bits) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two heads of
+// a thread
 #pragma once
 #include "rows.h"
 
@@ -35,107 +35,147 @@ __device__ __forceinline__ void ro_turn(uint64_t fraction, float scale, float &c
     s = scale * (q & 2u ? -b : b);
 }
 
-// Values i .. i + m - 1 of a head, m <= 8, the others zeros.
-template <uint32_t TYPE>
-__device__ __forceinline__ void ro_load(uint64_t head, uint32_t i, uint32_t m, float (&v)[8]) {
-    if (m == 8u) return row_load8<TYPE>(head, i, v);
+// Values i .. i + m - 1 of a head, m <= 8. FULL: every m is 8, and the values stay as they are in memory until they are used, so that
+// loads follow each other without a wait. Otherwise those past m are zeros.
+template <uint32_t TYPE, bool FULL>
+struct RoEight {
+    gd_u32x4 raw[TYPE == ROW_F32 ? 2 : 1];
+    float v[8];
+    __device__ __forceinline__ void load(uint64_t head, uint32_t i, uint32_t m) {
+        if constexpr (FULL) {
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) v[j] = j < m ? row_load(head, i + j, TYPE) : 0.f;
-}
-__device__ __forceinline__ void ro_store(uint64_t head, uint32_t i, uint32_t m, uint32_t type, const float (&v)[8]) {
-    row_store8(head, i, i + m, type, v);
-}
+            for (uint32_t j = 0; j < sizeof(raw) / 16u; ++j) raw[j] = gd_at<const gd_u32x4_any>(head + ((uint64_t)i << row_shift(TYPE)))[j];
+        } else if (m == 8u) {
+            row_load8<TYPE>(head, i, v);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) v[j] = j < m ? row_load(head, i + j, TYPE) : 0.f;
+        }
+    }
+    __device__ __forceinline__ void unpack() {
+        if constexpr (FULL) {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                if constexpr (TYPE == ROW_F32) v[j] = gd_bits_f32(raw[j >> 2][j & 3u]);
+                else v[j] = row_value16(raw[0][j >> 1] >> (16u * (j & 1u)) & 0xffffu, TYPE);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint64_t head, uint32_t i, uint32_t m, uint32_t type) const { row_store8(head, i, i + (FULL ? 8u : m), type, v); }
+};
 
-template <uint32_t TYPE>
-__device__ __forceinline__ void rotary_body(const GdArgs &a) {
+#define RO_TABLE 512u  // pairs of a head at most
+
+template <uint32_t TYPE, bool FULL>
+__device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, float *sines) {
     const uint32_t D = a.c[32], pairs = a.c[33], QH = a.c[34], KVH = a.c[35], n = a.c[36], types = a.c[37], flags = a.c[38];
-    const uint32_t per = a.c[42], groups = a.c[43], units = a.c[44], heads = QH + 2u * KVH;
-    const uint64_t FREQ = gd_addr(a, 26);
-    const uint32_t own = threadIdx.x / units, u = threadIdx.x - own * units, at_once = 256u / units;
-    if (own >= at_once) return;
-    const uint64_t item = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * at_once + own;
-    if (item >= (uint64_t)n * groups) return;
-    const uint32_t t = (uint32_t)item / groups, head0 = ((uint32_t)item - t * groups) * per;
+    const uint32_t sharers = a.c[42], units = a.c[43], turns = a.c[44], heads = QH + 2u * KVH;
+    const uint64_t id = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x, of = id / sharers;
+    if (of >= n) return;
+    const uint32_t t = (uint32_t)of;
+    // A thread takes one unit of every at_once-th head, two heads a turn; a group that shares a token its turns' heads.
+    const uint32_t at_once = 256u / units, own = threadIdx.x / units, u = threadIdx.x - own * units;
+    const uint32_t head0 = (uint32_t)(id - of * sharers) * turns * 2u * at_once + own;
     const uint32_t turning = (pairs + 7u) / 8u;  // units of pairs; the others' values are copied
-    // Where the two halves of a unit lie in a head, and how many values of each there are.
-    uint32_t at1, at2, m1, m2;
+    // The halves of a unit in a head that turns and in one that does not: their places and how many values of each there are.
+    uint32_t f1, f2, n1, n2;
     if (u < turning) {
         const uint32_t m = min(8u, pairs - 8u * u);
-        if (flags & 1u) {
-            at1 = 16u * u;
-            at2 = at1 + 8u;
-            m1 = min(8u, 2u * m);
-            m2 = 2u * m - m1;
-        } else {
-            at1 = 8u * u;
-            at2 = pairs + at1;
-            m1 = m2 = m;
-        }
+        const bool apart = !(flags & 1u);
+        f1 = apart ? 8u * u : 16u * u;
+        f2 = apart ? pairs + 8u * u : 16u * u + 8u;
+        n1 = apart ? m : min(8u, 2u * m);
+        n2 = apart ? m : 2u * m - n1;
     } else {
-        at1 = 2u * pairs + 16u * (u - turning);
-        at2 = at1 + 8u;
-        m1 = at1 < D ? min(8u, D - at1) : 0u;
-        m2 = at2 < D ? min(8u, D - at2) : 0u;
+        f1 = 2u * pairs + 16u * (u - turning);
+        f2 = f1 + 8u;
+        n1 = f1 < D ? min(8u, D - f1) : 0u;
+        n2 = f2 < D ? min(8u, D - f2) : 0u;
     }
-    // Units of the values' heads, which have nothing that turns.
     const uint32_t v1 = 16u * u, v2 = v1 + 8u, mv1 = v1 < D ? min(8u, D - v1) : 0u, mv2 = v2 < D ? min(8u, D - v2) : 0u;
+    const uint32_t to_q = types & 15u, to_cache = types >> 4;
 
-    float c[8], s[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        c[j] = 1.f;
-        s[j] = 0.f;
-    }
-    if (u < turning && head0 < QH + KVH) {
-        const int64_t position = ro_index(gd_addr(a, 28), t, flags & 2u);
-        const float scale = gd_bits_f32(a.c[39]);
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)  // the table's last pair is read again behind the end
-            ro_turn((uint64_t)position * gd_at<const uint64_t>(FREQ)[min(8u * u + j, pairs - 1u)], scale, c[j], s[j]);
-    }
-    uint64_t slot_offset = 0;
+    // Where the token's rows begin, and its place in the cache.
+    const uint64_t from_q = gd_addr(a, 0) + ((t * gd_addr(a, 2)) << row_shift(TYPE)), from_k = gd_addr(a, 8) + ((t * gd_addr(a, 10)) << row_shift(TYPE)),
+                   from_v = gd_addr(a, 12) + ((t * gd_addr(a, 14)) << row_shift(TYPE)), out_q = gd_addr(a, 4) + ((t * gd_addr(a, 6)) << row_shift(to_q));
+    uint64_t cache_k = gd_addr(a, 16), cache_v = gd_addr(a, 18);
     bool kept = false;
-    if (head0 + per > QH && KVH) {
+    if (KVH) {
         const int64_t slot = ro_index(gd_addr(a, 30), t, flags & 4u);
         kept = (uint64_t)slot < a.c[41];
         const uint32_t where = kept ? (uint32_t)slot : 0u, page = where / a.c[40];
-        slot_offset = page * gd_addr(a, 20) + (where - page * a.c[40]) * gd_addr(a, 24);
+        const uint64_t at = page * gd_addr(a, 20) + (where - page * a.c[40]) * gd_addr(a, 24);
+        cache_k += at;
+        cache_v += at;
     }
 #pragma unroll 1
-    for (uint32_t h = head0; h < min(head0 + per, heads); ++h) {
-        const bool value = h >= QH + KVH, query = h < QH;
-        if (!query && !kept) continue;
-        const uint32_t in_row = query ? h : value ? h - QH - KVH : h - QH;
-        const uint64_t from = query ? gd_addr(a, 0) : value ? gd_addr(a, 12) : gd_addr(a, 8);
-        const uint64_t stride = query ? gd_addr(a, 2) : value ? gd_addr(a, 14) : gd_addr(a, 10);
-        const uint64_t x = from + ((t * stride + (uint64_t)in_row * D) << row_shift(TYPE));
-        const uint32_t to = query ? types & 15u : types >> 4;
-        const uint64_t y = query ? gd_addr(a, 4) + ((t * gd_addr(a, 6) + (uint64_t)in_row * D) << row_shift(to))
-                                 : (value ? gd_addr(a, 18) : gd_addr(a, 16)) + slot_offset + in_row * gd_addr(a, 22);
-        const uint32_t f1 = value ? v1 : at1, f2 = value ? v2 : at2, n1 = value ? mv1 : m1, n2 = value ? mv2 : m2;
-        float p[8], q[8];
-        ro_load<TYPE>(x, f1, n1, p);
-        ro_load<TYPE>(x, f2, n2, q);
-        if (!value && u < turning) {
-            if (flags & 1u) {
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        // Two heads at a time: the second's loads are on their way with the first's, the first turn's while the angles are formed.
+        RoEight<TYPE, FULL> first[2], second[2];
+        uint64_t y[2];
+        bool stays[2], query[2], value[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float p1 = p[2 * j], q1 = q[2 * j];
-                    p[2 * j] = p1 * c[j] - p[2 * j + 1] * s[j];
-                    p[2 * j + 1] = p1 * s[j] + p[2 * j + 1] * c[j];
-                    q[2 * j] = q1 * c[4 + j] - q[2 * j + 1] * s[4 + j];
-                    q[2 * j + 1] = q1 * s[4 + j] + q[2 * j + 1] * c[4 + j];
-                }
-            } else {
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t head = head0 + (2u * turn + i) * at_once;
+            const bool there = own < at_once && head < heads;
+            const uint32_t h = there ? head : 0u;
+            query[i] = h < QH;
+            value[i] = h >= QH + KVH;
+            const uint32_t in_row = query[i] ? h : value[i] ? h - QH - KVH : h - QH;
+            const uint64_t x = (query[i] ? from_q : value[i] ? from_v : from_k) + ((uint64_t)(in_row * D) << row_shift(TYPE));
+            y[i] = query[i] ? out_q + ((uint64_t)(in_row * D) << row_shift(to_q)) : (value[i] ? cache_v : cache_k) + in_row * gd_addr(a, 22);
+            stays[i] = there && (query[i] || kept);
+            first[i].load(x, value[i] ? v1 : f1, value[i] ? mv1 : n1);
+            second[i].load(x, value[i] ? v2 : f2, value[i] ? mv2 : n2);
+        }
+        if (!turn) {
+            for (uint32_t i = threadIdx.x; i < pairs; i += 256u)
+                ro_turn((uint64_t)ro_index(gd_addr(a, 28), t, flags & 2u) * gd_at<const uint64_t>(gd_addr(a, 26))[i], gd_bits_f32(a.c[39]), cosines[i], sines[i]);
+            __syncthreads();
+        }
+        float c[8], s[8];  // of the thread's pairs (of a head's last ones the table's end is read again)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float p1 = p[j];
-                    p[j] = p1 * c[j] - q[j] * s[j];
-                    q[j] = p1 * s[j] + q[j] * c[j];
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t at = min(8u * u + j, RO_TABLE - 1u);
+            c[j] = cosines[at];
+            s[j] = sines[at];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            if (!stays[i]) continue;
+            first[i].unpack();
+            second[i].unpack();
+            auto &p = first[i].v, &q = second[i].v;
+            if (u < turning && !value[i]) {
+                if (flags & 1u) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p1 = p[2 * j], q1 = q[2 * j];
+                        p[2 * j] = p1 * c[j] - p[2 * j + 1] * s[j];
+                        p[2 * j + 1] = p1 * s[j] + p[2 * j + 1] * c[j];
+                        q[2 * j] = q1 * c[4 + j] - q[2 * j + 1] * s[4 + j];
+                        q[2 * j + 1] = q1 * s[4 + j] + q[2 * j + 1] * c[4 + j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float p1 = p[j];
+                        p[j] = p1 * c[j] - q[j] * s[j];
+                        q[j] = p1 * s[j] + q[j] * c[j];
+                    }
                 }
             }
+            const uint32_t to = query[i] ? to_q : to_cache;
+            first[i].store(y[i], value[i] ? v1 : f1, value[i] ? mv1 : n1, to);
+            second[i].store(y[i], value[i] ? v2 : f2, value[i] ? mv2 : n2, to);
         }
-        ro_store(y, f1, n1, to, p);
-        ro_store(y, f2, n2, to, q);
     }
+}
+
+// (full: whole units only)
+template <uint32_t TYPE>
+__device__ __forceinline__ void rotary_body(const GdArgs &a) {
+    __shared__ __align__(16) float cosines[RO_TABLE], sines[RO_TABLE];
+    if (a.c[32] % 16u == 0 && a.c[33] % 8u == 0) rotary_rows<TYPE, true>(a, cosines, sines);
+    else rotary_rows<TYPE, false>(a, cosines, sines);
 }

@@ -93,6 +93,7 @@ _PACK_ROTARY = struct.Struct("@4I" + 2 * "PQII" + "P").pack
 _PACK_APPEND = struct.Struct("@" + _CACHE + "4I" + 4 * "PQII" + "PP").pack
 _PACK_ATTENTION = struct.Struct("@" + _CACHE + 2 * "PQII" + "5IfPQPPIIPQ").pack
 _NO_ROWS = (0, 0, 0)
+_MOST = 0xffffffff
 
 
 def _count(n, what):
@@ -367,22 +368,26 @@ class Engine:
 
     def _rows(self, t, shape, what):
         """(address, stride, type) of a tensor of rows."""
+        code = _type_codes.get(t.dtype)
+        if code not in _ROW_TYPES:
+            code = _type(t, _ROW_TYPES, what)
         if t.shape != shape:
-            raise ValueError(f"{what}: shape {tuple(t.shape)}, not {shape}")
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, not {tuple(shape)}")
         if t.get_device() != self.adapter:
             raise ValueError(f"{what}: not on the engine's GPU")
         stride, step = t.stride()
         if step != 1 and shape[1] > 1:
             raise ValueError(f"{what}: the values of a row are not neighbours")
-        return t.data_ptr(), stride, _type(t, _ROW_TYPES, what)
+        return t.data_ptr(), stride, code
 
     def _flat(self, t, size, types, what):
         """Address of a contiguous tensor of `size` values."""
+        if _type_codes.get(t.dtype) not in types:
+            _type(t, types, what)
         if t.numel() != size or not t.is_contiguous():
             raise ValueError(f"{what}: shape {tuple(t.shape)}, not {size} neighbouring values")
         if t.get_device() != self.adapter:
             raise ValueError(f"{what}: not on the engine's GPU")
-        _type(t, types, what)
         return t.data_ptr()
 
     def linear(self, matrix: int, x, y, act: str = "none", accumulate: bool = False, scale: float = 1.0,
@@ -485,32 +490,36 @@ class Engine:
 
     def rotary(self, rotary: int, x, positions, y, heads: int, stream: int | None = None):
         """y = the heads of x (rows of `heads` heads) turned by positions (int32 or int64 [n]); y may be x."""
-        n, values = x.shape
-        _count(n, "rows of x")
+        shape = x.shape
+        n, values = shape
         if heads <= 0 or values % heads:
             raise ValueError(f"x: {values} values are not {heads} heads")
-        shape = (n, values)
+        if not (0 <= rotary <= _MOST and n <= _MOST and values <= _MOST):
+            raise ValueError("rotary, rows or values: not 32-bit counts")
         p = self._flat(positions, n, _INTS, "positions")
-        d = _PACK_ROTARY(_count(rotary, "rotary"), _count(heads, "heads"), _count(values // heads, "values of a head"),
-                         _type_codes[positions.dtype] == 4, *self._rows(x, shape, "x"), 0, *self._rows(y, shape, "y"), 0, p)
+        d = _PACK_ROTARY(rotary, heads, values // heads, _type_codes[positions.dtype] == 4, *self._rows(x, shape, "x"), 0,
+                         *self._rows(y, shape, "y"), 0, p)
         rc = lib().gm_rotary(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_rotary")
 
-    def _cache(self, k_cache, v_cache):
+    def _cache(self, k, v):
         """The fields of a gm_cache, of two tensors [pages, kv_heads, page_size, head_dim] of the same strides."""
-        shape, strides = k_cache.shape, k_cache.stride()
-        if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides or v_cache.dtype != k_cache.dtype:
+        shape, strides, dtype = k.shape, k.stride(), k.dtype
+        if len(shape) != 4 or v.shape != shape or v.stride() != strides or v.dtype != dtype:
             raise ValueError("k_cache and v_cache: [pages, kv_heads, page_size, head_dim] of one type and the same strides")
-        if strides[3] != 1 and shape[3] > 1:
-            raise ValueError("k_cache: the values of a head are not neighbours")
-        if k_cache.get_device() != self.adapter or v_cache.get_device() != self.adapter:
+        code = _type_codes.get(dtype)
+        if code not in _ROW_TYPES:
+            code = _type(k, _ROW_TYPES, "k_cache")
+        if k.get_device() != self.adapter or v.get_device() != self.adapter:
             raise ValueError("k_cache and v_cache: not on the engine's GPU")
         pages, heads, size, dim = shape
-        if max(shape) > 0xffffffff:
+        page, head, token, step = strides
+        if step != 1 and dim > 1:
+            raise ValueError("k_cache: the values of a head are not neighbours")
+        if max(shape) > _MOST:
             raise ValueError("k_cache: not 32-bit counts")
-        return (k_cache.data_ptr(), v_cache.data_ptr(), _type(k_cache, _ROW_TYPES, "k_cache"), pages, size, heads, dim, 0,
-                strides[0], strides[1], strides[2])
+        return k.data_ptr(), v.data_ptr(), code, pages, size, heads, dim, 0, page, head, token
 
     def cache_append(self, k, v, k_cache, v_cache, slots, rotary: int | None = None, positions=None, q=None, q_out=None,
                      stream: int | None = None):
@@ -518,27 +527,34 @@ class Engine:
         negative: skipped) of a cache [pages, kv_heads, page_size, head_dim], the keys turned by their positions; with q
         (rows of any number of heads) also q_out = q turned."""
         c = self._cache(k_cache, v_cache)
-        n, dim = k.shape[0], c[6]
-        _count(n, "rows of k")
+        n, dim, rows = k.shape[0], c[6], self._rows
         shape = (n, c[5] * dim)
         s = self._flat(slots, n, _INTS, "slots")
         p = wide = heads = 0
-        if rotary is not None:
+        if rotary is None:
+            rotary = NO_ROTARY
+        else:
             if positions is None:
                 raise ValueError("a rotary without positions")
             p = self._flat(positions, n, _INTS, "positions")
             wide = _type_codes[positions.dtype] == 4
-        if (q is None) != (q_out is None):
-            raise ValueError("q and q_out go together")
+            if rotary == NO_ROTARY:
+                raise ValueError(f"no rotary {rotary}")
         qr = qo = _NO_ROWS
         if q is not None:
+            if q_out is None:
+                raise ValueError("q without q_out")
             values = q.shape[1]
             if not dim or not values or values % dim:
                 raise ValueError(f"q: {values} values are not heads of {dim}")
-            heads = _count(values // dim, "heads of q")
-            qr, qo = self._rows(q, (n, values), "q"), self._rows(q_out, (n, values), "q_out")
-        d = _PACK_APPEND(*c, NO_ROTARY if rotary is None else _count(rotary, "rotary"), heads, _type_codes[slots.dtype] == 4, wide,
-                         *self._rows(k, shape, "k"), 0, *self._rows(v, shape, "v"), 0, *qr, 0, *qo, 0, s, p)
+            heads = values // dim
+            qr, qo = rows(q, (n, values), "q"), rows(q_out, (n, values), "q_out")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if not (0 <= rotary <= _MOST and n <= _MOST and heads <= _MOST):
+            raise ValueError("rotary, rows or heads: not 32-bit counts")
+        d = _PACK_APPEND(*c, rotary, heads, _type_codes[slots.dtype] == 4, wide, *rows(k, shape, "k"), 0, *rows(v, shape, "v"), 0,
+                         *qr, 0, *qo, 0, s, p)
         rc = lib().gm_cache_append(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_cache_append")
@@ -556,13 +572,13 @@ class Engine:
         every token sees all keys; a window limits it to the last `window` up to its own. scale: 1 / sqrt(head_dim).
         workspace: a uint8 tensor of attention_workspace() bytes, not shared with calls that may overlap."""
         c = self._cache(k_cache, v_cache)
-        n, values = q.shape
-        _count(n, "rows of q")
-        dim = c[6]
+        shape, dim = q.shape, c[6]
+        n, values = shape
         if not dim or not values or values % dim:
             raise ValueError(f"q: {values} values are not heads of {dim}")
         sequences, width = table.shape
-        _type(table, _INT32, "table")
+        if _type_codes.get(table.dtype) != 3:
+            _type(table, _INT32, "table")
         if table.get_device() != self.adapter:
             raise ValueError("table: not on the engine's GPU")
         row, step = table.stride()
@@ -581,11 +597,11 @@ class Engine:
         if workspace is not None:
             ws_bytes = workspace.numel()
             ws = self._flat(workspace, ws_bytes, _UINT8, "workspace")
-        shape = (n, values)
-        d = _PACK_ATTENTION(*c, *self._rows(q, shape, "q"), 0, *self._rows(out, shape, "out"), 0, _count(values // dim, "heads"),
-                            _count(sequences, "sequences"), _count(longest, "longest"), causal, _count(window, "window"),
-                            dim ** -0.5 if scale is None else scale, table.data_ptr(), row, lp, sp, _count(width, "table"), 0,
-                            ws, ws_bytes)
+        if not (n <= _MOST and values <= _MOST and sequences <= _MOST and width <= _MOST and 0 <= longest <= _MOST and 0 <= window <= _MOST):
+            raise ValueError("tokens, heads, sequences, longest, window or table: not 32-bit counts")
+        rows = self._rows
+        d = _PACK_ATTENTION(*c, *rows(q, shape, "q"), 0, *rows(out, shape, "out"), 0, values // dim, sequences, longest, causal, window,
+                            dim ** -0.5 if scale is None else scale, table.data_ptr(), row, lp, sp, width, 0, ws, ws_bytes)
         rc = lib().gm_attention(self._h, d, n, self._stream() if stream is None else stream)
         if rc:
             self._check(rc, "gm_attention")

@@ -101,14 +101,14 @@ class AttentionOps {
         c.set(35, kv_heads);
         c.set(36, n);
         const uint32_t units = std::max((pairs + 7) / 8 + (D - 2 * pairs + 15) / 16, (D + 15) / 16);
-        // Heads of a thread, which form its angles once: as many as leave 2^16 threads, at most 8.
-        uint32_t per = 1;
-        while (per < 8 && per * 2 <= all && (uint64_t)n * ((all + 2 * per - 1) / (2 * per)) * units >= 1u << 16) per *= 2;
-        const uint32_t groups = (all + per - 1) / per, at_once = 256 / units;
-        c.set(42, per);
-        c.set(43, groups);
-        c.set(44, units);
-        const uint64_t blocks = ((uint64_t)n * groups + at_once - 1) / at_once;
+        // A group's 256 threads take at_once heads together, two a thread and turn. Of few tokens a group takes one turn of a token,
+        // so that all are on their way at once; of many (256 compute units hold eight groups each) up to eight turns of it.
+        const uint32_t at_once = 256 / units, all_turns = (all + 2 * at_once - 1) / (2 * at_once);
+        const uint32_t turns = (uint64_t)n * all_turns > 2048 ? std::min(all_turns, 8u) : 1u, sharers = (all_turns + turns - 1) / turns;
+        c.set(42, sharers);
+        c.set(43, units);
+        c.set(44, turns);
+        const uint64_t blocks = (uint64_t)n * sharers;
         l.kernel = x.type == GM_F32 ? "rotary_f" : x.type == GM_BF16 ? "rotary_b" : "rotary_h";
         l.x = (uint32_t)std::min<uint64_t>(blocks, 65535);
         l.y = (uint32_t)((blocks + 65534) / 65535);

@@ -235,12 +235,11 @@ def test_rotary_grids(shim, pairs, dim):
                 rc, why, out = call(shim.plan_rotary, rotary(heads=heads, head_dim=dim), n, pairs)
             assert rc == 0, why
             x, y, w = out[0], out[1], out[4:]
-            per, groups, units = w[42], w[43], w[44]
-            assert 1 <= x <= 65535 and 1 <= y <= 65535 and 1 <= per <= 8 and units <= 256
-            assert groups * per >= heads + 2 * kv > (groups - 1) * per
-            turning = -(-pairs // 8)
-            assert units >= turning + -(-(dim - 2 * pairs) // 16) and units * 16 >= dim
-            assert x * y * (256 // units) >= n * groups
+            sharers, units, turns = w[42], w[43], w[44]
+            assert 1 <= x <= 65535 and 1 <= y <= 65535
+            assert units >= -(-pairs // 8) + -(-(dim - 2 * pairs) // 16) and units * 16 >= dim
+            assert units <= 256 and sharers * turns * 2 * (256 // units) >= heads + 2 * kv
+            assert x * y >= n * sharers
 
 
 # ---- attention ----
