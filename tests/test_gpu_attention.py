@@ -428,6 +428,92 @@ def test_offsets_past_32_bits(eng, type, counts):
     b.check()
 
 
+@pytest.mark.parametrize("counts", [[40, 1], [3, 20]], ids=str)
+def test_wide_cache_faults(eng, counts):
+    """Pages outside the cache, and keys and values that are not finite, in a cache that 32 bits do not span."""
+    size, dim, kv, pages = 16, 128, 2, 7
+    stride = (1 << 29) + 4096
+    k_all = torch.zeros(stride * pages, dtype=torch.bfloat16, device="cuda")
+    kc = k_all.as_strided((pages, kv, size, dim), (stride, size * dim, dim, 1))
+    vc = k_all[size * kv * dim:].as_strided((pages, kv, size, dim), (stride, size * dim, dim, 1))
+    b = Batch(eng, "bf16", 4, kv, dim, size, counts, [75, 30], seed=25, spare=0)
+    kc.copy_(b.kc)
+    vc.copy_(b.vc)
+    b.kc, b.vc = kc, vc
+    b.table[0, 1] = pages
+    vc[int(b.table[0, 2]), 1, 3, 5] = float("nan")
+    vc[int(b.table[1, 1]), 0, 13, 100] = float("-inf")  # the last token's
+    kc[int(b.table[1, 1]), 1, 13, 9] = float("nan")
+    for kw in (dict(), dict(window=20), dict(causal=False)):
+        print(f"wide cache {counts} {kw}", flush=True)
+        b.out.fill_(7.0)
+        b.run(**kw)
+        b.check(**kw)
+
+
+@pytest.mark.parametrize("dim", [8, 64, 136, 256])
+@pytest.mark.parametrize("counts,lengths", [([150, 70], [400, 1300]), ([20, 2], [65, 64])])
+def test_not_finite_in_tiles(eng, dim, counts, lengths):
+    """Values that are not finite in tiles that all rows see whole, in split ones, and next to the mask's edge."""
+    b = Batch(eng, "f16", 4, 2, dim, 48, counts, lengths, seed=26)
+    for s, length in enumerate(lengths):
+        at = lambda j: (int(b.table[s, j // 48]), slice(None), j % 48)  # noqa: E731
+        b.vc[at(length // 3)][0, dim - 1] = float("inf")
+        b.vc[at(length - counts[s])][1, 0] = float("nan")
+        b.vc[at(length - 1)][1, dim // 2] = float("-inf")
+    for kw in (dict(), dict(window=30), dict(causal=False)):
+        print(f"not finite in tiles {dim} {counts} {kw}", flush=True)
+        b.out.fill_(7.0)
+        b.run(**kw)
+        b.check(**kw)
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("group,counts", [(1, [16, 1, 15]), (1, [17, 16, 2]), (4, [4, 3]), (4, [5, 4]), (3, [43, 42]), (16, [8, 1]), (20, [1, 2])])
+def test_attention_around_tiles(eng, type, group, counts):
+    """Rows and keys around the sizes of tiles and around what a single launch takes."""
+    for first in (63, 64, 65, 255, 257, 1023, 1025, 2049):
+        lengths = [first] + [max(n, first // 2) for n in counts[1:]]
+        print(f"around {type} {group} {counts} {lengths}", flush=True)
+        b = Batch(eng, type, group, 1, 32, 64, counts, lengths, seed=first)
+        b.run()
+        b.check()
+
+
+@pytest.mark.parametrize("sequences", [512, 1024, 1025])
+def test_attention_entries(eng, sequences):
+    """As many tiles of rows as a group finds by itself, and one more; sequences of few rows among them."""
+    rng = np.random.default_rng(67)
+    counts = [int(n) for n in rng.choice([0, 1, 2, 9, 33], sequences)]
+    lengths = [int(rng.integers(max(1, n), 200)) for n in counts]
+    b = Batch(eng, "bf16", 2, 1, 16, 16, counts, lengths, seed=27)
+    print(f"entries {sequences}", flush=True)
+    b.run()
+    b.check()
+
+
+def test_graphs_of_tiles(eng):
+    """Captured calls of split tiles and of a list of units, one workspace; lengths change between replays."""
+    batches = [Batch(eng, "bf16", 8, 2, 64, 16, [90, 1, 20], [3000, 2000, 100], seed=28),
+               Batch(eng, "bf16", 8, 2, 64, 16, [18] * 520 + [0] * 520, [40] * 520 + [9] * 520, seed=29)]
+    batches[1].ws = batches[0].ws
+    graphs = []
+    for b in batches:
+        b.run()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            b.run()
+    for turn in range(3):
+        print(f"turn {turn}", flush=True)
+        for b, g in zip(batches, graphs):
+            b.out.fill_(7.0)
+            b.q.mul_(-1)
+            b.lengths.sub_(turn)
+            g.replay()
+        for b in batches:
+            b.check()
+
+
 # ---- together -------------------------------------------------------------------------------------
 
 class Decoder:
