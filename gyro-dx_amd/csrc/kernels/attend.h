@@ -344,7 +344,7 @@ __device__ __forceinline__ void at_share(const GdArgs &a, AtShare &s, uint32_t w
                 rows[k] = 1u;
             }
         }
-        own += keys[k];  // at most 2^24 each, 64 lanes' 4 in 32 bits
+        own += min(keys[k], 0xffffffu);  // of 2^24 at most; 64 lanes' 4 in 32 bits
     }
     __syncthreads();
     const uint32_t of_wave = (uint32_t)__builtin_amdgcn_readlane((int)gd_wave_scan_u32(own), 63);

@@ -132,10 +132,14 @@ template <typename F>
 __device__ __forceinline__ void aj_tiles(const GdArgs &a, uint32_t group, uint32_t groups, uint32_t splits, F entry) {
     const uint32_t KVH = a.c[31], D = a.c[30], wide = D > 128u ? 64u : D > 64u ? 32u : 16u, at_once = AJ_THREADS / wide;
     const uint64_t step = at_part_bytes(a, AT_ROWS) * KVH;
-    // A group's turn: at_once neighbouring rows of a split tile and head, which AT_ROWS is a multiple of.
-    const uint64_t turns = (uint64_t)splits * KVH * (AT_ROWS / at_once);
+    // A group's turn: at_once neighbouring rows of a split tile and head, which AT_ROWS is a multiple of, or fewer, down to one,
+    // while that leaves every turn a group of its own (20 rows of 16000 keys and two heads: 40 us with
+    // at_once rows a turn, 20 with one).
+    uint32_t own = at_once;
+    while (own > 1u && (uint64_t)splits * KVH * (AT_ROWS / own) * 2u <= groups) own >>= 1;
+    const uint64_t turns = (uint64_t)splits * KVH * (AT_ROWS / own);
     for (uint64_t turn = group; turn < turns; turn += groups) {
-        const uint32_t rest = (uint32_t)(turn / (AT_ROWS / at_once)), row0 = (uint32_t)(turn % (AT_ROWS / at_once)) * at_once, index = rest / KVH;
+        const uint32_t rest = (uint32_t)(turn / (AT_ROWS / own)), row0 = (uint32_t)(turn % (AT_ROWS / own)) * own, index = rest / KVH;
         AtItem o;
         uint32_t tile, slot, parts;
         if (!entry(index, o, tile, slot, parts)) continue;
@@ -143,9 +147,9 @@ __device__ __forceinline__ void aj_tiles(const GdArgs &a, uint32_t group, uint32
         const uint64_t at = at_slot(a, slot, o.head);
         if (parts <= 16u) {
             const uint32_t r = row0 + threadIdx.x / wide;
-            if (tile * AT_ROWS + r < o.rows) aj_by_lanes(a, at, step, parts, r, 4u * (threadIdx.x % wide), aj_out(a, o, tile * AT_ROWS + r));
+            if (r < row0 + own && tile * AT_ROWS + r < o.rows) aj_by_lanes(a, at, step, parts, r, 4u * (threadIdx.x % wide), aj_out(a, o, tile * AT_ROWS + r));
         } else {
-            for (uint32_t r = row0; r < row0 + at_once && tile * AT_ROWS + r < o.rows; ++r) {
+            for (uint32_t r = row0; r < row0 + own && tile * AT_ROWS + r < o.rows; ++r) {
                 aj_by_group<AT_ROWS>(a, at, step, parts, r, aj_out(a, o, tile * AT_ROWS + r));
                 __syncthreads();
             }

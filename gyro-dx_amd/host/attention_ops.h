@@ -233,8 +233,13 @@ class AttentionOps {
         const bool wide = d.cache.type == GM_F32;
         const uint32_t group = H / G;
         const uint64_t rows = (uint64_t)d.longest * group;
-        // Sequences of more than 16 rows go to attend_tile, the others, and all of fp32, to the kernels of few rows.
-        const bool many = !wide && rows > kFewRows, few = !many || d.starts;
+        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile where these have more
+        // keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a sequence's keys once for
+        // every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000 keys 18 against 24, of 16000 32 against 31; 256
+        // rows of 2000 24 against 27, of 4000 40 against 29).
+        const uint64_t row_tiles = (rows + kFewRows - 1) / kFewRows;
+        const unsigned __int128 pairs = (unsigned __int128)row_tiles * d.sequences * G;
+        const bool many = !wide && rows > kFewRows && pairs * capacity > kFewKeys, few = !many || d.starts;
         Constants &c = l.c;
         c.set(0, d.q.data);
         c.set64(2, d.q.stride);
@@ -274,21 +279,24 @@ class AttentionOps {
         uint64_t need = 0, join = 0, groups = 0;
         bool short_keys = false;
         if (few) {
-            const uint32_t keys = wide && D > 64 ? 16 : 32, tiles = wide ? (uint32_t)((rows + kFewRows - 1) / kFewRows) : 1;
+            const uint32_t keys = wide && D > 64 ? 16 : 32, tiles = many ? 1 : (uint32_t)row_tiles;
             const uint64_t entries = (uint64_t)d.sequences * tiles;
             require(entries * G < 1u << 31, "gm_attention: too many sequences");
             groups = entries * G;
             c.set(42, tiles);
             c.set(44, keys);
-            // Split where there may be keys for it, and entries enough to fill the GPU are not there anyway. Keys that one
-            // group takes may be taken by one of eight waves.
-            const uint32_t resident = (wide ? 256 : kResident[size]) * (d.sequences > 1 ? kPerGroup : 1);
-            short_keys = capacity <= (wide ? 2 : 1) * kAlone;
+            // Where one group's waves (eight, but for heads above 128 values) take all keys of 16 rows as fast as several and a
+            // join, by the pairs of row tiles and cache heads that there are to fill the GPU.
+            const uint64_t few_pairs = entries * G;
+            const uint32_t alone = wide ? (few_pairs >= kWidePairs ? 4096 : 512)
+                                        : (uint32_t)std::min<uint64_t>(D > 128 ? 1024 : 2048, std::max<uint64_t>(896, 16 * few_pairs));
+            short_keys = capacity <= alone;
+            const uint32_t resident = (wide ? 256 : kResident[size]) * (!wide && few_pairs >= kResident[size] / 2 ? kPerGroup : 1);
             if (entries <= kEntries && entries * G < 2 * resident && !short_keys) {
                 groups += resident;
                 c.set(41, resident);
-                c.set(45, kLeast / keys);
-                c.set(57, (wide ? 2 * kAlone : kLeast) / keys);
+                c.set(45, (wide ? 2 * kLeast : kLeast) / keys);
+                c.set(57, (wide ? alone : kLeast) / keys);
                 need = plan_at(D);
                 const uint32_t most = (uint32_t)std::min<uint64_t>(kFewRows, rows);
                 c.set(56, most);
@@ -307,7 +315,7 @@ class AttentionOps {
             c.set64(50, (uint64_t)(uintptr_t)d.workspace + slots_at(D));
             c.set(54, kSlots / G);
             c.set(55, D > 128 ? 32u : 64u);
-            c.set(58, kTileLeast);
+            c.set(58, entries * G >= kTilePairs ? 16u : 4u);
             if (entries <= kEntries) {
                 c.set(28, (uint32_t)tiles);
             } else {
@@ -332,10 +340,22 @@ class AttentionOps {
         if (join) l.add("attend_join", join);
         return l;
     }
-    // Few rows' keys: groups that the GPU holds, by the heads' size; parts for each of them where sequences differ; keys that
-    // make a part; and those that one group takes without a join.
-    static constexpr uint32_t kResident[3] = {512, 512, 256}, kPerGroup = 2, kLeast = 256, kAlone = 1024;
-    static constexpr uint32_t kTileLeast = 4;  // tiles that make a part of many rows' keys
+    // Few rows' keys: groups that the GPU holds, by the heads' size, and parts for each of them where row tiles and heads (half as many
+    // or more) differ in keys (us: 64 sequences of 91 to 8192 keys 110 with one part, 98 with two, of 4000 each 198 and 207; 4 of
+    // 4000 each 19.5 and 23).
+    static constexpr uint32_t kResident[3] = {512, 512, 256}, kPerGroup = 2;
+    // Keys that make a part (twice as many in fp32). 1500 keys of one sequence: 11.1 us with 128, 12.0 with 256, 14.0 with 512.
+    static constexpr uint32_t kLeast = 128;
+    // Keys of one group alone against several and a join, us, replayed (outside a graph the second launch costs its caller 2 more),
+    // 8 heads of 128 values: one sequence of 640 keys 10.9 and 10.8, of 1024
+    // 14.0 and 10.9; 8 of 1024 15.1 and 15.4, of 2048 24.6 and 19.5; 16 of 2048 26 and 31, of 4000 71 and 59; 32 of 2048 42 and 49.
+    // Heads of 256, 16 of 1024 31 and 38, of 1536 55 and 52. fp32: 8 tiles of 512 keys 11.9 and 13.0, of 1024 18 and 13; 112 of 1024 20
+    // and 27, of 4096 58 and 65.
+    static constexpr uint32_t kWidePairs = 96;
+    static constexpr uint32_t kFewKeys = 1u << 18;
+    // Many rows: tiles of rows and heads from which on a part has 16 tiles of keys at least, otherwise 4 (us: 1023 tokens of 32 heads
+    // alone, 256 such tiles, 44.5 with 4 and 34.6 with 16; 64 tokens of 4096 keys, 16 tiles, 28.4 and 36.5).
+    static constexpr uint32_t kTilePairs = 128;
 };
 
 }  // namespace gyro

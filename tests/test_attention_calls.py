@@ -266,8 +266,8 @@ def test_attention_refusals(shim):
                   attention(table_width=0), attention(table_width=1 << 27), attention(table_stride=1 << 41), attention(causal=0, window=4),
                   attention(scale=0.0), attention(scale=-1.0), attention(scale=float("nan")), attention(scale=float("inf")),
                   attention(table_width=1000, workspace=None), attention(table_width=1000, workspace=A + 128),
-                  attention(table_width=1000, workspace_bytes=4096), attention(heads=64, table_width=1, workspace=None),
-                  attention(heads=64, table_width=1, workspace_bytes=1 << 20), attention(cache=cache(pages=0)), attention(cache=cache(type=3)),
+                  attention(table_width=1000, workspace_bytes=4096), attention(heads=64, table_width=5000, workspace=None),
+                  attention(heads=64, table_width=5000, workspace_bytes=1 << 20), attention(cache=cache(pages=0)), attention(cache=cache(type=3)),
                   attention(cache=cache(pages=1 << 27)), (attention(sequences=1 << 28, longest=1), 1 << 28)])
     assert call(shim.plan_attention, attention(), 0)[2][0] == 0
 
@@ -293,9 +293,12 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
             names, w = names.split(), out[9:]
             grids = {name: out[1 + 2 * i] * out[2 + 2 * i] for i, name in enumerate(names)}
             assert len(names) == out[0] and all(1 <= v <= 65535 for v in out[1:1 + 2 * out[0]])
-            many = type and longest * group > 16
+            pairs = -(-longest * group // 16) * sequences * kv
+            many = bool(type) and longest * group > 16 and pairs * width * 16 > 1 << 18
             size = 64 if dim <= 64 else 128 if dim <= 128 else 256
-            build = "f32_" if not type else ("short_" if width * 16 <= 1024 and size < 256 else "few_") + "?bh"[type]
+            short = type and size < 256 and f"attend_short_{'?bh'[type]}{size}" in names
+            build = "f32_" if not type else ("short_" if short else "few_") + "?bh"[type]
+            assert not short or width * 16 <= min(2048, max(896, 16 * (sequences * kv if many else pairs)))
             few = f"attend_{build}{size}"
             tile = "attend_tile_%s%d" % ("?bh"[type], size)
             listed = many and sequences * -(-longest * group // 128) > 1024
@@ -306,7 +309,7 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
             if few in names:
                 split, tiles, keys, least = w[41], w[42], w[44], w[45]
                 assert keys == (16 if not type and dim > 64 else 32)
-                assert tiles == 1 if type else tiles * 16 >= longest * group > (tiles - 1) * 16
+                assert tiles == 1 if many else tiles * 16 >= longest * group > (tiles - 1) * 16
                 # A group for every entry and head, and for what splits add: of each entry less than its share of `split`.
                 assert split in (0, 256, 512, 1024) and grids[few] >= sequences * tiles * kv + split
                 assert not split or (sequences * tiles <= 1024 and width * 16 > w[57] * keys and least >= 1)

@@ -149,13 +149,16 @@ def test_append_no_tokens(eng):
 # ---- attention -----------------------------------------------------------------------------------
 
 class Batch:
-    """Sequences of counts[b] tokens over lengths[b] cached ones, on pages in any order."""
+    """Sequences of counts[b] tokens over lengths[b] cached ones, on pages in any order. The table spans `reach` keys at least:
+    calls choose their kernels by that."""
+
+    reach = 0
 
     def __init__(self, eng, dtype, heads, kv_heads, dim, size, counts, lengths, order="head", pad=0, shift=0, seed=0, spare=2, big=1.0):
         g = torch.Generator().manual_seed(seed + 17)
         self.eng, self.dtype, self.heads, self.counts = eng, DTYPES[dtype], heads, counts
         per = [-(-max(l, 0) // size) for l in lengths]
-        width, pages = max(1, *per) + 1, max(1, sum(per)) + spare
+        width, pages = max(1, *per, -(-self.reach // size)) + 1, max(1, sum(per)) + spare
         self.kc, self.vc = ref.make_cache(pages, kv_heads, size, dim, self.dtype, order, seed=seed)
         self.kc *= big
         table = torch.randint(0, pages, (len(counts), width), generator=g, dtype=torch.int32)
@@ -203,6 +206,13 @@ class Batch:
         assert op_reference.untouched(self.buf, self.out, 7.0)
 
 
+@pytest.fixture(params=[0, 1 << 18], ids=["narrow", "wide"])
+def reach(request):
+    Batch.reach = request.param
+    yield
+    Batch.reach = 0
+
+
 SHAPES = [  # heads, kv_heads, dim, page, counts, lengths
     (4, 4, 64, 16, [1], [1]),
     (8, 2, 128, 16, [1, 1, 1], [777, 31, 33]),
@@ -217,6 +227,7 @@ SHAPES = [  # heads, kv_heads, dim, page, counts, lengths
 ]
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("order", ["head", "token"])
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s[:4])))
@@ -235,6 +246,7 @@ def test_attention(eng, shape, type, order):
             b.check(**kw)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 def test_attention_empty_rows(eng, type):
     """Sequences without tokens, without keys, with fewer keys than tokens, lengths below zero and past the table."""
@@ -248,6 +260,7 @@ def test_attention_empty_rows(eng, type):
         b.check(**kw)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("counts,lengths", [([6, 1, 20], [200, 97, 20]), ([150], [400])])
 def test_attention_not_finite(eng, type, counts, lengths):
@@ -285,6 +298,7 @@ def test_attention_not_finite(eng, type, counts, lengths):
     b.check()
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f32"])
 def test_attention_only_minus_infinity(eng, type):
     """Scores of -infinity alone leave zeros, like no keys."""
@@ -296,6 +310,7 @@ def test_attention_only_minus_infinity(eng, type):
     assert (b.out[:b.n] == 0).all()
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("counts,lengths", [([1, 4], [300, 90]), ([100], [260])])
 def test_attention_bad_pages(eng, type, counts, lengths):
@@ -315,6 +330,7 @@ def test_attention_bad_pages(eng, type, counts, lengths):
     assert (b.out[:b.n] == 0).all()
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 def test_attention_large_scores(eng, type):
     """Scores of hundreds, whose weights fall to one key, rise late and fall again."""
@@ -324,6 +340,7 @@ def test_attention_large_scores(eng, type):
     b.check(scale=1.0, norm=False)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f32"])
 def test_attention_in_place(eng, type):
     """out at q's rows; the same results as apart."""
@@ -350,6 +367,7 @@ def test_attention_long(eng):
         assert all(torch.equal(first, x) for x in again)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type,dim", [("bf16", 128), ("f16", 64), ("bf16", 256), ("f16", 200)])
 def test_attention_split_tiles(eng, type, dim):
     """Rows of one or a few tiles whose keys many groups share, beside sequences of few rows; the same results every time."""
@@ -403,6 +421,7 @@ def test_attention_many_sequences(eng):
     b.check()
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16"])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 1]])
 def test_offsets_past_32_bits(eng, type, counts):
@@ -428,6 +447,7 @@ def test_offsets_past_32_bits(eng, type, counts):
     b.check()
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("counts", [[40, 1], [3, 20]], ids=str)
 def test_wide_cache_faults(eng, counts):
     """Pages outside the cache, and keys and values that are not finite, in a cache that 32 bits do not span."""
@@ -451,6 +471,7 @@ def test_wide_cache_faults(eng, counts):
         b.check(**kw)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("dim", [8, 64, 136, 256])
 @pytest.mark.parametrize("counts,lengths", [([150, 70], [400, 1300]), ([20, 2], [65, 64])])
 def test_not_finite_in_tiles(eng, dim, counts, lengths):
@@ -468,6 +489,7 @@ def test_not_finite_in_tiles(eng, dim, counts, lengths):
         b.check(**kw)
 
 
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f32"])
 @pytest.mark.parametrize("group,counts", [(1, [16, 1, 15]), (1, [17, 16, 2]), (4, [4, 3]), (4, [5, 4]), (3, [43, 42]), (16, [8, 1]), (20, [1, 2])])
 def test_attention_around_tiles(eng, type, group, counts):
