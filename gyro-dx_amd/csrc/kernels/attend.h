@@ -2,8 +2,8 @@
 // cache's heads, `group` = heads / kv_heads queries' heads each, are its rows: row r is head r % group of token r / group, so
 // that a page read once serves them all.
 //
-// Sequences of few rows (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and cache head and a
-// part of its keys, and finds out by itself which (af_share). Those of more (attend_tile.h): a group takes a unit, a tile of 128
+// Sequences of few rows or short ones (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and cache head and a
+// part of its keys, and finds out by itself which (af_share). The others (attend_tile.h): a group takes a unit, a tile of 128
 // rows and a run of its keys, of every head; of up to 1024 tiles it finds out by itself which (at_share), of more attend_plan
 // makes a list. Where keys are split, attend_join puts the parts together.
 //

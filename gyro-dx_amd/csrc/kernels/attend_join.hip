@@ -1,5 +1,6 @@
 // Joins the parts of rows whose keys several groups shared (attend.h). The first groups take the few rows' split entries, a
-// group a row, as these may have hundreds of parts; the others the many rows' split tiles, in turn.
+// group a row, as these may have hundreds of parts; the others the many rows' split tiles, in turn. Bound by latency (which were split,
+// statistics, parts): 5 to 10 us, of which the launch is 2.
 #include "attend.h"
 
 // Row r of a sequence and head in out.

@@ -1,5 +1,6 @@
 // Cuts the sequences of many rows into units for attend_tile (attend.h), one group for the launch: the tiles of 128 rows, whose
-// keys are split where one has more tiles of them than its share (at_fair), the units of most tiles first. Units of one size come in any order, which changes no result.
+// keys are split where one has more tiles of them than its share (at_fair), the units of most tiles first. Units of one size
+// come in any order, which changes no result.
 #include "attend.h"
 
 #define AP_CLASSES 32u

@@ -1,5 +1,5 @@
 // Attention of many rows (attend.h), 16-bit types: a group of four waves takes 128 rows, 32 a wave, and a run of tiles of 64 or 32
-// keys (attend_plan says which), which go from memory straight to LDS, two buffers of keys and of values in turn.
+// keys (its unit), which go from memory straight to LDS, two buffers of keys and of values in turn.
 //
 // Scores are K Q^T by v_mfma_f32_32x32x16: a lane holds half the keys of one row, the other half is lane ^ 32's, so the
 // running maximum needs one exchange per tile, the sum none until the end, and the weights are the second product's operand
@@ -10,7 +10,12 @@
 // precise.
 //
 // LDS is filled 1 KB an instruction in the order of lanes, so rows cannot be padded; instead their 16-byte pieces are swapped
-// by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v).
+// by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v; no conflict was counted).
+//
+// 4096 tokens of 32 heads over 8 of 128 values, causal: 159 us with the join (866 TFLOP/s; a large library product reaches 1131). Matrix
+// instructions fill 40% of all cycles and vector instructions 44%, at two waves a SIMD, which 248 registers allow. More buffers and earlier reads
+// of LDS gained nothing, a wave's higher priority around its products 6%, 32-bit offsets into the cache, groups that
+// find their units without a list and even rounds 5%. 128 rows halve the reads of 64; 256 would leave one wave a SIMD.
 #pragma once
 #include "attend16.h"
 #include <type_traits>
