@@ -15,7 +15,7 @@
 // Constants: 0 q 2 q stride 4 q_out 6 q_out stride 8 k 10 k stride 12 v 14 v stride 16 cache k 18 cache v 20 page stride
 // 22 head stride 24 token stride (bytes) 26 frequencies (0: nothing turns) 28 positions 30 slots 32 D 33 pairs 34 query heads
 // 35 kv heads (0: no cache) 36 tokens 37 types (q_out | cache << 4) 38 flags (1 interleaved, 2 positions in 64 bits, 4 slots
-// in 64 bits) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two heads of
+// in 64 bits, 8 q in place) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two heads of
 // a thread
 #pragma once
 #include "rows.h"
@@ -38,8 +38,8 @@ __device__ __forceinline__ void ro_turn(uint64_t fraction, float scale, float &c
     s = scale * (q & 2u ? -b : b);
 }
 
-// Values i .. i + m - 1 of a head, m <= 8. FULL: every m is 8, and the values stay as they are in memory until they are used, so that
-// loads follow each other without a wait. Otherwise those past m are zeros.
+// Values i .. i + 7 of a head. FULL: all of them are in it, and they stay as they are in memory until they are used, so that loads
+// follow each other without a wait; the last 8 - low are stored. Otherwise the first m <= 8 are there.
 template <uint32_t TYPE, bool FULL>
 struct RoEight {
     gd_u32x4 raw[TYPE == ROW_F32 ? 2 : 1];
@@ -64,8 +64,32 @@ struct RoEight {
             }
         }
     }
-    __device__ __forceinline__ void store(uint64_t head, uint32_t i, uint32_t m, uint32_t type) const { row_store8(head, i, i + (FULL ? 8u : m), type, v); }
+    __device__ __forceinline__ void store(uint64_t head, uint32_t i, uint32_t m, uint32_t low, uint32_t type) const {
+        if (!FULL || !low) return row_store8(head, i, i + (FULL ? 8u : m), type, v);
+#pragma unroll
+        for (uint32_t j = 1; j < 8; ++j)
+            if (j >= low) row_store(head, i + j, type, v[j]);
+    }
 };
+
+// Eight values from i on that are copied, as far as the head goes.
+template <bool FULL>
+__device__ __forceinline__ void ro_end(uint32_t D, uint32_t &i, uint32_t &m, uint32_t &low) {
+    if (FULL) {
+        const uint32_t at = min(i, D - 8u);
+        low = min(8u, i - at);
+        i = at;
+    } else {
+        m = i < D ? min(8u, D - i) : 0u;
+    }
+}
+
+// (fused in one way, wherever it stands)
+__device__ __forceinline__ void ro_pair(float &x, float &y, float c, float s) {
+    const float x1 = x;
+    x = fmaf(-y, s, x1 * c);
+    y = fmaf(y, c, x1 * s);
+}
 
 #define RO_TABLE 512u  // pairs of a head at most
 
@@ -80,22 +104,34 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
     const uint32_t at_once = 256u / units, own = threadIdx.x / units, u = threadIdx.x - own * units;
     const uint32_t head0 = (uint32_t)(id - of * sharers) * turns * 2u * at_once + own;
     const uint32_t turning = (pairs + 7u) / 8u;  // units of pairs; the others' values are copied
-    // The halves of a unit in a head that turns and in one that does not: their places and how many values of each there are.
-    uint32_t f1, f2, n1, n2;
+    // The halves of a unit in a head that turns and in one that does not: their places, and how many values of each there are. FULL: a
+    // half that would reach past the pairs or the head's end moves down to it, and begins to store at its own first value; pairs
+    // that two units turn need no such care but in place, as both have the same values.
+    uint32_t f1, f2, n1 = 8, n2 = 8, low1 = 0, low2 = 0, pair0 = 8u * u;
     if (u < turning) {
-        const uint32_t m = min(8u, pairs - 8u * u);
+        const uint32_t m = min(8u, pairs - pair0);
         const bool apart = !(flags & 1u);
-        f1 = apart ? 8u * u : 16u * u;
-        f2 = apart ? pairs + 8u * u : 16u * u + 8u;
-        n1 = apart ? m : min(8u, 2u * m);
-        n2 = apart ? m : 2u * m - n1;
+        if (FULL) {
+            pair0 -= 8u - m;
+            if (flags & 8u) {
+                low1 = apart ? 8u - m : min(8u, 16u - 2u * m);
+                low2 = apart ? 8u - m : max(8u, 16u - 2u * m) - 8u;
+            }
+        } else {
+            n1 = apart ? m : min(8u, 2u * m);
+            n2 = apart ? m : 2u * m - n1;
+        }
+        f1 = apart ? pair0 : 2u * pair0;
+        f2 = apart ? pairs + pair0 : 2u * pair0 + 8u;
     } else {
         f1 = 2u * pairs + 16u * (u - turning);
         f2 = f1 + 8u;
-        n1 = f1 < D ? min(8u, D - f1) : 0u;
-        n2 = f2 < D ? min(8u, D - f2) : 0u;
+        ro_end<FULL>(D, f1, n1, low1);
+        ro_end<FULL>(D, f2, n2, low2);
     }
-    const uint32_t v1 = 16u * u, v2 = v1 + 8u, mv1 = v1 < D ? min(8u, D - v1) : 0u, mv2 = v2 < D ? min(8u, D - v2) : 0u;
+    uint32_t v1 = 16u * u, v2 = v1 + 8u, mv1 = 8, mv2 = 8, vlow1 = 0, vlow2 = 0;
+    ro_end<FULL>(D, v1, mv1, vlow1);
+    ro_end<FULL>(D, v2, mv2, vlow2);
     const uint32_t to_q = types & 15u, to_cache = types >> 4;
 
     // Where the token's rows begin, and its place in the cache.
@@ -139,7 +175,7 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
         float c[8], s[8];  // of the thread's pairs (of a head's last ones the table's end is read again)
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
-            const uint32_t at = min(8u * u + j, RO_TABLE - 1u);
+            const uint32_t at = min(pair0 + j, RO_TABLE - 1u);
             c[j] = cosines[at];
             s[j] = sines[at];
         }
@@ -153,32 +189,25 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
                 if (flags & 1u) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float p1 = p[2 * j], q1 = q[2 * j];
-                        p[2 * j] = p1 * c[j] - p[2 * j + 1] * s[j];
-                        p[2 * j + 1] = p1 * s[j] + p[2 * j + 1] * c[j];
-                        q[2 * j] = q1 * c[4 + j] - q[2 * j + 1] * s[4 + j];
-                        q[2 * j + 1] = q1 * s[4 + j] + q[2 * j + 1] * c[4 + j];
+                        ro_pair(p[2 * j], p[2 * j + 1], c[j], s[j]);
+                        ro_pair(q[2 * j], q[2 * j + 1], c[4 + j], s[4 + j]);
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float p1 = p[j];
-                        p[j] = p1 * c[j] - q[j] * s[j];
-                        q[j] = p1 * s[j] + q[j] * c[j];
-                    }
+                    for (int j = 0; j < 8; ++j) ro_pair(p[j], q[j], c[j], s[j]);
                 }
             }
             const uint32_t to = query[i] ? to_q : to_cache;
-            first[i].store(y[i], value[i] ? v1 : f1, value[i] ? mv1 : n1, to);
-            second[i].store(y[i], value[i] ? v2 : f2, value[i] ? mv2 : n2, to);
+            first[i].store(y[i], value[i] ? v1 : f1, value[i] ? mv1 : n1, value[i] ? vlow1 : low1, to);
+            second[i].store(y[i], value[i] ? v2 : f2, value[i] ? mv2 : n2, value[i] ? vlow2 : low2, to);
         }
     }
 }
 
-// (full: whole units only)
+// (few pairs and small heads have no eight values to move down to)
 template <uint32_t TYPE>
 __device__ __forceinline__ void rotary_body(const GdArgs &a) {
     __shared__ __align__(16) float cosines[RO_TABLE], sines[RO_TABLE];
-    if (a.c[32] % 16u == 0 && a.c[33] % 8u == 0) rotary_rows<TYPE, true>(a, cosines, sines);
+    if (a.c[32] >= 8u && (!a.c[33] || a.c[33] >= 8u)) rotary_rows<TYPE, true>(a, cosines, sines);
     else rotary_rows<TYPE, false>(a, cosines, sines);
 }

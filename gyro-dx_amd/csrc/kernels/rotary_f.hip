@@ -1,3 +1,3 @@
 // Rotary positions and the cache's appending, rows of fp32 values (rotary.h).
 #include "rotary.h"
-GD_PIPELINE_NAMED(rotary_f, 256) { rotary_body<ROW_F32>(a); }
+GD_PIPELINE_NAMED_OCC(rotary_f, 256, 4) { rotary_body<ROW_F32>(a); }

@@ -1,3 +1,3 @@
 // Rotary positions and the cache's appending, rows of binary16 values (rotary.h).
 #include "rotary.h"
-GD_PIPELINE_NAMED(rotary_h, 256) { rotary_body<ROW_F16>(a); }
+GD_PIPELINE_NAMED_OCC(rotary_h, 256, 4) { rotary_body<ROW_F16>(a); }

@@ -125,7 +125,7 @@ class AttentionOps {
         turn(l, &r, &d.x, &d.y, d.heads, nullptr, nullptr, 0, d.head_dim, n);
         l.c.set(28, d.positions);
         l.c.set(37, d.y.type);
-        l.c.set(38, (r.layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u));
+        l.c.set(38, (r.layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u) | (d.x.data == d.y.data ? 8u : 0u));
         return l;
     }
 
@@ -176,7 +176,8 @@ class AttentionOps {
         if (r) c.set(28, d.positions);
         c.set(30, d.slots);
         c.set(37, (d.heads ? d.q_out.type : 0u) | d.cache.type << 4);
-        c.set(38, (r && r->layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u) | (d.slots_64 ? 4u : 0u));
+        c.set(38, (r && r->layout == GM_ROTARY_INTERLEAVED ? 1u : 0u) | (d.positions_64 ? 2u : 0u) | (d.slots_64 ? 4u : 0u) |
+                      (d.q.data == d.q_out.data ? 8u : 0u));
         c.set(40, d.cache.page_size);
         c.set(41, d.cache.pages * d.cache.page_size);
         return l;

@@ -64,6 +64,30 @@ def test_rotary(eng, layout, x, y):
         eng.release_rotary(index)
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_rotary_parts(eng, layout, type):
+    """Heads whose pairs, or what is behind them, are no whole eights; in place and apart alike."""
+    for n, H, D, R in ((3, 3, 20, 16), (6, 5, 24, 18), (2, 64, 8, 2), (9, 4, 72, 36), (40, 9, 200, 198), (1, 3, 9, 8), (5, 2, 1023, 1022),
+                       (70, 30, 250, 90), (2, 600, 120, 58), (11, 1, 16, 14)):
+        print(f"rotary parts {layout} {type}: {n} tokens, {H} heads of {D}, {R} turned", flush=True)
+        g = torch.Generator().manual_seed(n * D)
+        f, _ = frequencies(R)
+        index = eng.add_rotary(f, layout=layout)
+        x, _ = op_reference.wide_rows(torch.randn(n, H * D, generator=g), DTYPES[type], pad=1, shift=1)
+        p = positions_of(g, n, "near").cuda()
+        y, buf = op_reference.wide_rows(torch.zeros(n, H * D), DTYPES[type], pad=3, fill=7.0)
+        eng.rotary(index, x, p, y, heads=H, stream=stream())
+        torch.cuda.synchronize()
+        want, size = ref.rotary(x, H, p, f, layout, 1.0)
+        assert ((y.cpu().double() - want).abs() <= ref.rotary_bound(want, size, DTYPES[type])).all()
+        assert op_reference.untouched(buf, y, 7.0)
+        eng.rotary(index, x, p, x, heads=H, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(x, y)
+        eng.release_rotary(index)
+
+
 def test_rotary_far(eng):
     """Neighbouring positions far out turn by their distance: fp32 angles would not tell them apart."""
     f, _ = frequencies(64)
@@ -250,6 +274,7 @@ def test_attention(eng, shape, type, order):
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
 def test_attention_empty_rows(eng, type):
     """Sequences without tokens, without keys, with fewer keys than tokens, lengths below zero and past the table."""
+    Batch.reach = min(Batch.reach, 1 << 13)
     b = Batch(eng, type, 4, 2, 64, 16, [3, 0, 5, 2, 1, 40], [0, 50, 2, 37, 90, 17], seed=3)
     b.lengths[3] = -4
     b.lengths[4] = 1 << 30
@@ -383,7 +408,7 @@ def test_attention_split_tiles(eng, type, dim):
         assert torch.equal(first, b.out)
 
 
-@pytest.mark.parametrize("counts", [[700, 300, 20, 3, 40, 0, 130, 1, 90], [3, 200] * 20, [40] * 170 + [400]], ids=str)
+@pytest.mark.parametrize("counts", [[700, 300, 20, 3, 40, 0, 130, 1, 90], [3, 200] * 20, [40] * 170 + [400]], ids=["mixed", "alternating", "even"])
 def test_attention_many_split_tiles(eng, counts):
     """Split tiles among those that every wave of a group looks at, in every order; the same results every time."""
     rng = np.random.default_rng(63)
