@@ -12,7 +12,7 @@
 // LDS is filled 1 KB an instruction in the order of lanes, so rows cannot be padded; instead their 16-byte pieces are swapped
 // by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v; no conflict was counted).
 //
-// 4096 tokens of 32 heads over 8 of 128 values, causal: 159 us with the join (866 TFLOP/s; a large library product reaches 1131). Matrix
+// 4096 tokens of 32 heads over 8 of 128 values, causal: 156 us with the join (881 TFLOP/s; a large library product reaches 1131). Matrix
 // instructions fill 40% of all cycles and vector instructions 44%, at two waves a SIMD, which 248 registers allow. More buffers and earlier reads
 // of LDS gained nothing, a wave's higher priority around its products 6%, 32-bit offsets into the cache, groups that
 // find their units without a list and even rounds 5%. 128 rows halve the reads of 64; 256 would leave one wave a SIMD.

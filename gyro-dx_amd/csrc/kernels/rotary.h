@@ -2,21 +2,22 @@
 //   (y1, y2) = scale (x1 cos a - x2 sin a, x1 sin a + x2 cos a),  a = position * frequency of the pair
 // Rows of up to three kinds in one launch: queries (turned, to rows), keys (turned, to the cache's slots) and values
 // (as they are, to the slots). A group takes a token, or a part of one, forms its sines and cosines once, a pair a thread, and
-// turns its heads by them (one to eight tokens a group were timed alike): a thread takes units of 8 pairs (or 16 values that do not turn) of a head.
+// turns its heads by them; of many tokens a wave takes one, if its turns cover the heads. A thread takes units of 8 pairs (or 16 values
+// that do not turn) of a head.
 //
 // Angles: a frequency is a fraction of a turn in 64 bits, whole turns dropped; its product with the position modulo 2^64 is the
 // angle's fraction of a turn, exact but for the frequency's own last place. Its top two bits, rounded, are the quadrant; what is
 // left, at most an eighth of a turn, goes to fp32 and through the series of sine and cosine up to x^9 and x^10 (a remainder
 // below 2e-9). fp32 angles would be wrong in the first digit at a position of 10^6.
 //
-// Bound by memory where there are many tokens: 4096 of 32 + 2 x 8 heads of 128 bf16 values, 101 MB in and out, take 21 us (4.7 TB/s; a
-// copy of as many bytes 21.7), 1023 of 40 heads 6.7; of one token the launch, 3.3. Vector instructions fill 32% of the first's cycles.
+// Bound by memory where there are many tokens: 4096 of 32 + 2 x 8 heads of 128 bf16 values, 101 MB in and out, take 19 us (5.3 TB/s; a call
+// in a loop 21.0, a copy of as many bytes 21.7), 1023 of 40 heads 7.5; of one token the launch, 3.7.
 //
 // Constants: 0 q 2 q stride 4 q_out 6 q_out stride 8 k 10 k stride 12 v 14 v stride 16 cache k 18 cache v 20 page stride
 // 22 head stride 24 token stride (bytes) 26 frequencies (0: nothing turns) 28 positions 30 slots 32 D 33 pairs 34 query heads
 // 35 kv heads (0: no cache) 36 tokens 37 types (q_out | cache << 4) 38 flags (1 interleaved, 2 positions in 64 bits, 4 slots
 // in 64 bits, 8 q in place) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two heads of
-// a thread
+// a thread 45 a wave takes a token
 #pragma once
 #include "rows.h"
 
@@ -39,7 +40,7 @@ __device__ __forceinline__ void ro_turn(uint64_t fraction, float scale, float &c
 }
 
 // Values i .. i + 7 of a head. FULL: all of them are in it, and they stay as they are in memory until they are used, so that loads
-// follow each other without a wait; the last 8 - low are stored. Otherwise the first m <= 8 are there.
+// follow each other without a wait; low .. m - 1 are stored. Otherwise the first m <= 8 are there.
 template <uint32_t TYPE, bool FULL>
 struct RoEight {
     gd_u32x4 raw[TYPE == ROW_F32 ? 2 : 1];
@@ -65,10 +66,10 @@ struct RoEight {
         }
     }
     __device__ __forceinline__ void store(uint64_t head, uint32_t i, uint32_t m, uint32_t low, uint32_t type) const {
-        if (!FULL || !low) return row_store8(head, i, i + (FULL ? 8u : m), type, v);
+        if (!FULL || (!low && m == 8u)) return row_store8(head, i, i + m, type, v);
 #pragma unroll
-        for (uint32_t j = 1; j < 8; ++j)
-            if (j >= low) row_store(head, i + j, type, v[j]);
+        for (uint32_t j = 0; j < 8; ++j)
+            if (j >= low && j < m) row_store(head, i + j, type, v[j]);
     }
 };
 
@@ -98,20 +99,23 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
     const uint32_t D = a.c[32], pairs = a.c[33], QH = a.c[34], KVH = a.c[35], n = a.c[36], types = a.c[37], flags = a.c[38];
     const uint32_t sharers = a.c[42], units = a.c[43], turns = a.c[44], heads = QH + 2u * KVH;
     const uint64_t id = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x, of = id / sharers;
-    if (of >= n) return;
-    const uint32_t t = (uint32_t)of;
+    const bool narrow = a.c[45];  // a token a wave
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), width = narrow ? 64u : 256u, tid = threadIdx.x & (width - 1u);
+    if (of * (narrow ? 4u : 1u) >= n) return;
+    const uint32_t wanted = (uint32_t)of * (narrow ? 4u : 1u) + (narrow ? wave : 0u), t = min(wanted, n - 1u), table = narrow ? wave * (RO_TABLE / 4u) : 0u;
     // A thread takes one unit of every at_once-th head, two heads a turn; a group that shares a token its turns' heads.
-    const uint32_t at_once = 256u / units, own = threadIdx.x / units, u = threadIdx.x - own * units;
+    const uint32_t at_once = width / units, own = tid / units, u = tid - own * units;
     const uint32_t head0 = (uint32_t)(id - of * sharers) * turns * 2u * at_once + own;
     const uint32_t turning = (pairs + 7u) / 8u;  // units of pairs; the others' values are copied
     // The halves of a unit in a head that turns and in one that does not: their places, and how many values of each there are. FULL: a
     // half that would reach past the pairs or the head's end moves down to it, and begins to store at its own first value; pairs
-    // that two units turn need no such care but in place, as both have the same values.
+    // that two units turn need no such care but in place, as both have the same values. Fewer than eight pairs are one unit's, which
+    // reads on behind them.
     uint32_t f1, f2, n1 = 8, n2 = 8, low1 = 0, low2 = 0, pair0 = 8u * u;
     if (u < turning) {
         const uint32_t m = min(8u, pairs - pair0);
         const bool apart = !(flags & 1u);
-        if (FULL) {
+        if (FULL && pairs >= 8u) {
             pair0 -= 8u - m;
             if (flags & 8u) {
                 low1 = apart ? 8u - m : min(8u, 16u - 2u * m);
@@ -156,7 +160,7 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
             const uint32_t head = head0 + (2u * turn + i) * at_once;
-            const bool there = own < at_once && head < heads;
+            const bool there = own < at_once && head < heads && wanted < n;
             const uint32_t h = there ? head : 0u;
             query[i] = h < QH;
             value[i] = h >= QH + KVH;
@@ -168,14 +172,14 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
             second[i].load(x, value[i] ? v2 : f2, value[i] ? mv2 : n2);
         }
         if (!turn) {
-            for (uint32_t i = threadIdx.x; i < pairs; i += 256u)
-                ro_turn((uint64_t)ro_index(gd_addr(a, 28), t, flags & 2u) * gd_at<const uint64_t>(gd_addr(a, 26))[i], gd_bits_f32(a.c[39]), cosines[i], sines[i]);
+            for (uint32_t i = tid; i < pairs; i += width)
+                ro_turn((uint64_t)ro_index(gd_addr(a, 28), t, flags & 2u) * gd_at<const uint64_t>(gd_addr(a, 26))[i], gd_bits_f32(a.c[39]), cosines[table + i], sines[table + i]);
             __syncthreads();
         }
         float c[8], s[8];  // of the thread's pairs (of a head's last ones the table's end is read again)
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
-            const uint32_t at = min(pair0 + j, RO_TABLE - 1u);
+            const uint32_t at = min(table + pair0 + j, RO_TABLE - 1u);
             c[j] = cosines[at];
             s[j] = sines[at];
         }
@@ -204,10 +208,11 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
     }
 }
 
-// (few pairs and small heads have no eight values to move down to)
+// (smaller heads have no eight values to move down to, or to read on behind their pairs)
 template <uint32_t TYPE>
 __device__ __forceinline__ void rotary_body(const GdArgs &a) {
     __shared__ __align__(16) float cosines[RO_TABLE], sines[RO_TABLE];
-    if (a.c[32] >= 8u && (!a.c[33] || a.c[33] >= 8u)) rotary_rows<TYPE, true>(a, cosines, sines);
+    const uint32_t D = a.c[32], pairs = a.c[33];
+    if (D >= 8u && (!pairs || pairs >= 8u || D >= (a.c[38] & 1u ? 16u : pairs + 8u))) rotary_rows<TYPE, true>(a, cosines, sines);
     else rotary_rows<TYPE, false>(a, cosines, sines);
 }

@@ -102,13 +102,17 @@ class AttentionOps {
         c.set(36, n);
         const uint32_t units = std::max((pairs + 7) / 8 + (D - 2 * pairs + 15) / 16, (D + 15) / 16);
         // A group's 256 threads take at_once heads together, two a thread and turn. Of few tokens a group takes one turn of a token,
-        // so that all are on their way at once; of many (256 compute units hold eight groups each) up to eight turns of it.
-        const uint32_t at_once = 256 / units, all_turns = (all + 2 * at_once - 1) / (2 * at_once);
+        // so that all are on their way at once; of many (256 compute units hold eight groups each) up to eight turns of it, or, where
+        // eight turns of a wave cover the heads, four tokens, one a wave (us, 4096 tokens of 128 values: one head 20 and 9.5, 8 heads
+        // 13.0 and 7.2, 24 14.8 and 12.4; 32 and 8 + 8 into a cache 26.8 and 24.8).
+        const bool narrow = n > 2048 && units <= 64 && 16 * (64 / units) >= all && pairs <= 128;
+        const uint32_t at_once = (narrow ? 64 : 256) / units, all_turns = (all + 2 * at_once - 1) / (2 * at_once);
         const uint32_t turns = (uint64_t)n * all_turns > 2048 ? std::min(all_turns, 8u) : 1u, sharers = (all_turns + turns - 1) / turns;
+        c.set(45, narrow ? 1u : 0u);
         c.set(42, sharers);
         c.set(43, units);
         c.set(44, turns);
-        const uint64_t blocks = (uint64_t)n * sharers;
+        const uint64_t blocks = narrow ? ((uint64_t)n + 3) / 4 : (uint64_t)n * sharers;
         l.kernel = x.type == GM_F32 ? "rotary_f" : x.type == GM_BF16 ? "rotary_b" : "rotary_h";
         l.x = (uint32_t)std::min<uint64_t>(blocks, 65535);
         l.y = (uint32_t)((blocks + 65534) / 65535);
@@ -234,13 +238,13 @@ class AttentionOps {
         const bool wide = d.cache.type == GM_F32;
         const uint32_t group = H / G;
         const uint64_t rows = (uint64_t)d.longest * group;
-        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile where these have more
-        // keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a sequence's keys once for
+        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile these are more
+        // than 512 or have more keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a sequence's keys once for
         // every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000 keys 18 against 24, of 16000 32 against 31; 256
-        // rows of 2000 24 against 27, of 4000 40 against 29).
+        // rows of 2000 24 against 27, of 4000 40 against 29; 512 pairs of 300 keys 16 against 25, 1024 32 against 27).
         const uint64_t row_tiles = (rows + kFewRows - 1) / kFewRows;
         const unsigned __int128 pairs = (unsigned __int128)row_tiles * d.sequences * G;
-        const bool many = !wide && rows > kFewRows && pairs * capacity > kFewKeys, few = !many || d.starts;
+        const bool many = !wide && rows > kFewRows && (pairs > kFewPairs || pairs * capacity > kFewKeys), few = !many || d.starts;
         Constants &c = l.c;
         c.set(0, d.q.data);
         c.set64(2, d.q.stride);
@@ -353,7 +357,7 @@ class AttentionOps {
     // Heads of 256, 16 of 1024 31 and 38, of 1536 55 and 52. fp32: 8 tiles of 512 keys 11.9 and 13.0, of 1024 18 and 13; 112 of 1024 20
     // and 27, of 4096 58 and 65.
     static constexpr uint32_t kWidePairs = 96;
-    static constexpr uint32_t kFewKeys = 1u << 18;
+    static constexpr uint32_t kFewKeys = 1u << 18, kFewPairs = 512;
     // Many rows: tiles of rows and heads from which on a part has 16 tiles of keys at least, otherwise 4 (us: 1023 tokens of 32 heads
     // alone, 256 such tiles, 44.5 with 4 and 34.6 with 16; 64 tokens of 4096 keys, 16 tiles, 28.4 and 36.5).
     static constexpr uint32_t kTilePairs = 128;

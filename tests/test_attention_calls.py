@@ -235,11 +235,12 @@ def test_rotary_grids(shim, pairs, dim):
                 rc, why, out = call(shim.plan_rotary, rotary(heads=heads, head_dim=dim), n, pairs)
             assert rc == 0, why
             x, y, w = out[0], out[1], out[4:]
-            sharers, units, turns = w[42], w[43], w[44]
+            sharers, units, turns, narrow = w[42], w[43], w[44], w[45]
             assert 1 <= x <= 65535 and 1 <= y <= 65535
             assert units >= -(-pairs // 8) + -(-(dim - 2 * pairs) // 16) and units * 16 >= dim
-            assert units <= 256 and sharers * turns * 2 * (256 // units) >= heads + 2 * kv
-            assert x * y >= n * sharers
+            assert units <= 256 and sharers * turns * 2 * ((64 if narrow else 256) // units) >= heads + 2 * kv
+            assert not narrow or pairs <= 128 and sharers == 1 and n > 2048
+            assert x * y >= (-(-n // 4) if narrow else n * sharers)
 
 
 # ---- attention ----
@@ -294,7 +295,7 @@ def test_attention_launches(shim, type, heads, kv, dim, ragged):
             grids = {name: out[1 + 2 * i] * out[2 + 2 * i] for i, name in enumerate(names)}
             assert len(names) == out[0] and all(1 <= v <= 65535 for v in out[1:1 + 2 * out[0]])
             pairs = -(-longest * group // 16) * sequences * kv
-            many = bool(type) and longest * group > 16 and pairs * width * 16 > 1 << 18
+            many = bool(type) and longest * group > 16 and (pairs > 512 or pairs * width * 16 > 1 << 18)
             size = 64 if dim <= 64 else 128 if dim <= 128 else 256
             short = type and size < 256 and f"attend_short_{'?bh'[type]}{size}" in names
             build = "f32_" if not type else ("short_" if short else "few_") + "?bh"[type]

@@ -69,7 +69,8 @@ def test_rotary(eng, layout, x, y):
 def test_rotary_parts(eng, layout, type):
     """Heads whose pairs, or what is behind them, are no whole eights; in place and apart alike."""
     for n, H, D, R in ((3, 3, 20, 16), (6, 5, 24, 18), (2, 64, 8, 2), (9, 4, 72, 36), (40, 9, 200, 198), (1, 3, 9, 8), (5, 2, 1023, 1022),
-                       (70, 30, 250, 90), (2, 600, 120, 58), (11, 1, 16, 14)):
+                       (70, 30, 250, 90), (2, 600, 120, 58), (11, 1, 16, 14),
+                       (30, 2, 64, 14), (2051, 2, 64, 2), (2050, 5, 72, 36), (3001, 1, 128, 128), (2100, 16, 128, 64), (2100, 17, 128, 64)):
         print(f"rotary parts {layout} {type}: {n} tokens, {H} heads of {D}, {R} turned", flush=True)
         g = torch.Generator().manual_seed(n * D)
         f, _ = frequencies(R)
@@ -158,6 +159,35 @@ def test_append(eng, order, x, cache, wide, layout):
                 assert torch.equal(q, q_out)
         if index is not None:
             eng.release_rotary(index)
+
+
+@pytest.mark.parametrize("n,H,KVH,D,R", [(2101, 0, 8, 128, 128), (2102, 2, 3, 80, 20), (4099, 1, 1, 256, 256), (2103, 12, 4, 64, 62)])
+def test_append_many(eng, n, H, KVH, D, R):
+    """More tokens than groups; of few heads and many."""
+    print(f"append many {n} {H} {KVH} {D} {R}", flush=True)
+    g = torch.Generator().manual_seed(n)
+    kc, vc = (torch.zeros(n // 16 + 3, KVH, 16, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k, v, q = (torch.randn(n, heads * D, generator=g).bfloat16().cuda() for heads in (KVH, KVH, H))
+    slots = torch.randperm(kc.shape[0] * 16, generator=g)[:n]
+    slots[::7] = -1
+    p = positions_of(g, n, "near")
+    f, _ = frequencies(R)
+    index = eng.add_rotary(f)
+    q_out = torch.zeros_like(q)
+    eng.cache_append(k, v, kc, vc, slots.cuda(), rotary=index, positions=p.cuda(), q=q if H else None, q_out=q_out if H else None)
+    torch.cuda.synchronize()
+    kept = slots >= 0
+    flat = lambda c: c.permute(0, 2, 1, 3).reshape(-1, KVH * D).cpu()  # noqa: E731
+    want, size = ref.rotary(k, KVH, p, f, "half", 1.0)
+    assert ((flat(kc)[slots[kept]].double() - want[kept]).abs() <= ref.rotary_bound(want, size, torch.bfloat16)[kept]).all()
+    assert torch.equal(flat(vc)[slots[kept]], v.cpu()[kept])
+    others = torch.ones(kc.shape[0] * 16, dtype=torch.bool)
+    others[slots[kept]] = False
+    assert (flat(kc)[others] == 0).all() and (flat(vc)[others] == 0).all()
+    if H:
+        want, size = ref.rotary(q, H, p, f, "half", 1.0)
+        assert ((q_out.cpu().double() - want).abs() <= ref.rotary_bound(want, size, torch.bfloat16)).all()
+    eng.release_rotary(index)
 
 
 def test_append_no_tokens(eng):
