@@ -29,14 +29,17 @@ __device__ __forceinline__ at_f32x16 at_mfma(gd_u32x4 a, gd_u32x4 b, at_f32x16 c
 }
 
 // 16 bytes at each lane's address to LDS, from `lds` (of the wave) on in the order of lanes. Counted by vmcnt; at_landed waits.
+// (The load needs a wait state behind M0's write, which the compiler does not see to within a statement.)
 __device__ __forceinline__ void at_to_lds(uint32_t lds, uint64_t from) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from)
+                 : "memory", "m0");
 }
 // The same at a 32-bit offset from a uniform address.
 __device__ __forceinline__ void at_to_lds(uint32_t lds, uint64_t base, uint32_t offset) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base), hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
     const uint64_t uniform = (uint64_t)hi << 32 | (uint64_t)lo;
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(uniform)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset),
+                 "s"(uniform)
                  : "memory", "m0");
 }
 __device__ __forceinline__ void at_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }

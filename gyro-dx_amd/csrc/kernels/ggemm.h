@@ -47,8 +47,9 @@ __device__ __forceinline__ void gg_sync() {
 }
 
 // One global_load_lds_dwordx4: lane l writes the 16 bytes at gbase + voff into LDS byte
-// lds + 16 l (lds is uniform). M0 is set and used inside the one statement; the kernels that
-// stage this way use M0 nowhere else.
+// lds + 16 l (lds is uniform). M0 is set and used inside the one statement, with the wait state that
+// the load needs behind its write and the compiler adds to its own code only; the kernels that stage
+// this way use M0 nowhere else.
 __device__ __forceinline__ void gg_dma16(uint32_t lds, const void *gbase, uint32_t voff) {
     // The base and the LDS address are uniform; readfirstlane keeps them in scalar registers even
     // where the compiler has moved them to vector registers (it folds away otherwise). Its result
@@ -57,8 +58,8 @@ __device__ __forceinline__ void gg_dma16(uint32_t lds, const void *gbase, uint32
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
     const uint64_t sb = ((uint64_t)hi << 32) | (uint64_t)lo;
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff),
-                 "s"(sb)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+                 "v"(voff), "s"(sb)
                  : "memory", "m0");
 }
 
