@@ -57,7 +57,10 @@ __device__ __forceinline__ void gg_dma16(uint32_t lds, const void *gbase, uint32
     const uint64_t b = (uint64_t)(uintptr_t)gbase;
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
-    const uint64_t sb = ((uint64_t)hi << 32) | (uint64_t)lo;
+    uint64_t sb = ((uint64_t)hi << 32) | (uint64_t)lo;
+    // A load may read a scalar register five wait states after a vector instruction has written it; the
+    // statement below is two of them. (Once for all loads at a base, and outside of loops that keep it.)
+    asm("s_nop 2" : "+s"(sb));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                  "v"(voff), "s"(sb)
                  : "memory", "m0");

@@ -73,6 +73,14 @@ def folder(tmp_path_factory):
 needs_kernels = pytest.mark.skipif(not _objects() or not OBJDUMP.exists(), reason="kernels not built, or nothing to read them with")
 
 
+def scalars(operands):
+    """Scalar registers that an instruction's operands name."""
+    found = {int(n) for n in re.findall(r"\bs(\d+)\b", operands)}
+    for first, last in re.findall(r"\bs\[(\d+):(\d+)\]", operands):
+        found |= set(range(int(first), int(last) + 1))
+    return found | set(re.findall(r"\bvcc\b", operands))
+
+
 def to_lds(name, operands):
     return name.startswith(MEMORY) and ("_lds_" in name or re.search(r"\blds\b", operands))
 
@@ -103,3 +111,21 @@ def test_m0_before_loads_to_lds(co, folder):
         if to_lds(name, operands):
             at = c.too_close(i, 1, lambda n, o: n.startswith("s_") and re.match(r"m0\b", o))
             assert at is None, f"{co.stem}: {c.ops[at]} then {c.ops[i]}"
+
+
+@needs_kernels
+@pytest.mark.parametrize("co", _objects(), ids=lambda p: p.stem)
+def test_scalars_before_memory(co, folder):
+    """A vector instruction's write of a scalar register is five wait states or more before a memory instruction that reads it."""
+    c = code(co, folder)
+    for i, (name, operands) in enumerate(c.ops):
+        read = scalars(operands) if name.startswith(MEMORY) else set()
+        if not read:
+            continue
+
+        def writes(n, o):
+            results = 2 if "_co_" in n or n.startswith(("v_div_scale", "v_mad_u64", "v_mad_i64")) else 1
+            return n.startswith("v_") and scalars(",".join(o.split(",")[:results])) & read
+
+        at = c.too_close(i, 5, writes)
+        assert at is None, f"{co.stem}: {c.ops[at]} then {c.ops[i]}"
