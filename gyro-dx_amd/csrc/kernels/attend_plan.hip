@@ -25,7 +25,8 @@ GD_PIPELINE_NAMED(attend_plan, 1024) {
             uint32_t own = 0;
             if (s0 + tid < S) {
                 at_sequence(a, s0 + tid, o);
-                if (o.rows >= a.c[46]) own = (o.rows + AT_ROWS - 1u) / AT_ROWS;
+                // (of a sequence of more than `longest` tokens those alone: the list has room for no more)
+                if (o.rows >= a.c[46]) own = (min(o.rows, a.c[33] * a.c[29]) + AT_ROWS - 1u) / AT_ROWS;
             }
             const uint32_t upto = gd_wave_scan_u32(own);
             __syncthreads();  // the chunk before is done
