@@ -134,8 +134,8 @@ __device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, 
                                                         row_bits16(x[2], TYPE) | row_bits16(x[3], TYPE) << 16};
 }
 
-// Below every score that counts, and finite: the difference of two such is zero, not NaN.
-#define AT_LOWEST -1e30f
+// Where maxima begin: no finite score is below it, and the difference of two such is zero, not NaN.
+#define AT_LOWEST -3.402823466e38f
 
 // Few rows (attend_few.h, attend_f32.h).
 

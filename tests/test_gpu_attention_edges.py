@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import attention_reference as ref
-from test_gpu_attention import Batch, eng, stream  # noqa: F401 (a fixture)
+from test_gpu_attention import Batch, eng, reach, stream  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,39 @@ def test_more_tokens_than_the_bound(eng):  # noqa: F811
         got = b.out[first].cpu().double()
         assert ((got - want).abs() <= bound + ref.half_step(torch.bfloat16) * (want.abs() + bound)).all()
         assert (b.out[b.n:] == 7).all()
+
+
+@pytest.mark.usefixtures("reach")
+@pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("sign,ones", [(-1, 64), (1, 64)])
+def test_scores_of_any_size(eng, type, sign, ones):  # noqa: F811
+    """Finite scores count, whatever their size: the largest, which several keys share to the last bit, and no other. Weights are
+    one and zero then: the result is the mean of the values, off by the sum's roundings and its own."""
+    for counts, lengths in (([1, 3], [700, 90]), ([1], [9000]), ([150], [400]), ([18], [6000])):
+        for scale in (2.0 ** 105, 1.1e32, 1e20, 3e9, 2.0 ** 26, 5e4):
+            b = Batch(eng, type, 4, 2, 64, 16, counts, lengths, seed=42)
+            g = torch.Generator().manual_seed(43)
+            size = 2.0 ** torch.randint(0, 3, b.kc.shape[:3], generator=g)  # a key's values: 1, 2 or 4
+            b.kc.copy_(sign * size[..., None].expand_as(b.kc))
+            b.q.zero_()
+            for head in range(4):
+                b.q[:, 64 * head:64 * head + ones] = 1
+            b.out.fill_(7.0)
+            print(f"scores of {sign * ones} {scale:.1e} {type} {counts} {lengths}", flush=True)
+            b.run(scale=scale)
+            torch.cuda.synchronize()
+            table, vc, row = b.table.cpu().long(), b.vc.cpu().double(), 0
+            for s, (count, length) in enumerate(zip(counts, lengths)):
+                j = torch.arange(length)
+                page = table[s, j // 16]
+                keys, v = size[page, :, j % 16] * sign, vc[page, :, j % 16]  # [length, kv], [length, kv, dim]
+                for i in range(count):
+                    seen = length - count + i + 1
+                    for head in range(4):
+                        k, x = keys[:seen, head // 2], v[:seen, head // 2]
+                        top = x[k == k.max()]
+                        want, room = top.mean(0), top.abs().mean(0) * (len(top) / 4 + 130) * ref.ULP
+                        got = b.out[row, head * 64:(head + 1) * 64].cpu().double()
+                        least = 2.0 ** -25 if type == "f16" else 0
+                        assert ((got - want).abs() <= room + ref.half_step(b.dtype) * (want.abs() + room) + least).all(), (s, i, head)
+                    row += 1
