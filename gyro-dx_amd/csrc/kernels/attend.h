@@ -137,6 +137,17 @@ __device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, 
 // Where maxima begin: no finite score is below it, and the difference of two such is zero, not NaN.
 #define AT_LOWEST -3.402823466e38f
 
+// A weight is exp2(s scale - top), in one fused step. top is a product of that kind as well, but rounded: off by up to half a unit of
+// its last place, by which all of a row's weights are too large or small alike. From 2^20 on that is 2^-5 and more, and with no
+// bound: of scores of 10^10 all weights were zero, or infinite. Rows with such a top take both products rounded, so that the
+// largest score's weight is one.
+__device__ __forceinline__ bool at_far(float top) { return (fabsf(top) >= 1048576.f) & (top > AT_LOWEST); }
+__device__ __forceinline__ float at_from_top(float s, float scale, float top) {
+    float product = s * scale;
+    asm volatile("" : "+v"(product));  // (not to be fused)
+    return at_far(top) ? product - top : fmaf(s, scale, -top);
+}
+
 // Few rows (attend_few.h, attend_f32.h).
 
 // The larger (the sum) of the four lanes that hold a row's keys, 16 lanes apart.

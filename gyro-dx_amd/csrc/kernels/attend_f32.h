@@ -121,10 +121,15 @@ __device__ __forceinline__ void attend_f32_body(const GdArgs &a) {
         const float shrink = at_exp2(top - most);
         top = most;
         sum *= shrink;
+        const bool far = __ballot(at_far(most));
+        if (far)
+#pragma unroll
+            for (int i = 0; i < 4 * (int)BLOCKS; ++i) s[i >> 2][i & 3] = at_from_top(s[i >> 2][i & 3], scale, most);
+        const float by = far ? 1.f : scale, from = far ? 0.f : most;
 #pragma unroll
         for (uint32_t b = 0; b < BLOCKS; ++b) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][i] = at_exp2(fmaf(s[b][i], scale, -most));
+            for (int i = 0; i < 4; ++i) s[b][i] = at_exp2(fmaf(s[b][i], by, -from));
             sum += (s[b][0] + s[b][1]) + (s[b][2] + s[b][3]);
         }
 #pragma unroll

@@ -55,6 +55,7 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
 #pragma unroll
     for (uint32_t d = 0; d < DIMS; ++d) acc[d] = none;
     float top = AT_LOWEST, sum = 0.f;
+    bool far = false;  // some row's top is (at_far)
 
     // A tile's keys: a lane knows the place in the cache of key l % 32; k and v are on their way from when their registers are
     // free again, a tile ahead of their use. (Where there is none, the cache's first are loaded, and dropped later: at_key says
@@ -158,15 +159,20 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
             most = fmaxf(most, top);
             const float shrink = at_exp2(top - most);
             top = most;
+            far = __ballot(at_far(top));
             sum *= shrink;
 #pragma unroll
             for (uint32_t d = 0; d < DIMS; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[d][i] *= shrink;
         }
+        if (far)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = at_from_top(s[i >> 2][i & 3], scale, top);
+        const float by = far ? 1.f : scale, from = far ? 0.f : top;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            s[i >> 2][i & 3] = at_exp2(fmaf(s[i >> 2][i & 3], scale, -top));
+            s[i >> 2][i & 3] = at_exp2(fmaf(s[i >> 2][i & 3], by, -from));
             sum += s[i >> 2][i & 3];
         }
         gd_u32x4 large, small;  // the weights' parts

@@ -87,6 +87,7 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
     float top = AT_LOWEST, sum = 0.f;
+    bool far = false;  // some row's top is (at_far)
 
     // Load i of a wave brings keys 4 PER i + PER wave .. of a tile; a lane piece lane % CHUNKS of key lane / CHUNKS, which is the
     // piece of the head that belongs there. (Of shorter heads the others stay zeros.)
@@ -245,12 +246,17 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
                 most = fmaxf(most, top);
                 const float shrink = at_exp2(top - most);
                 top = most;
+                far = __ballot(at_far(top));
                 sum *= shrink;
 #pragma unroll
                 for (uint32_t d = 0; d < DIMS; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
             }
+            if (far)
+#pragma unroll
+                for (int i = 0; i < 16 * (int)BLOCKS; ++i) s[i >> 4][i & 15] = at_from_top(s[i >> 4][i & 15], scale, top);
+            const float by = far ? 1.f : scale, from = far ? 0.f : top;
             // The weights beside the next tile's scores (of the last one's: of what is in the buffer), with the first of V^T, whose
             // 16 keys and 32 channels an operand has in the order of the weights, behind.
             constexpr uint32_t PAIRS = 8u * BLOCKS;
@@ -261,7 +267,7 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
 #pragma unroll
                 for (uint32_t i = step * PAIRS / PRODUCTS; i < (step + 1u) * PAIRS / PRODUCTS; ++i) {
                     const uint32_t b = i >> 3, e = i & 7u;
-                    const float x = at_exp2(fmaf(s[b][2 * e], scale, -top)), y = at_exp2(fmaf(s[b][2 * e + 1], scale, -top));
+                    const float x = at_exp2(fmaf(s[b][2 * e], by, -from)), y = at_exp2(fmaf(s[b][2 * e + 1], by, -from));
                     w[b][e >> 2][e & 3u] = at_pair<TYPE>(x, y);
                     sum = at_add_pair<TYPE>(w[b][e >> 2][e & 3u], sum);  // the sum of what the values are weighed with
                 }

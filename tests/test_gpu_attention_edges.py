@@ -30,7 +30,7 @@ def test_more_tokens_than_the_bound(eng):  # noqa: F811
 
 @pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("sign,ones", [(-1, 64), (1, 64)])
+@pytest.mark.parametrize("sign,ones", [(-1, 64), (1, 64), (-1, 57), (1, 57)])
 def test_scores_of_any_size(eng, type, sign, ones):  # noqa: F811
     """Finite scores count, whatever their size: the largest, which several keys share to the last bit, and no other. Weights are
     one and zero then: the result is the mean of the values, off by the sum's roundings and its own."""
