@@ -141,7 +141,8 @@ __device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, 
 // its last place, by which all of a row's weights are too large or small alike. From 2^20 on that is 2^-5 and more, and with no
 // bound: of scores of 10^10 all weights were zero, or infinite. Rows with such a top take both products rounded, so that the
 // largest score's weight is one.
-__device__ __forceinline__ bool at_far(float top) { return (fabsf(top) >= 1048576.f) & (top > AT_LOWEST); }
+#define AT_FAR 1048576.f
+__device__ __forceinline__ bool at_far(float top) { return (fabsf(top) >= AT_FAR) & (top > AT_LOWEST); }
 __device__ __forceinline__ float at_from_top(float s, float scale, float top) {
     float product = s * scale;
     asm volatile("" : "+v"(product));  // (not to be fused)

@@ -7,8 +7,8 @@
 // from memory straight to operands. Values go through LDS, a wave's tile its own, and come back transposed
 // (ds_read_b64_tr_b16).
 //
-// The maximum that weights are relative to follows the running one only when that has grown by more than 2^8, so that the sums
-// are rarely rescaled; weights are at most 2^8 then, and as precise.
+// Weights are at most 2^8 in bf16, where the sums are rescaled only when the maximum has grown by as much; in binary16 they reach
+// 2^15 and every growth is followed, so that small ones lose least (at_grown).
 //
 // The weights are the sum of two 16-bit parts, so that they lose nothing: these rows are bound by memory, and the second
 // products run in its shadow.
@@ -155,8 +155,8 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, s[i >> 2][i & 3]);
         most = af_max(most) * scale;
-        if (__ballot(most > top + 8.f)) {
-            most = fmaxf(most, top);
+        if (__ballot(at_grown<TYPE>(most, top))) {
+            most = at_new_top<TYPE, 15>(most, top);
             const float shrink = at_exp2(top - most);
             top = most;
             far = __ballot(at_far(top));

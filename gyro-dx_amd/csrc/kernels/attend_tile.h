@@ -5,9 +5,8 @@
 // running maximum needs one exchange per tile, the sum none until the end, and the weights are the second product's operand
 // as they lie: O^T += V^T P^T, contracted over keys in the order in which lanes hold them; values come out of LDS transposed
 // (ds_read_b64_tr_b16). The next tile's scores are multiplied while this one's weights are worked out, which are independent: the
-// matrix unit and the vector unit work side by side within a wave. The maximum that weights are relative to follows the running
-// one only when that has grown by more than 2^8, so that the sums are rarely rescaled; weights are at most 2^8 then, and as
-// precise.
+// matrix unit and the vector unit work side by side within a wave. Sums are rescaled only when the maximum has grown by more than
+// 2^8, of binary16 2^4 (at_grown).
 //
 // LDS is filled 1 KB an instruction in the order of lanes, so rows cannot be padded; instead their 16-byte pieces are swapped
 // by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v; no conflict was counted).
@@ -242,8 +241,8 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
 #pragma unroll
             for (int i = 1; i < 16 * (int)BLOCKS; ++i) most = fmaxf(most, s[i >> 4][i & 15]);
             most = at_max_halves(most) * scale;
-            if (__ballot(most > top + 8.f)) {
-                most = fmaxf(most, top);
+            if (__ballot(at_grown<TYPE>(most, top))) {
+                most = at_new_top<TYPE, 11>(most, top);
                 const float shrink = at_exp2(top - most);
                 top = most;
                 far = __ballot(at_far(top));

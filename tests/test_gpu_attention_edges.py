@@ -1,4 +1,6 @@
 """Attention where its arithmetic and its bounds end, against 64-bit forms."""
+import math
+
 import pytest
 import torch
 
@@ -6,6 +8,7 @@ import attention_reference as ref
 from test_gpu_attention import Batch, eng, reach, stream  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
+HALF = ref.half_step(torch.float16)
 
 
 def test_more_tokens_than_the_bound(eng):  # noqa: F811
@@ -62,3 +65,29 @@ def test_scores_of_any_size(eng, type, sign, ones):  # noqa: F811
                         least = 2.0 ** -25 if type == "f16" else 0
                         assert ((got - want).abs() <= room + ref.half_step(b.dtype) * (want.abs() + room) + least).all(), (s, i, head)
                     row += 1
+
+
+@pytest.mark.usefixtures("reach")
+@pytest.mark.parametrize("counts,lengths", [([1, 2], [4000, 300]), ([40], [4000])], ids=["few", "many"])
+@pytest.mark.parametrize("below", [13, 17, 19, 21])
+def test_small_weights(eng, below, counts, lengths):  # noqa: F811
+    """Binary16 rows behind one key that takes nearly all weight and whose value is zero: the others' weights, e^-below of it, are
+    all that there is. A weight is rounded by half a step of the type or by 2^-36 of the largest (by 2^-25,
+    where the largest is 2^11 or more), whichever is more."""
+    b = Batch(eng, "f16", 4, 2, 64, 16, counts, lengths, seed=44)
+    b.q.fill_(1)
+    b.kc.zero_()
+    b.vc.add_(4).mul_(500)
+    for s in range(len(counts)):
+        b.kc[int(b.table[s, 0]), :, 3] = below / 8  # 64 / 8 of it, in nats
+        b.vc[int(b.table[s, 0]), :, 3] = 0
+    b.out.fill_(7.0)
+    print(f"weights {below} below, {counts}", flush=True)
+    b.run()
+    torch.cuda.synchronize()
+    want, bound, _ = ref.attention(b.q, b.kc, b.vc, b.table, b.lengths, counts, 4, 0.125, True, 0)
+    rounded = want.abs() * 2.0 ** -36 * math.exp(below)
+    err = (b.out[:b.n].cpu().double() - want).abs()
+    limit = bound + rounded + HALF * (want.abs() + bound + rounded) + 2.0 ** -25
+    print(f"  err / want {float((err / want.abs()).max()):.2e}, limit {float((limit / want.abs()).max()):.2e}", flush=True)
+    assert (err <= limit).all()
