@@ -10,8 +10,8 @@
 // Weights are at most 2^8 in bf16, where the sums are rescaled only when the maximum has grown by as much; in binary16 they reach
 // 2^15 and every growth is followed, so that small ones lose least (at_grown).
 //
-// The weights are the sum of two 16-bit parts, so that they lose nothing: these rows are bound by memory, and the second
-// products run in its shadow.
+// The weights are the sum of two 16-bit parts, 16 bits of them in bf16 and 22 in binary16: these rows are bound by memory, and the
+// second products run in its shadow.
 //
 // Bound by the cache's bytes: a token each of 64 sequences of 91 to 8192 keys, 8 heads of 128 values, 560 MB, 108 us (5.2 TB/s;
 // vector unit 16% of cycles, matrix unit 5%); one token over 131072 keys, 2 heads of 256, 268 MB, 53 us (5.1 TB/s). A wave has a
@@ -211,13 +211,12 @@ __device__ __forceinline__ void attend_few_body(const GdArgs &a) {
             const int32_t j = (int32_t)(32u * t + key);
             const bool seen = j <= work.last && j >= work.first;
             const uint64_t from = V + place(here, key);
-            // The key's weight is in the lanes of quarter key / 4 % 4, one of a pair in a word.
-            uint32_t pair = 0;
+            // The key's weight is in the lanes of quarter key / 4 % 4.
+            float weight = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if ((key >> 4) * 2u + (key >> 1 & 1u) == i) pair = large[i];
-            pair = __shfl(key & 1u ? pair >> 16 : pair & 0xffffu, col + 16u * (key >> 2 & 3u), 64);
-            const float weight = row_value16(pair, TYPE);
+            for (uint32_t i = 0; i < 8; ++i)
+                if ((key >> 4) * 4u + (key & 3u) == i) weight = s[i >> 2][i & 3];
+            weight = __shfl(weight, col + 16u * (key >> 2 & 3u), 64);
 #pragma unroll
             for (uint32_t d = 0; d < DIMS; ++d) {
                 const uint32_t dim = 16u * d + 4u * h;

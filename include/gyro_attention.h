@@ -76,8 +76,9 @@ GM_API int gm_cache_append(gm_engine *e, const gm_cache_append_desc *desc, uint3
  * A token that sees no key, or only keys whose score is -infinity, has zeros. What is not seen does not count, NaNs and
  * infinities among it. Rows of q behind the last sequence's are left in out as they were. Products of 16-bit types are exact
  * and summed in fp32, as are the softmax's statistics; its weights may be rounded to the type before they meet v, in
- * binary16, which has no smaller ones, by up to 2^-36 of a row's largest. out may be q's rows, of the same stride; it
- * overlaps nothing else. n * heads is at most 2^30, and n * heads / kv_heads / 128 + sequences at most 2^18 - 1024.
+ * binary16, which has no smaller ones, by up to 2^-36 of a row's largest; an infinite value times a weight that is zero then
+ * is NaN. out may be q's rows, of the same stride; it overlaps nothing else. n * heads is at most 2^30, and
+ * n * heads / kv_heads / 128 + sequences at most 2^18 - 1024.
  * The workspace (256-byte aligned, of gm_attention_workspace(heads, kv_heads, head_dim) bytes, which serve every call of that
  * shape) holds nothing between calls; calls that may overlap, replayed graphs among them, take one each. */
 typedef struct gm_attention_desc {

@@ -91,3 +91,30 @@ def test_small_weights(eng, below, counts, lengths):  # noqa: F811
     limit = bound + rounded + HALF * (want.abs() + bound + rounded) + 2.0 ** -25
     print(f"  err / want {float((err / want.abs()).max()):.2e}, limit {float((limit / want.abs()).max()):.2e}", flush=True)
     assert (err <= limit).all()
+
+
+@pytest.mark.parametrize("type", ["bf16", "f16"])
+def test_whole_weight_beside_infinity(eng, type):  # noqa: F811
+    """A key with one value that is not finite gives its others the whole weight, as rows of few tokens give every key's."""
+    heads, dim = 64, 64
+    b = Batch(eng, type, heads, heads, dim, 16, [1], [9], seed=45)
+    b.q.fill_(1)
+    b.kc.zero_()
+    page = int(b.table[0, 0])
+    b.kc[page, :, 2] = torch.linspace(-0.4, -0.01, heads)[:, None].to(b.kc)  # one key a little below the eight others
+    b.vc.zero_()
+    b.vc[page, :, 2] = 1 + 2.0 ** -6
+    b.vc[page, :, 2, 5] = float("inf")
+    b.run()
+    torch.cuda.synchronize()
+    k = b.kc[page, :, 2, 0].cpu().double()
+    w = torch.exp(8 * k) / (8 + torch.exp(8 * k))
+    got = b.out[0].cpu().double().reshape(heads, dim)
+    assert torch.isinf(got[:, 5]).all()
+    got = got[:, [d for d in range(dim) if d != 5]]
+    want = (w * (1 + 2.0 ** -6))[:, None]
+    # Two parts of a weight hold 16 bits or more; scores and sums as in attention_reference.
+    room = want * (2.0 ** -16 + (2 * (2 * dim + 6) * 3.2 + 140) * ref.ULP)
+    err = (got - want).abs()
+    print(f"  {type}: err / half a step {float((err / (ref.half_step(b.dtype) * want)).max()):.3f}", flush=True)
+    assert (err <= room + ref.half_step(b.dtype) * (want + room)).all()
