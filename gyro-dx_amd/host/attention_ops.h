@@ -238,13 +238,17 @@ class AttentionOps {
         const bool wide = d.cache.type == GM_F32;
         const uint32_t group = H / G;
         const uint64_t rows = (uint64_t)d.longest * group;
-        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile these are more
-        // than 512 or have more keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a sequence's keys once for
-        // every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000 keys 18 against 24, of 16000 32 against 31; 256
-        // rows of 2000 24 against 27, of 4000 40 against 29; 512 pairs of 300 keys 16 against 25, 1024 32 against 27).
+        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile if these tiles are more than
+        // 512 or have more keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a
+        // sequence's keys once for every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000 keys 18 against 24,
+        // of 16000 32 against 31; 256 rows of 2000 24 against 27, of 4000 40 against 29; 512 pairs of 300 keys 16 against 25, 1024
+        // 32 against 27). attend_tile loads straight to LDS, which wants addresses that are multiples of four bytes (4096 tokens of 32
+        // heads over 8 160 us, over a cache off by two bytes 2360; 256 tokens 14 and 26).
         const uint64_t row_tiles = (rows + kFewRows - 1) / kFewRows;
         const unsigned __int128 pairs = (unsigned __int128)row_tiles * d.sequences * G;
-        const bool many = !wide && rows > kFewRows && (pairs > kFewPairs || pairs * capacity > kFewKeys), few = !many || d.starts;
+        const bool direct = !wide && !(((uintptr_t)d.cache.k | (uintptr_t)d.cache.v | (d.cache.pages > 1 ? 2 * d.cache.page_stride : 0) |
+                                        (G > 1 ? 2 * d.cache.head_stride : 0) | (d.cache.page_size > 1 ? 2 * d.cache.token_stride : 0)) & 3);
+        const bool many = direct && rows > kFewRows && (pairs > kFewPairs || pairs * capacity > kFewKeys), few = !many || d.starts;
         Constants &c = l.c;
         c.set(0, d.q.data);
         c.set64(2, d.q.stride);

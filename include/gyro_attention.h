@@ -39,8 +39,8 @@ GM_API int gm_rotary(gm_engine *e, const gm_rotary_desc *desc, uint32_t n, void 
 
 /* Keys and values in `pages` pages of `page_size` tokens each: the key of token i of page p and head g starts at
  * k + p page_stride + g head_stride + i token_stride (values; at most 2^40 each), its head_dim values are neighbours;
- * values likewise at v. k and v are aligned to their type (16-byte aligned heads are read faster). pages * page_size is below
- * 2^31. */
+ * values likewise at v. k and v are aligned to their type. (Attention of prompts over a 16-bit cache takes up to 15 times as
+ * long where k, v or a stride is no multiple of four bytes.) pages * page_size is below 2^31. */
 typedef struct gm_cache {
     void *k, *v;
     uint32_t type; /* GM_F32, GM_BF16, GM_F16 */

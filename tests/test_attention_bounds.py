@@ -1,0 +1,23 @@
+"""Where the host's checks and choices for rotary positions, the cache and attention end (host/attention_ops.h), on the CPU."""
+import pytest
+from test_attention_calls import A, attention, cache, call, rows, shim  # noqa: F401 (a fixture)
+
+
+@pytest.mark.parametrize("type", [1, 2])
+def test_unaligned_caches(shim, type):  # noqa: F811
+    """Loads straight to LDS want addresses that are multiples of four bytes: a cache with others goes to the kernels that load to
+    registers, all its rows in tiles of 16."""
+    plain = dict(type=type, pages=100, page_stride=2 * 16 * 64 + 2, head_stride=16 * 64 + 2, token_stride=66)
+    for kw, direct in ((dict(), True), (dict(k=A + 2), False), (dict(v=2 * A + 2), False), (dict(k=A + 4, v=2 * A + 12), True),
+                       (dict(page_stride=2049), False), (dict(head_stride=1025), False), (dict(token_stride=65), False),
+                       (dict(pages=1, page_stride=2049), True), (dict(kv_heads=1, head_stride=1025), True),
+                       (dict(page_size=1, token_stride=65), True), (dict(page_stride=1 << 40), True), (dict(page_stride=(1 << 40) - 1), False)):
+        c = cache(**{**plain, **kw})
+        d = attention(cache=c, q=rows(type), out=rows(type, data=3 * A), heads=32 * c.kv_heads, sequences=2, longest=300, starts=A, table_width=1000)
+        rc, names, out = call(shim.plan_attention, d, 600)
+        assert rc == 0, names
+        names = names.split()
+        assert any(n.startswith("attend_tile") for n in names) == direct, (kw, names)
+        if not direct:
+            assert names[0].startswith("attend_few") and out[9 + 42] == 300 * 32 // 16 and out[9 + 46] == 0
+            assert out[1] * out[2] >= 2 * 600 * c.kv_heads

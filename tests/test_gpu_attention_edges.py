@@ -118,3 +118,56 @@ def test_whole_weight_beside_infinity(eng, type):  # noqa: F811
     err = (got - want).abs()
     print(f"  {type}: err / half a step {float((err / (ref.half_step(b.dtype) * want)).max()):.3f}", flush=True)
     assert (err <= room + ref.half_step(b.dtype) * (want + room)).all()
+
+
+@pytest.mark.usefixtures("reach")
+@pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("by", [1, 2], ids=["one", "two"])
+@pytest.mark.parametrize("counts,lengths", [([1, 3], [700, 90]), ([150, 20], [400, 90]), ([18], [5000])], ids=["few", "many", "split"])
+@pytest.mark.parametrize("dim", [64, 136])
+def test_caches_aligned_to_their_type(eng, type, by, counts, lengths, dim):  # noqa: F811
+    """k, v and every stride off 16 bytes by one value, or by two; values that are not finite among them."""
+    b = Batch(eng, type, 8, 2, dim, 16, counts, lengths, pad=by, shift=by, seed=46)
+    pages = b.kc.shape[0]
+    token = dim + by
+    head = 16 * token + by
+    page = 2 * head + by
+    for name, shift in (("kc", by), ("vc", 3 * by)):
+        flat = torch.full((pages * page + 16,), float("nan"), dtype=b.dtype, device="cuda")
+        cache = flat.as_strided((pages, 2, 16, dim), (page, head, token, 1), shift)
+        cache.copy_(getattr(b, name))
+        setattr(b, name, cache)
+    for kw in (dict(), dict(window=50), dict(causal=False)):
+        print(f"aligned to {by} {type} {counts} {dim} {kw}", flush=True)
+        b.out.fill_(7.0)
+        b.run(**kw)
+        b.check(**kw)
+    for s, length in enumerate(lengths):
+        at = lambda j: (int(b.table[s, j // 16]), slice(None), j % 16)  # noqa: E731
+        b.vc[at(length // 2)][0, dim - 1] = float("inf")
+        b.vc[at(length - 1)][1, 0] = float("nan")
+        b.kc[at(length - 1)][0, dim - 1] = float("nan")
+    b.out.fill_(7.0)
+    b.run()
+    b.check()
+
+
+@pytest.mark.usefixtures("reach")
+@pytest.mark.parametrize("by", [1, 2], ids=["one", "two"])
+@pytest.mark.parametrize("counts", [[3, 1], [40, 1]], ids=["few", "many"])
+def test_wide_caches_aligned_to_their_type(eng, by, counts):  # noqa: F811
+    """The same in caches that 32 bits do not span."""
+    size, dim, kv, pages = 16, 128, 2, 7
+    stride = (1 << 29) + 4096 + by
+    b = Batch(eng, "bf16", 4, kv, dim, size, counts, [75, 30], seed=47, spare=0)
+    flat = torch.zeros(stride * pages, dtype=torch.bfloat16, device="cuda")
+    for name, shift in (("kc", by), ("vc", size * kv * (dim + by) + 3 * by)):
+        cache = flat.as_strided((pages, kv, size, dim), (stride, size * (dim + by), dim + by, 1), shift)
+        cache.copy_(getattr(b, name))
+        setattr(b, name, cache)
+    b.vc[int(b.table[0, 2]), 1, 3, 5] = float("nan")
+    for kw in (dict(), dict(window=20), dict(causal=False)):
+        print(f"wide cache aligned to {by} {counts} {kw}", flush=True)
+        b.out.fill_(7.0)
+        b.run(**kw)
+        b.check(**kw)
