@@ -34,6 +34,20 @@ class AttentionOps {
 
     // ---- rotary positions ----
 
+    // The fraction of a turn, of 2^64, by which a frequency below 2^31 turns, rounded: m 2^-down (m of 53 bits) times 1 / (2 pi) in
+    // 128 bits, before rounding exact to 2^-21 of the last place, however many whole turns there are.
+    static uint64_t fraction(double frequency) {
+        constexpr uint64_t high = 0x28be60db9391054aull, low = 0x7f09d5f47d4d3770ull;  // 2^128 / (2 pi)
+        int e;
+        const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(frequency), &e), 53);
+        const uint32_t down = (uint32_t)(53 - e);  // at least 22
+        // m / (2 pi) in units of 2^-64, of which the last place is 2^22 or more.
+        const unsigned __int128 turns = (unsigned __int128)m * high + (uint64_t)((unsigned __int128)m * low >> 64);
+        if (down > 128) return 0;
+        const uint64_t whole = down < 128 ? (uint64_t)(turns >> down) : 0, f = whole + (uint64_t)(turns >> (down - 1) & 1);
+        return frequency < 0 ? 0 - f : f;
+    }
+
     static Rotary describe(const double *frequencies, uint32_t pairs, uint32_t layout, float scale, std::vector<uint64_t> &table) {
         require(frequencies && pairs && pairs <= 512, "a rotary has 1 to 512 pairs");
         require(layout <= GM_ROTARY_INTERLEAVED, "unknown rotary layout");
@@ -41,10 +55,7 @@ class AttentionOps {
         table.resize(pairs);
         for (uint32_t i = 0; i < pairs; ++i) {
             require(std::fabs(frequencies[i]) < 2147483648.0, "a rotary's frequencies are below 2^31 in magnitude");
-            // x87's 64-bit mantissa keeps the fraction's last places.
-            const long double turns = (long double)frequencies[i] / 6.283185307179586476925286766559L;
-            const long double scaled = std::floor((turns - std::floor(turns)) * 18446744073709551616.0L + 0.5L);
-            table[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
+            table[i] = fraction(frequencies[i]);
         }
         Rotary r;
         r.pairs = pairs;

@@ -1,4 +1,9 @@
 """Where the host's checks and choices for rotary positions, the cache and attention end (host/attention_ops.h), on the CPU."""
+import ctypes as C
+import math
+from fractions import Fraction
+
+import numpy as np
 import pytest
 from test_attention_calls import A, attention, cache, call, rows, shim  # noqa: F401 (a fixture)
 
@@ -21,3 +26,18 @@ def test_unaligned_caches(shim, type):  # noqa: F811
         if not direct:
             assert names[0].startswith("attend_few") and out[9 + 42] == 300 * 32 // 16 and out[9 + 46] == 0
             assert out[1] * out[2] >= 2 * 600 * c.kv_heads
+
+
+def test_frequencies_of_many_turns(shim):  # noqa: F811
+    """The table is off by half of its last place, 2^-65 of a turn (and 2^-21 of that place for digits of 2 pi behind 128 bits and
+    what is cut off), however many turns a position is: at positions below 2^36 angles are exact to 2^-29 of a turn before fp32."""
+    turn = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+    rng = np.random.default_rng(7)
+    f = np.concatenate([[0.0, -0.0, 5e-324, 2.0 ** -64, 1e-19, 0.5, 1, 6.283185307179586, 2.0 ** 30, 2.0 ** 31 - 2.0 ** -21, -1e9, 12345.678],
+                        rng.uniform(-1, 1, 200) * 2.0 ** rng.uniform(-70, 31, 200)])
+    out, why = (C.c_uint64 * len(f))(), C.create_string_buffer(200)
+    assert shim.plan_frequencies(f.ctypes.data, len(f), 0, 1.0, out, why) == 0
+    for v, got in zip(f, out):
+        turns = Fraction(float(v)) / turn
+        off = abs((turns - math.floor(turns)) * 2 ** 64 - got)
+        assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + Fraction(1, 2 ** 21), (v, got, float(off))

@@ -1,5 +1,6 @@
 """Attention where its arithmetic and its bounds end, against 64-bit forms."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -171,3 +172,23 @@ def test_wide_caches_aligned_to_their_type(eng, by, counts):  # noqa: F811
         b.out.fill_(7.0)
         b.run(**kw)
         b.check(**kw)
+
+
+def test_rotary_of_many_turns(eng):  # noqa: F811
+    """Angles of frequencies that are many turns a position, far out."""
+    f = [1.0, 100.0, 12345.678, 1e6, 1e9, 2.0 ** 31 - 1, -3e8, 6.283185307179586]
+    index = eng.add_rotary(f)
+    positions = torch.cat([(1 << 36) - torch.arange(1, 33), torch.arange(4)]).cuda()
+    x = torch.randn(len(positions), 16, generator=torch.Generator().manual_seed(48)).cuda()
+    y = torch.empty_like(x)
+    eng.rotary(index, x, positions, y, heads=1, stream=stream())
+    torch.cuda.synchronize()
+    eng.release_rotary(index)
+    turn = 2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+    angle = [[float(Fraction(v) * int(p) / turn % 1) * 2 * math.pi for v in f] for p in positions]
+    c, s = torch.tensor(angle, dtype=torch.float64).cos(), torch.tensor(angle, dtype=torch.float64).sin()
+    a, b = x[:, :8].cpu().double(), x[:, 8:].cpu().double()
+    want, size = torch.cat([a * c - b * s, a * s + b * c], 1), (a.abs() + b.abs()).repeat(1, 2)
+    # As in attention_reference, and 2^-29 of a turn (2 pi 2^-29 in a sine or cosine) for the position times the table's rounding.
+    bound = ref.rotary_bound(want, size, torch.float32) + 2 * math.pi * 2.0 ** -29 * size
+    assert ((y.cpu().double() - want).abs() <= bound).all()
