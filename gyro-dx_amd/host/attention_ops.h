@@ -181,8 +181,10 @@ class AttentionOps {
         }
         require(d.slots && (uintptr_t)d.slots % (d.slots_64 ? 8 : 4) == 0, "gm_cache_append: slots");
         require(!r || (d.positions && (uintptr_t)d.positions % (d.positions_64 ? 8 : 4) == 0), "gm_cache_append: positions");
-        // No two (page, head, token) may share an element: of two dimensions one's stride spans the other's extent.
+        // No two (page, head, token) may share an element: of two dimensions one's stride spans the other's extent. (Whether keys and
+        // values lie apart is the caller's to know; one array for both is told.)
         check_apart(d.cache);
+        require(d.cache.k != d.cache.v, "gm_cache_append: the cache's keys and values are one array");
         turn(l, r, d.heads ? &d.q : nullptr, &d.q_out, d.heads, &d.k, &d.v, G, D, n);
         Constants &c = l.c;
         c.set(16, d.cache.k);

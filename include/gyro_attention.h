@@ -53,7 +53,8 @@ typedef struct gm_cache {
  * (negative: a padded token) is skipped. Of two tokens with one slot either's values may stay, value by value. With q (rows
  * of `heads` heads, of every token) also q_out = q turned: q_out may be q's rows, as gm_rotary's y. k, v and q have one type.
  * slots int32, or int64 with slots_64; positions (absent without a rotary) alike. head_dim is at most 1024, n times the
- * heads of all three below 2^31; the cache's elements must be apart for different (page, head, token), and from all inputs. */
+ * heads of all three below 2^31; the cache's elements must be apart for different (page, head, token), its keys from its
+ * values, and both from all inputs. */
 #define GM_NO_ROTARY 0xffffffffu
 typedef struct gm_cache_append_desc {
     gm_cache cache;

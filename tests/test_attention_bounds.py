@@ -5,7 +5,7 @@ from fractions import Fraction
 
 import numpy as np
 import pytest
-from test_attention_calls import A, attention, cache, call, rows, shim  # noqa: F401 (a fixture)
+from test_attention_calls import A, append, attention, cache, call, rows, shim  # noqa: F401 (a fixture)
 
 
 @pytest.mark.parametrize("type", [1, 2])
@@ -41,3 +41,15 @@ def test_frequencies_of_many_turns(shim):  # noqa: F811
         turns = Fraction(float(v)) / turn
         off = abs((turns - math.floor(turns)) * 2 ** 64 - got)
         assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + Fraction(1, 2 ** 21), (v, got, float(off))
+
+
+def test_keys_and_values_of_one_address(shim):  # noqa: F811
+    """Appending keys and values to one array would leave either's: refused. Attention may read one array as both."""
+    d = append()
+    assert call(shim.plan_append, d, 3)[0] == 0
+    d.cache.v = d.cache.k
+    rc, why, _ = call(shim.plan_append, d, 3)
+    assert rc < 0 and "cache" in why
+    d = attention()
+    d.cache.v = d.cache.k
+    assert call(shim.plan_attention, d, 3)[0] == 0
