@@ -247,7 +247,7 @@ class AttentionOps {
         const uint64_t capacity = (uint64_t)d.table_width * d.cache.page_size;
         require(capacity < 1u << 29, "gm_attention: table_width * page_size is below 2^29");  // 2^25 tiles of 16 keys, 64 of them in 32 bits
         require(d.causal || !d.window, "gm_attention: a window without the causal mask");
-        require(d.scale > 0 && std::isfinite(d.scale), "gm_attention: scale");
+        require(d.scale > 0 && std::isfinite(d.scale * 1.44269504088896341f), "gm_attention: scale");  // (times log2 e in the kernels)
         const bool wide = d.cache.type == GM_F32;
         const uint32_t group = H / G;
         const uint64_t rows = (uint64_t)d.longest * group;

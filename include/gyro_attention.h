@@ -73,7 +73,7 @@ GM_API int gm_cache_append(gm_engine *e, const gm_cache_append_desc *desc, uint3
  * i < table_width (int32; cut to table_width * page_size, which is below 2^29).
  * Token i of q tokens stands at p = lengths[b] - q + i and sees the keys j <= p with `causal`, else all of its sequence's;
  * with a window w > 0 (and causal) only j > p - w. A key on a page outside the cache is seen by no token.
- *   out = sum_j softmax_j(scale q . k_j) v_j   (scale > 0)
+ *   out = sum_j softmax_j(scale q . k_j) v_j   (0 < scale < 2^127)
  * A token that sees no key, or only keys whose score is -infinity, has zeros. What is not seen does not count, NaNs and
  * infinities among it. Rows of q behind the last sequence's are left in out as they were. Products of 16-bit types are exact
  * and summed in fp32, as are the softmax's statistics; its weights may be rounded to the type before they meet v, in

@@ -53,3 +53,9 @@ def test_keys_and_values_of_one_address(shim):  # noqa: F811
     d = attention()
     d.cache.v = d.cache.k
     assert call(shim.plan_attention, d, 3)[0] == 0
+
+
+def test_scales(shim):  # noqa: F811
+    """The kernels' scale is times log2 e: one that leaves fp32 by that would make scores of zero NaN, and is refused."""
+    for scale, ok in ((2.3e38, True), (2.4e38, False), (3.4e38, False), (1e-44, True)):
+        assert (call(shim.plan_attention, attention(scale=scale), 3)[0] == 0) == ok, scale
