@@ -568,7 +568,7 @@ class Engine:
                   scale: float | None = None, causal: bool = True, window: int = 0, stream: int | None = None):
         """out = the attention of q's tokens (rows of heads) over the pages table[b] (int32 [sequences, width]) of each
         sequence's first lengths[b] keys (int32 [sequences]), the tokens' own among them. The sequences have equally many
-        tokens, or tokens starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1]) and at most `longest` of them. Without `causal`
+        tokens, or tokens starts[b] .. starts[b + 1] - 1 (int32 [sequences + 1]) and at most `longest` of them each. Without `causal`
         every token sees all keys; a window limits it to the last `window` up to its own. scale: 1 / sqrt(head_dim).
         workspace: a uint8 tensor of attention_workspace() bytes, not shared with calls that may overlap."""
         c = self._cache(k_cache, v_cache)
@@ -590,6 +590,8 @@ class Engine:
             sp = self._flat(starts, sequences + 1, _INT32, "starts")
             if longest is None:
                 raise ValueError("starts without the longest sequence's count")
+            if n < longest <= _MOST:
+                longest = n
         elif longest is None:
             if not sequences or n % sequences:
                 raise ValueError(f"q: {n} tokens are not of {sequences} equal sequences")

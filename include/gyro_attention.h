@@ -67,19 +67,20 @@ GM_API int gm_cache_append(gm_engine *e, const gm_cache_append_desc *desc, uint3
 /* Attention of new tokens over a paged cache that already holds theirs. q and out: rows of `heads` heads (a multiple of
  * kv_heads; head h reads the cache's head h / (heads / kv_heads)) of head_dim values, a multiple of 8 up to 256, of the
  * cache's type. Sequence b has the tokens starts[b] .. starts[b + 1] - 1 of q (int32 [sequences + 1], not falling), or,
- * with starts NULL, `longest` tokens from b * longest on (then n = sequences * longest); `longest` is at least every
- * sequence's count of tokens (of more, the first `longest` are certain to be computed, the rest may be left). Its keys are
- * the first lengths[b] places (int32, the new tokens' own among them) of the pages table[b * table_stride + i],
+ * with starts NULL, `longest` tokens from b * longest on (then n = sequences * longest); `longest`, at most n, is at least
+ * every sequence's count of tokens (of more, the first `longest` are certain to be computed, the rest may be left). Its keys
+ * are the first lengths[b] places (int32, the new tokens' own among them) of the pages table[b * table_stride + i],
  * i < table_width (int32; cut to table_width * page_size, which is below 2^29).
  * Token i of q tokens stands at p = lengths[b] - q + i and sees the keys j <= p with `causal`, else all of its sequence's;
  * with a window w > 0 (and causal) only j > p - w. A key on a page outside the cache is seen by no token.
  *   out = sum_j softmax_j(scale q . k_j) v_j   (0 < scale < 2^127)
- * A token that sees no key, or only keys whose score is -infinity, has zeros. What is not seen does not count, NaNs and
+ * A token that sees no key, or only keys whose score is -infinity (in fp32, times log2 e), has zeros. What is not seen does not count, NaNs and
  * infinities among it. Rows of q behind the last sequence's are left in out as they were. Products of 16-bit types are exact
  * and summed in fp32, as are the softmax's statistics; its weights may be rounded to the type before they meet v, in
  * binary16, which has no smaller ones, by up to 2^-36 of a row's largest; an infinite value times a weight that is zero then
  * is NaN. out may be q's rows, of the same stride; it overlaps nothing else. n * heads is at most 2^30, and
- * n * heads / kv_heads / 128 + sequences at most 2^18 - 1024.
+ * n * heads / kv_heads / 128 + sequences at most 2^18 - 1024; sequences * kv_heads, in fp32 and over caches not aligned to
+ * four bytes times the tiles of 16 rows in longest * heads / kv_heads, is below 2^31.
  * The workspace (256-byte aligned, of gm_attention_workspace(heads, kv_heads, head_dim) bytes, which serve every call of that
  * shape) holds nothing between calls; calls that may overlap, replayed graphs among them, take one each. */
 typedef struct gm_attention_desc {

@@ -5,6 +5,9 @@ from fractions import Fraction
 
 import numpy as np
 import pytest
+import torch
+from gyrodx import engine
+from gyrodx.engine import AttentionDesc, Engine
 from test_attention_calls import A, append, attention, cache, call, rows, shim  # noqa: F401 (a fixture)
 
 
@@ -59,3 +62,36 @@ def test_scales(shim):  # noqa: F811
     """The kernels' scale is times log2 e: one that leaves fp32 by that would make scores of zero NaN, and is refused."""
     for scale, ok in ((2.3e38, True), (2.4e38, False), (3.4e38, False), (1e-44, True)):
         assert (call(shim.plan_attention, attention(scale=scale), 3)[0] == 0) == ok, scale
+
+
+def test_binding_takes_any_bound(monkeypatch):
+    """A host's fixed bound on a sequence's tokens may be above the tokens of a call: no sequence has more than all of them, which
+    is what the library is told (it refuses more)."""
+    seen = []
+
+    class Library:
+        def gm_attention(self, handle, desc, n, on):
+            seen.append((AttentionDesc.from_buffer_copy(desc).longest, n))
+            return 0
+
+    monkeypatch.setattr(engine, "lib", Library)
+    e = Engine.__new__(Engine)
+    e._h, e.adapter, e._matrices = C.c_void_p(), -1, {}
+    x, kc = torch.zeros(6, 16), torch.zeros(5, 2, 16, 8)
+    table, lengths, starts = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    for longest in (2, 6, 7, 4096):
+        e.attention(x, kc, kc, table, lengths, x, starts=starts, longest=longest, stream=0)
+    assert seen == [(2, 6), (6, 6), (6, 6), (6, 6)]
+    e.attention(x, kc, kc, table, lengths, x, longest=7, stream=0)  # without starts: every sequence has as many
+    assert seen[-1] == (7, 6)
+
+
+def test_limits_as_stated(shim):  # noqa: F811
+    """`longest` up to n, and tiles of 16 rows of the longest sequence times all of them and the cache's heads below 2^31 in fp32."""
+    d = dict(heads=8, starts=A, table_width=100)
+    fp32 = cache(type=0, kv_heads=8, page_stride=8 * 1024)
+    for sequences, longest, n, ok in ((5000, 1 << 18, 1 << 20, True), (5000, 1 << 20, 1 << 20, False), (1 << 14, 1 << 18, 1 << 20, False),
+                                      ((1 << 14) - 1, 1 << 18, 1 << 20, True), (1, 1 << 21, 1 << 20, False)):
+        assert (sequences * -(-longest // 16) * 8 < 1 << 31 and longest <= n) == ok
+        rc, why, _ = call(shim.plan_attention, attention(cache=fp32, q=rows(0), out=rows(0, data=3 * A), sequences=sequences, longest=longest, **d), n)
+        assert (rc == 0) == ok, (sequences, longest, why)
