@@ -320,7 +320,7 @@ __device__ __forceinline__ void af_finish(const GdArgs &a, const AfWork &k, floa
 // compute unit) and an eighth more, so that tiles a little larger than that are not split into units that fill a second round
 // by half (40 tiles of 250 and 22 small ones, four heads: 4 parts each 288 us, 3 parts 230).
 __device__ __forceinline__ uint32_t at_fair(const GdArgs &a, uint64_t all) {
-    return (uint32_t)max((uint64_t)a.c[58], (all * a.c[31] * 9u + 4095u) / 4096u);
+    return (uint32_t)min(max((uint64_t)a.c[58], (all * a.c[31] * 9u + 4095u) / 4096u), (uint64_t)~0u);
 }
 
 // How the many rows' keys are shared out without a list: entry e is tile tiles - 1 - e / sequences of sequence e % sequences, the
