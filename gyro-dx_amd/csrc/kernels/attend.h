@@ -2,19 +2,20 @@
 // cache's heads, `group` = heads / kv_heads queries' heads each, are its rows: row r is head r % group of token r / group, so
 // that a page read once serves them all.
 //
-// Sequences of few rows or short ones (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and cache head and a
-// part of its keys, and finds out by itself which (af_share). The others (attend_tile.h): a group takes a unit, a tile of 128
-// rows and a run of its keys, of every head; of up to 1024 tiles it finds out by itself which (at_share), of more attend_plan
-// makes a list. Where keys are split, attend_join puts the parts together.
+// Sequences of few rows or short ones (attend_few.h, fp32 in attend_f32.h): a group takes a tile of 16 rows of a sequence and
+// cache head and a part of its keys, and finds out by itself which (af_share). The others (attend_tile.h): a group takes a
+// unit, a tile of 128 rows and a run of its keys, of every head; of up to 1024 tiles it finds out by itself which (at_share),
+// of more attend_plan makes a list. Where keys are split, attend_join puts the parts together.
 //
-// Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table
-// 20 table stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 tiles of 128 rows of the longest sequence 29 group 30 D 31 kv heads
-// 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 flags (1 causal, 2 32 bits span the cache) 39 window 40 scale times log2(e)
-// 41 groups that few rows' keys are split for (0: they are not) 42 tiles of few rows per sequence 43 type 44 keys of a tile
-// 45 tiles that make a part 46 rows of a sequence that units take it from (0: none) 47 groups of attend_join for
-// the few rows 48 units' list (0: none) 50 units' parts 52 logarithm of the page size, rounded up, and 59 its reciprocal 53 units that the list holds
-// 54 parts that the workspace holds, per head 55 keys of a tile of units 56 rows that attend_join takes of a few rows' tile
-// 57 tiles of keys up to which few rows' are not split 58 tiles that make a unit
+// Constants: 0 q 2 q stride 4 out 6 out stride 8 k 10 v 12 page stride 14 head stride 16 token stride (bytes) 18 table 20 table
+// stride 22 lengths 24 starts (0: `longest` tokens each) 26 few rows' parts 28 tiles of 128 rows of the longest sequence 29
+// group 30 D 31 kv heads 32 sequences 33 longest 34 tokens 35 pages 36 page size 37 table width 38 flags (1 causal, 2 32 bits
+// span the cache) 39 window 40 scale times log2(e) 41 groups that few rows' keys are split for (0: they are not) 42 tiles of
+// few rows per sequence 43 type 44 keys of a tile 45 tiles that make a part 46 rows of a sequence that units take it from (0:
+// none) 47 groups of attend_join for the few rows 48 units' list (0: none) 50 units' parts 52 logarithm of the page size,
+// rounded up, and 59 its reciprocal 53 units that the list holds 54 parts that the workspace holds, per head 55 keys of a tile
+// of units 56 rows that attend_join takes of a few rows' tile 57 tiles of keys up to which few rows' are not split 58 tiles
+// that make a unit
 
 #pragma once
 #include "rows.h"
@@ -137,10 +138,10 @@ __device__ __forceinline__ void at_store4(uint64_t row, uint32_t d, gd_f32x4 x, 
 // Where maxima begin: no finite score is below it, and the difference of two such is zero, not NaN.
 #define AT_LOWEST -3.402823466e38f
 
-// A weight is exp2(s scale - top), in one fused step. top is a product of that kind as well, but rounded: off by up to half a unit of
-// its last place, by which all of a row's weights are too large or small alike. From 2^20 on that is 2^-5 and more, and with no
-// bound: of scores of 10^10 all weights were zero, or infinite. Rows with such a top take both products rounded, so that the
-// largest score's weight is one.
+// A weight is exp2(s scale - top), in one fused step. top is a product of that kind as well, but rounded: off by up to half a
+// unit of its last place, by which all of a row's weights are too large or small alike. From 2^20 on that is 2^-5 and more, and
+// with no bound: of scores of 10^10 all weights were zero, or infinite. Rows with such a top take both products rounded, so
+// that the largest score's weight is one.
 #define AT_FAR 1048576.f
 __device__ __forceinline__ bool at_far(float top) { return (fabsf(top) >= AT_FAR) & (top > AT_LOWEST); }
 __device__ __forceinline__ float at_from_top(float s, float scale, float top) {
@@ -161,9 +162,9 @@ __device__ __forceinline__ float af_sum(float v) {
     return at_sum_halves(gd_bits_f32(r[0]) + gd_bits_f32(r[1]));
 }
 
-// How the few rows' keys are shared out: entry e is tile e % tiles of sequence e / tiles. One of more tiles of keys than a constant is
-// split into as many parts as leave none more than `share` tiles, a fair part of all entries' and heads' among the groups. The
-// split entries' parts come first, then the whole ones. Every wave works this out by itself, 64 entries at a time.
+// How the few rows' keys are shared out: entry e is tile e % tiles of sequence e / tiles. One of more tiles of keys than a
+// constant is split into as many parts as leave none more than `share` tiles, a fair part of all entries' and heads' among the
+// groups. The split entries' parts come first, then the whole ones. Every wave works this out by itself, 64 entries at a time.
 struct AfEntry {
     uint32_t rows, keys;  // of the sequence (0: none for this launch), tiles of keys
 };

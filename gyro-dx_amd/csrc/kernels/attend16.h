@@ -32,12 +32,12 @@ __device__ __forceinline__ float at_finite(uint32_t w, float c) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(at_f16x2, w), at_f16x2{(_Float16)0.f, (_Float16)0.f}, c, false);
 }
 
-// Weights are relative to a top that follows the running maximum only when that has grown by more than 2^GROWN, so that the sums
-// are rarely rescaled. bf16 has fp32's exponents, and GROWN 8. Binary16 ends at 2^-24: its weights are 2^LIFT larger, which the
-// sums share, as far as 2^16 allows. A weight is then rounded by half a unit of its last place or by 2^-25-LIFT of the largest.
-// (131,071 keys 19 nats below one whose value is zero: off by 67% with LIFT 0 and GROWN 8.) Rows bound by memory have LIFT 15, many
-// rows 11: 4096 tokens of 32 heads of 128 over 8, us: LIFT 7 170, 11 172, 13 175, heads of 256, 2048 tokens 171, 183, 195. A top that
-// is far has no room for LIFT in its last places, and needs none.
+// Weights are relative to a top that follows the running maximum only when that has grown by more than 2^GROWN, so that the
+// sums are rarely rescaled. bf16 has fp32's exponents, and GROWN 8. Binary16 ends at 2^-24: its weights are 2^LIFT larger,
+// which the sums share, as far as 2^16 allows. A weight is then rounded by half a unit of its last place or by 2^-25-LIFT of
+// the largest. (131,071 keys 19 nats below one whose value is zero: off by 67% with LIFT 0 and GROWN 8.) Rows bound by memory
+// have LIFT 15, many rows 11: 4096 tokens of 32 heads of 128 over 8, us: LIFT 7 170, 11 172, 13 175, heads of 256, 2048 tokens
+// 171, 183, 195. A top that is far has no room for LIFT in its last places, and needs none.
 template <uint32_t TYPE>
 __device__ __forceinline__ bool at_grown(float most, float top) { return most > top + (TYPE == ROW_F16 ? 15.f : 8.f); }
 template <uint32_t TYPE, uint32_t LIFT>

@@ -10,11 +10,11 @@
 // Weights are at most 2^8 in bf16, where the sums are rescaled only when the maximum has grown by as much; in binary16 they reach
 // 2^15 and every growth is followed, so that small ones lose least (at_grown).
 //
-// The weights are the sum of two 16-bit parts, 16 bits of them in bf16 and 22 in binary16: these rows are bound by memory, and the
-// second products run in its shadow.
+// The weights are the sum of two 16-bit parts, 16 bits of them in bf16 and 22 in binary16: these rows are bound by memory, and
+// the second products run in its shadow.
 //
 // Bound by the cache's bytes: a token each of 64 sequences of 91 to 8192 keys, 8 heads of 128 values, 560 MB, 108 us (5.2 TB/s;
-// vector unit 16% of cycles, matrix unit 5%); one token over 131072 keys, 2 heads of 256, 268 MB, 53 us (5.1 TB/s). A wave has a
+// vector unit 16% of cycles, matrix unit 5%); one token over 131072 keys, 2 heads of 256, 268 MB, 52 us (5.1 TB/s). A wave has a
 // tile of keys and one of values on their way at any time. Of short contexts the chain of dependent loads is the time: 777
 // keys by eight waves 12 us, 300 keys 8.5.
 #pragma once

@@ -1,6 +1,6 @@
 // Joins the parts of rows whose keys several groups shared (attend.h). The first groups take the few rows' split entries, a
-// group a row, as these may have hundreds of parts; the others the many rows' split tiles, in turn. Bound by latency (which were split,
-// statistics, parts): 5 to 10 us, of which the launch is 2.
+// group a row, as these may have hundreds of parts; the others the many rows' split tiles, in turn. Bound by latency (which
+// were split, statistics, parts): 5 to 10 us, of which the launch is 2.
 #include "attend.h"
 
 // Row r of a sequence and head in out.
@@ -29,7 +29,8 @@ __device__ __forceinline__ float aj_group(float v, float *waves, F join) {
     return v;
 }
 
-// A row of parts of ROWS rows, `step` bytes apart from `at` on, by the group: slices of it take parts in turn, four channels a thread.
+// A row of parts of ROWS rows, `step` bytes apart from `at` on, by the group: slices of it take parts in turn, four channels a
+// thread.
 template <uint32_t ROWS>
 __device__ __forceinline__ void aj_by_group(const GdArgs &a, uint64_t at, uint64_t step, uint32_t parts, uint32_t r, uint64_t out) {
     constexpr uint32_t HELD = 5, MOST = HELD * AJ_THREADS;  // few rows' keys are split for 1024 groups at most, an entry in one part more
@@ -127,8 +128,8 @@ __device__ __forceinline__ void aj_by_lanes(const GdArgs &a, uint64_t at, uint64
     if (d < D) aj_store(a, out, d, x, total);
 }
 
-// The rows of split tiles, `splits` of them, each of every head, among the groups from number `group` on. `entry` tells a split's sequence,
-// tile of rows, first slot and parts.
+// The rows of split tiles, `splits` of them, each of every head, among the groups from number `group` on. `entry` tells a
+// split's sequence, tile of rows, first slot and parts.
 template <typename F>
 __device__ __forceinline__ void aj_tiles(const GdArgs &a, uint32_t group, uint32_t groups, uint32_t splits, F entry) {
     const uint32_t KVH = a.c[31], D = a.c[30], wide = D > 128u ? 64u : D > 64u ? 32u : 16u, at_once = AJ_THREADS / wide;

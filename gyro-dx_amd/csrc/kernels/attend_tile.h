@@ -1,5 +1,5 @@
-// Attention of many rows (attend.h), 16-bit types: a group of four waves takes 128 rows, 32 a wave, and a run of tiles of 64 or 32
-// keys (its unit), which go from memory straight to LDS, two buffers of keys and of values in turn.
+// Attention of many rows (attend.h), 16-bit types: a group of four waves takes 128 rows, 32 a wave, and a run of tiles of 64 or
+// 32 keys (its unit), which go from memory straight to LDS, two buffers of keys and of values in turn.
 //
 // Scores are K Q^T by v_mfma_f32_32x32x16: a lane holds half the keys of one row, the other half is lane ^ 32's, so the
 // running maximum needs one exchange per tile, the sum none until the end, and the weights are the second product's operand
@@ -11,10 +11,16 @@
 // LDS is filled 1 KB an instruction in the order of lanes, so rows cannot be padded; instead their 16-byte pieces are swapped
 // by the row's number such that every read finds its lanes in different banks (at_tile_k, at_tile_v; no conflict was counted).
 //
-// 4096 tokens of 32 heads over 8 of 128 values, causal: 156 us with the join (881 TFLOP/s; a large library product reaches 1131). Matrix
-// instructions fill 40% of all cycles and vector instructions 44%, at two waves a SIMD, which 248 registers allow. More buffers and earlier reads
-// of LDS gained nothing, a wave's higher priority around its products 6%, 32-bit offsets into the cache, groups that
-// find their units without a list and even rounds 5%. 128 rows halve the reads of 64; 256 would leave one wave a SIMD.
+// Weights are rounded once to the type before they meet the values, at most half a step and both ways alike, and summed as
+// rounded: a second product for what is lost, as attend_few.h has it, would be half of the second products' work again, and the
+// matrix unit is what bounds this kernel. Against 64 bits a bf16 prompt is off by 0.0020, with its result's rounding alone by
+// 0.0016.
+//
+// 4096 tokens of 32 heads over 8 of 128 values, causal: 158 us with the join (869 TFLOP/s; a large library product reaches
+// 1131). Matrix instructions fill 40% of all cycles and vector instructions 45%, at two waves a SIMD, which 249 registers
+// allow. More buffers and earlier reads of LDS gained nothing, a wave's higher priority around its products 6%, 32-bit offsets
+// into the cache, groups that find their units without a list and even rounds 5%. 128 rows halve the reads of 64; 256 would
+// leave one wave a SIMD.
 #pragma once
 #include "attend16.h"
 #include <type_traits>
@@ -158,8 +164,8 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
     uint32_t soon = page(unit_from + 2u);
     asm volatile("" : "+v"(soon));
     at_f32x16 s[BLOCKS];
-    // A tile's scores, a product a step: its operand is read AHEAD steps before, `beside` is work to run beside it. The steps stay
-    // in this order (the scheduler would put one kind of work after the other).
+    // A tile's scores, a product a step: its operand is read AHEAD steps before, `beside` is work to run beside it. The steps
+    // stay in this order (the scheduler would put one kind of work after the other).
     constexpr uint32_t PRODUCTS = STEPS * BLOCKS, AHEAD = 3;
     gd_u32x4 operand[AHEAD];
     uint32_t base_k = 0;
@@ -256,8 +262,8 @@ __device__ __forceinline__ void attend_tile_of(const GdArgs &a, const AtUnit &un
 #pragma unroll
                 for (int i = 0; i < 16 * (int)BLOCKS; ++i) s[i >> 4][i & 15] = at_from_top(s[i >> 4][i & 15], scale, top);
             const float by = far ? 1.f : scale, from = far ? 0.f : top;
-            // The weights beside the next tile's scores (of the last one's: of what is in the buffer), with the first of V^T, whose
-            // 16 keys and 32 channels an operand has in the order of the weights, behind.
+            // The weights beside the next tile's scores (of the last one's: of what is in the buffer), with the first of V^T,
+            // whose 16 keys and 32 channels an operand has in the order of the weights, behind.
             constexpr uint32_t PAIRS = 8u * BLOCKS;
             constexpr uint32_t SUMS = 2u * BLOCKS * DIMS, RING = 4;
             gd_u32x4 w[BLOCKS][2], x[RING];

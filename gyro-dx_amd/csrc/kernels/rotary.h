@@ -1,8 +1,8 @@
 // Heads turned by their positions, and new tokens' keys and values on their way into a paged cache:
 //   (y1, y2) = scale (x1 cos a - x2 sin a, x1 sin a + x2 cos a),  a = position * frequency of the pair
-// Rows of up to three kinds in one launch: queries (turned, to rows), keys (turned, to the cache's slots) and values
-// (as they are, to the slots). A group takes a token, or a part of one, forms its sines and cosines once, a pair a thread, and
-// turns its heads by them; of many tokens a wave takes one, if its turns cover the heads. A thread takes units of 8 pairs (or 16 values
+// Rows of up to three kinds in one launch: queries (turned, to rows), keys (turned, to the cache's slots) and values (as they
+// are, to the slots). A group takes a token, or a part of one, forms its sines and cosines once, a pair a thread, and turns its
+// heads by them; of many tokens a wave takes one, if its turns cover the heads. A thread takes units of 8 pairs (or 16 values
 // that do not turn) of a head.
 //
 // Angles: a frequency is a fraction of a turn in 64 bits, whole turns dropped; its product with the position modulo 2^64 is the
@@ -10,14 +10,14 @@
 // left, at most an eighth of a turn, goes to fp32 and through the series of sine and cosine up to x^9 and x^10 (a remainder
 // below 2e-9). fp32 angles would be wrong in the first digit at a position of 10^6.
 //
-// Bound by memory where there are many tokens: 4096 of 32 + 2 x 8 heads of 128 bf16 values, 101 MB in and out, take 19 us (5.3 TB/s; a call
-// in a loop 21.0, a copy of as many bytes 21.7), 1023 of 40 heads 7.5; of one token the launch, 3.7.
+// Bound by memory where there are many tokens: 4096 of 32 + 2 x 8 heads of 128 bf16 values, 101 MB in and out, take 18.7 us
+// (5.4 TB/s; a call in a loop 21.3, a copy of as many bytes 21.7), 1023 of 40 heads 7.3; of one token the launch, 3.8.
 //
-// Constants: 0 q 2 q stride 4 q_out 6 q_out stride 8 k 10 k stride 12 v 14 v stride 16 cache k 18 cache v 20 page stride
-// 22 head stride 24 token stride (bytes) 26 frequencies (0: nothing turns) 28 positions 30 slots 32 D 33 pairs 34 query heads
-// 35 kv heads (0: no cache) 36 tokens 37 types (q_out | cache << 4) 38 flags (1 interleaved, 2 positions in 64 bits, 4 slots
-// in 64 bits, 8 q in place) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two heads of
-// a thread 45 a wave takes a token
+// Constants: 0 q 2 q stride 4 q_out 6 q_out stride 8 k 10 k stride 12 v 14 v stride 16 cache k 18 cache v 20 page stride 22
+// head stride 24 token stride (bytes) 26 frequencies (0: nothing turns) 28 positions 30 slots 32 D 33 pairs 34 query heads 35
+// kv heads (0: no cache) 36 tokens 37 types (q_out | cache << 4) 38 flags (1 interleaved, 2 positions in 64 bits, 4 slots in 64
+// bits, 8 q in place) 39 scale 40 page size 41 pages * page size 42 groups that share a token 43 units per head 44 turns of two
+// heads of a thread 45 a wave takes a token
 #pragma once
 #include "rows.h"
 
@@ -39,8 +39,8 @@ __device__ __forceinline__ void ro_turn(uint64_t fraction, float scale, float &c
     s = scale * (q & 2u ? -b : b);
 }
 
-// Values i .. i + 7 of a head. FULL: all of them are in it, and they stay as they are in memory until they are used, so that loads
-// follow each other without a wait; low .. m - 1 are stored. Otherwise the first m <= 8 are there.
+// Values i .. i + 7 of a head. FULL: all of them are in it, and they stay as they are in memory until they are used, so that
+// loads follow each other without a wait; low .. m - 1 are stored. Otherwise the first m <= 8 are there.
 template <uint32_t TYPE, bool FULL>
 struct RoEight {
     gd_u32x4 raw[TYPE == ROW_F32 ? 2 : 1];
@@ -107,10 +107,10 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
     const uint32_t at_once = width / units, own = tid / units, u = tid - own * units;
     const uint32_t head0 = (uint32_t)(id - of * sharers) * turns * 2u * at_once + own;
     const uint32_t turning = (pairs + 7u) / 8u;  // units of pairs; the others' values are copied
-    // The halves of a unit in a head that turns and in one that does not: their places, and how many values of each there are. FULL: a
-    // half that would reach past the pairs or the head's end moves down to it, and begins to store at its own first value; pairs
-    // that two units turn need no such care but in place, as both have the same values. Fewer than eight pairs are one unit's, which
-    // reads on behind them.
+    // The halves of a unit in a head that turns and in one that does not: their places, and how many values of each there are.
+    // FULL: a half that would reach past the pairs or the head's end moves down to it, and begins to store at its own first
+    // value; pairs that two units turn need no such care but in place, as both have the same values. Fewer than eight pairs are
+    // one unit's, which reads on behind them.
     uint32_t f1, f2, n1 = 8, n2 = 8, low1 = 0, low2 = 0, pair0 = 8u * u;
     if (u < turning) {
         const uint32_t m = min(8u, pairs - pair0);
@@ -153,7 +153,8 @@ __device__ __forceinline__ void rotary_rows(const GdArgs &a, float *cosines, flo
     }
 #pragma unroll 1
     for (uint32_t turn = 0; turn < turns; ++turn) {
-        // Two heads at a time: the second's loads are on their way with the first's, the first turn's while the angles are formed.
+        // Two heads at a time: the second's loads are on their way with the first's, the first turn's while the angles are
+        // formed.
         RoEight<TYPE, FULL> first[2], second[2];
         uint64_t y[2];
         bool stays[2], query[2], value[2];

@@ -34,8 +34,8 @@ class AttentionOps {
 
     // ---- rotary positions ----
 
-    // The fraction of a turn, of 2^64, by which a frequency below 2^31 turns, rounded: m 2^-down (m of 53 bits) times 1 / (2 pi) in
-    // 128 bits, before rounding exact to 2^-21 of the last place, however many whole turns there are.
+    // The fraction of a turn, of 2^64, by which a frequency below 2^31 turns, rounded: m 2^-down (m of 53 bits) times 1 / (2
+    // pi) in 128 bits, before rounding exact to 2^-21 of the last place, however many whole turns there are.
     static uint64_t fraction(double frequency) {
         constexpr uint64_t high = 0x28be60db9391054aull, low = 0x7f09d5f47d4d3770ull;  // 2^128 / (2 pi)
         int e;
@@ -112,10 +112,11 @@ class AttentionOps {
         c.set(35, kv_heads);
         c.set(36, n);
         const uint32_t units = std::max((pairs + 7) / 8 + (D - 2 * pairs + 15) / 16, (D + 15) / 16);
-        // A group's 256 threads take at_once heads together, two a thread and turn. Of few tokens a group takes one turn of a token,
-        // so that all are on their way at once; of many (256 compute units hold eight groups each) up to eight turns of it, or, where
-        // eight turns of a wave cover the heads, four tokens, one a wave (us, 4096 tokens of 128 values: one head 20 and 9.5, 8 heads
-        // 13.0 and 7.2, 24 14.8 and 12.4; 32 and 8 + 8 into a cache 26.8 and 24.8).
+        // A group's 256 threads take at_once heads together, two a thread and turn. Of few tokens a group takes one turn of a
+        // token, so that all are on their way at once; of many (256 compute units hold eight groups each) up to eight turns of
+        // it, or, where eight turns of a wave cover the heads, four tokens, one a wave (us, 4096 tokens of 128 values: one head
+        // 20 and 9.5, 8 heads 13.0 and 7.2, 24 14.8 and 12.4; 32 and 8 + 8 into a cache 26.8 and 24.8; replayed, 2048 tokens of
+        // 8 heads 6.7 and 4.3, of 32 and 8 + 8 13.2 and 12.2, 1023 tokens 4.6 and 3.8, 8.1 and 9.9).
         const bool narrow = n > 2048 && units <= 64 && 16 * (64 / units) >= all && pairs <= 128;
         const uint32_t at_once = (narrow ? 64 : 256) / units, all_turns = (all + 2 * at_once - 1) / (2 * at_once);
         const uint32_t turns = (uint64_t)n * all_turns > 2048 ? std::min(all_turns, 8u) : 1u, sharers = (all_turns + turns - 1) / turns;
@@ -181,8 +182,8 @@ class AttentionOps {
         }
         require(d.slots && (uintptr_t)d.slots % (d.slots_64 ? 8 : 4) == 0, "gm_cache_append: slots");
         require(!r || (d.positions && (uintptr_t)d.positions % (d.positions_64 ? 8 : 4) == 0), "gm_cache_append: positions");
-        // No two (page, head, token) may share an element: of two dimensions one's stride spans the other's extent. (Whether keys and
-        // values lie apart is the caller's to know; one array for both is told.)
+        // No two (page, head, token) may share an element: of two dimensions one's stride spans the other's extent. (Whether
+        // keys and values lie apart is the caller's to know; one array for both is told.)
         check_apart(d.cache);
         require(d.cache.k != d.cache.v, "gm_cache_append: the cache's keys and values are one array");
         turn(l, r, d.heads ? &d.q : nullptr, &d.q_out, d.heads, &d.k, &d.v, G, D, n);
@@ -251,12 +252,12 @@ class AttentionOps {
         const bool wide = d.cache.type == GM_F32;
         const uint32_t group = H / G;
         const uint64_t rows = (uint64_t)d.longest * group;
-        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile if these tiles are more than
-        // 512 or have more keys to read (as far as the table tells) than 2^18: below that the kernels of few rows, which read a
-        // sequence's keys once for every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000 keys 18 against 24,
-        // of 16000 32 against 31; 256 rows of 2000 24 against 27, of 4000 40 against 29; 512 pairs of 300 keys 16 against 25, 1024
-        // 32 against 27). attend_tile loads straight to LDS, which wants addresses that are multiples of four bytes (4096 tokens of 32
-        // heads over 8 160 us, over a cache off by two bytes 2360; 256 tokens 14 and 26).
+        // Tiles of 16 rows of all sequences and cache heads. Rows past 16 of a sequence go to attend_tile if these tiles are
+        // more than 512 or have more keys to read (as far as the table tells) than 2^18: below that the kernels of few rows,
+        // which read a sequence's keys once for every 16 rows but start faster, are ahead (us, 8 cache heads: 64 rows of 4000
+        // keys 18 against 24, of 16000 32 against 31; 256 rows of 2000 24 against 27, of 4000 40 against 29; 512 pairs of 300
+        // keys 16 against 25, 1024 32 against 27). attend_tile loads straight to LDS, which wants addresses that are multiples
+        // of four bytes (4096 tokens of 32 heads over 8 160 us, over a cache off by two bytes 2360; 256 tokens 14 and 26).
         const uint64_t row_tiles = (rows + kFewRows - 1) / kFewRows;
         const unsigned __int128 pairs = (unsigned __int128)row_tiles * d.sequences * G;
         const bool direct = !wide && !(((uintptr_t)d.cache.k | (uintptr_t)d.cache.v | (d.cache.pages > 1 ? 2 * d.cache.page_stride : 0) |
@@ -362,21 +363,20 @@ class AttentionOps {
         if (join) l.add("attend_join", join);
         return l;
     }
-    // Few rows' keys: groups that the GPU holds, by the heads' size, and parts for each of them where row tiles and heads (half as many
-    // or more) differ in keys (us: 64 sequences of 91 to 8192 keys 110 with one part, 98 with two, of 4000 each 198 and 207; 4 of
-    // 4000 each 19.5 and 23).
+    // Few rows' keys: groups that the GPU holds, by the heads' size, and parts for each of them where row tiles and heads (half
+    // as many or more) differ in keys (us: 64 sequences of 91 to 8192 keys 110 with one part, 98 with two, of 4000 each 198 and
+    // 207; 4 of 4000 each 19.5 and 23).
     static constexpr uint32_t kResident[3] = {512, 512, 256}, kPerGroup = 2;
     // Keys that make a part (twice as many in fp32). 1500 keys of one sequence: 11.1 us with 128, 12.0 with 256, 14.0 with 512.
     static constexpr uint32_t kLeast = 128;
-    // Keys of one group alone against several and a join, us, replayed (outside a graph the second launch costs its caller 2 more),
-    // 8 heads of 128 values: one sequence of 640 keys 10.9 and 10.8, of 1024
-    // 14.0 and 10.9; 8 of 1024 15.1 and 15.4, of 2048 24.6 and 19.5; 16 of 2048 26 and 31, of 4000 71 and 59; 32 of 2048 42 and 49.
-    // Heads of 256, 16 of 1024 31 and 38, of 1536 55 and 52. fp32: 8 tiles of 512 keys 11.9 and 13.0, of 1024 18 and 13; 112 of 1024 20
-    // and 27, of 4096 58 and 65.
+    // Keys of one group alone against several and a join, us, replayed (outside a graph the second launch costs its caller 2
+    // more), 8 heads of 128 values: one sequence of 640 keys 10.9 and 10.8, of 1024 14.0 and 10.9; 8 of 1024 15.1 and 15.4, of
+    // 2048 24.6 and 19.5; 16 of 2048 26 and 31, of 4000 71 and 59; 32 of 2048 42 and 49. Heads of 256, 16 of 1024 31 and 38, of
+    // 1536 55 and 52. fp32: 8 tiles of 512 keys 11.9 and 13.0, of 1024 18 and 13; 112 of 1024 20 and 27, of 4096 58 and 65.
     static constexpr uint32_t kWidePairs = 96;
     static constexpr uint32_t kFewKeys = 1u << 18, kFewPairs = 512;
-    // Many rows: tiles of rows and heads from which on a part has 16 tiles of keys at least, otherwise 4 (us: 1023 tokens of 32 heads
-    // alone, 256 such tiles, 44.5 with 4 and 34.6 with 16; 64 tokens of 4096 keys, 16 tiles, 28.4 and 36.5).
+    // Many rows: tiles of rows and heads from which on a part has 16 tiles of keys at least, otherwise 4 (us: 1023 tokens of 32
+    // heads alone, 256 such tiles, 44.5 with 4 and 34.6 with 16; 64 tokens of 4096 keys, 16 tiles, 28.4 and 36.5).
     static constexpr uint32_t kTilePairs = 128;
 };
 

@@ -19,7 +19,8 @@ extern "C" {
  * magnitude below 2^31), and is multiplied by `scale`:
  *   (y1, y2) = scale (x1 cos a - x2 sin a, x1 sin a + x2 cos a)
  * GM_ROTARY_HALF: x1 = x[j], x2 = x[pairs + j]; GM_ROTARY_INTERLEAVED: x1 = x[2 j], x2 = x[2 j + 1]. The values behind
- * them are copied. Angles are exact to 2^-27 of a turn for positions below 2^36 in magnitude (64-bit fixed point, modulo whole turns). */
+ * them are copied. Angles are exact to 2^-27 of a turn for positions below 2^36 in magnitude (64-bit fixed point, modulo whole
+ * turns). */
 enum { GM_ROTARY_HALF = 0, GM_ROTARY_INTERLEAVED = 1 };
 /* Uploads frequencies (1 to 512 pairs) and returns their index. */
 GM_API int gm_add_rotary(gm_engine *e, const double *frequencies, uint32_t pairs, uint32_t layout, float scale,
@@ -74,11 +75,11 @@ GM_API int gm_cache_append(gm_engine *e, const gm_cache_append_desc *desc, uint3
  * Token i of q tokens stands at p = lengths[b] - q + i and sees the keys j <= p with `causal`, else all of its sequence's;
  * with a window w > 0 (and causal) only j > p - w. A key on a page outside the cache is seen by no token.
  *   out = sum_j softmax_j(scale q . k_j) v_j   (0 < scale < 2^127)
- * A token that sees no key, or only keys whose score is -infinity (in fp32, times log2 e), has zeros. What is not seen does not count, NaNs and
- * infinities among it. Rows of q behind the last sequence's are left in out as they were. Products of 16-bit types are exact
- * and summed in fp32, as are the softmax's statistics; its weights may be rounded to the type before they meet v, in
- * binary16, which has no smaller ones, by up to 2^-36 of a row's largest; an infinite value times a weight that is zero then
- * is NaN. out may be q's rows, of the same stride; it overlaps nothing else. n * heads is at most 2^30, and
+ * A token that sees no key, or only keys whose score is -infinity (in fp32, times log2 e), has zeros. What is not seen does
+ * not count, NaNs and infinities among it. Rows of q behind the last sequence's are left in out as they were. Products of
+ * 16-bit types are exact and summed in fp32, as are the softmax's statistics; its weights may be rounded to the type before
+ * they meet v, in binary16, which has no smaller ones, by up to 2^-36 of a row's largest; an infinite value times a weight that
+ * is zero then is NaN. out may be q's rows, of the same stride; it overlaps nothing else. n * heads is at most 2^30, and
  * n * heads / kv_heads / 128 + sequences at most 2^18 - 1024; sequences * kv_heads, in fp32 and over caches not aligned to
  * four bytes times the tiles of 16 rows in longest * heads / kv_heads, is below 2^31.
  * The workspace (256-byte aligned, of gm_attention_workspace(heads, kv_heads, head_dim) bytes, which serve every call of that
