@@ -69,6 +69,24 @@ def test_scores_of_any_size(eng, type, sign, ones):  # noqa: F811
 
 
 @pytest.mark.usefixtures("reach")
+@pytest.mark.parametrize("type", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("window", [0, 70])
+def test_scores_of_any_size_side_by_side(eng, type, window):  # noqa: F811
+    """Rows whose scores are of every size, in one tile: the ordinary ones lose nothing by the others, of which the first
+    begin with small scores and grow, and none is NaN."""
+    for counts, lengths in (([5, 3], [700, 90]), ([2], [9000]), ([150, 40], [400, 300]), ([18], [6000])):
+        b = Batch(eng, type, 4, 2, 64, 16, counts, lengths, seed=49)
+        b.q[0::3] *= 200
+        b.q[1::9] *= 60
+        b.kc[:, :, 5::8] *= 100
+        for scale in (0.125, 300.0):
+            b.out.fill_(7.0)
+            print(f"side by side {type} {counts} {lengths} {scale}", flush=True)
+            b.run(scale=scale, window=window)
+            b.check(scale=scale, window=window, norm=False)
+
+
+@pytest.mark.usefixtures("reach")
 @pytest.mark.parametrize("counts,lengths", [([1, 2], [4000, 300]), ([40], [4000])], ids=["few", "many"])
 @pytest.mark.parametrize("below", [13, 17, 19, 21])
 def test_small_weights(eng, below, counts, lengths):  # noqa: F811
